@@ -8,6 +8,7 @@
 #include <mutex>
 #include <unordered_map>
 
+#include "beam_api.h"
 #include "chain_api.h"
 #include "divisor.h"
 #include "gemm_api.h"
@@ -1077,6 +1078,7 @@ Tensor prefill_attention_tc(const Tensor& q, const Tensor& k_cache, const Tensor
 #include "bindings_streams.inc"
 #include "bindings_recurrent.inc"
 #include "bindings_mixed.inc"
+#include "bindings_beam.inc"
 
 // ---- sampling ---------------------------------------------------------------------------------------------------------
 std::vector<Tensor> argmax(const Tensor& logits, c10::optional<Tensor> mask, double softcap, double inv_scale) {
@@ -1874,6 +1876,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mixed_decode", &mixed_decode, py::arg("q"), py::arg("mix"), py::arg("k_cache"), py::arg("v_cache"), py::arg("block_tables"), py::arg("ctx_lens"),
         py::arg("H"), py::arg("KV"), py::arg("scale"), py::arg("window"), py::arg("splits"), py::arg("gate") = py::none(), py::arg("out_mult") = 1.0,
         py::arg("out") = py::none());
+  m.def("beam_select", &beam_select, py::arg("logits"), py::arg("scores"), py::arg("k"), py::arg("mask") = py::none(), py::arg("softcap") = 0.0,
+        py::arg("inv_scale") = 1.0, py::arg("splits") = 0);
+  m.def("beam_move", &beam_move, py::arg("tensors"), py::arg("slots"), py::arg("parents"), py::arg("rows") = py::none(), py::arg("paged") = false);
   m.def("q4_quantize", &q4_quantize);
   m.def("q4_dequantize", &q4_dequantize, py::arg("packed"), py::arg("scales"), py::arg("to_bf16") = false);
 }

@@ -393,3 +393,39 @@ def stream_read(streams, read):
 def log_softmax_at(logits: torch.Tensor, idx: torch.Tensor) -> torch.Tensor:
     lf = logits.float()
     return lf.gather(-1, idx) - torch.logsumexp(lf, dim=-1, keepdim=True)
+
+
+# ---------------------------------------------------------------------------------------------------------------- beam search
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, allowed: Optional[torch.Tensor], softcap: float, inv_scale: float):
+    """The ``k`` largest finite ``scores[b, w] + log softmax(z[b, w])[v]`` per request, in 64 bits; see ``ops.beam.beam_select``."""
+    B, W = scores.shape
+    V = logits.shape[1]
+    x = logits.double()
+    gone = x == -math.inf
+    z = x * inv_scale
+    if softcap > 0:
+        z = softcap * torch.tanh(z / softcap)
+    z = z.masked_fill(gone if allowed is None else gone | ~allowed, -math.inf)
+    top = torch.where(z.isnan(), -math.inf, z).amax(dim=-1, keepdim=True).clamp_min(torch.finfo(torch.float32).min)
+    logp = z - top - (z - top).exp().sum(dim=-1, keepdim=True).log()
+    value = (scores.double().reshape(B * W, 1) + logp).reshape(B, W * V)
+    value, at = torch.sort(torch.where(value.isfinite(), value, -math.inf), dim=-1, descending=True, stable=True)
+    value, at = value[:, :k], at[:, :k]
+    none = value == -math.inf
+    return value.float(), torch.where(none, -1, at // V), torch.where(none, -1, at % V)
+
+
+def beam_move(t: torch.Tensor, slots: torch.Tensor, parents: torch.Tensor, rows: Optional[torch.Tensor]) -> None:
+    """``t[slots[b, j]] = t[slots[b, parents[b, j]]]`` at once; with ``rows`` the first ``rows[b]`` rows of the third dimension only."""
+    if slots.numel() and (int(slots.min()) < 0 or int(slots.max()) >= t.shape[0]):
+        raise IndexError("beam slot outside the tensor")
+    W = parents.shape[1]
+    for b in range(parents.shape[0]):
+        moves = [(int(slots[b, j]), int(slots[b, p])) for j, p in enumerate(parents[b].tolist()) if 0 <= p < W and p != j]
+        n = slice(None) if rows is None else slice(0, max(0, int(rows[b])))
+        old = [t[s].clone() if rows is None else t[s, :, n].clone() for _, s in moves]
+        for (d, _), o in zip(moves, old):
+            if rows is None:
+                t[d] = o
+            else:
+                t[d, :, n] = o
