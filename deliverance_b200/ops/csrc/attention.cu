@@ -8,6 +8,7 @@
 // and (window == 0 or j > p - window)  (reference: core/.../generator/CausalSelfAttention.java:458-532,
 // tensor/.../operations/TensorOperations.java:225-271, tensor/.../VectorTensorMathUtils.java:34-78).
 #include "common.cuh"
+#include "beam_api.h"
 #include "gemm_api.h"
 #include "io.cuh"
 
@@ -258,6 +259,7 @@ struct DecodeSlices {
   }
   __device__ int count() const { return hi - skip; }
 };
+__device__ __forceinline__ int window_first(int ctx, int window) { return window > 0 && ctx > window ? ctx - window : 0; }
 // Of `splits` CTAs per (sequence, KV head) as many work as have min_slices slices each: a short context is not worth a merge.
 __device__ __forceinline__ int decode_used_splits(int slices, int splits, int min_slices) { return max(1, min(splits, slices / min_slices)); }
 
@@ -540,13 +542,23 @@ template <bool ROPE>
 struct DecodeRope {};
 template <>
 struct DecodeRope<true> : DecodeRopeArgs {};
-template <int D, int EXT, int NW, bool PLAN, bool ROPE>
+// SCORES: every score goes to fp32 [B, H, pitch] as well (keys at or behind the pitch do not; -inf outside the window), and every CTA writes its maxima and sums, for what adds the
+// probabilities to the keys' weights (evict.cu). This form looks at what it is given: lengths end with the block table, pages outside the cache are read as page 0 and reported.
+template <bool SCORES>
+struct DecodeScores {};
+template <>
+struct DecodeScores<true> {
+  float* out;
+  int pitch, max_ctx, pages;
+  int* status;
+};
+template <int D, int EXT, int NW, bool PLAN, bool ROPE, bool SCORES>
 __global__ void __launch_bounds__(NW * 32, (D <= 128 && NW == 4 ? 2 : 1)) decode_attn_mma_kernel(
     const __nv_bfloat16* __restrict__ q, long long q_stride, const __nv_bfloat16* __restrict__ k_cache,
     const __nv_bfloat16* __restrict__ v_cache, const int* __restrict__ block_tables, int bt_stride,
     const int* __restrict__ ctx_lens, __nv_bfloat16* __restrict__ out, float* part_o, float* part_ml, int* __restrict__ arrivals,
     int H, int KV, int page_size, float scale, float softcap, int window, int splits, int min_slices, const DecodeOptions<EXT> opt,
-    const DecodePlan<PLAN> plan, const DecodeRope<ROPE> rope) {
+    const DecodePlan<PLAN> plan, const DecodeRope<ROPE> rope, const DecodeScores<SCORES> scores) {
   pdl_trigger();  // first: the next kernel may then be set up (and a GEMM prefetch its weights) while this one still waits
   pdl_wait();
   using L = DecodeMma<D, NW>;
@@ -565,7 +577,11 @@ __global__ void __launch_bounds__(NW * 32, (D <= 128 && NW == 4 ? 2 : 1)) decode
   const int g = lane >> 2, t4 = lane & 3;
   const int h0 = kvh * heads_per_kv + (EXT == 1 ? (blockIdx.y % groups) * 16 : 0);  // first query head of this CTA
   const int G = EXT == 1 ? min(16, (kvh + 1) * heads_per_kv - h0) : heads_per_kv;
-  const int ctx = ctx_lens[b];
+  int ctx = ctx_lens[b];
+  if constexpr (SCORES) {
+    if ((ctx < 0 || ctx > scores.max_ctx) && tid == 0) atomicCAS(scores.status, kStatusOk, kStatusBadArgs);
+    ctx = max(0, min(ctx, scores.max_ctx));
+  }
   const DecodeSlices list(ctx, window, EXT == 1 ? keep_first : 0);
   const int first_key = list.first_key, kept = list.kept, sl_kept = list.n_kept, sl_skip = list.skip;
   int used;
@@ -609,7 +625,14 @@ __global__ void __launch_bounds__(NW * 32, (D <= 128 && NW == 4 ? 2 : 1)) decode
     // 16 keys x D of K and V: 2 * 16 * CPR chunks over 32 lanes (zeros behind the real widths)
     if ((j & 31) == 0 && j + lane < n_mine) {
       const int sl = slice_at(first + NW * (j + lane));
-      my_row = (block_tables[static_cast<long long>(b) * bt_stride + sl / per_page] * KV + kvh) * page_size + sl % per_page * 16;
+      int at = block_tables[static_cast<long long>(b) * bt_stride + sl / per_page];
+      if constexpr (SCORES) {
+        if (at < 0 || at >= scores.pages) {
+          atomicCAS(scores.status, kStatusOk, kStatusBadArgs);
+          at = 0;
+        }
+      }
+      my_row = (at * KV + kvh) * page_size + sl % per_page * 16;
     }
     const int key0 = slice_at(first + NW * j) * 16;
     const long long row0 = __shfl_sync(0xffffffffu, my_row, j & 31);
@@ -813,6 +836,16 @@ __global__ void __launch_bounds__(NW * 32, (D <= 128 && NW == 4 ? 2 : 1)) decode
         mx[e >> 1] = fmaxf(mx[e >> 1], v);
       }
     }
+    if constexpr (SCORES) {
+      if (key0 < scores.pitch) {  // (the pitch is a multiple of 16)
+        float* at = scores.out + (static_cast<long long>(b) * H + h0 + g) * scores.pitch + key0 + 2 * t4;
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          if (g < G) *reinterpret_cast<float2*>(at + nt * 8) = make_float2(sc[nt][0], sc[nt][1]);
+          if (g + 8 < G) *reinterpret_cast<float2*>(at + 8ll * scores.pitch + nt * 8) = make_float2(sc[nt][2], sc[nt][3]);
+        }
+      }
+    }
     float alpha[2], m_new[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -922,6 +955,9 @@ __global__ void __launch_bounds__(NW * 32, (D <= 128 && NW == 4 ? 2 : 1)) decode
     }
     if (used == 1) {
       finish(r, d, m, n0, n1, den);
+      if constexpr (SCORES) {
+        if (d == 0) *reinterpret_cast<float2*>(part_ml + (static_cast<long long>(b) * H + h0 + r) * splits * 2) = make_float2(m, den);
+      }
     } else {
       const long long base = (static_cast<long long>(b) * H + h0 + r) * splits + sp;
       *reinterpret_cast<float2*>(part_o + base * dv + d) = make_float2(n0, n1);
@@ -987,35 +1023,38 @@ __global__ void __launch_bounds__(NW * 32, (D <= 128 && NW == 4 ? 2 : 1)) decode
   }
 }
 
-template <int D, int EXT, bool PLAN = false, bool ROPE = false>
+int decode_min_slices(int B, int KV, int G) { return static_cast<long long>(B) * KV * ((G + 15) / 16) >= 64 ? 16 : 3; }
+
+template <int D, int EXT, bool PLAN = false, bool ROPE = false, bool SCORES = false>
 static int launch_decode_mma_t(const void* q, long long q_stride, const void* kc, const void* vc, const int* bt, int bt_stride,
                                const int* ctx, void* out, float* po, float* pml, int* arrivals, int B, int H, int KV, int page,
-                               float scale, float cap, int window, int splits, const int* used, cudaStream_t st, int dk = D, int dv = D, AttnExtra x = {}, const DecodeRope<ROPE>& rope = {}) {
+                               float scale, float cap, int window, int splits, const int* used, cudaStream_t st, int dk = D, int dv = D, AttnExtra x = {}, const DecodeRope<ROPE>& rope = {},
+                               const DecodeScores<SCORES>& scores = {}) {
   constexpr int NW = D > 128 ? 6 : 4;
   using L = DecodeMma<D, NW>;
   using Extra = std::conditional_t<EXT != 0, AttnExtra, NoExtra>;
   if constexpr (!PLAN) {
     if (used != nullptr && splits > 1)
-      return launch_decode_mma_t<D, EXT, true, ROPE>(q, q_stride, kc, vc, bt, bt_stride, ctx, out, po, pml, nullptr, B, H, KV, page, scale, cap, window, splits, used, st, dk, dv, x, rope);
+      return launch_decode_mma_t<D, EXT, true, ROPE, SCORES>(q, q_stride, kc, vc, bt, bt_stride, ctx, out, po, pml, nullptr, B, H, KV, page, scale, cap, window, splits, used, st, dk, dv, x, rope, scores);
   }
   // the in-kernel merge keeps its weights in the warp-merge area of shared memory
   if (splits > 1 && (H / KV) * (splits + 1) > L::kMerge / 4) arrivals = nullptr;
   // `splits` is an upper bound. No CTA takes less than 16 slices (128 pairs x 576 keys: 13.5 us against 21.0), or 3 where a few sequences have the GPU to
   // themselves (8 pairs x 777 keys: 16 splits 5.4, 32 splits 6.6).
-  const int min_slices = static_cast<long long>(B) * KV * ((H / KV + 15) / 16) >= 64 ? 16 : 3;
+  const int min_slices = decode_min_slices(B, KV, H / KV);
   static PerDeviceOnce attr_once;
   if (attr_once.first()) {
-    cudaFuncSetAttribute(decode_attn_mma_kernel<D, EXT, NW, PLAN, ROPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+    cudaFuncSetAttribute(decode_attn_mma_kernel<D, EXT, NW, PLAN, ROPE, SCORES>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
   }
   dim3 grid(B, KV * ((H / KV + 15) / 16), splits);
   DecodeOptions<EXT> opt;
   if constexpr (EXT != 0) opt = {dk, dv, x};
   DecodePlan<PLAN> plan;
   if constexpr (PLAN) plan.used = used;
-  launch_pdl(decode_attn_mma_kernel<D, EXT, NW, PLAN, ROPE>, dim3(grid), dim3(NW * 32), L::kBytes, st, static_cast<const __nv_bfloat16*>(q), q_stride,
+  launch_pdl(decode_attn_mma_kernel<D, EXT, NW, PLAN, ROPE, SCORES>, dim3(grid), dim3(NW * 32), L::kBytes, st, static_cast<const __nv_bfloat16*>(q), q_stride,
                                                           static_cast<const __nv_bfloat16*>(kc), static_cast<const __nv_bfloat16*>(vc), bt,
                                                           bt_stride, ctx, static_cast<__nv_bfloat16*>(out), po, pml, arrivals, H, KV, page, scale,
-                                                          cap, window, splits, min_slices, opt, plan, rope);
+                                                          cap, window, splits, min_slices, opt, plan, rope, scores);
   if (splits > 1 && arrivals == nullptr) {
     dim3 g2(B, H);
     const dim3 block((dv + 31) / 32 * 32);
@@ -1065,6 +1104,76 @@ int launch_decode_attention_rope(const void* qkv, long long pitch, const DecodeR
   if (D != 64) return 1;
   return launch_decode_mma_t<64, 0, false, true>(qkv, pitch, a->k_cache, a->v_cache, bt, bt_stride, ctx, out, po, pml, nullptr, B, H, KV, page, scale, cap, window, splits,
                                                  used, st, 64, 64, {}, rope);
+}
+
+int launch_decode_attention_scores(const void* q, long long q_stride, const void* kc, const void* vc, const int* bt, int bt_stride, const int* ctx, void* out, float* po,
+                                   float* pml, float* scores, int pitch, int pages, int max_ctx, int* status, int B, int H, int KV, int D, int page, float scale, float cap,
+                                   int window, int splits, const int* used, cudaStream_t st) {
+  if (B == 0) return 0;
+  if (H / KV > 16 || page % 16 != 0 || q_stride % 2 != 0) return 1;
+  const DecodeScores<true> s{scores, pitch, max_ctx, pages, status};
+#define DLV_DEC_SCORES(DD)                                                                                                                                              \
+  return launch_decode_mma_t<DD, 0, false, false, true>(q, q_stride, kc, vc, bt, bt_stride, ctx, out, po, pml, nullptr, B, H, KV, page, scale, cap, window, splits, used, st, \
+                                                        DD, DD, {}, {}, s)
+  switch (D) {
+    case 64: DLV_DEC_SCORES(64);
+    case 128: DLV_DEC_SCORES(128);
+    case 256: DLV_DEC_SCORES(256);
+    default: return 1;
+  }
+#undef DLV_DEC_SCORES
+}
+
+// Probabilities of a decode step, added to the keys' weights: exp(score - maximum) / sum per head, summed over the query heads of a KV head in order.
+// grid (B * KV, keys / 1024). The second sequence on a slot adds nothing and is reported, so that no two CTAs write one weight.
+__global__ void __launch_bounds__(256) weigh_kernel(const WeighArgs a) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ float top[16], inv[16];
+  const int b = blockIdx.x / a.KV, kvh = blockIdx.x % a.KV, t = threadIdx.x, lane = t & 31, warp = t >> 5, G = a.H / a.KV;
+  const int ctx = max(0, min(a.ctx[b], a.max_ctx)), keys = min(ctx, a.capacity);
+  if (static_cast<int>(blockIdx.y) * 1024 >= keys) return;
+  const long long slot = a.slots[b];
+  if (slot == 0) return;
+  bool bad = slot < 0 || slot >= a.num_slots;
+  for (int i = t; i < b; i += 256) bad = bad || a.slots[i] == slot;
+  if (__syncthreads_or(bad)) {
+    if (t == 0) atomicCAS(a.status, kStatusOk, kStatusBadArgs);
+    return;
+  }
+  int used = a.splits;
+  if (a.used != nullptr) used = a.used[b * kDecodePlanStride];
+  else used = decode_used_splits(DecodeSlices(ctx, a.window, 0).count(), used, a.min_slices);
+  for (int g = warp; g < G; g += 8) {
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (static_cast<long long>(b) * a.H + kvh * G + g) * a.splits;
+    float m = -INFINITY, l = 0.f;
+    for (int s = lane; s < used; s += 32) m = fmaxf(m, ml[s].x);
+    m = warp_max(m);
+    for (int s = lane; s < used; s += 32) l += ml[s].x == -INFINITY ? 0.f : expf(ml[s].x - m) * ml[s].y;
+    l = warp_sum(l);
+    if (lane == 0) {
+      top[g] = m;
+      inv[g] = l > 0.f ? 1.f / l : 0.f;
+    }
+  }
+  __syncthreads();
+  const float* s0 = a.scores + (static_cast<long long>(b) * a.H + kvh * G) * a.S;
+  float* w = a.weights + (slot * a.KV + kvh) * a.capacity;
+  for (int key = blockIdx.y * 1024 + t; key < min(keys, static_cast<int>(blockIdx.y) * 1024 + 1024); key += 256) {
+    float p = 0.f;
+    if (window_first(ctx, a.window) <= key) {
+      for (int g = 0; g < G; ++g) {
+        const float s = s0[static_cast<long long>(g) * a.S + key];
+        p += s == -INFINITY ? 0.f : expf(s - top[g]) * inv[g];
+      }
+      w[key] += p;
+    }
+  }
+}
+
+void launch_weigh(const WeighArgs& a, cudaStream_t st) {
+  const int keys = a.max_ctx < a.capacity ? a.max_ctx : a.capacity;
+  if (a.B > 0 && keys > 0) launch_pdl(weigh_kernel, dim3(a.B * a.KV, (keys + 1023) / 1024), dim3(256), 0, st, a);
 }
 
 int launch_decode_attention_mma(const void* q, long long q_stride, const void* kc, const void* vc, const int* bt, int bt_stride, const int* ctx, void* out,

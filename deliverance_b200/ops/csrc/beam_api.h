@@ -48,4 +48,40 @@ struct BeamMoveArgs {
 // unit: bytes that one access moves (16, 4 or 2): all sizes and addresses are multiples of it
 void launch_beam_move(const BeamMoveArgs& a, int B, int unit, cudaStream_t st);
 
+// ---- bounded cache ----------------------------------------------------------------------------------------------------
+constexpr int kEvictLayers = 96;  // layers of one launch (the table travels as a kernel parameter)
+
+struct EvictLayer {
+  void *k, *v;     // [pages, KV, page, D]
+  float* weights;  // [slots, KV, capacity]
+  int k_bytes, v_bytes;  // bytes of a row
+};
+struct EvictArgs {
+  EvictLayer layer[kEvictLayers];
+  const int* tables;      // [B, table_width]
+  const int* out_tables;  // [B, out_width]
+  const int* ctx;         // [B]
+  const long long* slots; // [B]
+  int* kept;              // [layers, B, KV, keep]
+  int* lens;              // [B]
+  int* status;
+  int layers, B, KV, page, pages, num_slots, capacity, table_width, out_width, keep, recent;
+};
+// unit: bytes of one access (16, 4 or 2). Two launches.
+void launch_evict(const EvictArgs& a, int unit, cudaStream_t st);
+
+// Adds the probabilities of a decode step to the weights: scores fp32 [B, H, S] (scaled and capped, -inf where masked), part_ml [B, H, splits, 2] of the
+// attention kernel, used: its plan or null (then min_slices).
+struct WeighArgs {
+  const float* scores;
+  const float* part_ml;
+  const int* ctx;
+  const int* used;
+  const long long* slots;
+  float* weights;  // [num_slots, KV, capacity]
+  int* status;
+  int B, H, KV, S, splits, window, min_slices, num_slots, capacity, max_ctx;
+};
+void launch_weigh(const WeighArgs& a, cudaStream_t st);
+
 }  // namespace dlv

@@ -1878,6 +1878,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("out") = py::none());
   m.def("beam_select", &beam_select, py::arg("logits"), py::arg("scores"), py::arg("k"), py::arg("mask") = py::none(), py::arg("softcap") = 0.0,
         py::arg("inv_scale") = 1.0, py::arg("splits") = 0);
+  m.def("decode_attention_weighted", &decode_attention_weighted);
+  m.def("evict_keys", &evict_keys);
   m.def("beam_move", &beam_move, py::arg("tensors"), py::arg("slots"), py::arg("parents"), py::arg("rows") = py::none(), py::arg("paged") = false);
   m.def("q4_quantize", &q4_quantize);
   m.def("q4_dequantize", &q4_dequantize, py::arg("packed"), py::arg("scales"), py::arg("to_bf16") = false);

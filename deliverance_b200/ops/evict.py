@@ -1,0 +1,70 @@
+"""A cache of bounded length: the attention weights that every cached key has received are added up, and from time to time the keys that received
+the least are dropped.
+
+Every sequence has a row ``weights[slot]`` per layer, fp32 ``[KV, capacity]``: entry i is the sum, over the decode steps since the key came into row i and
+over the query heads that share the KV head, of the probabilities it had. :func:`decode_attention_weighted` is decode attention that also adds a step's
+probabilities. :func:`evict_keys` keeps, per layer, sequence and KV head, the newest rows and the heaviest of the others, in their order, in the first rows of
+the sequence's pages. KV heads keep different keys, but all of them equally many, so that block tables and lengths stay what they are for the rest of
+the framework. Keys carry their rotary positions with them; what changes is the row that they lie in.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from .. import ops
+from . import ref
+
+
+def decode_attention_weighted(q, k_cache, v_cache, block_tables, ctx_lens, H, scale, weights, slots, softcap=0.0, window=0, splits=1, even=False, plan=None):
+    """:func:`ops.decode_attention`, which also adds every key's probabilities to ``weights[slots[b], kv head, row]`` (fp32 ``[slots, KV, capacity]``, in place;
+    ``slots`` int64 ``[B]``). Rows of a sequence at or behind the capacity are attended to and not counted. Slot 0 is the scratch slot: a sequence with slot 0 adds nothing. The other
+    slots of a call are different ones; a second sequence on a slot, or a slot outside ``weights``, adds nothing and is reported by :func:`ops.check_status` (on the CPU:
+    raised)."""
+    if weights.dim() != 3 or weights.dtype != torch.float32 or weights.shape[1] != k_cache.shape[1]:
+        raise ValueError("weights must be fp32 [slots, KV, capacity]")
+    if slots.dim() != 1 or slots.shape[0] != q.shape[0] or slots.dtype != torch.int64:
+        raise ValueError("slots must be int64, one per query row")
+    if ops._cuda(q):
+        B, KV = q.shape[0], k_cache.shape[1]
+        splits, used = ops.decode_launch(splits, even, plan, ctx_lens, B, H, KV, k_cache.shape[3], int(window))
+        out, launches = ops.require_ext().decode_attention_weighted(q, k_cache, v_cache, block_tables, ctx_lens, H, scale, softcap, int(window), splits, weights, slots, used)
+        ops._count(launches)
+        return out
+    return ref.decode_attention_weighted(q, k_cache, v_cache, block_tables, ctx_lens, H, scale, weights, slots, softcap, window)
+
+
+def evict_keys(k_caches, v_caches, weights, block_tables, ctx_lens, slots, keep: int, recent: int, out_tables: Optional[torch.Tensor] = None):
+    """Shorten sequences of more than ``keep`` rows to ``keep``: the last ``recent`` rows and, of the others, those with the largest weights (equal weights, and NaN
+    as the smallest: the earliest; rows at or behind the capacity count as weight 0). What is kept moves, in order, to the first rows of ``out_tables[b]`` (default: of ``block_tables[b]``) in all layers, its weights to the first entries of
+    ``weights[layer][slots[b]]``; the weights behind them, up to the old length, become zero. Sequences that are short enough keep everything, and with ``out_tables`` move too.
+
+    ``k_caches`` / ``v_caches``: per layer ``[pages, KV, page, D]`` (widths may differ); ``weights``: per layer fp32 ``[slots, KV, capacity]``; ``block_tables`` / ``out_tables`` int32 ``[B, pages]``,
+    ``ctx_lens`` int32 ``[B]``, ``slots`` int64 ``[B]``, all different (0, the scratch slot: only for sequences of length 0). An entry of ``out_tables`` is either the page that ``block_tables`` has in the same place or a page that no sequence of the call reads.
+    Returns the rows that were kept, int32 ``[layers, B, KV, keep]`` (-1 behind a sequence's end), and the new lengths, int32 ``[B]``."""
+    k_caches, v_caches, weights = list(k_caches), list(v_caches), list(weights)
+    if not k_caches or not len(k_caches) == len(v_caches) == len(weights):
+        raise ValueError("one key cache, value cache and weight tensor per layer")
+    if not 0 <= recent <= keep or keep < 1:
+        raise ValueError("0 <= recent <= keep, 1 <= keep")
+    first = k_caches[0]
+    for k, v, w in zip(k_caches, v_caches, weights):
+        if k.dim() != 4 or v.dim() != 4 or w.dim() != 3 or k.shape[:3] != first.shape[:3] or v.shape[:3] != first.shape[:3] or k.dtype != v.dtype or k.dtype != first.dtype:
+            raise ValueError("caches must be [pages, KV, page, D] of one type, with the same pages and KV heads in all layers")
+        if w.dtype != torch.float32 or w.shape != weights[0].shape or w.shape[1] != k.shape[1]:
+            raise ValueError("weights must be fp32 [slots, KV, capacity], the same in all layers")
+    if len({t.data_ptr() for t in k_caches + v_caches if t.numel()}) < sum(1 for t in k_caches + v_caches if t.numel()):
+        raise ValueError("a cache that several layers share cannot be shortened for one of them")
+    B = ctx_lens.shape[0]
+    if block_tables.dim() != 2 or block_tables.shape[0] != B or slots.shape != (B,) or slots.dtype != torch.int64 or block_tables.dtype != torch.int32 or ctx_lens.dtype != torch.int32:
+        raise ValueError("block_tables int32 [B, pages], ctx_lens int32 [B], slots int64 [B]")
+    out = block_tables if out_tables is None else out_tables
+    if out.dim() != 2 or out.shape[0] != B or out.dtype != torch.int32:
+        raise ValueError("out_tables must be int32 [B, pages]")
+    if ops._cuda(first):
+        e = ops.require_ext()
+        kept, lens, launches = e.evict_keys(k_caches, v_caches, weights, block_tables, ctx_lens, slots, keep, recent, out)
+        ops._count(launches)
+        return kept, lens
+    return ref.evict_keys(k_caches, v_caches, weights, block_tables, ctx_lens, slots, keep, recent, out)

@@ -429,3 +429,69 @@ def beam_move(t: torch.Tensor, slots: torch.Tensor, parents: torch.Tensor, rows:
                 t[d] = o
             else:
                 t[d, :, n] = o
+
+
+# ---------------------------------------------------------------------------------------------------------------- bounded cache
+def decode_attention_weighted(q, k_cache, v_cache, block_tables, ctx_lens, H, scale, weights, slots, softcap: float = 0.0, window: int = 0) -> torch.Tensor:
+    """Decode attention that adds every key's probabilities, summed over the query heads of a KV head, to ``weights[slots[b]]``; see ``ops.evict``."""
+    B, KV, D = q.shape[0], k_cache.shape[1], k_cache.shape[3]
+    used = [int(s) for s in slots.tolist() if s != 0]
+    if len(set(used)) < len(used) or any(not 0 < s < weights.shape[0] for s in used):
+        raise IndexError("weight slots must be different ones inside the weights")
+    out = torch.zeros(B, KV, H // KV, v_cache.shape[3], dtype=q.dtype)
+    for b in range(B):
+        n, slot = int(ctx_lens[b]), int(slots[b])
+        if n == 0:
+            continue
+        pages = block_tables[b, : -(-n // k_cache.shape[2])].long()
+        k, v = (t[pages].permute(1, 0, 2, 3).reshape(KV, -1, t.shape[3])[:, :n].float() for t in (k_cache, v_cache))
+        s = torch.matmul(q[b].float().reshape(KV, H // KV, D), k.transpose(1, 2)) * scale
+        if softcap and softcap > 0:
+            s = torch.tanh(s / softcap) * softcap
+        if window and 0 < window < n:
+            s[:, :, : n - window] = -math.inf
+        p = torch.softmax(s, dim=-1)
+        out[b] = torch.matmul(p, v).to(q.dtype)
+        if slot != 0:
+            m = min(n, weights.shape[2])
+            weights[slot, :, :m] += p.sum(dim=1)[:, :m]
+    return out.reshape(B, -1)
+
+
+def evict_keys(k_caches, v_caches, weights, block_tables, ctx_lens, slots, keep: int, recent: int, out_tables):
+    """The newest ``recent`` rows and the heaviest of the others move to the front, per layer, sequence and KV head; see ``ops.evict.evict_keys``."""
+    B, L, (pages, KV, P, _) = ctx_lens.shape[0], len(k_caches), k_caches[0].shape
+    cap = weights[0].shape[2]
+    kept = torch.full((L, B, KV, keep), -1, dtype=torch.int32)
+    lens = ctx_lens.clamp(max=keep)
+    used = [int(s) for s, n in zip(slots.tolist(), ctx_lens.tolist()) if n > 0]
+    if len(set(used)) < len(used) or any(not 0 < s < weights[0].shape[0] for s in used):
+        raise IndexError("weight slots must be different ones inside the weights")
+    for b in range(B):
+        n, slot = int(ctx_lens[b]), int(slots[b])
+        m = min(n, keep)
+        if m == 0:
+            continue
+        src, dst = block_tables[b, : -(-n // P)].long(), out_tables[b, : -(-m // P)].long()
+        if any(int(t.min()) < 0 or int(t.max()) >= pages for t in (src, dst)):
+            raise IndexError("page outside the cache")
+        j = torch.arange(m)
+        for layer in range(L):
+            w = weights[layer][slot]
+            full = torch.zeros(KV, n)
+            full[:, : min(n, cap)] = w[:, : min(n, cap)]
+            if n > keep:
+                old = full[:, : n - recent]
+                order = torch.sort(torch.where(old.isnan(), -math.inf, old), dim=-1, descending=True, stable=True).indices
+                # (NaN comes behind -inf)
+                order = torch.gather(order, 1, torch.sort(torch.gather(old.isnan().int(), 1, order), dim=-1, stable=True).indices)[:, : keep - recent]
+                rows = torch.cat([order.sort(dim=-1).values, torch.arange(n - recent, n).expand(KV, -1)], dim=-1)
+                w[:, : min(n, cap)] = torch.nn.functional.pad(full.gather(1, rows), (0, max(0, n - keep)))[:, : min(n, cap)]
+            else:
+                rows = j.expand(KV, -1)
+            kept[layer, b, :, :m] = rows.to(torch.int32)
+            for t in (k_caches[layer], v_caches[layer]):
+                new = torch.stack([t[src[rows[h] // P], h, rows[h] % P] for h in range(KV)])
+                for h in range(KV):
+                    t[dst[j // P], h, j % P] = new[h]
+    return kept, lens

@@ -1,0 +1,282 @@
+"""Decode attention that adds up its keys' weights, and the eviction that goes by them, against plain statements in 64 bits. On the CPU and, on a GPU
+box, on the CUDA kernels."""
+import math
+
+import pytest
+import torch
+
+from deliverance_b200 import ops
+from deliverance_b200.ops.evict import decode_attention_weighted, evict_keys
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+BF16, F32 = torch.bfloat16, torch.float32
+P = 32
+
+
+def tables_for(lens, first=1, extra=0):
+    need = [-(-n // P) for n in lens]
+    order = (torch.randperm(sum(need)) + first).to(torch.int32)
+    t = torch.zeros(len(lens), max(max(need), 1) + extra, dtype=torch.int32)
+    at = 0
+    for i, n in enumerate(need):
+        t[i, :n] = order[at : at + n]
+        at += n
+    return t, first + sum(need)
+
+
+def dense(cache, table, n):
+    return cache[table[: -(-n // P)].long()].permute(1, 0, 2, 3).reshape(cache.shape[1], -1, cache.shape[3])[:, :n].double()
+
+
+def plain_attention(q, k, v, table, lens, KV, scale, softcap, window):
+    """fp64 outputs [B, H * D] and per sequence the probabilities summed over a KV head's query heads, [KV, n]."""
+    B, D = q.shape[0], k.shape[3]
+    out, sums = torch.zeros(B, q.shape[1], dtype=torch.float64), []
+    for b, n in enumerate(lens):
+        K, V = dense(k, table[b], n), dense(v, table[b], n)
+        s = q[b].double().view(KV, -1, D) @ K.transpose(1, 2) * scale
+        if softcap:
+            s = softcap * torch.tanh(s / softcap)
+        if window and n > window:
+            s[:, :, : n - window] = -math.inf
+        p = torch.softmax(s, -1) if n else s
+        sums.append(p.sum(1))
+        out[b] = (p @ V).flatten()
+    return out, sums
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("KV,G", [(1, 1), (2, 4), (3, 5), (1, 16), (8, 8)])
+@pytest.mark.parametrize("lens,splits", [([1], 1), ([33, 0, 1, 500], 1), ([700, 31, 32], 8), ([3001, 2], 32), ([64] * 70, 3)])
+def test_weighted_attention_matches_plain(device, D, KV, G, lens, splits):
+    if device == "cpu" and sum(lens) * KV * G * D > 3e7:
+        pytest.skip("large for the CPU")
+    run_attention(device, D, KV, G, lens, splits, 0.0, 0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("softcap,window", [(50.0, 0), (0.5, 0), (0.0, 100), (50.0, 17)])
+def test_weighted_attention_softcap_window(device, D, softcap, window):
+    run_attention(device, D, 2, 2, [777, 16, 100, 101], 6, softcap, window)
+
+
+def run_attention(device, D, KV, G, lens, splits, softcap, window, capacity=None, extra=1):
+    B, H = len(lens), KV * G
+    table, pages = tables_for(lens, extra=extra)
+    q = torch.randn(B, H * D).to(BF16)
+    k, v = torch.randn(pages, KV, P, D).to(BF16), torch.randn(pages, KV, P, D).to(BF16)
+    # what lies behind a sequence's end must not matter
+    for b, n in enumerate(lens):
+        if n % P:
+            k[table[b, n // P].long(), :, n % P :] = math.nan
+            v[table[b, n // P].long(), :, n % P :] = math.nan
+    cap = capacity or max(lens) + 7
+    start = torch.rand(B + 2, KV, cap)
+    slots = torch.randperm(B) + 1
+    to = lambda t: t.to(device)  # noqa: E731
+    w = to(start.clone())
+    ctx = torch.tensor(lens, dtype=torch.int32)
+    scale = D**-0.5
+    out = decode_attention_weighted(to(q), to(k), to(v), to(table), to(ctx), H, scale, w, to(slots), softcap, window, splits)
+    if device == "cuda":
+        ops.check_status(0)
+    want, sums = plain_attention(q, k, v, table, lens, KV, scale, softcap, window)
+    out, w = out.cpu().double(), w.cpu().double()
+    # Output: probabilities rounded to bf16 (2^-8 of each, against sum p |v| <= max |v|) and the result's own rounding; fp32 in between is far below.
+    for b, n in enumerate(lens):
+        top = float(dense(v, table[b], n).abs().max()) if n else 0.0
+        assert (out[b] - want[b]).abs().max() <= 2**-8 * (want[b].abs().max() + top) + 1e-6, b
+    # Weights: a score s = scale * q.k carries D + 2 fp32 roundings of at most sum |q k| * scale (here below 5 sqrt(D) for normal values), exp and __expf 2^-22 + 2^-23 |s|, the sum over n
+    # probabilities and heads n * 2^-24 at the worst; relative to the probability. The addition rounds to 2^-24 of the entry.
+    expect = start.double()
+    for b, n in enumerate(lens):
+        m = min(n, cap)
+        expect[slots[b], :, :m] += sums[b][:, :m]
+    for b, n in enumerate(lens):
+        m = min(n, cap)
+        slack = 5 * math.sqrt(D) * (D + 2) * 2**-24 + 64 * 2**-23 + n * 2**-24
+        d = (w[slots[b], :, :m] - expect[slots[b], :, :m]).abs()
+        assert (d <= sums[b][:, :m] * slack + expect[slots[b], :, :m] * 2**-23).all(), (b, float(d.max()))
+        assert torch.equal(w[slots[b], :, m:], start[slots[b], :, m:].double())
+    for s in range(B + 2):
+        if s not in slots.tolist():
+            assert torch.equal(w[s], start[s].double())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_weights_shorter_than_the_sequence(device):
+    run_attention(device, 64, 2, 4, [300, 90, 129], 4, 0.0, 0, capacity=100)
+    run_attention(device, 128, 1, 2, [300, 90, 129], 1, 0.0, 0, capacity=129, extra=40)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_weights_add_up_over_steps(device):
+    """Ten steps on one cache: every step adds one per query head in all; strided query rows."""
+    KV, G, D, n = 2, 3, 64, 210
+    table, pages = tables_for([n, n - 50])
+    k, v = torch.randn(pages, KV, P, D).to(BF16).to(device), torch.randn(pages, KV, P, D).to(BF16).to(device)
+    w = torch.zeros(3, KV, 256, device=device)
+    for i in range(10):
+        q = torch.randn(2, KV * G * D + 64).to(BF16).to(device)[:, 2 : 2 + KV * G * D]
+        decode_attention_weighted(q, k, v, table.to(device), torch.tensor([n, n - 50], dtype=torch.int32, device=device), KV * G, 0.125, w,
+                                  torch.tensor([2, 1], device=device), splits=1 + i % 4)
+    total = w.double().sum(-1).cpu()
+    assert (total[1:] - 10 * G).abs().max() < 10 * G * 1e-5 and float(total[0].abs().max()) == 0
+    assert float(w[2, :, n:].abs().max()) == 0 and float(w[1, :, n - 50 :].abs().max()) == 0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_scratch_slot_adds_nothing(device):
+    """Padded rows of a captured step share slot 0."""
+    KV, D = 1, 64
+    k, v = torch.randn(3, KV, P, D).to(BF16).to(device), torch.randn(3, KV, P, D).to(BF16).to(device)
+    w = torch.zeros(2, KV, 64, device=device)
+    decode_attention_weighted(torch.randn(3, D).to(BF16).to(device), k, v, torch.tensor([[1], [0], [0]], dtype=torch.int32, device=device),
+                              torch.tensor([20, 1, 1], dtype=torch.int32, device=device), 1, 0.125, w, torch.tensor([1, 0, 0], device=device))
+    assert float(w[0].abs().max()) == 0 and abs(float(w[1].sum()) - 1) < 1e-5
+    if device == "cuda":
+        ops.check_status(0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("slots", [[1, 1], [1, 9], [-1, 1]])
+def test_bad_slots_are_reported(device, slots):
+    KV, D = 1, 64
+    k, v = torch.randn(3, KV, P, D).to(BF16).to(device), torch.randn(3, KV, P, D).to(BF16).to(device)
+    w = torch.zeros(3, KV, 64, device=device)
+    args = (torch.randn(2, D).to(BF16).to(device), k, v, torch.tensor([[1], [2]], dtype=torch.int32, device=device), torch.tensor([20, 10], dtype=torch.int32, device=device))
+    with pytest.raises((IndexError, RuntimeError)):
+        decode_attention_weighted(*args, 1, 0.125, w, torch.tensor(slots, device=device))
+        ops.check_status(0)
+    if device == "cuda":  # the good one counted, the bad one did not
+        assert abs(float(w.sum()) - 1) < 1e-5
+    kept_w = w.clone()
+    with pytest.raises((IndexError, RuntimeError)):
+        evict_keys([k], [v], [w], args[3], args[4], torch.tensor(slots, device=device), 5, 2)
+        ops.check_status(0)
+    bad = [s for s in range(3) if s not in slots]
+    assert torch.equal(w[bad], kept_w[bad])
+
+
+# ---------------------------------------------------------------------------------------------------------------- eviction
+def plain_evict(w, n, keep, recent):
+    """Rows kept of one head: fp64 weights [n]."""
+    if n <= keep:
+        return list(range(n))
+    old = sorted(range(n - recent), key=lambda i: (math.isnan(w[i]), -w[i] if not math.isnan(w[i]) else 0.0, i))[: keep - recent]
+    return sorted(old) + list(range(n - recent, n))
+
+
+def run_evict(device, lens, keep, recent, L=2, KV=2, D=64, DV=None, dtype=BF16, capacity=None, out="same", weights=None, shared=()):
+    B = len(lens)
+    table, pages = tables_for(lens, extra=1)
+    target = table.clone()
+    if out != "same":
+        fresh, pages = tables_for([min(n, keep) for n in lens], pages)
+        if out == "fresh":
+            target = fresh
+        else:  # the first pages are held by others, the rest are the sequence's own
+            for b in range(B):
+                for j in range(min(shared[b], fresh.shape[1])):
+                    if j < -(-min(lens[b], keep) // P):
+                        target[b, j] = fresh[b, j]
+    k = [torch.randn(pages, KV, P, D).to(dtype) for _ in range(L)]
+    v = [torch.randn(pages, KV, P, DV or D).to(dtype) for _ in range(L)]
+    cap = capacity or max(lens) + 5
+    w = weights if weights is not None else [torch.where(torch.rand(B + 2, KV, cap) < 0.3, 0.0, torch.randn(B + 2, KV, cap).exp()) for _ in range(L)]
+    slots = torch.randperm(B) + 1
+    to = lambda t: t.clone().to(device)  # noqa: E731
+    K, V, Wt = [to(t) for t in k], [to(t) for t in v], [to(t) for t in w]
+    kept, new = evict_keys(K, V, Wt, to(table), torch.tensor(lens, dtype=torch.int32).to(device), to(slots), keep, recent, None if out == "same" else to(target))
+    if device == "cuda":
+        ops.check_status(0)
+    assert kept.dtype == torch.int32 and new.tolist() == [min(n, keep) for n in lens]
+    kept = kept.cpu()
+    for i in range(L):
+        want_k, want_v, want_w = k[i].clone(), v[i].clone(), w[i].clone()
+        for b, n in enumerate(lens):
+            s, m = int(slots[b]), min(n, keep)
+            for h in range(KV):
+                full = w[i][s, h, : min(n, cap)].tolist() + [0.0] * (n - min(n, cap))
+                rows = plain_evict(full, n, keep, recent)
+                assert kept[i, b, h].tolist() == rows + [-1] * (keep - m), (i, b, h)
+                for t, o in ((k[i], want_k), (v[i], want_v)):
+                    for j, r in enumerate(rows):
+                        o[target[b, j // P].long(), h, j % P] = t[table[b, r // P].long(), h, r % P]
+                if n > keep:
+                    c = min(n, cap)
+                    want_w[s, h, :c] = torch.tensor(([full[r] for r in rows] + [0.0] * n)[:c])
+        assert torch.equal(K[i].cpu(), want_k) and torch.equal(V[i].cpu(), want_v)
+        assert torch.equal(torch.nan_to_num(Wt[i].cpu(), -5.0), torch.nan_to_num(want_w, -5.0))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("lens,keep,recent", [([1], 1, 0), ([2], 1, 0), ([2], 1, 1), ([0, 5, 70], 33, 8), ([100, 64, 65, 63], 64, 64), ([100, 97], 96, 0), ([513, 512, 3], 200, 31), ([1500], 1030, 100)])
+@pytest.mark.parametrize("out", ["same", "fresh", "mixed"])
+def test_evict_matches_plain(device, lens, keep, recent, out):
+    run_evict(device, lens, keep, recent, out=out, shared=[i % 3 for i in range(1, 1 + len(lens))])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D,DV,dtype", [(128, 128, BF16), (256, 64, BF16), (6, 6, BF16), (5, 3, BF16), (20, 20, F32), (5, 7, F32), (1032, 1032, F32)])
+def test_evict_widths(device, D, DV, dtype):
+    run_evict(device, [90, 200], 64, 10, L=1, D=D, DV=DV, dtype=dtype)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_evict_ties_infinities_nan(device):
+    """All weights equal, all zero, infinities of both signs, NaN, negative zero."""
+    L, KV, n = 1, 2, 700
+    for fill in (0.0, 1.5, math.nan):
+        run_evict(device, [n], 300, 20, L=L, KV=KV, weights=[torch.full((3, KV, n), fill)])
+    w = torch.randn(3, KV, n)
+    w[:, :, ::3] = math.nan
+    w[:, :, 1::7] = math.inf
+    w[:, :, 2::5] = -math.inf
+    w[:, :, 4::9] = 0.0
+    w[:, :, 5::9] = -0.0
+    for keep in (50, 350, 600, 699):
+        run_evict(device, [n], keep, 20, L=L, KV=KV, weights=[w])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_evict_beyond_the_capacity(device):
+    run_evict(device, [400, 90, 150], 120, 30, capacity=100)
+    run_evict(device, [400, 90, 150], 64, 30, capacity=150)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_evict_many_layers(device):
+    run_evict(device, [70], 40, 10, L=100, KV=1, D=8)
+
+
+@pytest.mark.gpu
+def test_evict_long_sequences():
+    """More rows than the selection holds in registers; offsets of rows far into a page table."""
+    run_evict("cuda", [9000, 4097], 4000, 500, L=1, KV=1, D=8)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals(device):
+    KV, D = 2, 64
+    k, w = torch.zeros(4, KV, P, D, dtype=BF16, device=device), torch.zeros(3, KV, 64, device=device)
+    v = k.clone()
+    t, n, s = torch.ones(1, 2, dtype=torch.int32, device=device), torch.tensor([40], dtype=torch.int32, device=device), torch.ones(1, dtype=torch.int64, device=device)
+    q = torch.zeros(1, 4 * D, dtype=BF16, device=device)
+    for bad in (lambda: evict_keys([], [], [], t, n, s, 8, 2), lambda: evict_keys([k], [v], [w], t, n, s, 8, 9), lambda: evict_keys([k], [v], [w], t, n, s, 0, 0),
+                lambda: evict_keys([k], [k], [w], t, n, s, 8, 2), lambda: evict_keys([k], [v], [w[:, :1]], t, n, s, 8, 2), lambda: evict_keys([k], [v], [w.double()], t, n, s, 8, 2),
+                lambda: evict_keys([k], [v.float()], [w], t, n, s, 8, 2), lambda: evict_keys([k], [v], [w], t.long(), n, s, 8, 2), lambda: evict_keys([k], [v], [w], t, n, s.int(), 8, 2),
+                lambda: evict_keys([k], [v], [w], t, n, s, 8, 2, t[0]), lambda: decode_attention_weighted(q, k, v, t, n, 4, 0.1, w[0], s),
+                lambda: decode_attention_weighted(q, k, v, t, n, 4, 0.1, w, s.int()), lambda: decode_attention_weighted(q, k, v, t, n, 4, 0.1, w.half(), s)):
+        with pytest.raises((ValueError, RuntimeError)):
+            bad()
+    if device == "cuda":
+        for bad in (lambda: evict_keys([k], [v], [w], t, n, s, 40, 2, t[:, :1]), lambda: decode_attention_weighted(q.float(), k, v, t, n, 4, 0.1, w, s),
+                    lambda: decode_attention_weighted(torch.zeros(1, 34 * D, dtype=BF16, device=device), k, v, t, n, 34, 0.1, w, s), lambda: decode_attention_weighted(q, k, v, t.cpu(), n, 4, 0.1, w, s)):
+            with pytest.raises(RuntimeError):
+                bad()
+    with pytest.raises((IndexError, RuntimeError)):  # a page outside the cache: left out, and reported
+        evict_keys([k], [v], [w], torch.tensor([[1, 7]], dtype=torch.int32, device=device), n, s, 38, 2)
+        ops.check_status(0)
