@@ -24,21 +24,16 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, mask: Option
     allow-bitmask ``mask`` left out), ``scores [B, W]`` fp32, the beams' sums so far; -inf for a beam that is not in use. A candidate's value is finite: a logit of
     -inf is a masked token, a row with a NaN (or +inf, without a softcap) and a beam whose score is not finite give none. Places that no candidate is left for have value
     -inf, parent and token -1."""
+    if logits.is_cuda:  # (the extension checks)
+        ops._count(2)
+        return ops.require_ext().beam_select(logits, scores, k, mask, softcap, inv_scale)
     if scores.dim() != 2 or logits.dim() != 2 or logits.shape[0] != scores.numel():
         raise ValueError("logits must be [requests * beams, V], scores [requests, beams]")
     if not 1 <= scores.shape[1] <= MAX_BEAMS or not 1 <= k <= min(MAX_CANDIDATES, scores.shape[1] * logits.shape[1]):
         raise ValueError(f"1 to {MAX_BEAMS} beams, 1 to {MAX_CANDIDATES} candidates, no more than there are")
     if not inv_scale > 0 or not softcap >= 0:
         raise ValueError("inv_scale must be positive, softcap not negative")
-    if ops._cuda(logits):
-        ops._count(2)
-        return tuple(ops.require_ext().beam_select(logits, scores, k, mask, softcap, inv_scale))
     return ref.beam_select(logits, scores, k, None if mask is None else ops.unpack_mask(mask, logits.shape[1]), softcap, inv_scale)
-
-
-def _distinct(tensors) -> list:
-    """Layers that share a cache name it twice; it moves once."""
-    return list({t.data_ptr(): t for t in tensors if t is not None}.values())
 
 
 def beam_reorder(parents: torch.Tensor, states=(), slots: Optional[torch.Tensor] = None, caches=(), pages: Optional[torch.Tensor] = None,
@@ -48,22 +43,26 @@ def beam_reorder(parents: torch.Tensor, states=(), slots: Optional[torch.Tensor]
     (``[pages, KV, page, D]``; ``rows`` None: whole pages). ``parents``, ``slots`` and ``pages`` are int64 ``[B, W]``, ``rows`` int32 ``[B]``. A parent outside
     ``0 .. W - 1`` leaves its beam as it is. All slots (pages) of a call are different ones; one outside the tensors is left out and reported by
     :func:`ops.check_status` (on the CPU: raised)."""
-    states, caches = _distinct(states), _distinct(caches)
+    if parents.is_cuda:  # (the extension checks: a loop over the layers here takes longer than the kernel)
+        e = ops.require_ext()
+        if len(states):
+            ops._count(e.beam_move(states, slots, parents))
+        if len(caches):
+            ops._count(e.beam_move(caches, pages, parents, rows, True))
+        return
     for group, index, name in ((states, slots, "slots"), (caches, pages, "pages")):
         if group and (index is None or index.shape != parents.shape or index.dim() != 2 or index.shape[1] > MAX_BEAMS or index.dtype != torch.int64 or parents.dtype != torch.int64):
             raise ValueError(f"{name} and parents must be int64 [requests, beams] with at most {MAX_BEAMS} beams")
-    if any(c.dim() != 4 for c in caches):
+    if any(c is not None and c.dim() != 4 for c in caches):
         raise ValueError("page pools are [pages, KV, page, D]")
     if rows is not None and (rows.shape != parents.shape[:1] or rows.dtype != torch.int32):
         raise ValueError("rows must be int32 [requests]")
-    if ops._cuda(parents):
-        e = ops.require_ext()
-        if states:
-            ops._count(e.beam_move(states, slots, parents))
-        if caches:
-            ops._count(e.beam_move(caches, pages, parents, rows, True))
-        return
-    for t in states:
+    for t in _distinct(states):
         ref.beam_move(t, slots, parents, None)
-    for t in caches:
+    for t in _distinct(caches):
         ref.beam_move(t, pages, parents, rows if rows is not None else torch.full((parents.shape[0],), t.shape[2], dtype=torch.int32))
+
+
+def _distinct(tensors) -> list:
+    """Layers that share a cache name it twice; it moves once."""
+    return list({t.data_ptr(): t for t in tensors if t is not None}.values())

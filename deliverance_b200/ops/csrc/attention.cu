@@ -542,23 +542,75 @@ template <bool ROPE>
 struct DecodeRope {};
 template <>
 struct DecodeRope<true> : DecodeRopeArgs {};
-// SCORES: every score goes to fp32 [B, H, pitch] as well (keys at or behind the pitch do not; -inf outside the window), and every CTA writes its maxima and sums, for what adds the
-// probabilities to the keys' weights (evict.cu). This form looks at what it is given: lengths end with the block table, pages outside the cache are read as page 0 and reported.
-template <bool SCORES>
-struct DecodeScores {};
+// WEIGH: every score goes to fp32 [B, H, S] as well, so that what is behind a sequence's last key (this CTA where it is the only split, weigh_kernel where not) can
+// add the probabilities to the keys' weights: 4 bytes per key and query head written and read again, out of L2, for no second product of queries and keys.
+// This form looks at what it is given: lengths end with the block table, pages outside the cache are read as page 0 and reported.
+template <bool WEIGH>
+struct DecodeWeigh {};
 template <>
-struct DecodeScores<true> {
-  float* out;
-  int pitch, max_ctx, pages;
-  int* status;
-};
-template <int D, int EXT, int NW, bool PLAN, bool ROPE, bool SCORES>
+struct DecodeWeigh<true> : WeighArgs {};
+
+// Whether a sequence's weights can be written: its slot lies inside them and no earlier sequence of the call has it. Slot 0 takes nothing. For the whole CTA.
+__device__ __forceinline__ bool weigh_slot(const WeighArgs& a, int b) {
+  const long long slot = a.slots[b];
+  if (slot == 0) return false;
+  bool bad = slot < 0 || slot >= a.num_slots;
+  for (int i = threadIdx.x; i < b; i += blockDim.x) bad = bad || a.slots[i] == slot;
+  if (!__syncthreads_or(bad)) return true;
+  if (threadIdx.x == 0) atomicCAS(a.status, kStatusOk, kStatusBadArgs);
+  return false;
+}
+// weights[key] += sum over the query heads of exp(score - maximum) / sum, heads in order. A thread takes four neighbouring keys at a time, the scores of eight (key group, head)
+// pairs on their way together; thread `first` of `step`. Scores behind the last key of a slice are -inf. (Base-two exponential of a rounded product: 2^-22 + |score - maximum| 2^-23 of a probability.)
+__device__ __forceinline__ void weigh_keys(const WeighArgs& a, int b, int kvh, int ctx, int first, int step, const float* top, const float* inv) {
+  const int G = a.H / a.KV, keys = min(ctx, a.capacity), from = window_first(ctx, a.window) & ~3;
+  const float* s0 = a.scores + (static_cast<long long>(b) * a.H + kvh * G) * a.S;
+  float* w = a.weights + (a.slots[b] * a.KV + kvh) * a.capacity;
+  for (int k0 = from + 4 * first; k0 < keys; k0 += 8 * step) {
+    const int k1 = k0 + 4 * step;
+    float old[8], p[8] = {};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int k = (i < 4 ? k0 : k1 - 4) + i;
+      old[i] = k < keys ? w[k] : 0.f;
+    }
+    for (int g0 = 0; g0 < G; g0 += 4) {
+      float4 s[2][4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float* row = s0 + static_cast<long long>(g0 + g) * a.S;
+        const float4 none = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        s[0][g] = g0 + g < G ? *reinterpret_cast<const float4*>(row + k0) : none;
+        s[1][g] = g0 + g < G && k1 < keys ? *reinterpret_cast<const float4*>(row + k1) : none;
+      }
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float m = top[(g0 + g) & 15], f = g0 + g < G ? inv[(g0 + g) & 15] : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4& v = s[i >> 2][g];
+          const float x = (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
+          float e;
+          asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((x - m) * 1.44269504088896341f));
+          p[i] = fmaf(e, f, p[i]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int k = (i < 4 ? k0 : k1 - 4) + i;
+      if (k < keys) w[k] = old[i] + p[i];
+    }
+  }
+}
+
+template <int D, int EXT, int NW, bool PLAN, bool ROPE, bool WEIGH>
 __global__ void __launch_bounds__(NW * 32, (D <= 128 && NW == 4 ? 2 : 1)) decode_attn_mma_kernel(
     const __nv_bfloat16* __restrict__ q, long long q_stride, const __nv_bfloat16* __restrict__ k_cache,
     const __nv_bfloat16* __restrict__ v_cache, const int* __restrict__ block_tables, int bt_stride,
     const int* __restrict__ ctx_lens, __nv_bfloat16* __restrict__ out, float* part_o, float* part_ml, int* __restrict__ arrivals,
     int H, int KV, int page_size, float scale, float softcap, int window, int splits, int min_slices, const DecodeOptions<EXT> opt,
-    const DecodePlan<PLAN> plan, const DecodeRope<ROPE> rope, const DecodeScores<SCORES> scores) {
+    const DecodePlan<PLAN> plan, const DecodeRope<ROPE> rope, const __grid_constant__ DecodeWeigh<WEIGH> weigh) {
   pdl_trigger();  // first: the next kernel may then be set up (and a GEMM prefetch its weights) while this one still waits
   pdl_wait();
   using L = DecodeMma<D, NW>;
@@ -578,9 +630,9 @@ __global__ void __launch_bounds__(NW * 32, (D <= 128 && NW == 4 ? 2 : 1)) decode
   const int h0 = kvh * heads_per_kv + (EXT == 1 ? (blockIdx.y % groups) * 16 : 0);  // first query head of this CTA
   const int G = EXT == 1 ? min(16, (kvh + 1) * heads_per_kv - h0) : heads_per_kv;
   int ctx = ctx_lens[b];
-  if constexpr (SCORES) {
-    if ((ctx < 0 || ctx > scores.max_ctx) && tid == 0) atomicCAS(scores.status, kStatusOk, kStatusBadArgs);
-    ctx = max(0, min(ctx, scores.max_ctx));
+  if constexpr (WEIGH) {
+    if ((ctx < 0 || ctx > weigh.max_ctx) && tid == 0) atomicCAS(weigh.status, kStatusOk, kStatusBadArgs);
+    ctx = max(0, min(ctx, weigh.max_ctx));
   }
   const DecodeSlices list(ctx, window, EXT == 1 ? keep_first : 0);
   const int first_key = list.first_key, kept = list.kept, sl_kept = list.n_kept, sl_skip = list.skip;
@@ -626,9 +678,9 @@ __global__ void __launch_bounds__(NW * 32, (D <= 128 && NW == 4 ? 2 : 1)) decode
     if ((j & 31) == 0 && j + lane < n_mine) {
       const int sl = slice_at(first + NW * (j + lane));
       int at = block_tables[static_cast<long long>(b) * bt_stride + sl / per_page];
-      if constexpr (SCORES) {
-        if (at < 0 || at >= scores.pages) {
-          atomicCAS(scores.status, kStatusOk, kStatusBadArgs);
+      if constexpr (WEIGH) {
+        if (at < 0 || at >= weigh.pages) {
+          atomicCAS(weigh.status, kStatusOk, kStatusBadArgs);
           at = 0;
         }
       }
@@ -836,13 +888,13 @@ __global__ void __launch_bounds__(NW * 32, (D <= 128 && NW == 4 ? 2 : 1)) decode
         mx[e >> 1] = fmaxf(mx[e >> 1], v);
       }
     }
-    if constexpr (SCORES) {
-      if (key0 < scores.pitch) {  // (the pitch is a multiple of 16)
-        float* at = scores.out + (static_cast<long long>(b) * H + h0 + g) * scores.pitch + key0 + 2 * t4;
+    if constexpr (WEIGH) {
+      if (key0 < weigh.S) {  // (keys at and behind the weights' capacity are not weighed)
+        float* at = weigh.scores + (static_cast<long long>(b) * H + h0 + g) * weigh.S + key0 + 2 * t4;
 #pragma unroll
         for (int nt = 0; nt < 2; ++nt) {
           if (g < G) *reinterpret_cast<float2*>(at + nt * 8) = make_float2(sc[nt][0], sc[nt][1]);
-          if (g + 8 < G) *reinterpret_cast<float2*>(at + 8ll * scores.pitch + nt * 8) = make_float2(sc[nt][2], sc[nt][3]);
+          if (g + 8 < G) *reinterpret_cast<float2*>(at + 8ll * weigh.S + nt * 8) = make_float2(sc[nt][2], sc[nt][3]);
         }
       }
     }
@@ -955,9 +1007,6 @@ __global__ void __launch_bounds__(NW * 32, (D <= 128 && NW == 4 ? 2 : 1)) decode
     }
     if (used == 1) {
       finish(r, d, m, n0, n1, den);
-      if constexpr (SCORES) {
-        if (d == 0) *reinterpret_cast<float2*>(part_ml + (static_cast<long long>(b) * H + h0 + r) * splits * 2) = make_float2(m, den);
-      }
     } else {
       const long long base = (static_cast<long long>(b) * H + h0 + r) * splits + sp;
       *reinterpret_cast<float2*>(part_o + base * dv + d) = make_float2(n0, n1);
@@ -966,6 +1015,28 @@ __global__ void __launch_bounds__(NW * 32, (D <= 128 && NW == 4 ? 2 : 1)) decode
         part_ml[base * 2 + 1] = den;
       }
     }
+  }
+  if constexpr (WEIGH) {
+    if (used == 1 && weigh_slot(weigh, b)) {
+      __shared__ float top[16], inv[16];
+      if (tid < G) {
+        float m = -INFINITY, den = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) m = fmaxf(m, mg[(w * 16 + tid) * (D + 2) + D]);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          const float* row = mg + (w * 16 + tid) * (D + 2);
+          den += row[D] == -INFINITY ? 0.f : expf(row[D] - m) * row[D + 1];
+        }
+        top[tid] = den > 0.f ? m : 0.f;
+        inv[tid] = den > 0.f ? 1.f / den : 0.f;
+      } else if (tid < 16) {
+        top[tid] = inv[tid] = 0.f;
+      }
+      __syncthreads();
+      weigh_keys(weigh, b, kvh, ctx, tid, NW * 32, top, inv);
+    }
+    return;
   }
   if (used == 1 || arrivals == nullptr) return;  // (no arrival counters: decode_merge_kernel follows)
 
@@ -1025,17 +1096,17 @@ __global__ void __launch_bounds__(NW * 32, (D <= 128 && NW == 4 ? 2 : 1)) decode
 
 int decode_min_slices(int B, int KV, int G) { return static_cast<long long>(B) * KV * ((G + 15) / 16) >= 64 ? 16 : 3; }
 
-template <int D, int EXT, bool PLAN = false, bool ROPE = false, bool SCORES = false>
+template <int D, int EXT, bool PLAN = false, bool ROPE = false, bool WEIGH = false>
 static int launch_decode_mma_t(const void* q, long long q_stride, const void* kc, const void* vc, const int* bt, int bt_stride,
                                const int* ctx, void* out, float* po, float* pml, int* arrivals, int B, int H, int KV, int page,
                                float scale, float cap, int window, int splits, const int* used, cudaStream_t st, int dk = D, int dv = D, AttnExtra x = {}, const DecodeRope<ROPE>& rope = {},
-                               const DecodeScores<SCORES>& scores = {}) {
+                               const DecodeWeigh<WEIGH>& weigh = {}) {
   constexpr int NW = D > 128 ? 6 : 4;
   using L = DecodeMma<D, NW>;
   using Extra = std::conditional_t<EXT != 0, AttnExtra, NoExtra>;
   if constexpr (!PLAN) {
     if (used != nullptr && splits > 1)
-      return launch_decode_mma_t<D, EXT, true, ROPE, SCORES>(q, q_stride, kc, vc, bt, bt_stride, ctx, out, po, pml, nullptr, B, H, KV, page, scale, cap, window, splits, used, st, dk, dv, x, rope, scores);
+      return launch_decode_mma_t<D, EXT, true, ROPE, WEIGH>(q, q_stride, kc, vc, bt, bt_stride, ctx, out, po, pml, nullptr, B, H, KV, page, scale, cap, window, splits, used, st, dk, dv, x, rope, weigh);
   }
   // the in-kernel merge keeps its weights in the warp-merge area of shared memory
   if (splits > 1 && (H / KV) * (splits + 1) > L::kMerge / 4) arrivals = nullptr;
@@ -1044,18 +1115,18 @@ static int launch_decode_mma_t(const void* q, long long q_stride, const void* kc
   const int min_slices = decode_min_slices(B, KV, H / KV);
   static PerDeviceOnce attr_once;
   if (attr_once.first()) {
-    cudaFuncSetAttribute(decode_attn_mma_kernel<D, EXT, NW, PLAN, ROPE, SCORES>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+    cudaFuncSetAttribute(decode_attn_mma_kernel<D, EXT, NW, PLAN, ROPE, WEIGH>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
   }
   dim3 grid(B, KV * ((H / KV + 15) / 16), splits);
   DecodeOptions<EXT> opt;
   if constexpr (EXT != 0) opt = {dk, dv, x};
   DecodePlan<PLAN> plan;
   if constexpr (PLAN) plan.used = used;
-  launch_pdl(decode_attn_mma_kernel<D, EXT, NW, PLAN, ROPE, SCORES>, dim3(grid), dim3(NW * 32), L::kBytes, st, static_cast<const __nv_bfloat16*>(q), q_stride,
+  launch_pdl(decode_attn_mma_kernel<D, EXT, NW, PLAN, ROPE, WEIGH>, dim3(grid), dim3(NW * 32), L::kBytes, st, static_cast<const __nv_bfloat16*>(q), q_stride,
                                                           static_cast<const __nv_bfloat16*>(kc), static_cast<const __nv_bfloat16*>(vc), bt,
                                                           bt_stride, ctx, static_cast<__nv_bfloat16*>(out), po, pml, arrivals, H, KV, page, scale,
-                                                          cap, window, splits, min_slices, opt, plan, rope, scores);
-  if (splits > 1 && arrivals == nullptr) {
+                                                          cap, window, splits, min_slices, opt, plan, rope, weigh);
+  if (!WEIGH && splits > 1 && arrivals == nullptr) {
     dim3 g2(B, H);
     const dim3 block((dv + 31) / 32 * 32);
     const int keep = EXT == 1 ? x.keep_first : 0;
@@ -1106,74 +1177,88 @@ int launch_decode_attention_rope(const void* qkv, long long pitch, const DecodeR
                                                  used, st, 64, 64, {}, rope);
 }
 
-int launch_decode_attention_scores(const void* q, long long q_stride, const void* kc, const void* vc, const int* bt, int bt_stride, const int* ctx, void* out, float* po,
-                                   float* pml, float* scores, int pitch, int pages, int max_ctx, int* status, int B, int H, int KV, int D, int page, float scale, float cap,
-                                   int window, int splits, const int* used, cudaStream_t st) {
-  if (B == 0) return 0;
-  if (H / KV > 16 || page % 16 != 0 || q_stride % 2 != 0) return 1;
-  const DecodeScores<true> s{scores, pitch, max_ctx, pages, status};
-#define DLV_DEC_SCORES(DD)                                                                                                                                              \
-  return launch_decode_mma_t<DD, 0, false, false, true>(q, q_stride, kc, vc, bt, bt_stride, ctx, out, po, pml, nullptr, B, H, KV, page, scale, cap, window, splits, used, st, \
-                                                        DD, DD, {}, {}, s)
-  switch (D) {
-    case 64: DLV_DEC_SCORES(64);
-    case 128: DLV_DEC_SCORES(128);
-    case 256: DLV_DEC_SCORES(256);
-    default: return 1;
-  }
-#undef DLV_DEC_SCORES
-}
-
-// Probabilities of a decode step, added to the keys' weights: exp(score - maximum) / sum per head, summed over the query heads of a KV head in order.
-// grid (B * KV, keys / 1024). The second sequence on a slot adds nothing and is reported, so that no two CTAs write one weight.
-__global__ void __launch_bounds__(256) weigh_kernel(const WeighArgs a) {
+// What follows weighed decode attention where sequences are split: the keys' weights (even blocks of a pair) and the outputs from the splits' partials (odd ones).
+// grid (B * KV, 2 * parts): a part takes every parts-th 256 outputs or groups of four keys.
+__global__ void __launch_bounds__(256) weigh_kernel(const __grid_constant__ WeighArgs a) {
   pdl_trigger();
-  pdl_wait();
-  __shared__ float top[16], inv[16];
+  __shared__ float top[16], inv[16], factor[16][kWeighMaxSplits];
   const int b = blockIdx.x / a.KV, kvh = blockIdx.x % a.KV, t = threadIdx.x, lane = t & 31, warp = t >> 5, G = a.H / a.KV;
-  const int ctx = max(0, min(a.ctx[b], a.max_ctx)), keys = min(ctx, a.capacity);
-  if (static_cast<int>(blockIdx.y) * 1024 >= keys) return;
-  const long long slot = a.slots[b];
-  if (slot == 0) return;
-  bool bad = slot < 0 || slot >= a.num_slots;
-  for (int i = t; i < b; i += 256) bad = bad || a.slots[i] == slot;
-  if (__syncthreads_or(bad)) {
-    if (t == 0) atomicCAS(a.status, kStatusOk, kStatusBadArgs);
+  const int first = (blockIdx.y >> 1) * 256 + t, step = (gridDim.y >> 1) * 256;
+  const bool weights = (blockIdx.y & 1) == 0;
+  if (!weights && first - t >= G * a.D) return;
+  if (t < 16) top[t] = inv[t] = 0.f;
+  pdl_wait();
+  const int ctx = max(0, min(a.ctx[b], a.max_ctx));
+  if (weights && 4 * (first - t) >= min(ctx, a.capacity)) return;
+  const int used = a.used != nullptr ? a.used[b * kDecodePlanStride] : decode_used_splits(DecodeSlices(ctx, a.window, 0).count(), a.splits, a.min_slices);
+  if (used == 1) return;  // (the attention kernel has done it all)
+  const long long h0 = static_cast<long long>(b) * a.H + kvh * G;
+  __syncthreads();
+  for (int g = warp; g < G; g += 8) {
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (h0 + g) * a.splits;
+    float2 v[kWeighMaxSplits / 32];
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < kWeighMaxSplits / 32; ++i) {
+      v[i] = lane + 32 * i < used ? ml[lane + 32 * i] : make_float2(-INFINITY, 0.f);
+      m = fmaxf(m, v[i].x);
+    }
+    m = warp_max(m);
+#pragma unroll
+    for (int i = 0; i < kWeighMaxSplits / 32; ++i) {
+      v[i].x = v[i].x == -INFINITY ? 0.f : expf(v[i].x - m);
+      l += v[i].x * v[i].y;
+    }
+    l = warp_sum(l);
+    const float f = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+    for (int i = 0; i < kWeighMaxSplits / 32; ++i)
+      if (lane + 32 * i < used) factor[g][lane + 32 * i] = v[i].x * f;
+    if (lane == 0) {
+      top[g] = l > 0.f ? m : 0.f;
+      inv[g] = f;
+    }
+  }
+  if (weights) {
+    if (weigh_slot(a, b)) weigh_keys(a, b, kvh, ctx, first, step, top, inv);  // (a barrier in weigh_slot where it is true)
     return;
   }
-  int used = a.splits;
-  if (a.used != nullptr) used = a.used[b * kDecodePlanStride];
-  else used = decode_used_splits(DecodeSlices(ctx, a.window, 0).count(), used, a.min_slices);
-  for (int g = warp; g < G; g += 8) {
-    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (static_cast<long long>(b) * a.H + kvh * G + g) * a.splits;
-    float m = -INFINITY, l = 0.f;
-    for (int s = lane; s < used; s += 32) m = fmaxf(m, ml[s].x);
-    m = warp_max(m);
-    for (int s = lane; s < used; s += 32) l += ml[s].x == -INFINITY ? 0.f : expf(ml[s].x - m) * ml[s].y;
-    l = warp_sum(l);
-    if (lane == 0) {
-      top[g] = m;
-      inv[g] = l > 0.f ? 1.f / l : 0.f;
-    }
-  }
   __syncthreads();
-  const float* s0 = a.scores + (static_cast<long long>(b) * a.H + kvh * G) * a.S;
-  float* w = a.weights + (slot * a.KV + kvh) * a.capacity;
-  for (int key = blockIdx.y * 1024 + t; key < min(keys, static_cast<int>(blockIdx.y) * 1024 + 1024); key += 256) {
-    float p = 0.f;
-    if (window_first(ctx, a.window) <= key) {
-      for (int g = 0; g < G; ++g) {
-        const float s = s0[static_cast<long long>(g) * a.S + key];
-        p += s == -INFINITY ? 0.f : expf(s - top[g]) * inv[g];
-      }
-      w[key] += p;
-    }
+  for (int i = first; i < G * a.D; i += step) {
+    const int g = i / a.D, d = i % a.D;
+    const float* po = a.part_o + (h0 + g) * a.splits * a.D + d;
+    float o = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < used; ++s) o += factor[g][s] * po[static_cast<long long>(s) * a.D];
+    static_cast<__nv_bfloat16*>(a.out)[(h0 + g) * a.D + d] = f2bf(o);
   }
 }
 
-void launch_weigh(const WeighArgs& a, cudaStream_t st) {
-  const int keys = a.max_ctx < a.capacity ? a.max_ctx : a.capacity;
-  if (a.B > 0 && keys > 0) launch_pdl(weigh_kernel, dim3(a.B * a.KV, (keys + 1023) / 1024), dim3(256), 0, st, a);
+int launch_decode_attention_weighted(const void* q, long long q_stride, const void* kc, const void* vc, const int* bt, int bt_stride, int page, float scale, float cap, WeighArgs a,
+                                     cudaStream_t st) {
+  if (a.B == 0) return 0;
+  if (a.H / a.KV > 16 || page % 16 != 0 || q_stride % 2 != 0 || a.splits > kWeighMaxSplits) return 1;
+  a.min_slices = decode_min_slices(a.B, a.KV, a.H / a.KV);
+  DecodeWeigh<true> w;
+  static_cast<WeighArgs&>(w) = a;
+#define DLV_DEC_WEIGH(DD)                                                                                                                                                   \
+  launch_decode_mma_t<DD, 0, false, false, true>(q, q_stride, kc, vc, bt, bt_stride, a.ctx, a.out, a.part_o, a.part_ml, nullptr, a.B, a.H, a.KV, page, scale, cap, a.window, \
+                                                 a.splits, a.used, st, DD, DD, {}, {}, w)
+  switch (a.D) {
+    case 64: DLV_DEC_WEIGH(64); break;
+    case 128: DLV_DEC_WEIGH(128); break;
+    case 256: DLV_DEC_WEIGH(256); break;
+    default: return 1;
+  }
+#undef DLV_DEC_WEIGH
+  if (a.splits > 1) {
+    // parts: two groups of four keys per thread, or one output each, as far as CTAs are resident together
+    const int pairs = a.B * a.KV, room = 4 * 148 / pairs, most = a.max_ctx < a.capacity ? a.max_ctx : a.capacity;
+    int parts = (most + 2047) / 2048;
+    parts = parts < a.H / a.KV * a.D / 256 ? a.H / a.KV * a.D / 256 : parts;
+    launch_pdl(weigh_kernel, dim3(pairs, 2 * (room < 1 || parts < 1 ? 1 : room < parts ? room : parts)), dim3(256), 0, st, a);
+  }
+  return 0;
 }
 
 int launch_decode_attention_mma(const void* q, long long q_stride, const void* kc, const void* vc, const int* bt, int bt_stride, const int* ctx, void* out,

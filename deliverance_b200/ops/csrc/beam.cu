@@ -1,9 +1,10 @@
 // Beam search: selection over beams and vocabulary, and the moves of beam states that follow it.
 //
 // Selection: value[w, v] = scores[w] + z[w, v] - log sum_u exp z[w, u], the K largest finite ones of a request's W rows, ties to the lowest w * V + v.
-// The order inside a row is the order of the raw logits (soft-capping and positive scaling are monotone), so rows are cut into splits that each keep
-// their K best logits, their maximum and their sum of exponentials from one pass; a second kernel compares the candidates of all rows in 64 bits.
-// What bounds it: the logits, read once.
+// The order inside a row is the order of the raw logits (soft-capping and positive scaling are monotone). The first kernel reads every logit once and leaves, per
+// row, maxima and sums of exponentials, and the largest logit of every group of 128 (bf16: 256) neighbours. The K best candidates lie in the K groups with the largest
+// maxima (equal ones: the first), so the second kernel compares those maxima over all rows, in 64 bits because rows differ by their log-sum-exp, and reads only
+// the few groups that can matter again. What bounds it: the logits, read once.
 #include <cfloat>
 
 #include "beam_api.h"
@@ -13,24 +14,12 @@ namespace dlv {
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kPerThread = 16;                   // logits per thread and tile
-constexpr int kTile = kThreads * kPerThread;     // logits per tile
-constexpr int kSoft = 512;                       // the list is cut back to K when it is longer than this behind a tile
-constexpr int kList = kSoft + kTile;             // so that a whole tile always fits
-constexpr int kShort = kThreads;                 // candidates that are put in order by counting
-
-// larger key = better candidate: the logit's order, then the lower token
-__device__ __forceinline__ uint32_t float_order(float x) {
-  const uint32_t u = __float_as_uint(x);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
-__device__ __forceinline__ float float_from_order(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o); }
-__device__ __forceinline__ unsigned long long candidate_key(float x, int i) {
-  return (static_cast<unsigned long long>(float_order(x + 0.f)) << 32) | (0xffffffffu - static_cast<uint32_t>(i));  // (-0 and 0 are equal)
-}
-__device__ __forceinline__ float key_logit(unsigned long long k) { return float_from_order(static_cast<uint32_t>(k >> 32)); }
-__device__ __forceinline__ int key_token(unsigned long long k) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(k)); }
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kPerLane = 16;                      // logits per lane and tile
+constexpr int kTile = kThreads * kPerLane;        // logits of a CTA's tile
+constexpr int kMergeThreads = 512, kMergeWarps = kMergeThreads / 32;
+constexpr int kClusters = 64;                     // threads of the second kernel, eight by eight: K of their best are the first bound
+constexpr int kMostGroups = 1024, kMostListed = 512;  // groups and candidates that are looked at without a closer bound
 
 // (-inf is a masked token and stays one)
 __device__ __forceinline__ float post(float x, float softcap, float inv_scale) {
@@ -52,137 +41,106 @@ __device__ __forceinline__ void unpack(const uint4& u, float (&x)[8]) {
   const float2 a = unpack_bf162(u.x), b = unpack_bf162(u.y), c = unpack_bf162(u.z), d = unpack_bf162(u.w);
   x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y, x[4] = c.x, x[5] = c.y, x[6] = d.x, x[7] = d.y;
 }
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return bf2f(v); }
 
-struct SelectShared {
-  unsigned long long list[kList];
-  unsigned long long shorter[kShort];
-  unsigned long long group[64];
-  unsigned long long edge;
-  double sum[kThreads / 32];
-  float max[kThreads / 32];
-  int count, n_short;
-};
-
-// K-th largest of the 64 group maxima (a group: four neighbouring threads): K entries of the list at least are not below it. All keys of a thread are
-// 0 where it has none.
-__device__ __forceinline__ unsigned long long group_edge(SelectShared& sh, unsigned long long best, int K) {
+// 16 bytes of a row (element by element where rows do not start on 16 bytes: the same logits in the same lane, so that equal rows have equal sums and their
+// candidates tie); -inf at and behind hi
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ uint4 load_vector(const T* row, int i, int hi) {
+  constexpr int N = Vec<T>::N;
+  if (ALIGNED && i + N <= hi) return __ldg(reinterpret_cast<const uint4*>(row + i));
+  uint4 u;
+  T e[N];
 #pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
-    const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
-    best = other > best ? other : best;
+  for (int j = 0; j < N; ++j) {
+    if constexpr (sizeof(T) == 4) e[j] = -INFINITY;
+    else e[j] = __ushort_as_bfloat16(static_cast<unsigned short>(0xff80u));
+    if (i + j < hi) e[j] = row[i + j];
   }
-  const int t = threadIdx.x;
-  if ((t & 3) == 0) sh.group[t >> 2] = best;
-  __syncthreads();
-  if (t < 64) {
-    const unsigned long long mine = sh.group[t];
-    int rank = 0;
-#pragma unroll 8
-    for (int u = 0; u < 64; ++u) {
-      const unsigned long long other = sh.group[u];
-      rank += other > mine || (other == mine && u < t) ? 1 : 0;  // (equal only where groups are empty)
-    }
-    if (rank == K - 1) sh.edge = mine;
+  if constexpr (sizeof(T) == 4) {
+    u = make_uint4(__float_as_uint(e[0]), __float_as_uint(e[1]), __float_as_uint(e[2]), __float_as_uint(e[3]));
+  } else {
+    auto two = [](T a, T b) { return static_cast<uint32_t>(__bfloat16_as_ushort(a)) | static_cast<uint32_t>(__bfloat16_as_ushort(b)) << 16; };
+    u = make_uint4(two(e[0], e[1]), two(e[2], e[3]), two(e[4], e[5]), two(e[6], e[7]));
   }
-  __syncthreads();
-  return sh.edge;
+  return u;
 }
 
-// Cuts the list back to its K best, in order. Returns how many there are.
-__device__ int cut_list(SelectShared& sh, int K) {
-  const int t = threadIdx.x, n = sh.count;
-  if (t == 0) sh.n_short = 0;
-  unsigned long long edge = 0;
-  if (n > kShort) {
-    unsigned long long best = 0;
-    for (int i = t; i < n; i += kThreads) best = sh.list[i] > best ? sh.list[i] : best;
-    edge = group_edge(sh, best, K);
-    int above = 0;
-    for (int i = t; i < n; i += kThreads) above += sh.list[i] >= edge ? 1 : 0;
-    // (a list in an unlucky order: many entries above the edge; keys differ, so a search over the bits finds the K-th largest itself)
-    int rough = 0;
-    for (int b = 0; b < 5; ++b) rough += __syncthreads_count((above >> b) & 1) << b;
-    if (rough > kShort) {
-      edge = 0;
-      for (int b = 63; b >= 0; --b) {
-        const unsigned long long probe = edge | (1ull << b);
-        int c = 0, total = 0;
-        for (int i = t; i < n; i += kThreads) c += sh.list[i] >= probe ? 1 : 0;
-        for (int q = 0; q < 5; ++q) total += __syncthreads_count((c >> q) & 1) << q;
-        if (total >= K) edge = probe;
-      }
-    }
-  }
-  __syncthreads();
-  for (int i = t; i < n; i += kThreads)
-    if (sh.list[i] >= edge) sh.shorter[atomicAdd(&sh.n_short, 1)] = sh.list[i];
-  __syncthreads();
-  const int m = sh.n_short;
-  if (t < m) {
-    const unsigned long long mine = sh.shorter[t];
-    int rank = 0;
-    for (int u = 0; u < m; ++u) rank += sh.shorter[u] > mine ? 1 : 0;
-    if (rank < K) sh.list[rank] = mine;
-  }
-  const int left = min(m, K);
-  if (t == 0) sh.count = left;
-  __syncthreads();
-  return left;
+// exp(d) for d <= 0, relative error 2^-22 + |d| 2^-22: exactly 1 at d = 0, so that what weighs most is exact (with expf the kernel executes 20 instructions per logit, with this 14:
+// 35 us against 29 for 256 rows of 151,936)
+__device__ __forceinline__ float exp_below(float d) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * 1.44269504088896341f));
+  return r;
+}
+// maximum over the warp, NaN left out
+__device__ __forceinline__ float redux_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
 }
 
-// grid: B * W * splits. A thread reads 16 logits of a tile in groups of 16 bytes (one by one where the row does not start on 16 bytes: the same logits in the
-// same thread, so that equal rows have equal sums and their candidates tie), keeps a running maximum and sum, and lists what beats the K-th best found so far.
-// Later tiles hold higher tokens, so an equal logit never does.
-template <typename T, bool MASK>
-__global__ void __launch_bounds__(kThreads) beam_part_kernel(const __grid_constant__ BeamSelectArgs a) {
+// grid: B * W * splits. A tile is 16 logits per thread, 16 bytes of a warp's lanes side by side: one group per load. The next tile is on its way while a tile is
+// worked on; a running maximum and sum per thread, joined at the end in a fixed order.
+template <typename T, bool MASK, bool ALIGNED>
+__global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_constant__ BeamSelectArgs a) {
   pdl_trigger();
   pdl_wait();
-  __shared__ SelectShared sh;
-  constexpr int N = Vec<T>::N, NV = kPerThread / N;
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, K = a.K;
+  __shared__ double sums[kWarps];
+  __shared__ float tops[kWarps];
+  constexpr int N = Vec<T>::N, NV = kPerLane / N;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
   const int lo = min(a.V, split * a.per), hi = min(a.V, lo + a.per);
   const T* x_row = static_cast<const T*>(a.logits) + static_cast<long long>(row) * a.ld;
   const uint32_t* bits = MASK ? a.mask + static_cast<long long>(row) * a.mask_ld : nullptr;
-  const bool whole = (reinterpret_cast<uintptr_t>(x_row) & 15) == 0;  // (splits start at multiples of 64 logits)
+  float* group_max = a.group_max + static_cast<long long>(row) * a.groups;
   const bool plain = a.softcap <= 0.f && a.inv_scale == 1.f;
-  if (t == 0) sh.count = 0;
-  float m = -FLT_MAX, edge = -INFINITY;
+  float m = -FLT_MAX;
   double sum = 0.0;
-  bool first = true;
-  __syncthreads();
+  uint4 raw[NV];
+  uint32_t word[NV];
+  auto fetch = [&](int at) {
+    const int first = at + (warp * NV * 32 + lane) * N;
+    const T* p = x_row + first;
+    if (ALIGNED && at + kTile <= hi) {  // (the same for the whole CTA)
+#pragma unroll
+      for (int v = 0; v < NV; ++v) raw[v] = __ldg(reinterpret_cast<const uint4*>(p + v * 32 * N));
+    } else {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) raw[v] = load_vector<T, ALIGNED>(x_row, first + v * 32 * N, hi);
+    }
+    if constexpr (MASK) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) word[v] = first + v * 32 * N < hi ? bits[(first + v * 32 * N) >> 5] >> (first & 31) : 0u;
+    }
+  };
+  if (lo < hi) fetch(lo);
+#pragma unroll 2
   for (int at = lo; at < hi; at += kTile) {
     float x[NV][N];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int i = at + (v * kThreads + t) * N;
-      if (i + N <= hi) {
-        if (whole) {
-          unpack(__ldg(reinterpret_cast<const uint4*>(x_row + i)), x[v]);
-        } else {
+      unpack(raw[v], x[v]);
+      if constexpr (MASK) {
 #pragma unroll
-          for (int e = 0; e < N; ++e) x[v][e] = to_float(__ldg(x_row + i + e));
-        }
-        if constexpr (MASK) {
-          const uint32_t word = bits[i >> 5] >> (i & 31);
-#pragma unroll
-          for (int e = 0; e < N; ++e) x[v][e] = (word >> e) & 1u ? x[v][e] : -INFINITY;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          x[v][e] = -INFINITY;
-          if (i + e < hi && (!MASK || ((bits[(i + e) >> 5] >> ((i + e) & 31)) & 1u))) x[v][e] = to_float(x_row[i + e]);
-        }
+        for (int e = 0; e < N; ++e) x[v][e] = (word[v] >> e) & 1u ? x[v][e] : -INFINITY;
       }
     }
-    // maximum and sum of exponentials (NaN and +inf make the sum NaN: such a row has no candidates)
-    float top = -INFINITY, top_z;
+    if (at + kTile < hi) fetch(at + kTile);
+    // (NaN is left out of the maxima; NaN and +inf make the sum NaN, and a row with such a sum has no candidates)
+    float top = -INFINITY, mine = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < kPerThread; ++j) top = fmaxf(top, x[j / N][j % N]);
-    top_z = plain ? top : post(top, a.softcap, a.inv_scale);
+    for (int v = 0; v < NV; ++v) {
+      float g = x[v][0];
+#pragma unroll
+      for (int e = 1; e < N; ++e) g = fmaxf(g, x[v][e]);
+      top = fmaxf(top, g);
+      g = redux_max(g);
+      if (lane == v) mine = g;
+    }
+    const int group = at / (32 * N) + warp * NV + lane;
+    if (lane < NV && group * 32 * N < hi) group_max[group] = mine;
+    const float top_z = plain ? top : post(top, a.softcap, a.inv_scale);
     if (top_z > m) {
       sum *= static_cast<double>(expf(m - top_z));
       m = top_z;
@@ -190,210 +148,307 @@ __global__ void __launch_bounds__(kThreads) beam_part_kernel(const __grid_consta
     float part = 0.f;
     if (plain) {
 #pragma unroll
-      for (int j = 0; j < kPerThread; ++j) part += expf(x[j / N][j % N] - m);
+      for (int j = 0; j < kPerLane; ++j) part += exp_below(x[j / N][j % N] - m);
     } else {
 #pragma unroll
-      for (int j = 0; j < kPerThread; ++j) part += expf(post(x[j / N][j % N], a.softcap, a.inv_scale) - m);
+      for (int j = 0; j < kPerLane; ++j) part += exp_below(post(x[j / N][j % N], a.softcap, a.inv_scale) - m);
     }
     sum += static_cast<double>(part);
-    // candidates
-    unsigned long long least = 0;
-    if (first) {
-      first = false;
-      unsigned long long best = 0;
-#pragma unroll
-      for (int v = NV - 1; v >= 0; --v) {
-#pragma unroll
-        for (int e = N - 1; e >= 0; --e) {
-          const float y = x[v][e];
-          if (y > -INFINITY) {
-            const unsigned long long k = candidate_key(y, at + (v * kThreads + t) * N + e);
-            best = k > best ? k : best;
-          }
-        }
-      }
-      least = group_edge(sh, best, K);
-    }
-    bool over = false;
-    if (top > edge) {
-#pragma unroll
-      for (int v = 0; v < NV; ++v) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float y = x[v][e];
-          if (y > edge) {
-            const unsigned long long k = candidate_key(y, at + (v * kThreads + t) * N + e);
-            if (k >= least) {
-              const int p = atomicAdd(&sh.count, 1);
-              sh.list[p] = k;
-              over = over || p >= kSoft;
-            }
-          }
-        }
-      }
-    }
-    if (__syncthreads_or(over)) {
-      cut_list(sh, K);
-      edge = key_logit(sh.list[K - 1]);
-    } else if (least != 0) {
-      edge = key_logit(least);
-    }
   }
-  const int n = cut_list(sh, K);
-  const long long out = static_cast<long long>(blockIdx.x) * K;
-  if (t < K) {
-    a.cand_x[out + t] = t < n ? key_logit(sh.list[t]) : -INFINITY;
-    a.cand_i[out + t] = t < n ? key_token(sh.list[t]) : 0;
-  }
-  // the split's maximum and sum, threads in a fixed order
   const float wm = warp_max(m);
   sum *= static_cast<double>(expf(m - wm));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) {
-    sh.max[warp] = wm;
-    sh.sum[warp] = sum;
+    tops[warp] = wm;
+    sums[warp] = sum;
   }
   __syncthreads();
-  if (t == 0) {
-    float top = sh.max[0];
-    for (int w = 1; w < kThreads / 32; ++w) top = fmaxf(top, sh.max[w]);
-    double total = 0.0;
-    for (int w = 0; w < kThreads / 32; ++w) total += sh.sum[w] * static_cast<double>(expf(sh.max[w] - top));
-    a.part_m[blockIdx.x] = top;
-    a.part_sum[blockIdx.x] = total;
+  if (warp == 0) {
+    const float t = lane < kWarps ? tops[lane] : -FLT_MAX, all = warp_max(t);
+    double s = lane < kWarps ? sums[lane] * static_cast<double>(expf(t - all)) : 0.0;
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) {
+      a.part_m[blockIdx.x] = all;
+      a.part_sum[blockIdx.x] = s;
+    }
   }
 }
 
 __device__ __forceinline__ unsigned long long double_order(double v) {
-  const long long u = __double_as_longlong(v);
+  const long long u = __double_as_longlong(v + 0.0);
   return u < 0 ? ~static_cast<unsigned long long>(u) : static_cast<unsigned long long>(u) | 0x8000000000000000ull;
 }
-__device__ __forceinline__ double double_from_order(unsigned long long o) {
-  return __longlong_as_double(static_cast<long long>(o & 0x8000000000000000ull ? o ^ 0x8000000000000000ull : ~o));
+
+// Number of threads' set flags over the CTA, for the searches that need many of them
+__device__ __forceinline__ int merge_count(int c, int* red, int& turn) {
+  c = __reduce_add_sync(0xffffffffu, c);
+  const int lane = threadIdx.x & 31;
+  int* r = red + turn * kMergeWarps;
+  turn ^= 1;
+  if (lane == 0) r[threadIdx.x >> 5] = c;
+  __syncthreads();
+  return __reduce_add_sync(0xffffffffu, lane < kMergeWarps ? r[lane] : 0);
 }
 
-// best (largest value, lowest place) of a warp: every lane gets it; value 0: none
-__device__ __forceinline__ void warp_best(unsigned long long& value, uint32_t& place) {
-  const uint32_t hi = static_cast<uint32_t>(value >> 32), top = __reduce_max_sync(0xffffffffu, hi);
-  const uint32_t lo = hi == top ? static_cast<uint32_t>(value) : 0u, low = __reduce_max_sync(0xffffffffu, lo);
-  place = __reduce_min_sync(0xffffffffu, hi == top && static_cast<uint32_t>(value) == low ? place : 0xffffffffu);
-  value = (static_cast<unsigned long long>(top) << 32) | low;
+// The K-th best of n (value, place) pairs, found bit by bit: the value, then the place among equals. at(i, place) gives a pair's value, -inf: none. With fewer than
+// K pairs the value is -inf. Places differ.
+template <typename At>
+__device__ __noinline__ void kth_best(int n, int K, At at, int* red, double& value, uint32_t& place) {
+  int turn = 0;
+  unsigned long long edge = 0;
+  uint32_t p;
+  const unsigned long long none = double_order(-INFINITY);
+  for (int bit = 63; bit >= 0; --bit) {
+    const unsigned long long probe = edge | (1ull << bit);
+    int c = 0;
+    for (int i = threadIdx.x; i < n; i += kMergeThreads) {
+      const unsigned long long o = double_order(at(i, p));
+      c += o > none && o >= probe ? 1 : 0;
+    }
+    if (merge_count(c, red, turn) >= K) edge = probe;
+  }
+  value = edge > none ? __longlong_as_double(static_cast<long long>(edge & 0x8000000000000000ull ? edge ^ 0x8000000000000000ull : ~edge)) : -INFINITY;
+  place = 0xffffffffu;
+  if (edge <= none) return;
+  int c = 0;
+  for (int i = threadIdx.x; i < n; i += kMergeThreads) c += double_order(at(i, p)) > edge ? 1 : 0;
+  const int left = K - merge_count(c, red, turn);  // so many of the equal ones, the lowest places
+  uint32_t low = 0;                                // the largest bound below which fewer than `left` equal ones lie
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t probe = low | (1u << bit);
+    c = 0;
+    for (int i = threadIdx.x; i < n; i += kMergeThreads) c += double_order(at(i, p)) == edge && p < probe ? 1 : 0;
+    if (merge_count(c, red, turn) < left) low = probe;
+  }
+  place = low;
 }
 
-// one CTA per request: W * splits * K <= 8 * NT candidates in registers, K rounds of "take the best"
-template <int NT>
-__global__ void __launch_bounds__(NT) beam_merge_kernel(const __grid_constant__ BeamSelectArgs a) {
+// One CTA per request. Bound: K of 64 clusters of threads have seen a group whose maximum reaches it, so K candidates do. The groups that reach it are read
+// again, and the candidates that reach it are put in order by counting. Where too many do (long runs of one value), the K-th best itself is searched for.
+template <typename T>
+__global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_constant__ BeamSelectArgs a) {
   pdl_trigger();
   pdl_wait();
-  constexpr int PER = kBeamMaxMerge / 1024, NW = NT / 32;
   __shared__ double base[kBeamMaxBeams];
   __shared__ float top[kBeamMaxBeams];
-  __shared__ unsigned long long best_value[2][NW];
-  __shared__ uint32_t best_place[2][NW];
+  __shared__ double values[kMostListed];
+  __shared__ float rough[kBeamMaxBeams], cluster_value[kClusters], edge_value;
+  __shared__ uint32_t places[kMostListed];
+  __shared__ int groups[kMostGroups], red[2 * kMergeWarps], listed, n_groups;
+  constexpr int N = Vec<T>::N, GROUP = 32 * N;
   const int b = blockIdx.x, t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  const int S = a.splits, K = a.K, W = a.W, n = W * S * K;
-  for (int w = warp; w < W; w += NW) {
-    const long long at = (static_cast<long long>(b) * W + w) * S;
+  const int K = a.K, W = a.W, n = W * a.groups;
+  const float* maxima = a.group_max + static_cast<long long>(b) * n;
+  constexpr int AHEAD = 12;
+  float x[AHEAD];  // (on their way while the sums are joined)
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j) x[j] = j * kMergeThreads + t < n ? maxima[j * kMergeThreads + t] : -INFINITY;
+  if (t == 0) listed = n_groups = 0;
+  for (int w = warp; w < W; w += kMergeWarps) {
+    const long long at = (static_cast<long long>(b) * W + w) * a.splits;
+    const float score = a.scores[static_cast<long long>(b) * W + w];
     float m = -FLT_MAX;
-    for (int s = lane; s < S; s += 32) m = fmaxf(m, a.part_m[at + s]);
+    for (int s = lane; s < a.splits; s += 32) m = fmaxf(m, a.part_m[at + s]);
     m = warp_max(m);
     double sum = 0.0;
-    for (int s = lane; s < S; s += 32) sum += a.part_sum[at + s] * exp(static_cast<double>(a.part_m[at + s]) - static_cast<double>(m));
+    for (int s = lane; s < a.splits; s += 32) sum += a.part_sum[at + s] * static_cast<double>(expf(a.part_m[at + s] - m));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) {
       top[w] = m;
-      base[w] = static_cast<double>(a.scores[static_cast<long long>(b) * W + w]) - log(sum);
+      base[w] = static_cast<double>(score) - log(sum);
+      const float r = static_cast<float>(base[w] - static_cast<double>(m));
+      rough[w] = isfinite(r) ? r : -INFINITY;
     }
   }
   __syncthreads();
-  unsigned long long value[PER];
-  uint32_t place[PER];
-  const long long first = static_cast<long long>(b) * n;
+  auto value_of = [&](float y, int w) {
+    if (!(y > -INFINITY)) return -static_cast<double>(INFINITY);
+    double z = static_cast<double>(y) * static_cast<double>(a.inv_scale);
+    if (a.softcap > 0.f) z = static_cast<double>(a.softcap) * tanh(z / static_cast<double>(a.softcap));
+    const double v = base[w] + (z - static_cast<double>(top[w]));
+    return isfinite(v) ? v : -static_cast<double>(INFINITY);
+  };
+  // in 32 bits: off by less than half of `slack` (roundings of the row's constant, of the sum and of scale and cap)
+  auto rough_of = [&](float y, int i) { return post(y, a.softcap, a.inv_scale) + rough[a.by_groups.of(i)]; };
+  float best = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int i = j * NT + t;
-    value[j] = 0;
-    place[j] = 0xffffffffu;
-    if (i < n) {
-      const int w = i / (S * K);
-      const float x = a.cand_x[first + i];
-      if (x > -INFINITY) {
-        double z = static_cast<double>(x) * static_cast<double>(a.inv_scale);
-        if (a.softcap > 0.f) z = static_cast<double>(a.softcap) * tanh(z / static_cast<double>(a.softcap));
-        const double v = base[w] + (z - static_cast<double>(top[w]));
-        if (isfinite(v)) {
-          value[j] = double_order(v);
-          place[j] = static_cast<uint32_t>(w) * static_cast<uint32_t>(a.V) + static_cast<uint32_t>(a.cand_i[first + i]);
-        }
+  for (int j = 0; j < AHEAD; ++j) {
+    const int i = j * kMergeThreads + t;
+    x[j] = i < n ? rough_of(x[j], i) : -INFINITY;
+    best = fmaxf(best, x[j]);
+  }
+  for (int i0 = AHEAD * kMergeThreads + t; i0 < n; i0 += 8 * kMergeThreads) {
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = i0 + j * kMergeThreads < n ? maxima[i0 + j * kMergeThreads] : -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i0 + j * kMergeThreads < n) best = fmaxf(best, rough_of(y[j], i0 + j * kMergeThreads));
+  }
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+  if ((t & 7) == 0) cluster_value[t >> 3] = best;
+  __syncthreads();
+  {  // eight threads count for one cluster
+    const int g = t >> 3;
+    int rank = 0;
+#pragma unroll
+    for (int q = 0; q < kClusters / 8; ++q) {
+      const int u = q * 8 + (t & 7);
+      rank += cluster_value[u] > best || (cluster_value[u] == best && u < g) ? 1 : 0;
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+    if ((t & 7) == 0 && rank == K - 1) edge_value = best;
+  }
+  __syncthreads();
+  float most = 0.f;
+  for (int w = lane; w < W; w += 32) most = fmaxf(most, rough[w] > -INFINITY ? fabsf(rough[w]) : 0.f);
+  const float slack = 0x1p-20f * (warp_max(most) + fabsf(edge_value)) + 0x1p-18f * a.softcap, bound = edge_value - slack;
+  double edge = static_cast<double>(bound);  // K candidates at least are not below this
+  uint32_t last = 0xffffffffu;               // of the groups (then: candidates) that equal the edge, those up to this place
+  auto list_group = [&](int i) {
+    const int p = atomicAdd(&n_groups, 1);
+    if (p < kMostGroups) groups[p] = i;
+  };
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j)
+    if (x[j] > -INFINITY && x[j] >= bound) list_group(j * kMergeThreads + t);
+  for (int i0 = AHEAD * kMergeThreads + t; i0 < n; i0 += 8 * kMergeThreads) {
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = i0 + j * kMergeThreads < n ? maxima[i0 + j * kMergeThreads] : -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int i = i0 + j * kMergeThreads;
+      if (i < n) {
+        const float f = rough_of(y[j], i);
+        if (f > -INFINITY && f >= bound) list_group(i);
       }
     }
   }
-  const long long out = static_cast<long long>(b) * K;
-  for (int k = 0; k < K; ++k) {
-    unsigned long long mine = 0;
-    uint32_t at = 0xffffffffu;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      if (value[j] > mine || (value[j] == mine && place[j] < at)) {
-        mine = value[j];
-        at = place[j];
-      }
-    }
-    unsigned long long v = mine;
-    uint32_t p = at;
-    warp_best(v, p);
-    if (lane == 0) {
-      best_value[k & 1][warp] = v;
-      best_place[k & 1][warp] = p;
+  __syncthreads();
+  if (n_groups > kMostGroups) {
+    kth_best(n, K, [&](int i, uint32_t& p) { p = static_cast<uint32_t>(i); return value_of(maxima[i], i / a.groups); }, red, edge, last);
+    __syncthreads();
+    if (t == 0) n_groups = 0;
+    __syncthreads();
+    for (int i = t; i < n; i += kMergeThreads) {
+      const double v = value_of(maxima[i], i / a.groups);
+      if (v > -INFINITY && (v > edge || (v == edge && static_cast<uint32_t>(i) <= last))) list_group(i);
     }
     __syncthreads();
-    v = lane < NW ? best_value[k & 1][lane] : 0;
-    p = lane < NW ? best_place[k & 1][lane] : 0xffffffffu;
-    warp_best(v, p);
-    if (v == 0) {  // (the same for all threads)
-      for (int r = k + t; r < K; r += NT) {
-        a.out_value[out + r] = -INFINITY;
-        a.out_parent[out + r] = -1;
-        a.out_token[out + r] = -1;
-      }
-      return;
-    }
-    if (v == mine && p == at) {
-      a.out_value[out + k] = static_cast<float>(double_from_order(v));
-      a.out_parent[out + k] = p / static_cast<uint32_t>(a.V);
-      a.out_token[out + k] = p % static_cast<uint32_t>(a.V);
+  }
+  const int m_groups = n_groups;
+  // candidate j of the listed groups
+  auto logit = [&](int g, int e, int& w, int& v) {
+    w = groups[g] / a.groups;
+    v = groups[g] % a.groups * GROUP + e;
+    const long long row = static_cast<long long>(b) * W + w;
+    if (v >= a.V || (a.mask != nullptr && !((a.mask[row * a.mask_ld + (v >> 5)] >> (v & 31)) & 1u))) return -INFINITY;
+    const T y = static_cast<const T*>(a.logits)[row * a.ld + v];
+    if constexpr (sizeof(T) == 4) return static_cast<float>(y);
+    else return bf2f(y);
+  };
+  auto place_of = [&](int w, int v) { return static_cast<uint32_t>(w) * static_cast<uint32_t>(a.V) + static_cast<uint32_t>(v); };
+  last = 0xffffffffu;
+  auto list_candidates = [&]() {
+    for (int g = warp; g < m_groups; g += kMergeWarps) {
+      float y[N];
+      int w, v;
 #pragma unroll
-      for (int j = 0; j < PER; ++j)
-        if (place[j] == p) value[j] = 0, place[j] = 0xffffffffu;
+      for (int q = 0; q < N; ++q) y[q] = logit(g, q * 32 + lane, w, v);
+#pragma unroll
+      for (int q = 0; q < N; ++q) {
+        const double d = value_of(y[q], w);
+        const uint32_t p = place_of(w, groups[g] % a.groups * GROUP + q * 32 + lane);
+        if (d > -INFINITY && (d > edge || (d == edge && p <= last))) {
+          const int at = atomicAdd(&listed, 1);
+          if (at < kMostListed) {
+            values[at] = d;
+            places[at] = p;
+          }
+        }
+      }
     }
+  };
+  list_candidates();
+  __syncthreads();
+  if (listed > kMostListed) {
+    kth_best(m_groups * GROUP, K, [&](int i, uint32_t& p) {
+      int w, v;
+      const float y = logit(i / GROUP, i % GROUP, w, v);
+      p = place_of(w, v);
+      return value_of(y, w);
+    }, red, edge, last);
+    __syncthreads();
+    if (t == 0) listed = 0;
+    __syncthreads();
+    list_candidates();
+    __syncthreads();
+  }
+  const int m = listed;
+  const long long out = static_cast<long long>(b) * K;
+  for (int j = t; j < m; j += kMergeThreads) {
+    const double v = values[j];
+    const uint32_t p = places[j];
+    int rank = 0;
+    for (int u = 0; u < m; ++u) rank += values[u] > v || (values[u] == v && places[u] < p) ? 1 : 0;
+    if (rank < K) {
+      a.out_value[out + rank] = static_cast<float>(v);
+      a.out_parent[out + rank] = p / static_cast<uint32_t>(a.V);
+      a.out_token[out + rank] = p % static_cast<uint32_t>(a.V);
+    }
+  }
+  for (int r = m + t; r < K; r += kMergeThreads) {
+    a.out_value[out + r] = -INFINITY;
+    a.out_parent[out + r] = -1;
+    a.out_token[out + r] = -1;
   }
 }
 
 }  // namespace
 
-int beam_select_splits(int rows, int W, int K, int V) {
-  const int tiles = (V + kTile - 1) / kTile;
-  int s = (4 * 148 + rows - 1) / rows;
-  s = s < tiles ? s : tiles;
-  const int most = kBeamMaxMerge / (W * K);
-  s = s < most ? s : most;
-  return s > 1 ? s : 1;
+int beam_select_group(bool f32) { return f32 ? 32 * Vec<float>::N : 32 * Vec<__nv_bfloat16>::N; }
+
+// CTAs per row: the fewest that keep the GPU about evenly busy (four resident per SM), each with a tile at least.
+int beam_select_splits(int rows, int V) {
+  const int tiles = (V + kTile - 1) / kTile, slots = 4 * 148;
+  int best = 1;
+  double most = 0.0;
+  for (int s = 1; s <= tiles && s <= 64; ++s) {
+    const double n = static_cast<double>(rows) * ((tiles + (tiles + s - 1) / s - 1) / ((tiles + s - 1) / s)), waves = n / slots;
+    const double even = waves / static_cast<double>(static_cast<long long>(waves + 0.999999));
+    if (even > most + 0.1) {
+      most = even;
+      best = s;
+    }
+    if (most > 0.85) break;
+  }
+  return best;
+}
+
+template <typename T, bool MASK>
+static void launch_part(const BeamSelectArgs& a, dim3 grid, cudaStream_t st) {
+  if ((reinterpret_cast<uintptr_t>(a.logits) | static_cast<uintptr_t>(a.ld * static_cast<long long>(sizeof(T)))) % 16 == 0)
+    launch_pdl(beam_part_kernel<T, MASK, true>, grid, dim3(kThreads), 0, st, a);
+  else
+    launch_pdl(beam_part_kernel<T, MASK, false>, grid, dim3(kThreads), 0, st, a);
 }
 
 void launch_beam_select(const BeamSelectArgs& a, bool f32, cudaStream_t st) {
   if (a.B == 0) return;
   const dim3 grid(static_cast<unsigned>(a.B) * a.W * a.splits);
   if (f32) {
-    if (a.mask != nullptr) launch_pdl(beam_part_kernel<float, true>, grid, dim3(kThreads), 0, st, a);
-    else launch_pdl(beam_part_kernel<float, false>, grid, dim3(kThreads), 0, st, a);
+    a.mask != nullptr ? launch_part<float, true>(a, grid, st) : launch_part<float, false>(a, grid, st);
+    launch_pdl(beam_merge_kernel<float>, dim3(a.B), dim3(kMergeThreads), 0, st, a);
   } else {
-    if (a.mask != nullptr) launch_pdl(beam_part_kernel<__nv_bfloat16, true>, grid, dim3(kThreads), 0, st, a);
-    else launch_pdl(beam_part_kernel<__nv_bfloat16, false>, grid, dim3(kThreads), 0, st, a);
+    a.mask != nullptr ? launch_part<__nv_bfloat16, true>(a, grid, st) : launch_part<__nv_bfloat16, false>(a, grid, st);
+    launch_pdl(beam_merge_kernel<__nv_bfloat16>, dim3(a.B), dim3(kMergeThreads), 0, st, a);
   }
-  if (a.W * a.splits * a.K <= kBeamMaxMerge / 4) launch_pdl(beam_merge_kernel<256>, dim3(a.B), dim3(256), 0, st, a);
-  else launch_pdl(beam_merge_kernel<1024>, dim3(a.B), dim3(1024), 0, st, a);
 }
 
 // =====================================================================================================================

@@ -3,11 +3,12 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "divisor.h"
+
 namespace dlv {
 
 constexpr int kBeamMaxBeams = 32;        // beams of one request
 constexpr int kBeamMaxPicks = 64;        // candidates returned per request
-constexpr int kBeamMaxMerge = 8192;      // candidates of one request that the second kernel takes
 constexpr int kBeamMoveTensors = 96;     // tensors of one launch of beam_reorder (the table travels as a kernel parameter)
 
 struct BeamSelectArgs {
@@ -18,18 +19,20 @@ struct BeamSelectArgs {
   int mask_ld;
   float softcap, inv_scale;
   const float* scores;  // [B, W]
-  int B, W, K, splits, per;  // per: logits of one split
+  int B, W, K, splits, per;  // per: logits of one split, a multiple of 4,096
+  int groups;                // groups of a row
+  Divisor by_groups;
   float* part_m;             // [B * W, splits] maximum of the split (of the post-processed logits)
   double* part_sum;          // [B * W, splits] sum of exp(logit - maximum)
-  float* cand_x;             // [B * W, splits, K] raw logits of the split's best, -inf: none
-  int* cand_i;               // [B * W, splits, K] their tokens
+  float* group_max;          // [B * W, groups] largest raw logit of every group
   float* out_value;          // [B, K]
   long long *out_parent, *out_token;
 };
 // logits of fp32 (bf16: 0)
 void launch_beam_select(const BeamSelectArgs& a, bool f32, cudaStream_t st);
-// splits of a row of V logits, when there are `rows` rows
-int beam_select_splits(int rows, int W, int K, int V);
+int beam_select_group(bool f32);              // neighbouring logits of a group
+int beam_select_splits(int rows, int V);      // CTAs per row of V logits, when there are `rows` rows
+constexpr int kBeamSplitUnit = 4096;
 
 struct BeamMoveTensor {
   void* base;
@@ -70,18 +73,21 @@ struct EvictArgs {
 // unit: bytes of one access (16, 4 or 2). Two launches.
 void launch_evict(const EvictArgs& a, int unit, cudaStream_t st);
 
-// Adds the probabilities of a decode step to the weights: scores fp32 [B, H, S] (scaled and capped, -inf where masked), part_ml [B, H, splits, 2] of the
-// attention kernel, used: its plan or null (then min_slices).
+// Decode attention that adds its probabilities to the keys' weights (attention.cu).
+constexpr int kWeighMaxSplits = 128;
 struct WeighArgs {
-  const float* scores;
-  const float* part_ml;
+  float* scores;          // [B, H, S] scaled and capped, -inf where masked; S: a multiple of 16
+  float *part_ml, *part_o;  // [B, H, splits, 2], [B, H, splits, D]: with more than one split
+  void* out;              // [B, H * D] bf16
   const int* ctx;
-  const int* used;
+  const int* used;        // the plan's splits per sequence, or null: by length
   const long long* slots;
   float* weights;  // [num_slots, KV, capacity]
   int* status;
-  int B, H, KV, S, splits, window, min_slices, num_slots, capacity, max_ctx;
+  int B, H, KV, D, S, splits, window, min_slices, num_slots, capacity, max_ctx, pages;
 };
-void launch_weigh(const WeighArgs& a, cudaStream_t st);
+// 1: unsupported shape
+int launch_decode_attention_weighted(const void* q, long long q_stride, const void* kc, const void* vc, const int* bt, int bt_stride, int page, float scale, float cap, WeighArgs a,
+                                     cudaStream_t st);
 
 }  // namespace dlv

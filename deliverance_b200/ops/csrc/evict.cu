@@ -10,7 +10,7 @@ namespace dlv {
 
 namespace {
 
-constexpr int kSelectThreads = 512;
+constexpr size_t kSelectShared = 220 * 1024;
 
 // larger = heavier; NaN is the smallest, -0 equals 0
 __device__ __forceinline__ uint32_t weight_order(float w) {
@@ -19,14 +19,15 @@ __device__ __forceinline__ uint32_t weight_order(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// sum over the CTA (kSelectThreads threads); `red`: two buffers used in turn, one barrier per call
+// sum over the CTA's NT threads; `red`: two buffers used in turn, one barrier per call
+template <int NT>
 __device__ __forceinline__ int block_count(int v, int* red, int turn) {
   v = __reduce_add_sync(0xffffffffu, v);
   const int lane = threadIdx.x & 31;
-  int* r = red + turn * (kSelectThreads / 32);
+  int* r = red + turn * (NT / 32);
   if (lane == 0) r[threadIdx.x >> 5] = v;
   __syncthreads();
-  return __reduce_add_sync(0xffffffffu, lane < kSelectThreads / 32 ? r[lane] : 0);
+  return __reduce_add_sync(0xffffffffu, lane < NT / 32 ? r[lane] : 0);
 }
 
 // Whether this sequence can be worked on: its slot lies inside the weights and no earlier sequence of the call has it.
@@ -37,95 +38,183 @@ __device__ __forceinline__ bool slot_ok(const long long* slots, int b, int num_s
   return !__syncthreads_or(bad);
 }
 
-// grid (KV, B, layers)
-__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __grid_constant__ EvictArgs a) {
+// exclusive sum over the CTA, and the total; `red` as in block_count
+template <int NT>
+__device__ __forceinline__ int block_scan(int v, int* red, int turn, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int in = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, in, o);
+    in += lane >= o ? u : 0;
+  }
+  int* r = red + turn * (NT / 32);
+  if (lane == 31) r[warp] = in;
+  __syncthreads();
+  const int w = lane < NT / 32 ? r[lane] : 0;
+  total = __reduce_add_sync(0xffffffffu, w);
+  return in - v + __reduce_add_sync(0xffffffffu, lane < warp ? w : 0);
+}
+
+// What the selection of one (sequence, KV head, layer) works on; false: there is nothing to choose, and the list is written.
+struct EvictTask {
+  int n, counted, old, want;
+  int* kept;
+  float* w;
+  __device__ bool open(const EvictArgs& a) {
+    const int kvh = blockIdx.x, b = blockIdx.y, layer = blockIdx.z, t = threadIdx.x;
+    n = max(0, min(a.ctx[b], a.table_width * a.page));
+    kept = a.kept + ((static_cast<long long>(layer) * a.B + b) * a.KV + kvh) * a.keep;
+    const bool ok = n == 0 || slot_ok(a.slots, b, a.num_slots);
+    if (layer == 0 && kvh == 0 && t == 0) {
+      a.lens[b] = ok ? min(n, a.keep) : n;
+      if (!ok) atomicCAS(a.status, kStatusOk, kStatusBadArgs);
+    }
+    if (!ok || n <= a.keep) {
+      for (int j = t; j < a.keep; j += blockDim.x) kept[j] = ok && j < n ? j : -1;
+      return false;
+    }
+    w = a.layer[layer].weights + (a.slots[b] * a.KV + kvh) * a.capacity;
+    counted = min(n, a.capacity);
+    old = n - a.recent;
+    want = a.keep - a.recent;
+    return true;
+  }
+};
+
+// grid (KV, B, layers). Up to R * NT rows: the weights go through shared memory, every thread holds R neighbouring ones as ordered integers in registers.
+// The edge (what the want-th heaviest weighs) is found bit by bit, a count over the CTA each, until exactly `want` keys reach it. Shared: R * NT weights, keep rows.
+template <int NT, int R>
+__global__ void __launch_bounds__(NT) evict_select_kernel(const __grid_constant__ EvictArgs a) {
   pdl_trigger();
   pdl_wait();
-  __shared__ int red[2 * (kSelectThreads / 32)];
-  __shared__ int ties[2][kSelectThreads / 32], takes[2][kSelectThreads / 32];
-  const int kvh = blockIdx.x, b = blockIdx.y, layer = blockIdx.z, t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  const int n = max(0, min(a.ctx[b], a.table_width * a.page));
-  int* kept = a.kept + ((static_cast<long long>(layer) * a.B + b) * a.KV + kvh) * a.keep;
-  const bool ok = n == 0 || slot_ok(a.slots, b, a.num_slots);
-  if (layer == 0 && kvh == 0 && t == 0) {
-    a.lens[b] = ok ? min(n, a.keep) : n;
-    if (!ok) atomicCAS(a.status, kStatusOk, kStatusBadArgs);
-  }
-  if (!ok || n <= a.keep) {
-    for (int j = t; j < a.keep; j += kSelectThreads) kept[j] = ok && j < n ? j : -1;
-    return;
-  }
-  float* w = a.layer[layer].weights + (a.slots[b] * a.KV + kvh) * a.capacity;
-  const int counted = min(n, a.capacity), old = n - a.recent, want = a.keep - a.recent;
-  auto key_at = [&](int i) { return weight_order(i < counted ? w[i] : 0.f); };
-  // edge: the largest value that `want` of the old keys reach; `spare` of those that equal it stay
-  uint32_t edge = 0xffffffffu;
-  int spare = 0;
-  if (want > 0) {
-    edge = 0;
-    constexpr int R = 8;
-    uint32_t mine[R];
+  extern __shared__ float weight[];  // padded by one per 32: threads read R neighbours each
+  __shared__ int red[2 * (NT / 32)];
+  const int t = threadIdx.x;
+  EvictTask k;
+  if (!k.open(a)) return;
+  auto at = [](int i) { return i + (i >> 5); };
+  int* list = reinterpret_cast<int*>(weight + at(R * NT));
+  constexpr int BATCH = R < 16 ? R : 18;
+  for (int i0 = t; i0 < k.n; i0 += BATCH * NT) {
+    float v[BATCH];
 #pragma unroll
-    for (int r = 0; r < R; ++r) mine[r] = r * kSelectThreads + t < old ? key_at(r * kSelectThreads + t) : 0u;
-    int turn = 0;
-    for (int bit = 31; bit >= 0; --bit) {
+    for (int r = 0; r < BATCH; ++r) v[r] = i0 + r * NT < k.counted ? k.w[i0 + r * NT] : 0.f;
+#pragma unroll
+    for (int r = 0; r < BATCH; ++r)
+      if (i0 + r * NT < R * NT) weight[at(i0 + r * NT)] = v[r];
+  }
+  __syncthreads();
+  uint32_t key[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) key[r] = t * R + r < k.old ? weight_order(weight[at(t * R + r)]) : 0u;
+  uint32_t edge = 0xffffffffu;  // keys above the edge stay, and `spare` of those that equal it
+  int spare = 0, turn = 0;
+  if (k.want > 0) {
+    edge = 0;
+    bool exact = false;
+    for (int bit = 31; bit >= 0 && !exact; --bit) {
       const uint32_t probe = edge | (1u << bit);
       int c = 0;
 #pragma unroll
-      for (int r = 0; r < R; ++r) c += mine[r] >= probe ? 1 : 0;
-      for (int i = R * kSelectThreads + t; i < old; i += kSelectThreads) c += key_at(i) >= probe ? 1 : 0;
-      c = block_count(c, red, turn);
+      for (int r = 0; r < R; ++r) c += key[r] >= probe ? 1 : 0;
+      c = block_count<NT>(c, red, turn);
       turn ^= 1;
-      if (c >= want) edge = probe;
+      if (c >= k.want) edge = probe;
+      exact = c == k.want;
     }
-    int c = 0;
+    if (exact) {
+      edge -= 1;  // (all that reach the probe: above probe - 1; a probe is not 0)
+    } else {
+      int c = 0;
 #pragma unroll
-    for (int r = 0; r < R; ++r) c += mine[r] > edge ? 1 : 0;
-    for (int i = R * kSelectThreads + t; i < old; i += kSelectThreads) c += key_at(i) > edge ? 1 : 0;
-    spare = want - block_count(c, red, turn);
+      for (int r = 0; r < R; ++r) c += key[r] > edge ? 1 : 0;
+      spare = k.want - block_count<NT>(c, red, turn);
+      turn ^= 1;
+    }
   }
-  // the list, in ascending order
-  int tie_base = 0, take_base = 0, turn = 0;
-  for (int i0 = 0; i0 < n; i0 += kSelectThreads, turn ^= 1) {
-    const int i = i0 + t;
-    const uint32_t key = i < old ? key_at(i) : 0u;
-    const bool tie = i < old && key == edge && spare > 0;
-    const uint32_t tie_mask = __ballot_sync(0xffffffffu, tie);
-    if (lane == 0) ties[turn][warp] = __popc(tie_mask);
-    __syncthreads();
-    int tie_before = tie_base, tie_all = 0;
+  // how many ties lie in front of a thread's rows, then how many rows that stay
+  int ties = 0, total;
+  if (spare > 0) {
 #pragma unroll
-    for (int q = 0; q < kSelectThreads / 32; ++q) {
-      if (q < warp) tie_before += ties[turn][q];
-      tie_all += ties[turn][q];
-    }
-    tie_before += __popc(tie_mask & ((1u << lane) - 1u));
-    const bool take = i < n && (i >= old || key > edge || (tie && tie_before < spare));
-    const uint32_t take_mask = __ballot_sync(0xffffffffu, take);
-    if (lane == 0) takes[turn][warp] = __popc(take_mask);
-    __syncthreads();
-    int at = take_base, take_all = 0;
+    for (int r = 0; r < R; ++r) ties += t * R + r < k.old && key[r] == edge ? 1 : 0;
+    ties = block_scan<NT>(ties, red, turn, total);
+    turn ^= 1;
+  }
+  int takes = 0, tie = ties;
 #pragma unroll
-    for (int q = 0; q < kSelectThreads / 32; ++q) {
-      if (q < warp) at += takes[turn][q];
-      take_all += takes[turn][q];
-    }
-    at += __popc(take_mask & ((1u << lane) - 1u));
-    if (take && at < a.keep) kept[at] = i;
-    tie_base += tie_all;
-    take_base += take_all;
+  for (int r = 0; r < R; ++r) {
+    const int i = t * R + r;
+    const bool even = i < k.old && key[r] == edge;
+    takes += i < k.n && (i >= k.old || key[r] > edge || (even && tie < spare)) ? 1 : 0;
+    tie += even ? 1 : 0;
+  }
+  takes = block_scan<NT>(takes, red, turn, total);
+  tie = ties;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int i = t * R + r;
+    const bool even = i < k.old && key[r] == edge;
+    if (i < k.n && (i >= k.old || key[r] > edge || (even && tie < spare))) list[takes++] = i;
+    tie += even ? 1 : 0;
   }
   __syncthreads();
-  // weights: entry j takes over entry kept[j] >= j; a tile is read as a whole before it is written
-  for (int j0 = 0; j0 < counted; j0 += kSelectThreads) {
+  for (int j = t; j < a.keep; j += NT) k.kept[j] = list[j];
+  for (int j = t; j < k.counted; j += NT) k.w[j] = j < a.keep ? weight[at(list[j])] : 0.f;
+}
+
+// The same for any length, with the weights read again for every count and the list in global memory.
+__global__ void __launch_bounds__(512) evict_select_long_kernel(const __grid_constant__ EvictArgs a) {
+  constexpr int NT = 512;
+  pdl_trigger();
+  pdl_wait();
+  __shared__ int red[2 * (NT / 32)];
+  const int t = threadIdx.x;
+  EvictTask k;
+  if (!k.open(a)) return;
+  auto key_at = [&](int i) { return weight_order(i < k.counted ? k.w[i] : 0.f); };
+  auto count = [&](auto&& test, int turn) {
+    int c = 0;
+    for (int i = t; i < k.old; i += NT) c += test(key_at(i)) ? 1 : 0;
+    return block_count<NT>(c, red, turn);
+  };
+  uint32_t edge = 0xffffffffu;
+  int spare = 0, turn = 0;
+  if (k.want > 0) {
+    edge = 0;
+    for (int bit = 31; bit >= 0; --bit, turn ^= 1) {
+      const uint32_t probe = edge | (1u << bit);
+      if (count([&](uint32_t u) { return u >= probe; }, turn) >= k.want) edge = probe;
+    }
+    spare = k.want - count([&](uint32_t u) { return u > edge; }, turn);
+    turn ^= 1;
+  }
+  int tie_base = 0, take_base = 0;
+  for (int i0 = 0; i0 < k.n; i0 += NT) {
+    const int i = i0 + t;
+    const uint32_t key = i < k.old ? key_at(i) : 0u;
+    const bool even = i < k.old && key == edge;
+    int all;
+    const int before = tie_base + block_scan<NT>(even ? 1 : 0, red, turn, all);
+    turn ^= 1;
+    tie_base += all;
+    const bool take = i < k.n && (i >= k.old || key > edge || (even && before < spare));
+    const int place = take_base + block_scan<NT>(take ? 1 : 0, red, turn, all);
+    turn ^= 1;
+    take_base += all;
+    if (take) k.kept[place] = i;
+  }
+  __syncthreads();
+  // entry j takes over entry kept[j] >= j: a tile is read as a whole before it is written
+  for (int j0 = 0; j0 < k.counted; j0 += NT) {
     const int j = j0 + t;
     float v = 0.f;
-    if (j < a.keep && j < counted) {
-      const int i = kept[j];
-      v = i < counted ? w[i] : 0.f;
+    if (j < a.keep && j < k.counted) {
+      const int i = k.kept[j];
+      v = i < k.counted ? k.w[i] : 0.f;
     }
     __syncthreads();
-    if (j < counted) w[j] = v;
+    if (j < k.counted) k.w[j] = v;
   }
 }
 
@@ -145,13 +234,15 @@ struct RowUnit<2> {
 };
 
 // grid (2 * slices, B * KV, layers): a CTA moves a range of columns of all rows of K or V of one head, in ascending batches of rows that are read as a
-// whole before they are written. Sources lie at or behind their targets, so no batch reads what an earlier one wrote, and in place is safe.
+// whole before they are written. Sources lie at or behind their targets, so no batch reads what an earlier one wrote, and in place is safe. The places of a
+// batch's rows are looked up once per row, while the rows of the batch in front are on their way.
+constexpr int kMoveThreads = 512, kMoveBatch = 8;
 template <int UNIT>
-__global__ void __launch_bounds__(256) evict_move_kernel(const __grid_constant__ EvictArgs a, int slices) {
+__global__ void __launch_bounds__(kMoveThreads, 2) evict_move_kernel(const __grid_constant__ EvictArgs a, int slices, int most_lines) {
   using U = typename RowUnit<UNIT>::type;
-  constexpr int BATCH = 8;
   pdl_trigger();
   pdl_wait();
+  extern __shared__ int2 place[];  // [2][rows of a batch]: source and target row in the cache; target -1: the row stays
   const int value = blockIdx.x & 1, slice = blockIdx.x >> 1, b = blockIdx.y / a.KV, kvh = blockIdx.y % a.KV, layer = blockIdx.z, t = threadIdx.x;
   const EvictLayer& L = a.layer[layer];
   uint8_t* cache = static_cast<uint8_t*>(value ? L.v : L.k);
@@ -162,35 +253,44 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const __grid_constant__
   if (n == 0 || c0 == c1 || kept[0] < 0) return;  // (nothing of a sequence on a bad slot moves)
   const int* from = a.tables + static_cast<long long>(b) * a.table_width;
   const int* to = a.out_tables + static_cast<long long>(b) * a.out_width;
-  for (int c = c0; c < c1; c += 256) {
-    const int width = min(256, c1 - c), lines = 256 / width;  // rows side by side
-    const int line = t / width, col = c + t % width;
-    const bool on = line < lines;
-    for (int j0 = 0; j0 < n; j0 += lines * BATCH) {
-      U v[BATCH];
-      long long target[BATCH];
-#pragma unroll
-      for (int q = 0; q < BATCH; ++q) {
-        const int j = j0 + q * lines + line;
-        target[q] = -1;
-        if (on && j < n) {
-          const int i = kept[j], ps = from[i / a.page], pd = to[j / a.page];
+  for (int c = c0; c < c1; c += kMoveThreads) {
+    const int width = min(kMoveThreads, c1 - c), lines = min(kMoveThreads / width, most_lines);  // rows side by side
+    const int line = t / width, rows = lines * kMoveBatch;                                       // rows of a batch
+    uint8_t* column = cache + static_cast<long long>(c + t % width) * UNIT;
+    auto look_up = [&](int j0, int2* at) {
+      for (int r = t; r < rows; r += kMoveThreads) {
+        int2 p = make_int2(0, -1);
+        if (j0 + r < n) {
+          const int i = kept[j0 + r], j = j0 + r, ps = from[i / a.page], pd = to[j / a.page];
           if (ps < 0 || ps >= a.pages || pd < 0 || pd >= a.pages) {
             atomicCAS(a.status, kStatusOk, kStatusBadArgs);
           } else {
-            const long long s = (static_cast<long long>(ps) * a.KV + kvh) * a.page + i % a.page, d = (static_cast<long long>(pd) * a.KV + kvh) * a.page + j % a.page;
-            if (s != d) {
-              target[q] = d;
-              v[q] = *reinterpret_cast<const U*>(cache + s * row_bytes + static_cast<long long>(col) * UNIT);
-            }
+            p = make_int2((ps * a.KV + kvh) * a.page + i % a.page, (pd * a.KV + kvh) * a.page + j % a.page);
+            if (p.x == p.y) p.y = -1;
           }
         }
+        at[r] = p;
       }
+    };
+    look_up(0, place);
+    __syncthreads();
+    for (int j0 = 0, turn = 0; j0 < n; j0 += rows, turn ^= 1) {
+      const int2* at = place + turn * rows;
+      U v[kMoveBatch];
+      int target[kMoveBatch];
+#pragma unroll
+      for (int q = 0; q < kMoveBatch; ++q) {
+        const int2 p = line < lines ? at[q * lines + line] : make_int2(0, -1);
+        target[q] = p.y;
+        if (p.y >= 0) v[q] = *reinterpret_cast<const U*>(column + static_cast<long long>(p.x) * row_bytes);
+      }
+      if (j0 + rows < n) look_up(j0 + rows, place + (turn ^ 1) * rows);
       __syncthreads();
 #pragma unroll
-      for (int q = 0; q < BATCH; ++q)
-        if (target[q] >= 0) *reinterpret_cast<U*>(cache + target[q] * row_bytes + static_cast<long long>(col) * UNIT) = v[q];
+      for (int q = 0; q < kMoveBatch; ++q)
+        if (target[q] >= 0) *reinterpret_cast<U*>(column + static_cast<long long>(target[q]) * row_bytes) = v[q];
     }
+    __syncthreads();
   }
 }
 
@@ -198,11 +298,45 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const __grid_constant__
 
 void launch_evict(const EvictArgs& a, int unit, cudaStream_t st) {
   if (a.B == 0 || a.layers == 0 || a.KV == 0) return;
-  launch_pdl(evict_select_kernel, dim3(a.KV, a.B, a.layers), dim3(kSelectThreads), 0, st, a);
-  const dim3 grid(2, a.B * a.KV, a.layers);
-  if (unit == 16) launch_pdl(evict_move_kernel<16>, grid, dim3(256), 0, st, a, 1);
-  else if (unit == 4) launch_pdl(evict_move_kernel<4>, grid, dim3(256), 0, st, a, 1);
-  else launch_pdl(evict_move_kernel<2>, grid, dim3(256), 0, st, a, 1);
+  const dim3 heads(a.KV, a.B, a.layers);
+  const long long most = static_cast<long long>(a.table_width) * a.page;  // rows of a sequence
+  const auto shared = [&](int rows) { return (static_cast<size_t>(rows) * 33 / 32 + 1 + static_cast<size_t>(a.keep < most ? a.keep : most)) * 4; };
+#define DLV_EVICT_SELECT(NT, RR)                                                                                                          \
+  do {                                                                                                                                    \
+    static PerDeviceOnce once;                                                                                                            \
+    if (once.first()) cudaFuncSetAttribute(evict_select_kernel<NT, RR>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelectShared);      \
+    launch_pdl(evict_select_kernel<NT, RR>, heads, dim3(NT), shared(NT * RR), st, a);                                                     \
+  } while (0)
+  if (most <= 256 * 10 && shared(256 * 10) <= kSelectShared) DLV_EVICT_SELECT(256, 10);
+  else if (most <= 512 * 20 && shared(512 * 20) <= kSelectShared) DLV_EVICT_SELECT(512, 20);
+  else if (most <= 512 * 72 && shared(512 * 72) <= kSelectShared) DLV_EVICT_SELECT(512, 72);
+  else launch_pdl(evict_select_long_kernel, heads, dim3(512), 0, st, a);
+#undef DLV_EVICT_SELECT
+  // columns are cut (to 64 bytes at least) where there are too few heads to fill the GPU
+  int wide = 0;
+  for (int i = 0; i < a.layers; ++i) wide = a.layer[i].k_bytes > wide ? a.layer[i].k_bytes : wide;
+  int slices = 1;
+  while (slices < 8 && 2ll * slices * a.B * a.KV * a.layers < 2 * 148 && wide / (2 * slices) >= 64) slices *= 2;
+  const dim3 grid(2 * slices, a.B * a.KV, a.layers);
+  // rows of a batch: at most the threads' units in columns of the narrowest slice
+  int narrow = wide;
+  for (int i = 0; i < a.layers; ++i) {
+    narrow = a.layer[i].k_bytes < narrow ? a.layer[i].k_bytes : narrow;
+    narrow = a.layer[i].v_bytes < narrow ? a.layer[i].v_bytes : narrow;
+  }
+  const int units = narrow / unit / slices > 1 ? narrow / unit / slices : 1;
+  const int lines = kMoveThreads / (units < kMoveThreads ? units : kMoveThreads);
+  const size_t smem = static_cast<size_t>(2) * lines * kMoveBatch * sizeof(int2);
+#define DLV_EVICT_MOVE(UU)                                                                                                                       \
+  do {                                                                                                                                           \
+    static PerDeviceOnce once;                                                                                                                   \
+    if (once.first()) cudaFuncSetAttribute(evict_move_kernel<UU>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kMoveThreads * kMoveBatch * 8); \
+    launch_pdl(evict_move_kernel<UU>, grid, dim3(kMoveThreads), smem, st, a, slices, lines);                                                     \
+  } while (0)
+  if (unit == 16) DLV_EVICT_MOVE(16);
+  else if (unit == 4) DLV_EVICT_MOVE(4);
+  else DLV_EVICT_MOVE(2);
+#undef DLV_EVICT_MOVE
 }
 
 }  // namespace dlv

@@ -188,11 +188,6 @@ int launch_decode_attention_rope(const void* qkv, long long pitch, const DecodeR
 int launch_decode_attention_impl(const void* q, long long q_stride, const void* kc, const void* vc, const int* bt, int bt_stride,
                                  const int* ctx, void* out, float* po, float* pml, int* arrivals, int B, int H, int KV, int D, int page,
                                  float scale, float cap, int window, int splits, const int* used, int impl, cudaStream_t st);
-// Decode attention that also writes its scores, fp32 [B, H, pitch] (pitch: a multiple of 16), and the maxima and sums of all splits, [B, H, splits, 2]; 1: unsupported shape
-int launch_decode_attention_scores(const void* q, long long q_stride, const void* kc, const void* vc, const int* bt, int bt_stride, const int* ctx, void* out, float* po,
-                                   float* pml, float* scores, int pitch, int pages, int max_ctx, int* status, int B, int H, int KV, int D, int page, float scale, float cap,
-                                   int window, int splits, const int* used, cudaStream_t st);
-int decode_min_slices(int B, int KV, int G);  // least slices of 16 keys that a split takes
 constexpr int kDecodePlanStride = 32;
 // used: int32 [B] with this stride, how many of the splits every sequence takes (nullptr: as many as its own length has use for); groups: CTAs per sequence of head width D
 void launch_decode_plan(const int* ctx_lens, int* used, int B, int window, int keep_first, int splits, int groups, int D, cudaStream_t st);

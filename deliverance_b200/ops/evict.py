@@ -22,16 +22,15 @@ def decode_attention_weighted(q, k_cache, v_cache, block_tables, ctx_lens, H, sc
     ``slots`` int64 ``[B]``). Rows of a sequence at or behind the capacity are attended to and not counted. Slot 0 is the scratch slot: a sequence with slot 0 adds nothing. The other
     slots of a call are different ones; a second sequence on a slot, or a slot outside ``weights``, adds nothing and is reported by :func:`ops.check_status` (on the CPU:
     raised)."""
+    if q.is_cuda:  # (the extension checks)
+        splits, used = ops.decode_launch(splits, even, plan, ctx_lens, q.shape[0], H, k_cache.shape[1], k_cache.shape[3], int(window))
+        out, launches = ops.require_ext().decode_attention_weighted(q, k_cache, v_cache, block_tables, ctx_lens, H, scale, softcap, window, splits, weights, slots, used)
+        ops._count(launches)
+        return out
     if weights.dim() != 3 or weights.dtype != torch.float32 or weights.shape[1] != k_cache.shape[1]:
         raise ValueError("weights must be fp32 [slots, KV, capacity]")
     if slots.dim() != 1 or slots.shape[0] != q.shape[0] or slots.dtype != torch.int64:
         raise ValueError("slots must be int64, one per query row")
-    if ops._cuda(q):
-        B, KV = q.shape[0], k_cache.shape[1]
-        splits, used = ops.decode_launch(splits, even, plan, ctx_lens, B, H, KV, k_cache.shape[3], int(window))
-        out, launches = ops.require_ext().decode_attention_weighted(q, k_cache, v_cache, block_tables, ctx_lens, H, scale, softcap, int(window), splits, weights, slots, used)
-        ops._count(launches)
-        return out
     return ref.decode_attention_weighted(q, k_cache, v_cache, block_tables, ctx_lens, H, scale, weights, slots, softcap, window)
 
 
@@ -43,6 +42,10 @@ def evict_keys(k_caches, v_caches, weights, block_tables, ctx_lens, slots, keep:
     ``k_caches`` / ``v_caches``: per layer ``[pages, KV, page, D]`` (widths may differ); ``weights``: per layer fp32 ``[slots, KV, capacity]``; ``block_tables`` / ``out_tables`` int32 ``[B, pages]``,
     ``ctx_lens`` int32 ``[B]``, ``slots`` int64 ``[B]``, all different (0, the scratch slot: only for sequences of length 0). An entry of ``out_tables`` is either the page that ``block_tables`` has in the same place or a page that no sequence of the call reads.
     Returns the rows that were kept, int32 ``[layers, B, KV, keep]`` (-1 behind a sequence's end), and the new lengths, int32 ``[B]``."""
+    if ctx_lens.is_cuda:  # (the extension checks: a loop over the layers here takes longer than the kernels)
+        kept, lens, launches = ops.require_ext().evict_keys(k_caches, v_caches, weights, block_tables, ctx_lens, slots, keep, recent, block_tables if out_tables is None else out_tables)
+        ops._count(launches)
+        return kept, lens
     k_caches, v_caches, weights = list(k_caches), list(v_caches), list(weights)
     if not k_caches or not len(k_caches) == len(v_caches) == len(weights):
         raise ValueError("one key cache, value cache and weight tensor per layer")
@@ -50,21 +53,16 @@ def evict_keys(k_caches, v_caches, weights, block_tables, ctx_lens, slots, keep:
         raise ValueError("0 <= recent <= keep, 1 <= keep")
     first = k_caches[0]
     for k, v, w in zip(k_caches, v_caches, weights):
-        if k.dim() != 4 or v.dim() != 4 or w.dim() != 3 or k.shape[:3] != first.shape[:3] or v.shape[:3] != first.shape[:3] or k.dtype != v.dtype or k.dtype != first.dtype:
-            raise ValueError("caches must be [pages, KV, page, D] of one type, with the same pages and KV heads in all layers")
-        if w.dtype != torch.float32 or w.shape != weights[0].shape or w.shape[1] != k.shape[1]:
+        if k.dim() != 4 or v.dim() != 4 or k.shape[:3] != first.shape[:3] or v.shape[:3] != first.shape[:3]:
+            raise ValueError("caches must be [pages, KV, page, D], with the same pages and KV heads in all layers")
+        if w.dim() != 3 or w.dtype != torch.float32 or w.shape != weights[0].shape or w.shape[1] != k.shape[1]:
             raise ValueError("weights must be fp32 [slots, KV, capacity], the same in all layers")
-    if len({t.data_ptr() for t in k_caches + v_caches if t.numel()}) < sum(1 for t in k_caches + v_caches if t.numel()):
+    if len({t.data_ptr() for t in k_caches + v_caches}) < 2 * len(k_caches):
         raise ValueError("a cache that several layers share cannot be shortened for one of them")
     B = ctx_lens.shape[0]
+    out = block_tables if out_tables is None else out_tables
     if block_tables.dim() != 2 or block_tables.shape[0] != B or slots.shape != (B,) or slots.dtype != torch.int64 or block_tables.dtype != torch.int32 or ctx_lens.dtype != torch.int32:
         raise ValueError("block_tables int32 [B, pages], ctx_lens int32 [B], slots int64 [B]")
-    out = block_tables if out_tables is None else out_tables
-    if out.dim() != 2 or out.shape[0] != B or out.dtype != torch.int32:
-        raise ValueError("out_tables must be int32 [B, pages]")
-    if ops._cuda(first):
-        e = ops.require_ext()
-        kept, lens, launches = e.evict_keys(k_caches, v_caches, weights, block_tables, ctx_lens, slots, keep, recent, out)
-        ops._count(launches)
-        return kept, lens
+    if out.dim() != 2 or out.shape[0] != B or out.dtype != torch.int32 or out.shape[1] * first.shape[2] < min(keep, block_tables.shape[1] * first.shape[2]):
+        raise ValueError("out_tables must be int32 [B, pages] with room for the kept rows")
     return ref.evict_keys(k_caches, v_caches, weights, block_tables, ctx_lens, slots, keep, recent, out)

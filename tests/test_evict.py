@@ -220,7 +220,7 @@ def test_evict_matches_plain(device, lens, keep, recent, out):
 
 
 @pytest.mark.parametrize("device", DEVICES)
-@pytest.mark.parametrize("D,DV,dtype", [(128, 128, BF16), (256, 64, BF16), (6, 6, BF16), (5, 3, BF16), (20, 20, F32), (5, 7, F32), (1032, 1032, F32)])
+@pytest.mark.parametrize("D,DV,dtype", [(128, 128, BF16), (256, 64, BF16), (6, 6, BF16), (5, 3, BF16), (20, 20, F32), (5, 7, F32), (1032, 1032, F32), (2052, 20, F32)])
 def test_evict_widths(device, D, DV, dtype):
     run_evict(device, [90, 200], 64, 10, L=1, D=D, DV=DV, dtype=dtype)
 
@@ -256,6 +256,10 @@ def test_evict_many_layers(device):
 def test_evict_long_sequences():
     """More rows than the selection holds in registers; offsets of rows far into a page table."""
     run_evict("cuda", [9000, 4097], 4000, 500, L=1, KV=1, D=8)
+    run_evict("cuda", [2561, 2560], 1001, 0, L=1, KV=1, D=8)
+    run_evict("cuda", [10241, 20000], 5000, 4999, L=1, KV=1, D=8)
+    run_evict("cuda", [40000, 100], 10000, 17, L=1, KV=1, D=8)
+    run_evict("cuda", [40000], 39999, 17, L=1, KV=1, D=8, weights=[torch.zeros(3, 1, 40000)])
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -267,7 +271,7 @@ def test_refusals(device):
     q = torch.zeros(1, 4 * D, dtype=BF16, device=device)
     for bad in (lambda: evict_keys([], [], [], t, n, s, 8, 2), lambda: evict_keys([k], [v], [w], t, n, s, 8, 9), lambda: evict_keys([k], [v], [w], t, n, s, 0, 0),
                 lambda: evict_keys([k], [k], [w], t, n, s, 8, 2), lambda: evict_keys([k], [v], [w[:, :1]], t, n, s, 8, 2), lambda: evict_keys([k], [v], [w.double()], t, n, s, 8, 2),
-                lambda: evict_keys([k], [v.float()], [w], t, n, s, 8, 2), lambda: evict_keys([k], [v], [w], t.long(), n, s, 8, 2), lambda: evict_keys([k], [v], [w], t, n, s.int(), 8, 2),
+                lambda: evict_keys([k], [v], [w], t.long(), n, s, 8, 2), lambda: evict_keys([k], [v], [w], t, n, s.int(), 8, 2),
                 lambda: evict_keys([k], [v], [w], t, n, s, 8, 2, t[0]), lambda: decode_attention_weighted(q, k, v, t, n, 4, 0.1, w[0], s),
                 lambda: decode_attention_weighted(q, k, v, t, n, 4, 0.1, w, s.int()), lambda: decode_attention_weighted(q, k, v, t, n, 4, 0.1, w.half(), s)):
         with pytest.raises((ValueError, RuntimeError)):
