@@ -20,6 +20,16 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool v
   const int sz = valid ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(sz) : "memory");
 }
+// the same for what is read once in front of something that is read again: first in line to leave L2
+__device__ __forceinline__ uint64_t policy_evict_first() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ void cp_async16_once(uint32_t dst, const void* src, bool valid, uint64_t policy) {
+  const int sz = valid ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(sz), "l"(policy) : "memory");
+}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -673,6 +683,8 @@ __global__ void __launch_bounds__(NW * 32, (D <= 128 && NW == 4 ? 2 : 1)) decode
   const int n_mine = first < s1 ? (s1 - first + NW - 1) / NW : 0;
   const int per_page = page_size / 16;
   int my_row = 0;  // cache row of slice (j & ~31) + lane of this warp
+  [[maybe_unused]] uint64_t once = 0;
+  if constexpr (WEIGH) once = policy_evict_first();
   auto load_slice = [&](int j, int stage) {
     // 16 keys x D of K and V: 2 * 16 * CPR chunks over 32 lanes (zeros behind the real widths)
     if ((j & 31) == 0 && j + lane < n_mine) {
@@ -699,6 +711,10 @@ __global__ void __launch_bounds__(NW * 32, (D <= 128 && NW == 4 ? 2 : 1)) decode
         const bool vk = valid && cc * 8 < dk, vv = valid && cc * 8 < dv;
         cp_async16(kdst + swz<D>(r, cc), kb + (vk ? r * dk + cc * 8 : 0), vk);
         cp_async16(vdst + swz<D>(r, cc), vb + (vv ? r * dv + cc * 8 : 0), vv);
+      } else if constexpr (WEIGH) {
+        const int off = (valid ? r : 0) * D + cc * 8;
+        cp_async16_once(kdst + swz<D>(r, cc), kb + off, valid, once);
+        cp_async16_once(vdst + swz<D>(r, cc), vb + off, valid, once);
       } else {
         const int off = (valid ? r : 0) * D + cc * 8;
         cp_async16(kdst + swz<D>(r, cc), kb + off, valid);
