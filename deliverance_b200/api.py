@@ -14,6 +14,7 @@ import logging
 import os
 import uuid
 from dataclasses import dataclass, field
+from types import SimpleNamespace
 from typing import Callable, Optional
 
 import torch
@@ -208,6 +209,10 @@ class CausalLanguageModel:
         return gen
 
     def generate(self, prompt, params: Optional[GeneratorParameters] = None, on_event=None, session: Optional[str] = None) -> Response:
+        if params is not None and params.num_beams > 1:
+            if on_event is not None:
+                raise ValueError("beam search has no token events")
+            return self.generate_beams(prompt, params)[0]
         gen = self.submit(prompt, params, on_event, session)
         self.engine.run([gen.request])
         return gen.finish()
@@ -215,9 +220,29 @@ class CausalLanguageModel:
     def generate_many(self, prompts: list, params: Optional[GeneratorParameters] = None) -> list[Response]:
         import copy
 
+        if params is not None and params.num_beams > 1:
+            return [self.generate(p, params) for p in prompts]
         gens = [self.submit(p, copy.deepcopy(params) if params else None) for p in prompts]
         self.engine.run([g.request for g in gens])
         return [g.finish() for g in gens]
+
+    def generate_beams(self, prompt, params: GeneratorParameters) -> list[Response]:
+        """``params.num_beams`` answers of a beam search, best first (``Response.score``)."""
+        if getattr(prompt, "has_tools", False):
+            raise ValueError("beam search does not combine with tools")
+        if isinstance(prompt, PromptContext):
+            prompt = prompt.prompt
+        ids = self.encode_prompt(prompt) if isinstance(prompt, str) else [int(t) for t in prompt]
+        out = []
+        for r in self.engine.generate_beams([ids], params)[0]:
+            gen = Generation(self, params, None, "", False)
+            gen.starts_in_reasoning = isinstance(prompt, str) and prompt_ends_inside_reasoning(prompt)
+            for token in r.token_ids:
+                gen.detok_special.push(token)
+                gen.detok_plain.push(token)
+            gen.request = SimpleNamespace(response=lambda r=r: r)
+            out.append(gen.finish())
+        return out
 
     def close(self) -> None:
         pass

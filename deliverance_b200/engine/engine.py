@@ -20,6 +20,7 @@ import torch
 from .. import ops
 from ..kv.paged import KvCacheSettings, PagedKVCache, compose_salt
 from ..models.batch import ForwardBatch, make_batch
+from ..ops.evict import evict_keys
 from ..params import FinishReason, GeneratorParameters, Response, TokenLogProb
 from .sampler import Sampler, SamplingState
 
@@ -58,6 +59,9 @@ class Request:
     resumed: bool = False  # re-admitted after a preemption: the prefill only rebuilds the cache, nothing is sampled from it
     preemptions: int = 0
     replay: bool = False  # tokens are given step by step (Engine.replay_step), the scheduler leaves it alone
+    evicted: int = 0  # rows dropped from a bounded cache: the cache row of position p is p - evicted
+    weight_slot: int = -1  # its row of key weights
+    observed: int = 0  # decode steps whose attention its weights hold
     t_progress: float = 0.0
 
     def __post_init__(self):
@@ -111,6 +115,13 @@ class Engine:
         self.special_ids = frozenset(special_ids)
         self.sampler = Sampler(decode_token)
         layout = model.kv_layout()
+        kvs = self.config.kv
+        self.bounded = kvs.keep_tokens > 0  # sequences are shortened while they decode
+        if self.bounded:
+            if not 0 <= kvs.keep_recent <= kvs.keep_tokens or kvs.keep_every < 1 or 0 < kvs.keep_capacity <= kvs.keep_tokens:
+                raise ValueError("a bounded cache needs 0 <= keep_recent <= keep_tokens, keep_every >= 1 and keep_capacity > keep_tokens (or 0)")
+            if not getattr(model, "supports_key_weights", lambda: False)():
+                raise ValueError("this model's cache cannot be bounded: it needs attention over all cached rows in every layer")
         pages = self.config.num_pages or self._auto_pages(layout)
         tp = getattr(model, "tp", None)
         if self.config.num_pages is None and tp is not None and tp.enabled and tp.collectives is not None:
@@ -119,7 +130,8 @@ class Engine:
             mine = torch.tensor([float(pages)], dtype=torch.float32, device=self.device)
             pages = int(min(float(t.item()) for t in tp.collectives.all_gather(mine)))
         self.hybrid = any(layout.get("state_shapes") or [])  # recurrent layers: every sequence holds a state slot
-        self.kv = PagedKVCache(layout, pages, self.device, model.dtype, self.config.kv, self._state_slots(layout))
+        self.kv = PagedKVCache(layout, pages, self.device, model.dtype, self.config.kv, self._state_slots(layout), self.config.max_seqs if self.bounded else 0,
+                               self._weight_capacity())
         self.page_size = self.kv.page_size
         self.max_pages_per_seq = (self.cfg.max_position_embeddings + self.page_size - 1) // self.page_size
         self.waiting: list[Request] = []
@@ -144,11 +156,18 @@ class Engine:
     def _state_slots(self, layout) -> int:
         return (self.config.max_state_slots or self.config.max_seqs) if any(layout.get("state_shapes") or []) else 0
 
+    def _weight_capacity(self) -> int:
+        """Rows of a sequence that have a weight."""
+        n = self.config.kv.keep_capacity or self.cfg.max_position_embeddings
+        return (min(n, self.cfg.max_position_embeddings) + 31) // 32 * 32 if self.bounded else 0
+
     def _auto_pages(self, layout) -> int:
         per = max(1, PagedKVCache.bytes_per_page(layout, self.config.kv.block_size, self.model.dtype))
         if self.device.type == "cuda":
             free, _ = torch.cuda.mem_get_info(self.device)
             free -= (1 + self._state_slots(layout)) * PagedKVCache.bytes_per_state_slot(layout)
+            if self.bounded:
+                free -= 4 * len(layout["layer_kinds"]) * (1 + self.config.max_seqs) * layout["kv_heads"] * self._weight_capacity()
             budget = int(max(0, free) * self.config.kv_memory_fraction)
             # enough for max_seqs full contexts, never more than the budget
             want = self.config.max_seqs * ((self.cfg.max_position_embeddings + self.config.kv.block_size - 1) // self.config.kv.block_size) + 1
@@ -160,6 +179,15 @@ class Engine:
                     stopper=None) -> Request:
         params = params or GeneratorParameters()
         params.validate()
+        if params.num_beams > 1:
+            raise ValueError("beam search runs through Engine.generate, generate_batch or generate_beams")
+        r = self._new_request(prompt, params, on_token)
+        r.guide = guide
+        r.stopper = stopper
+        self.waiting.append(r)
+        return r
+
+    def _new_request(self, prompt: list[int], params: GeneratorParameters, on_token=None) -> Request:
         ctx = self.cfg.max_position_embeddings
         limit = min(params.ntokens or ctx, ctx)
         if len(prompt) == 0:
@@ -173,13 +201,10 @@ class Engine:
         r = Request(self._next_id, [int(t) for t in prompt], params, on_token)
         self._next_id += 1
         r.sampling = SamplingState.create(params, self.special_ids)
-        r.guide = guide
-        r.stopper = stopper
         r.limit = limit
         r.t_submit = time.perf_counter()
         r.salt = compose_salt(params.cache_salt, params.lora_adapter or getattr(self.model, "active_lora", None),
                               self.model.tp.rank, self.model.tp.size)
-        self.waiting.append(r)
         return r
 
     def abort(self, r: Request, reason: FinishReason = FinishReason.CANCELLED) -> None:
@@ -204,6 +229,8 @@ class Engine:
             if not self.kv.free_slots:
                 return False
             r.state_slot = self.kv.alloc_state_slot()
+        if self.bounded:  # (as many rows as places)
+            r.weight_slot, r.observed = self.kv.alloc_weight_slot(), 0
         # Recurrent (conv / SSM) state is not idempotent: a snapshot taken after L tokens may only be resumed at token L. A hit
         # that covers the whole prompt would have to replay the last token on a state that already absorbed it, so hybrid
         # models only take checkpoints strictly shorter than the prompt and prefill the remainder from the restored state.
@@ -226,10 +253,17 @@ class Engine:
         r.t_done = time.perf_counter()
         if r in self.running:
             self.running.remove(r)
+        self._release(r)
+
+    def _release(self, r: Request) -> None:
+        """Give back what a request holds of the cache."""
         self.kv.release_pages(r.pages)
         if r.state_slot >= 0:
             self.kv.free_state_slot(r.state_slot)
             r.state_slot = -1
+        if r.weight_slot >= 0:
+            self.kv.free_weight_slot(r.weight_slot)
+            r.weight_slot = -1
 
     # ------------------------------------------------------------------------------------------------ memory pressure
     def _preempt(self, v: Request) -> None:
@@ -237,11 +271,8 @@ class Engine:
         rebuilds its cache by prefilling prompt + generated tokens (recompute; its own prompt is usually a prefix-cache hit).
         Sampling state, guide, stop detector and the tokens produced so far stay with the request, so its output is unchanged."""
         self.running.remove(v)
-        self.kv.release_pages(v.pages)
-        if v.state_slot >= 0:
-            self.kv.free_state_slot(v.state_slot)
-            v.state_slot = -1
-        v.state, v.computed, v.state_snapshots = WAITING, 0, {}
+        self._release(v)
+        v.state, v.computed, v.state_snapshots, v.evicted = WAITING, 0, {}, 0
         v.resumed = bool(v.output)
         v.fill = v.prompt + v.output[:-1] if v.output else v.prompt
         v.preemptions += 1
@@ -276,7 +307,7 @@ class Engine:
             fused.scatter = None
 
     def _new_pages(self, r: Request, n_tokens: int) -> int:
-        return max(0, (n_tokens + self.page_size - 1) // self.page_size - len(r.pages))
+        return max(0, (n_tokens - r.evicted + self.page_size - 1) // self.page_size - len(r.pages))
 
     def _reserve(self, r: Request, n_tokens: int) -> bool:
         """Pages for the first ``n_tokens`` positions of ``r``. Under pressure, requests admitted after ``r`` are preempted
@@ -358,7 +389,8 @@ class Engine:
         return finished
 
     # ------------------------------------------------------------------------------------------------ prefill
-    def _prefill_step(self, reqs: list[Request]) -> Optional[list]:
+    def _prefill_step(self, reqs: list[Request], take=None) -> Optional[list]:
+        """One batch of prompt portions. ``take(requests, logits)``: what is done with those whose prompt is complete (default: sample)."""
         budget = self.config.max_batch_tokens
         seqs, chosen = [], []
         for r in reqs:
@@ -404,7 +436,7 @@ class Engine:
         finished = []
         if done_reqs:
             sub = logits.index_select(0, torch.tensor(done_rows, device=logits.device)) if len(done_rows) != logits.shape[0] else logits
-            finished = self._sample_and_advance(done_reqs, sub)
+            finished = (take or self._sample_and_advance)(done_reqs, sub)
         return finished
 
     def _portion(self, r: Request, n: int) -> dict:
@@ -484,16 +516,64 @@ class Engine:
     # ------------------------------------------------------------------------------------------------ decode
     def _decode_inputs(self, reqs: list[Request]):
         seqs = []
+        if self.bounded:
+            self._shorten(reqs)
         for r in reqs:
             pos = r.total_len - 1 + r.pending  # position of the token being fed (the last sampled one)
-            self.kv.ensure_pages(r.pages, pos + 1)
+            self.kv.ensure_pages(r.pages, pos + 1 - r.evicted)
             seqs.append({"tokens": [r.output[-1] if r.output else 0], "start": pos, "pages": r.pages, "state_slot": max(r.state_slot, 0),
-                         "rid": (r.rid, r.preemptions)})
+                         "rid": (r.rid, r.preemptions, r.evicted)})
+            if self.bounded:
+                seqs[-1]["cached"], seqs[-1]["key_slot"] = pos - r.evicted, r.weight_slot
+                r.observed += 1
             if self.needs_prev:
                 # the token in front of the one being fed: with a step in flight that is the newest token the host knows
                 before = len(r.output) - (1 if r.pending == 0 else 0)
                 seqs[-1]["prev"] = r.output[before - 1] if before > 0 else r.prompt[-1]
         return seqs
+
+    def _shorten(self, reqs: list[Request]) -> None:
+        """Bounded cache: sequences that hold more than ``keep_tokens`` rows and have been observed long enough (or have no weights left) drop the rows that had the
+        least attention. Their own pages are filled from the front; a page that others hold too (cached prefixes) is replaced by a new one, or, where
+        there is none, the sequence waits. Launched behind the step in flight and in front of the next one."""
+        s, ps = self.config.kv, self.page_size
+        keep, cap = s.keep_tokens, self.kv.key_weights[0].shape[2]
+        due, targets = [], []
+        for r in reqs:
+            rows = r.total_len - 1 + r.pending - r.evicted
+            if rows <= keep or (r.observed < s.keep_every and rows < cap):
+                continue
+            n = (keep + ps - 1) // ps
+            shared = [i for i in range(n) if self.kv.allocator.ref[r.pages[i]] > 1]
+            if shared and not self.kv.can_allocate(len(shared)):
+                continue
+            fresh: list[int] = []
+            self.kv.ensure_pages(fresh, len(shared) * ps)
+            target = r.pages[:n]
+            for i, p in zip(shared, fresh):
+                target[i] = p
+            due.append((r, rows))
+            targets.append(target)
+        if not due:
+            return
+        table = torch.zeros(len(due), max((rows + ps - 1) // ps for _, rows in due), dtype=torch.int32)
+        out = torch.zeros(len(due), max(len(t) for t in targets), dtype=torch.int32)
+        for i, ((r, rows), target) in enumerate(zip(due, targets)):
+            n = (rows + ps - 1) // ps
+            table[i, :n] = torch.tensor(r.pages[:n], dtype=torch.int32)
+            out[i, : len(target)] = torch.tensor(target, dtype=torch.int32)
+        dev = self.device
+        evict_keys(self.kv.k, self.kv.v, self.kv.key_weights, table.to(dev), torch.tensor([rows for _, rows in due], dtype=torch.int32).to(dev),
+                   torch.tensor([r.weight_slot for r, _ in due], dtype=torch.int64).to(dev), keep, s.keep_recent, out.to(dev))
+        for (r, rows), target in zip(due, targets):
+            for p in r.pages:
+                if p not in target:
+                    self.kv.allocator.release(p)
+            r.pages[:] = target
+            r.evicted += rows - keep
+            r.observed = 0
+        self.metrics["evictions"] = self.metrics.get("evictions", 0) + len(due)
+        self.metrics["evicted_rows"] = self.metrics.get("evicted_rows", 0) + sum(rows - keep for _, rows in due)
 
     def _plain_greedy(self, reqs: list[Request]) -> bool:
         return all(r.guide is None and r.sampling.greedy and not r.params.logprobs for r in reqs)
@@ -626,7 +706,8 @@ class Engine:
     def _graph_decode(self, seqs: list[dict], dev_tokens: Optional[torch.Tensor] = None) -> torch.Tensor:
         B = len(seqs)
         bucket = next(b for b in _BUCKETS if b >= B)
-        even = self._even([s["start"] + 1 for s in seqs] + [1] * (bucket - B))
+        rows = [s.get("cached", s["start"]) for s in seqs]  # cache rows of the new keys
+        even = self._even([p + 1 for p in rows] + [1] * (bucket - B))
         g = self._graphs.get(bucket if even else -bucket)
         if g is None:
             g = self._capture(bucket, even)
@@ -642,8 +723,8 @@ class Engine:
         starts = [s["start"] for s in seqs]
         h["tok"][:n] = torch.tensor([s["tokens"][0] for s in seqs], dtype=torch.int32)
         h["pos"][:n] = torch.tensor(starts, dtype=torch.int32)
-        h["slots"][:n] = torch.tensor([s["pages"][p // ps] * ps + p % ps for s, p in zip(seqs, starts)], dtype=torch.int64)
-        h["ctx"][:n] = torch.tensor([p + 1 for p in starts], dtype=torch.int32)
+        h["slots"][:n] = torch.tensor([s["pages"][p // ps] * ps + p % ps for s, p in zip(seqs, rows)], dtype=torch.int64)
+        h["ctx"][:n] = torch.tensor([p + 1 for p in rows], dtype=torch.int32)
         width = max(len(s["pages"]) for s in seqs)
         bt = h["bt"]
         owners = g["bt_owners"][slot]
@@ -664,6 +745,9 @@ class Engine:
             h["prev"][:n] = torch.tensor([s["prev"] for s in seqs], dtype=torch.int32)
         if self.hybrid:
             h["st"][:n] = torch.tensor([s["state_slot"] for s in seqs], dtype=torch.int64)
+        if self.bounded:
+            h["ks"][:n] = torch.tensor([s.get("key_slot", 0) for s in seqs], dtype=torch.int64)
+            h["ks"][n:] = 0
         if n < bucket:
             h["tok"][n:] = 0
             h["pos"][n:] = 0
@@ -683,6 +767,8 @@ class Engine:
             b.state_slots.copy_(h["st"], non_blocking=True)
         if b.prev_ids is not None:
             b.prev_ids.copy_(h["prev"], non_blocking=True)
+        if b.key_slots is not None:
+            b.key_slots.copy_(h["ks"], non_blocking=True)
         self.metrics["h2d_bytes"] = self.metrics.get("h2d_bytes", 0) + bucket * (4 + 4 + 8 + 4 + 4 * width + (4 if b.prev_ids is not None else 0))
         g["graph"].replay()
         self.metrics["graph_replays"] += 1
@@ -705,6 +791,7 @@ class Engine:
             decode_even=even,
             state_slots=torch.zeros(bucket, dtype=torch.int64, device=dev) if self.hybrid else None,
             prev_ids=torch.zeros(bucket, dtype=torch.int32, device=dev) if self.needs_prev else None,
+            key_slots=torch.zeros(bucket, dtype=torch.int64, device=dev) if self.bounded else None,
         )
         # warm up outside capture (lazy handles, function attributes, scratch), then capture
         side = torch.cuda.Stream(device=dev)
@@ -728,6 +815,7 @@ class Engine:
             "bt": torch.zeros(bucket, self.max_pages_per_seq, dtype=torch.int32, pin_memory=pin),
             "st": torch.zeros(bucket, dtype=torch.int64, pin_memory=pin),
             "prev": torch.zeros(bucket, dtype=torch.int32, pin_memory=pin),
+            "ks": torch.zeros(bucket, dtype=torch.int64, pin_memory=pin),
         } for _ in range(2)]
         g = {"graph": graph, "batch": batch, "logits": logits, "host": host, "launches": launches, "calls": 0,
              "bt_owners": [[None] * bucket, [None] * bucket]}
@@ -825,6 +913,10 @@ class Engine:
 
     def generate(self, prompt: list[int], params: Optional[GeneratorParameters] = None, on_token=None, guide=None,
                  stopper=None) -> Response:
+        if params is not None and params.num_beams > 1:
+            if on_token is not None or guide is not None or stopper is not None:
+                raise ValueError("beam search has no token events, guides or stop detectors")
+            return self.generate_beams([prompt], params)[0][0]
         r = self.add_request(prompt, params, on_token, guide, stopper)
         self.run([r])
         if self.device.type == "cuda":
@@ -836,8 +928,16 @@ class Engine:
     def generate_batch(self, prompts: list[list[int]], params: Optional[GeneratorParameters] = None) -> list[Response]:
         import copy
 
+        if params is not None and params.num_beams > 1:
+            return [hypotheses[0] for hypotheses in self.generate_beams(prompts, params)]
         rs = [self.add_request(p, copy.deepcopy(params) if params else None) for p in prompts]
         self.run(rs)
         if self.device.type == "cuda":
             ops.check_status(self.device.index)
         return [r.response() for r in rs]
+
+    def generate_beams(self, prompts: list[list[int]], params: GeneratorParameters) -> list[list[Response]]:
+        """Beam search: for every prompt ``params.num_beams`` hypotheses, best first (``engine.beams``). The engine must be idle."""
+        from .beams import BeamSearch
+
+        return BeamSearch(self, params).run(prompts)

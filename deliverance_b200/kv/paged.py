@@ -44,6 +44,13 @@ class KvCacheSettings:
     anchors: tuple = (32, 64, 128)
     enabled: bool = True
     compression: str = "NONE"  # NONE | LZ4 | DEFLATE | MSE_TURBOQUANT (host snapshots only, see kv.turboquant)
+    # Bounded cache: a decoding sequence that holds more than keep_tokens rows is shortened to that many every keep_every steps, to its newest keep_recent rows
+    # and those of the others that had the most attention since (ops.evict). 0: off. Rows at or behind keep_capacity (0: the model's context) are not weighed;
+    # a sequence that reaches it is shortened at once.
+    keep_tokens: int = 0
+    keep_recent: int = 128
+    keep_every: int = 64
+    keep_capacity: int = 0
 
     def checkpoint_lengths(self, n_tokens: int) -> list[int]:
         """Prefix lengths (multiples of the block size, at most ``max_prefix_tokens``) at which a prompt of ``n_tokens`` is
@@ -230,7 +237,7 @@ class PagedKVCache:
     """Device storage + allocator + prefix cache for one model replica (one tensor-parallel rank)."""
 
     def __init__(self, layout: dict, num_pages: int, device, dtype, settings: Optional[KvCacheSettings] = None,
-                 max_state_slots: int = 0):
+                 max_state_slots: int = 0, weight_slots: int = 0, weight_capacity: int = 0):
         self.settings = settings or KvCacheSettings()
         self.page_size = self.settings.block_size
         if self.page_size % 32:
@@ -271,6 +278,13 @@ class PagedKVCache:
                 for name, shape in (shapes or {}).items():
                     t = torch.zeros((1 + max_state_slots,) + tuple(shape), dtype=torch.float32, device=self.device)
                     self.state.setdefault(name, {})[i] = t
+
+        # attention weights of a bounded cache: per layer fp32 [1 + slots, KV, capacity] (slot 0 is scratch), one allocation
+        self.key_weights: Optional[list] = None
+        self.free_weight_slots = list(range(weight_slots, 0, -1))
+        if weight_slots > 0:
+            self._weights = torch.zeros(len(kinds), 1 + weight_slots, heads[0], weight_capacity, dtype=torch.float32, device=self.device)
+            self.key_weights = list(self._weights.unbind(0))
 
     def layer(self, i: int):
         return self.k[i], self.v[i]
@@ -351,6 +365,18 @@ class PagedKVCache:
         if s <= 0 or s in self.free_slots:
             raise RuntimeError(f"state slot {s} is not in use")
         self.free_slots.append(s)
+
+    def alloc_weight_slot(self) -> int:
+        if not self.free_weight_slots:
+            raise MemoryError("no free row of key weights")
+        s = self.free_weight_slots.pop()
+        self._weights[:, s].zero_()
+        return s
+
+    def free_weight_slot(self, s: int) -> None:
+        if s <= 0 or s in self.free_weight_slots:
+            raise RuntimeError(f"key weight slot {s} is not in use")
+        self.free_weight_slots.append(s)
 
     def snapshot_state(self, slot: int) -> dict:
         return {name: {i: t[slot].clone() for i, t in layers.items()} for name, layers in self.state.items()}

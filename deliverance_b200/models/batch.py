@@ -27,6 +27,7 @@ class ForwardBatch:
     ctx_len_host: list = field(default_factory=list)
     token_types: Optional[torch.Tensor] = None  # bert
     prev_ids: Optional[torch.Tensor] = None  # [T] int32 token before each token of its sequence (-1: none), for models that read it
+    key_slots: Optional[torch.Tensor] = None  # [S] int64 decode: rows of key weights that the step's attention adds to (0: none), for a bounded cache
     plans: dict = field(default_factory=dict)  # per-batch work plans of model mechanisms, built once and shared by the layers
     _tiles: dict = field(default_factory=dict)  # tile height -> (tile_seq, tile_q0) device tensors
     host_tables: Optional[tuple] = None  # decode: block tables on the host and the page size, what ``rows_apart`` looks at
@@ -86,7 +87,8 @@ def make_batch(seqs: list[dict], page_size: int, device, max_pages: Optional[int
     """Build a batch from host-side sequence descriptions.
 
     Each entry: ``{"tokens": [new token ids], "start": first position, "pages": [page ids], "state_slot": int}``. An entry may
-    carry ``"prev"``, the token in front of its first one (-1 at the start of a sequence): ``prev_ids`` is then filled.
+    carry ``"prev"``, the token in front of its first one (-1 at the start of a sequence): ``prev_ids`` is then filled; ``"cached"``, the rows that its
+    sequence holds where that is not ``"start"`` (a shortened cache); ``"key_slot"``, its row of key weights.
     """
     from ..ops import even_lengths, prefill_tiles
 
@@ -107,27 +109,28 @@ def make_batch(seqs: list[dict], page_size: int, device, max_pages: Optional[int
     for i, s in enumerate(seqs):
         n = len(s["tokens"])
         start = int(s["start"])
+        row0 = int(s.get("cached", start))  # cache row of the first token
         pages = s["pages"]
-        need = (start + n + page_size - 1) // page_size
+        need = (row0 + n + page_size - 1) // page_size
         if need > len(pages):
             raise ValueError(f"sequence {i}: {need} pages needed, {len(pages)} given")
         pages_t = torch.tensor(pages, dtype=torch.int64)
         bt[i, : len(pages)] = pages_t
         qs.append(row)
         ql.append(n)
-        cl.append(start + n)
+        cl.append(row0 + n)
         if n <= 16:  # decode rows and short tails: plain lists (a tensor op per sequence would cost more than the loop)
             for j in range(n):
-                p = start + j
+                p = row0 + j
                 short[0].append(int(s["tokens"][j]))
-                short[1].append(p)
+                short[1].append(start + j)
                 short[2].append(pages[p // page_size] * page_size + p % page_size)
         else:
             # vectorised: a prompt chunk has thousands of tokens, and the device waits while the host builds the next chunk
             flush_short()
-            p = torch.arange(start, start + n, dtype=torch.int64)
+            p = torch.arange(row0, row0 + n, dtype=torch.int64)
             toks.append(torch.as_tensor(s["tokens"], dtype=torch.int32))
-            pos.append(p.to(torch.int32))
+            pos.append((p + (start - row0)).to(torch.int32))
             slots.append(pages_t[p // page_size] * page_size + p % page_size)
         row += n
     flush_short()
@@ -144,6 +147,9 @@ def make_batch(seqs: list[dict], page_size: int, device, max_pages: Optional[int
     state_slots = None
     if any("state_slot" in s for s in seqs):
         state_slots = t([int(s.get("state_slot", 0)) for s in seqs], torch.int64)
+    key_slots = None
+    if is_decode and any("key_slot" in s for s in seqs):
+        key_slots = t([int(s.get("key_slot", 0)) for s in seqs], torch.int64)
     prev_ids = None
     if any("prev" in s for s in seqs):
         prev = []
@@ -156,5 +162,5 @@ def make_batch(seqs: list[dict], page_size: int, device, max_pages: Optional[int
         q_len=t(ql, torch.int32), ctx_len=t(cl, torch.int32), block_tables=bt.to(dev, non_blocking=True), is_decode=is_decode,
         logits_rows=t(last, torch.int64), tile_seq=t(ts, torch.int32) if ts else None, tile_q0=t(t0, torch.int32) if ts else None,
         state_slots=state_slots, q_len_host=ql, ctx_len_host=cl, prev_ids=prev_ids, decode_even=is_decode and even_lengths(cl),
-        host_tables=(bt, page_size) if is_decode else None,
+        host_tables=(bt, page_size) if is_decode else None, key_slots=key_slots,
     )

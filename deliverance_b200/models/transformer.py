@@ -25,6 +25,7 @@ from ..ckpt.loader import ShardSpec, WeightLoader, shard_dense, shard_q4
 from ..ckpt.safetensors_io import Q4Tensor
 from ..config import ModelConfig
 from ..ops import LinearWeight, ref
+from ..ops.evict import decode_attention_weighted
 from ..parallel.context import SINGLE, TensorParallelContext, TensorParallelPlanner
 from .batch import ForwardBatch
 
@@ -359,7 +360,7 @@ class DecoderModel:
         k_cache, v_cache = kv.layer(i)
         local_rope = lw.kind == "sliding" and self.cos_local is not None
         cos, sin = (self.cos_local, self.sin_local) if local_rope else (self.cos, self.sin)
-        inside = (self.rope_in_attention and batch.is_decode and self._sp is None and ops.rope_in_attention(x.device, x.shape[0], self.n_heads, self.n_kv, cfg.head_dim) and
+        inside = (self.rope_in_attention and batch.is_decode and batch.key_slots is None and self._sp is None and ops.rope_in_attention(x.device, x.shape[0], self.n_heads, self.n_kv, cfg.head_dim) and
                   batch.rows_apart())  # (else every new key is in the cache before any row reads it)
         if inside:  # norm + rotary + cache write in the attention kernel
             with self._stage("causalselfattention.qkv_projection"):
@@ -386,6 +387,9 @@ class DecoderModel:
                 a = ops.decode_attention_rope(q, batch.positions, batch.slots, lw.q_norm, lw.k_norm, cos, sin, k_cache, v_cache, batch.block_tables, batch.ctx_len,
                                               self.n_heads, cfg.scale, cfg.attn_softcap, window, batch.decode_splits, cfg.norm_eps, cfg.norm_weight_offset,
                                               batch.decode_even, lambda *a: batch.decode_plan(i, *a))
+            elif batch.is_decode and batch.key_slots is not None:  # bounded cache
+                a = decode_attention_weighted(q, k_cache, v_cache, batch.block_tables, batch.ctx_len, self.n_heads, cfg.scale, kv.key_weights[i], batch.key_slots,
+                                              cfg.attn_softcap, 0, batch.decode_splits, batch.decode_even, lambda *a: batch.decode_plan(i, *a))
             elif batch.is_decode:
                 a = ops.decode_attention(q, k_cache, v_cache, batch.block_tables, batch.ctx_len, self.n_heads, cfg.scale,
                                          cfg.attn_softcap, window, batch.decode_splits, even=batch.decode_even,
@@ -611,6 +615,13 @@ class DecoderModel:
             shapes = self._mamba_shape().state_shapes()
             out["state_shapes"] = [shapes if k == "mamba" else None for k in kinds]
         return out
+
+    def supports_key_weights(self) -> bool:
+        """Whether the cache of this model can be bounded (``KvCacheSettings.keep_tokens``): attention over all cached rows in every layer, so that which row a
+        key lies in does not matter."""
+        cfg = self.cfg
+        return (type(self) is DecoderModel and all(cfg.layer_type(i) != "mamba" and not cfg.window(i) for i in range(cfg.num_layers)) and
+                self.n_heads // self.n_kv <= 16)
 
     def weight_bytes(self) -> int:
         n = self.embed.numel() * self.embed.element_size()

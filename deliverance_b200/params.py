@@ -6,6 +6,7 @@
 from __future__ import annotations
 
 import enum
+import math
 from dataclasses import dataclass, field
 from typing import Any, Callable, Optional
 
@@ -44,8 +45,17 @@ class GeneratorParameters:
     top_p: Optional[float] = None
     uniform_top_p: Optional[float] = None
     lora_adapter: Optional[str] = None
+    num_beams: int = 1  # > 1: beam search (Engine.generate_beams); deterministic, without guides, stop strings and log-probabilities
+    length_penalty: float = 1.0  # a hypothesis of n tokens ranks by its log-probability / n ** length_penalty
 
     def validate(self) -> None:
+        if not 1 <= self.num_beams <= 32:
+            raise ValueError("num_beams must be 1 to 32")
+        if self.num_beams > 1 and (self.temperature != 0 or self.xtc_threshold or self.logprobs or self.stop_words or
+                                   any(x is not None for x in (self.guided_choice, self.guided_regex, self.guided_json, self.top_k, self.top_p, self.uniform_top_p))):
+            raise ValueError("beam search does not combine with sampling, guides, stop strings or log-probabilities")
+        if not math.isfinite(self.length_penalty):
+            raise ValueError("length_penalty must be finite")
         modes = sum(x is not None for x in (self.guided_choice, self.guided_regex, self.guided_json))
         if modes > 1:
             raise ValueError("only one of guided_choice, guided_regex, guided_json may be set")
@@ -97,6 +107,7 @@ class Response:
     tool_calls: list[ToolCall] = field(default_factory=list)
     token_ids: list[int] = field(default_factory=list)
     prefix_hit_tokens: int = 0
+    score: Optional[float] = None  # beam search: log-probability of the tokens / n ** length_penalty
 
     @property
     def tokens_per_second(self) -> float:

@@ -116,6 +116,8 @@ class ServerConfig:
 _KV_KEYS = {"deliverance.kv.prefix.max-tokens": ("max_prefix_tokens", int), "deliverance.kv.prefix.checkpoint-policy": ("policy", str.upper),
             "deliverance.kv.prefix.max-checkpoints": ("checkpoints", int), "deliverance.kv.prefix.compression": ("compression", str.upper),
             "deliverance.kv.prefix.enabled": ("enabled", lambda v: v.lower() == "true"), "deliverance.kv.prefix.max-entries": ("max_entries", int),
+            "deliverance.kv.keep-tokens": ("keep_tokens", int), "deliverance.kv.keep-recent": ("keep_recent", int),
+            "deliverance.kv.keep-every": ("keep_every", int), "deliverance.kv.keep-capacity": ("keep_capacity", int),
             "deliverance.kv.prefix.block-size": ("block_size", int), "deliverance.kv.context-rows-per-page-target": ("block_size", int)}
 
 

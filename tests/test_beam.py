@@ -264,3 +264,160 @@ def test_reorder_refusals(device):
     with pytest.raises((IndexError, RuntimeError)):  # a slot outside: left out, and reported
         beam_reorder(torch.tensor([[1, 0]], device=device), [t], torch.tensor([[1, 4]], device=device))
         ops.check_status(0)
+
+
+# ---------------------------------------------------------------------------------------------------------------- engine
+def tiny_model(tmp, family, device="cpu", **over):
+    from deliverance_b200.ckpt.loader import WeightLoader
+    from deliverance_b200.ckpt.tiny import write_tiny_model
+    from deliverance_b200.config import load_config
+    from deliverance_b200.models.transformer import DecoderModel
+
+    d = str(tmp / family)
+    write_tiny_model(d, family, seed=11, std=over.pop("std", 0.2), **over)
+    cfg = load_config(d)
+    if family == "fopivik":
+        from deliverance_b200.models.fopivik import FopivikModel as Model
+    elif family == "gevovik":
+        from deliverance_b200.models.gevovik import GevovikModel as Model
+    else:
+        Model = DecoderModel
+    return Model(cfg, device).load(WeightLoader(d))
+
+
+def engine_of(model, **kw):
+    from deliverance_b200.engine.engine import Engine, EngineConfig
+    from deliverance_b200.kv.paged import KvCacheSettings
+
+    kv = kw.pop("kv", None) or KvCacheSettings()
+    return Engine(model, EngineConfig(num_pages=kw.pop("pages", 256), max_batch_tokens=kw.pop("chunk", 64), kv=kv, max_seqs=kw.pop("max_seqs", 16), **kw))
+
+
+def params_of(**kw):
+    from deliverance_b200.params import GeneratorParameters
+
+    return GeneratorParameters(**kw)
+
+
+def plain_beams(model, prompt, W, steps, eos, lp):
+    """Beam search by its definition: every hypothesis is run from the start at every step."""
+    from deliverance_b200.params import FinishReason
+
+    def logp(tokens):
+        e = engine_of(model)
+        r = e.open_replay()
+        z = e.replay_step([(r, tokens, [len(tokens) - 1])])[0].double()
+        return torch.log_softmax(z, -1)
+
+    alive, ended = [(0.0, [])], []
+    for n in range(1, steps + 1):
+        cand = []
+        for w, (score, toks) in enumerate(alive):
+            for v, x in enumerate((logp(prompt + toks) + score).tolist()):
+                cand.append((-x, w, v))
+        cand = sorted(cand)[: 2 * W]
+        nxt = []
+        for rank, (x, w, v) in enumerate(cand):
+            if v in eos or n == steps:
+                if rank < W:
+                    ended.append((-x / n**lp, alive[w][1] + [v], FinishReason.STOP_TOKEN if v in eos else FinishReason.MAX_TOKENS))
+            elif len(nxt) < W:
+                nxt.append((-x, alive[w][1] + [v]))
+        ended = sorted(ended, key=lambda h: -h[0])[:W]
+        alive = nxt
+        if not alive or (len(ended) >= W and max(s for s, _ in alive) / n**lp <= ended[-1][0]):
+            break
+    return ended
+
+
+@pytest.mark.parametrize("family,n,W,steps,lp,eos", [("llama", 5, 3, 6, 1.0, ()), ("llama", 31, 4, 5, 0.0, (7, 9)), ("llama", 32, 2, 4, 2.0, (3,)), ("qwen3", 63, 3, 4, 1.0, ()),
+                                                      ("granitemoehybrid", 20, 3, 5, 1.0, ()), ("fopivik", 33, 2, 4, 1.0, ()), ("gevovik", 30, 3, 5, 1.0, ())])
+def test_engine_beams_match_plain(tmp_path, family, n, W, steps, lp, eos):
+    model = tiny_model(tmp_path, family)
+    prompt = [(7 * i * i + 3 * i + 11) % 200 + 3 for i in range(n)]
+    if eos:  # end tokens that come up: the likeliest continuations of the plain search without any
+        eos = tuple({h[1][k] for h in plain_beams(model, prompt, W, steps, (), lp)[:2] for k in (2,)})
+    want = plain_beams(model, prompt, W, steps, eos, lp)
+    e = engine_of(model)
+    e.eos_ids = frozenset(eos)
+    free = e.kv.allocator.available()
+    got = e.generate_beams([prompt], params_of(num_beams=W, max_tokens=steps, length_penalty=lp))[0]
+    assert [r.token_ids for r in got] == [h[1] for h in want]
+    assert [r.finish_reason for r in got] == [h[2] for h in want]
+    # fp32 models, run in other orders: logits differ by rounding (2^-24 of sums of hundreds of terms of order one)
+    assert max(abs(r.score - h[0]) for r, h in zip(got, want)) < 1e-3
+    assert got[0].prompt_tokens == n and not e.running and not e.waiting
+    e.kv.audit([])
+    e.kv.prefix.clear()
+    assert e.kv.allocator.available() == free
+    if e.hybrid:
+        assert len(e.kv.free_slots) == 16
+
+
+def test_engine_beams_in_batches_and_repeats(tmp_path):
+    """Prompts of one call share steps, some end before others; cached prefixes and other requests in between change nothing."""
+    model = tiny_model(tmp_path, "llama")
+    prompts = [[(5 * i * i + k * i + 2 * k + 1) % 200 + 3 for i in range(n)] for k, n in enumerate((3, 40, 64, 33, 70))]
+    p = params_of(num_beams=3, max_tokens=20)
+    e = engine_of(model, max_seqs=7)  # two prompts at a time
+    alone = [engine_of(model).generate_beams([q], p)[0] for q in prompts]
+    both = e.generate_beams(prompts, p)
+    e.generate(prompts[1], params_of(max_tokens=4))
+    again = e.generate_beams(prompts[::-1], p)[::-1]
+    for a, b, c in zip(alone, both, again):
+        assert [r.token_ids for r in a] == [r.token_ids for r in b] == [r.token_ids for r in c]
+    e.kv.audit([])
+    greedy = [r.token_ids for r in engine_of(model).generate_batch(prompts, params_of(max_tokens=20))]
+    assert [engine_of(model).generate(q, p).token_ids for q in prompts] == [a[0].token_ids for a in alone]
+    assert [r.token_ids for r in engine_of(model).generate_batch(prompts, p)] == [a[0].token_ids for a in alone]
+    assert len(greedy) == 5
+
+
+def test_engine_beams_refusals(tmp_path):
+    model = tiny_model(tmp_path, "llama")
+    e = engine_of(model, pages=16, max_seqs=4)
+    prompt = list(range(3, 40))
+    for bad in (dict(num_beams=33), dict(num_beams=0), dict(num_beams=2, temperature=0.5), dict(num_beams=2, logprobs=True), dict(num_beams=2, stop_words=["x"]),
+                dict(num_beams=2, guided_choice=["a"]), dict(num_beams=2, length_penalty=math.inf)):
+        with pytest.raises(ValueError):
+            e.generate_beams([prompt], params_of(max_tokens=4, **bad))
+    with pytest.raises(ValueError):
+        e.generate_beams([prompt], params_of(num_beams=5, max_tokens=4))  # more beams than places
+    with pytest.raises(ValueError):
+        e.add_request(prompt, params_of(num_beams=2))
+    with pytest.raises(MemoryError):
+        e.generate_beams([prompt], params_of(num_beams=4, max_tokens=200))
+    with pytest.raises(ValueError):
+        e.generate_beams([[]], params_of(num_beams=2, max_tokens=4))
+    e.add_request(prompt, params_of(max_tokens=4))
+    with pytest.raises(RuntimeError):
+        e.generate_beams([prompt], params_of(num_beams=2, max_tokens=4))
+    e.run()
+    e.kv.audit([])
+    assert len(e.generate_beams([prompt], params_of(num_beams=2, max_tokens=4))[0]) == 2
+    e.kv.audit([])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("family,over", [("qwen3", dict(hidden_size=256, num_attention_heads=4, num_key_value_heads=2, head_dim=64)), ("granitemoehybrid", dict(hidden_size=256, num_attention_heads=4, num_key_value_heads=2, head_dim=64, mamba_d_head=64, mamba_n_heads=8)),
+                                         ("qwen3", dict(hidden_size=256, num_attention_heads=4, num_key_value_heads=2, head_dim=128))])
+def test_engine_beams_on_the_gpu(tmp_path, family, over):
+    """Captured steps and steps launched one by one give the same hypotheses, and their scores are those of the CPU model for these tokens."""
+    cpu, gpu = tiny_model(tmp_path, family, **over), tiny_model(tmp_path, family, "cuda", **over)
+    prompts = [[(7 * i * i + 3 * i + k) % 200 + 3 for i in range(n)] for k, n in enumerate((31, 64, 90))]
+    p = params_of(num_beams=4, max_tokens=40)
+    got = []
+    for graphs in (True, False):
+        e = engine_of(gpu, cuda_graphs=graphs)
+        got.append(e.generate_beams(prompts, p))
+        e.kv.audit([])
+    assert [[r.token_ids for r in h] for h in got[0]] == [[r.token_ids for r in h] for h in got[1]]
+    for prompt, hyps in zip(prompts, got[0]):
+        assert hyps[0].score >= hyps[-1].score and len({tuple(r.token_ids) for r in hyps}) == 4
+        e = engine_of(cpu)
+        r = e.open_replay()
+        toks = prompt + hyps[0].token_ids
+        z = torch.log_softmax(e.replay_step([(r, toks, list(range(len(prompt) - 1, len(toks) - 1)))]).double(), -1)
+        want = float(z.gather(1, torch.tensor(hyps[0].token_ids).view(-1, 1)).sum()) / len(hyps[0].token_ids)
+        # bf16 activations over a few layers: a log-probability is off by some hundredths, here their mean over 40 tokens
+        assert abs(hyps[0].score - want) < 0.1
