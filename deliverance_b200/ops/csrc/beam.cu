@@ -288,26 +288,31 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
     for (int j = 0; j < 8; ++j)
       if (i0 + j * kMergeThreads < n) best = fmaxf(best, rough_of(y[j], i0 + j * kMergeThreads));
   }
+  // a value that K at least of the CTA's threads' best reach: the K-th best of 64 clusters of eight threads
+  auto bound_of = [&](float mine) {
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
-  if ((t & 7) == 0) cluster_value[t >> 3] = best;
-  __syncthreads();
-  {  // eight threads count for one cluster
-    const int g = t >> 3;
+    for (int o = 1; o < 8; o <<= 1) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+    if ((t & 7) == 0) cluster_value[t >> 3] = mine;
+    __syncthreads();
+    const int g = t >> 3;  // eight threads count for one cluster
     int rank = 0;
 #pragma unroll
     for (int q = 0; q < kClusters / 8; ++q) {
       const int u = q * 8 + (t & 7);
-      rank += cluster_value[u] > best || (cluster_value[u] == best && u < g) ? 1 : 0;
+      rank += cluster_value[u] > mine || (cluster_value[u] == mine && u < g) ? 1 : 0;
     }
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
-    if ((t & 7) == 0 && rank == K - 1) edge_value = best;
-  }
-  __syncthreads();
+    if ((t & 7) == 0 && rank == K - 1) edge_value = mine;
+    __syncthreads();
+    return edge_value;
+  };
+  const float reached = bound_of(best);
   float most = 0.f;
   for (int w = lane; w < W; w += 32) most = fmaxf(most, rough[w] > -INFINITY ? fabsf(rough[w]) : 0.f);
-  const float slack = 0x1p-20f * (warp_max(most) + fabsf(edge_value)) + 0x1p-18f * a.softcap, bound = edge_value - slack;
+  most = warp_max(most);
+  auto below = [&](float v) { return v - (0x1p-20f * (most + fabsf(v)) + 0x1p-18f * a.softcap); };
+  const float bound = below(reached);
   double edge = static_cast<double>(bound);  // K candidates at least are not below this
   uint32_t last = 0xffffffffu;               // of the groups (then: candidates) that equal the edge, those up to this place
   auto list_group = [&](int i) {
@@ -345,8 +350,8 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
   const int m_groups = n_groups;
   // candidate j of the listed groups
   auto logit = [&](int g, int e, int& w, int& v) {
-    w = groups[g] / a.groups;
-    v = groups[g] % a.groups * GROUP + e;
+    w = a.by_groups.of(groups[g]);
+    v = (groups[g] - w * a.groups) * GROUP + e;
     const long long row = static_cast<long long>(b) * W + w;
     if (v >= a.V || (a.mask != nullptr && !((a.mask[row * a.mask_ld + (v >> 5)] >> (v & 31)) & 1u))) return -INFINITY;
     const T y = static_cast<const T*>(a.logits)[row * a.ld + v];
@@ -356,7 +361,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
   auto place_of = [&](int w, int v) { return static_cast<uint32_t>(w) * static_cast<uint32_t>(a.V) + static_cast<uint32_t>(v); };
   last = 0xffffffffu;
   auto list_candidates = [&]() {
-    for (int g = warp; g < m_groups; g += kMergeWarps) {
+    for (int g = warp; g < m_groups && *static_cast<volatile int*>(&listed) <= kMostListed; g += kMergeWarps) {
       float y[N];
       int w, v;
 #pragma unroll
@@ -364,7 +369,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
 #pragma unroll
       for (int q = 0; q < N; ++q) {
         const double d = value_of(y[q], w);
-        const uint32_t p = place_of(w, groups[g] % a.groups * GROUP + q * 32 + lane);
+        const uint32_t p = place_of(w, (groups[g] - w * a.groups) * GROUP + q * 32 + lane);
         if (d > -INFINITY && (d > edge || (d == edge && p <= last))) {
           const int at = atomicAdd(&listed, 1);
           if (at < kMostListed) {
@@ -375,20 +380,38 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
       }
     }
   };
-  list_candidates();
+  const bool loose = m_groups > 4 * K + 16 || reached == -INFINITY;
+  if (!loose) list_candidates();
   __syncthreads();
-  if (listed > kMostListed) {
-    kth_best(m_groups * GROUP, K, [&](int i, uint32_t& p) {
-      int w, v;
-      const float y = logit(i / GROUP, i % GROUP, w, v);
-      p = place_of(w, v);
-      return value_of(y, w);
-    }, red, edge, last);
+  if (loose || listed > kMostListed) {  // a closer bound, from the candidates themselves: rows that a mask leaves few tokens, few groups
+    float mine = -INFINITY;
+    for (int g = warp; g < m_groups; g += kMergeWarps) {
+#pragma unroll
+      for (int q = 0; q < N; ++q) {
+        int w, v;
+        const float y = logit(g, q * 32 + lane, w, v);
+        mine = fmaxf(mine, post(y, a.softcap, a.inv_scale) + rough[w]);
+      }
+    }
     __syncthreads();
+    edge = fmax(edge, static_cast<double>(below(bound_of(mine))));
     if (t == 0) listed = 0;
     __syncthreads();
     list_candidates();
     __syncthreads();
+    if (listed > kMostListed) {
+      kth_best(m_groups * GROUP, K, [&](int i, uint32_t& p) {
+        int w, v;
+        const float y = logit(i / GROUP, i % GROUP, w, v);
+        p = place_of(w, v);
+        return value_of(y, w);
+      }, red, edge, last);
+      __syncthreads();
+      if (t == 0) listed = 0;
+      __syncthreads();
+      list_candidates();
+      __syncthreads();
+    }
   }
   const int m = listed;
   const long long out = static_cast<long long>(b) * K;
