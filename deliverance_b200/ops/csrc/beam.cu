@@ -81,7 +81,8 @@ __device__ __forceinline__ float redux_max(float v) {
 
 // grid: B * W * splits. A tile is 16 logits per thread, 16 bytes of a warp's lanes side by side: one group per load. The next tile is on its way while a tile is
 // worked on; a running maximum and sum per thread, joined at the end in a fixed order.
-template <typename T, bool MASK, bool ALIGNED>
+// PLAIN: neither scale nor cap.
+template <typename T, bool MASK, bool ALIGNED, bool PLAIN>
 __global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_constant__ BeamSelectArgs a) {
   pdl_trigger();
   pdl_wait();
@@ -94,7 +95,6 @@ __global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_con
   const T* x_row = static_cast<const T*>(a.logits) + static_cast<long long>(row) * a.ld;
   const uint32_t* bits = MASK ? a.mask + static_cast<long long>(row) * a.mask_ld : nullptr;
   float* group_max = a.group_max + static_cast<long long>(row) * a.groups;
-  const bool plain = a.softcap <= 0.f && a.inv_scale == 1.f;
   float m = -FLT_MAX;
   double sum = 0.0;
   uint4 raw[NV];
@@ -140,19 +140,14 @@ __global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_con
     }
     const int group = at / (32 * N) + warp * NV + lane;
     if (lane < NV && group * 32 * N < hi) group_max[group] = mine;
-    const float top_z = plain ? top : post(top, a.softcap, a.inv_scale);
+    const float top_z = PLAIN ? top : post(top, a.softcap, a.inv_scale);
     if (top_z > m) {
       sum *= static_cast<double>(expf(m - top_z));
       m = top_z;
     }
     float part = 0.f;
-    if (plain) {
 #pragma unroll
-      for (int j = 0; j < kPerLane; ++j) part += exp_below(x[j / N][j % N] - m);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kPerLane; ++j) part += exp_below(post(x[j / N][j % N], a.softcap, a.inv_scale) - m);
-    }
+    for (int j = 0; j < kPerLane; ++j) part += exp_below((PLAIN ? x[j / N][j % N] : post(x[j / N][j % N], a.softcap, a.inv_scale)) - m);
     sum += static_cast<double>(part);
   }
   const float wm = warp_max(m);
@@ -180,6 +175,10 @@ __device__ __forceinline__ unsigned long long double_order(double v) {
   const long long u = __double_as_longlong(v + 0.0);
   return u < 0 ? ~static_cast<unsigned long long>(u) : static_cast<unsigned long long>(u) | 0x8000000000000000ull;
 }
+
+// (out of line: the second kernel runs once through its code, and fetching copies of the hyperbolic tangent between what always runs takes it 0.4 us)
+__device__ __noinline__ double capped(double z, double cap) { return cap * tanh(z / cap); }
+__device__ __noinline__ float capped(float z, float cap) { return cap * tanhf(z / cap); }
 
 // Number of threads' set flags over the CTA, for the searches that need many of them
 __device__ __forceinline__ int merge_count(int c, int* red, int& turn) {
@@ -267,12 +266,16 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
   auto value_of = [&](float y, int w) {
     if (!(y > -INFINITY)) return -static_cast<double>(INFINITY);
     double z = static_cast<double>(y) * static_cast<double>(a.inv_scale);
-    if (a.softcap > 0.f) z = static_cast<double>(a.softcap) * tanh(z / static_cast<double>(a.softcap));
+    if (a.softcap > 0.f) z = capped(z, static_cast<double>(a.softcap));
     const double v = base[w] + (z - static_cast<double>(top[w]));
     return isfinite(v) ? v : -static_cast<double>(INFINITY);
   };
   // in 32 bits: off by less than half of `slack` (roundings of the row's constant, of the sum and of scale and cap)
-  auto rough_of = [&](float y, int i) { return post(y, a.softcap, a.inv_scale) + rough[a.by_groups.of(i)]; };
+  auto rough_post = [&](float y) {
+    y *= a.inv_scale;
+    return a.softcap > 0.f && y > -INFINITY ? capped(y, a.softcap) : y;
+  };
+  auto rough_of = [&](float y, int i) { return rough_post(y) + rough[a.by_groups.of(i)]; };
   float best = -INFINITY;
 #pragma unroll
   for (int j = 0; j < AHEAD; ++j) {
@@ -360,7 +363,31 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
   };
   auto place_of = [&](int w, int v) { return static_cast<uint32_t>(w) * static_cast<uint32_t>(a.V) + static_cast<uint32_t>(v); };
   last = 0xffffffffu;
-  auto list_candidates = [&]() {
+  const bool loose = m_groups > 4 * K + 16 || reached == -INFINITY;
+#pragma unroll 1
+  for (int round = loose ? 1 : 0;; ++round) {
+    if (round == 1) {  // a closer bound, from the candidates themselves: rows that a mask leaves few tokens, few groups
+      float mine = -INFINITY;
+#pragma unroll 1
+      for (int g = warp; g < m_groups; g += kMergeWarps) {
+#pragma unroll
+        for (int q = 0; q < N; ++q) {
+          int w, v;
+          const float y = logit(g, q * 32 + lane, w, v);
+          mine = fmaxf(mine, rough_post(y) + rough[w]);
+        }
+      }
+      __syncthreads();
+      edge = fmax(edge, static_cast<double>(below(bound_of(mine))));
+    } else if (round == 2) {  // long runs of one value
+      kth_best(m_groups * GROUP, K, [&](int i, uint32_t& p) {
+        int w, v;
+        const float y = logit(i / GROUP, i % GROUP, w, v);
+        p = place_of(w, v);
+        return value_of(y, w);
+      }, red, edge, last);
+    }
+#pragma unroll 1
     for (int g = warp; g < m_groups && *static_cast<volatile int*>(&listed) <= kMostListed; g += kMergeWarps) {
       float y[N];
       int w, v;
@@ -379,39 +406,11 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
         }
       }
     }
-  };
-  const bool loose = m_groups > 4 * K + 16 || reached == -INFINITY;
-  if (!loose) list_candidates();
-  __syncthreads();
-  if (loose || listed > kMostListed) {  // a closer bound, from the candidates themselves: rows that a mask leaves few tokens, few groups
-    float mine = -INFINITY;
-    for (int g = warp; g < m_groups; g += kMergeWarps) {
-#pragma unroll
-      for (int q = 0; q < N; ++q) {
-        int w, v;
-        const float y = logit(g, q * 32 + lane, w, v);
-        mine = fmaxf(mine, post(y, a.softcap, a.inv_scale) + rough[w]);
-      }
-    }
     __syncthreads();
-    edge = fmax(edge, static_cast<double>(below(bound_of(mine))));
+    if (listed <= kMostListed) break;
+    __syncthreads();
     if (t == 0) listed = 0;
     __syncthreads();
-    list_candidates();
-    __syncthreads();
-    if (listed > kMostListed) {
-      kth_best(m_groups * GROUP, K, [&](int i, uint32_t& p) {
-        int w, v;
-        const float y = logit(i / GROUP, i % GROUP, w, v);
-        p = place_of(w, v);
-        return value_of(y, w);
-      }, red, edge, last);
-      __syncthreads();
-      if (t == 0) listed = 0;
-      __syncthreads();
-      list_candidates();
-      __syncthreads();
-    }
   }
   const int m = listed;
   const long long out = static_cast<long long>(b) * K;
@@ -456,10 +455,12 @@ int beam_select_splits(int rows, int V) {
 
 template <typename T, bool MASK>
 static void launch_part(const BeamSelectArgs& a, dim3 grid, cudaStream_t st) {
-  if ((reinterpret_cast<uintptr_t>(a.logits) | static_cast<uintptr_t>(a.ld * static_cast<long long>(sizeof(T)))) % 16 == 0)
-    launch_pdl(beam_part_kernel<T, MASK, true>, grid, dim3(kThreads), 0, st, a);
-  else
-    launch_pdl(beam_part_kernel<T, MASK, false>, grid, dim3(kThreads), 0, st, a);
+  const bool aligned = (reinterpret_cast<uintptr_t>(a.logits) | static_cast<uintptr_t>(a.ld * static_cast<long long>(sizeof(T)))) % 16 == 0;
+  const bool plain = a.softcap <= 0.f && a.inv_scale == 1.f;
+  if (aligned && plain) launch_pdl(beam_part_kernel<T, MASK, true, true>, grid, dim3(kThreads), 0, st, a);
+  else if (aligned) launch_pdl(beam_part_kernel<T, MASK, true, false>, grid, dim3(kThreads), 0, st, a);
+  else if (plain) launch_pdl(beam_part_kernel<T, MASK, false, true>, grid, dim3(kThreads), 0, st, a);
+  else launch_pdl(beam_part_kernel<T, MASK, false, false>, grid, dim3(kThreads), 0, st, a);
 }
 
 void launch_beam_select(const BeamSelectArgs& a, bool f32, cudaStream_t st) {

@@ -111,27 +111,41 @@ __global__ void __launch_bounds__(NT) evict_select_kernel(const __grid_constant_
   uint32_t edge = 0xffffffffu;  // keys above the edge stay, and `spare` of those that equal it
   int spare = 0, turn = 0;
   if (k.want > 0) {
+    __shared__ uint32_t few[NT];
+    __shared__ int n_few;
+    if (t == 0) n_few = 0;
     edge = 0;
+    int reach = k.old, above = 0, bit = 31;  // keys that reach the edge, and those beyond the range that is still open above it
     bool exact = false;
-    for (int bit = 31; bit >= 0 && !exact; --bit) {
+    for (; bit >= 0 && !exact && reach - above > NT; --bit) {
       const uint32_t probe = edge | (1u << bit);
       int c = 0;
 #pragma unroll
       for (int r = 0; r < R; ++r) c += key[r] >= probe ? 1 : 0;
       c = block_count<NT>(c, red, turn);
       turn ^= 1;
-      if (c >= k.want) edge = probe;
+      if (c >= k.want) edge = probe, reach = c;
+      else above = c;
       exact = c == k.want;
     }
-    if (exact) {
-      edge -= 1;  // (all that reach the probe: above probe - 1; a probe is not 0)
-    } else {
-      int c = 0;
+    if (bit >= 0 && !exact) {  // one open key per thread from here on
+      __syncthreads();
 #pragma unroll
-      for (int r = 0; r < R; ++r) c += key[r] > edge ? 1 : 0;
-      spare = k.want - block_count<NT>(c, red, turn);
-      turn ^= 1;
+      for (int r = 0; r < R; ++r)
+        if (t * R + r < k.old && (static_cast<unsigned long long>(key[r]) >> (bit + 1)) == (static_cast<unsigned long long>(edge) >> (bit + 1))) few[atomicAdd(&n_few, 1)] = key[r];
+      __syncthreads();
+      const uint32_t mine = t < n_few ? few[t] : 0u;
+      const int beyond = above;
+      for (; bit >= 0 && !exact; --bit) {
+        const uint32_t probe = edge | (1u << bit);
+        const int c = beyond + __syncthreads_count(mine >= probe);
+        if (c >= k.want) edge = probe;
+        exact = c == k.want;
+        if (c < k.want) above = c;
+      }
     }
+    if (exact) edge -= 1;  // (all that reach the probe: above probe - 1; a probe is not 0)
+    else spare = k.want - above;
   }
   // how many ties lie in front of a thread's rows, then how many rows that stay
   int ties = 0, total;
@@ -155,7 +169,7 @@ __global__ void __launch_bounds__(NT) evict_select_kernel(const __grid_constant_
   for (int r = 0; r < R; ++r) {
     const int i = t * R + r;
     const bool even = i < k.old && key[r] == edge;
-    if (i < k.n && (i >= k.old || key[r] > edge || (even && tie < spare))) list[takes++] = i;
+    if (i < k.n && (i >= k.old || key[r] > edge || (even && tie < spare)) && takes < a.keep) list[takes++] = i;
     tie += even ? 1 : 0;
   }
   __syncthreads();
@@ -307,9 +321,9 @@ void launch_evict(const EvictArgs& a, int unit, cudaStream_t st) {
     if (once.first()) cudaFuncSetAttribute(evict_select_kernel<NT, RR>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelectShared);      \
     launch_pdl(evict_select_kernel<NT, RR>, heads, dim3(NT), shared(NT * RR), st, a);                                                     \
   } while (0)
-  if (most <= 256 * 10 && shared(256 * 10) <= kSelectShared) DLV_EVICT_SELECT(256, 10);
+  if (most <= 512 * 5 && shared(512 * 5) <= kSelectShared) DLV_EVICT_SELECT(512, 5);
   else if (most <= 512 * 20 && shared(512 * 20) <= kSelectShared) DLV_EVICT_SELECT(512, 20);
-  else if (most <= 512 * 72 && shared(512 * 72) <= kSelectShared) DLV_EVICT_SELECT(512, 72);
+  else if (most <= 1024 * 36 && shared(1024 * 36) <= kSelectShared) DLV_EVICT_SELECT(1024, 36);
   else launch_pdl(evict_select_long_kernel, heads, dim3(512), 0, st, a);
 #undef DLV_EVICT_SELECT
   // columns are cut (to 64 bytes at least) where there are too few heads to fill the GPU
