@@ -615,7 +615,7 @@ __device__ __forceinline__ void weigh_keys(const WeighArgs& a, int b, int kvh, i
 }
 
 template <int D, int EXT, int NW, bool PLAN, bool ROPE, bool WEIGH>
-__global__ void __launch_bounds__(NW * 32, (D <= 128 && NW == 4 ? 2 : 1)) decode_attn_mma_kernel(
+__global__ void __launch_bounds__(NW * 32, (WEIGH && D <= 64 ? 4 : D <= 128 && NW == 4 ? 2 : 1)) decode_attn_mma_kernel(
     const __nv_bfloat16* __restrict__ q, long long q_stride, const __nv_bfloat16* __restrict__ k_cache,
     const __nv_bfloat16* __restrict__ v_cache, const int* __restrict__ block_tables, int bt_stride,
     const int* __restrict__ ctx_lens, __nv_bfloat16* __restrict__ out, float* part_o, float* part_ml, int* __restrict__ arrivals,

@@ -496,19 +496,18 @@ struct MoveUnit<2> {
   using type = unsigned short;
 };
 
-// grid (units of a slot / 256, tensors, requests)
+// grid (parts of a slot, tensors, requests): a part takes every gridDim.x-th 256 units
 template <int UNIT, int MAXW>
 __global__ void __launch_bounds__(256) beam_move_kernel(const __grid_constant__ BeamMoveArgs a) {
   using U = typename MoveUnit<UNIT>::type;
   pdl_trigger();
   pdl_wait();
-  __shared__ long long from[MAXW], to[MAXW];  // slots; to < 0: the beam stays
+  __shared__ long long from[MAXW], to[MAXW];  // byte offsets of slots; to < 0: the beam stays
   const int b = blockIdx.z, t = threadIdx.x;
   const BeamMoveTensor& d = a.t[blockIdx.y];
   const int rows = a.rows != nullptr ? max(0, min(a.rows[b], a.max_rows)) : a.max_rows;
-  const long long part = static_cast<long long>(rows) * d.row_bytes / UNIT;  // units of one segment that move
-  const long long u = static_cast<long long>(blockIdx.x) * 256 + t;
-  if (static_cast<long long>(blockIdx.x) * 256 >= part * d.segments) return;
+  const long long part = static_cast<long long>(rows) * d.row_bytes / UNIT, all = part * d.segments;  // units of one segment that move, of a slot
+  if (static_cast<long long>(blockIdx.x) * 256 >= all) return;
   if (t < MAXW) {
     long long s = -1, r = -1;
     if (t < a.W) {
@@ -522,20 +521,22 @@ __global__ void __launch_bounds__(256) beam_move_kernel(const __grid_constant__ 
         }
       }
     }
-    from[t] = s;
-    to[t] = r;
+    from[t] = s * d.slot_bytes;
+    to[t] = r < 0 ? -1 : r * d.slot_bytes;
   }
   __syncthreads();
-  if (u >= part * d.segments) return;
-  const long long seg = u / part;
-  uint8_t* base = static_cast<uint8_t*>(d.base) + seg * (d.slot_bytes / d.segments) + (u - seg * part) * UNIT;
-  U v[MAXW];
+  const long long pitch = d.slot_bytes / d.segments;
+  for (long long u = static_cast<long long>(blockIdx.x) * 256 + t; u < all; u += static_cast<long long>(gridDim.x) * 256) {
+    const long long seg = all == part ? 0 : u / part;
+    uint8_t* base = static_cast<uint8_t*>(d.base) + seg * pitch + (u - seg * part) * UNIT;
+    U v[MAXW];
 #pragma unroll
-  for (int j = 0; j < MAXW; ++j)
-    if (to[j] >= 0) v[j] = *reinterpret_cast<const U*>(base + from[j] * d.slot_bytes);
+    for (int j = 0; j < MAXW; ++j)
+      if (to[j] >= 0) v[j] = *reinterpret_cast<const U*>(base + from[j]);
 #pragma unroll
-  for (int j = 0; j < MAXW; ++j)
-    if (to[j] >= 0) *reinterpret_cast<U*>(base + to[j] * d.slot_bytes) = v[j];
+    for (int j = 0; j < MAXW; ++j)
+      if (to[j] >= 0) *reinterpret_cast<U*>(base + to[j]) = v[j];
+  }
 }
 
 template <int UNIT>
@@ -553,7 +554,10 @@ void launch_beam_move(const BeamMoveArgs& a, int B, int unit, cudaStream_t st) {
     units = u > units ? u : units;
   }
   if (B == 0 || a.n == 0 || units == 0) return;
-  const dim3 grid(static_cast<unsigned>((units + 255) / 256), a.n, B);
+  // looking the slots up takes a CTA as long as moving a unit, so pages, of which a slot has little, get fewer CTAs (16 x 8 beams, 44 pools: 10.3 us with 16 per SM, 11.3 with 64;
+  // 32 x 16 beams 54 and 65; states of 2 MB 363 and 345)
+  const long long parts = (units + 255) / 256, room = 148 * (a.paged ? 16 : 64) / (static_cast<long long>(a.n) * B);
+  const dim3 grid(static_cast<unsigned>(room < 1 ? 1 : room < parts ? room : parts), a.n, B);
   if (unit == 16) move_by_width<16>(a, grid, st);
   else if (unit == 4) move_by_width<4>(a, grid, st);
   else move_by_width<2>(a, grid, st);

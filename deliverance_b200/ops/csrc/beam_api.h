@@ -47,6 +47,7 @@ struct BeamMoveArgs {
   const int* rows;           // [B], null: max_rows everywhere
   int* status;
   int n, W, num_slots, max_rows;
+  bool paged;
 };
 // unit: bytes that one access moves (16, 4 or 2): all sizes and addresses are multiples of it
 void launch_beam_move(const BeamMoveArgs& a, int B, int unit, cudaStream_t st);
