@@ -505,24 +505,25 @@ __global__ void __launch_bounds__(256) beam_move_kernel(const __grid_constant__ 
   __shared__ long long from[MAXW], to[MAXW];  // byte offsets of slots; to < 0: the beam stays
   const int b = blockIdx.z, t = threadIdx.x;
   const BeamMoveTensor& d = a.t[blockIdx.y];
-  const int rows = a.rows != nullptr ? max(0, min(a.rows[b], a.max_rows)) : a.max_rows;
+  // (everything that the moves depend on is asked for at once)
+  const int filled = a.rows != nullptr ? a.rows[b] : a.max_rows;
+  long long slot = -1, parent = -1;
+  if (t < a.W) {
+    slot = a.slots[static_cast<long long>(b) * a.W + t];
+    parent = a.parents[static_cast<long long>(b) * a.W + t];
+  }
+  const int rows = max(0, min(filled, a.max_rows));
   const long long part = static_cast<long long>(rows) * d.row_bytes / UNIT, all = part * d.segments;  // units of one segment that move, of a slot
   if (static_cast<long long>(blockIdx.x) * 256 >= all) return;
-  if (t < MAXW) {
-    long long s = -1, r = -1;
-    if (t < a.W) {
-      const long long p = a.parents[static_cast<long long>(b) * a.W + t];
-      if (p >= 0 && p < a.W && p != t) {
-        r = a.slots[static_cast<long long>(b) * a.W + t];
-        s = a.slots[static_cast<long long>(b) * a.W + p];
-        if (r < 0 || r >= a.num_slots || s < 0 || s >= a.num_slots) {
-          atomicCAS(a.status, kStatusOk, kStatusBadArgs);
-          r = -1;
-        }
-      }
+  if (t < 32) {
+    const bool moves = parent >= 0 && parent < a.W && parent != t;
+    const long long source = __shfl_sync(0xffffffffu, slot, moves ? static_cast<int>(parent) : t);
+    const bool good = slot >= 0 && slot < a.num_slots && source >= 0 && source < a.num_slots;
+    if (moves && !good) atomicCAS(a.status, kStatusOk, kStatusBadArgs);
+    if (t < MAXW) {
+      from[t] = source * d.slot_bytes;
+      to[t] = moves && good ? slot * d.slot_bytes : -1;
     }
-    from[t] = s * d.slot_bytes;
-    to[t] = r < 0 ? -1 : r * d.slot_bytes;
   }
   __syncthreads();
   const long long pitch = d.slot_bytes / d.segments;
