@@ -570,46 +570,58 @@ __device__ __forceinline__ bool weigh_slot(const WeighArgs& a, int b) {
   if (threadIdx.x == 0) atomicCAS(a.status, kStatusOk, kStatusBadArgs);
   return false;
 }
-// weights[key] += sum over the query heads of exp(score - maximum) / sum, heads in order. A thread takes four neighbouring keys at a time, the scores of eight (key group, head)
-// pairs on their way together; thread `first` of `step`. Scores behind the last key of a slice are -inf. (Base-two exponential of a rounded product: 2^-22 + |score - maximum| 2^-23 of a probability.)
+// weights[key] += sum over the query heads of exp(score - maximum) / sum, heads in order. A thread takes U groups of four neighbouring keys at a time, the scores of four heads on
+// their way together; thread `first` of `step`. Scores behind the last key of a slice are -inf. (Base-two exponential of a rounded product: 2^-22 + |score - maximum| 2^-23 of a probability.)
+template <int U>
 __device__ __forceinline__ void weigh_keys(const WeighArgs& a, int b, int kvh, int ctx, int first, int step, const float* top, const float* inv) {
   const int G = a.H / a.KV, keys = min(ctx, a.capacity), from = window_first(ctx, a.window) & ~3;
   const float* s0 = a.scores + (static_cast<long long>(b) * a.H + kvh * G) * a.S;
   float* w = a.weights + (a.slots[b] * a.KV + kvh) * a.capacity;
-  for (int k0 = from + 4 * first; k0 < keys; k0 += 8 * step) {
-    const int k1 = k0 + 4 * step;
-    float old[8], p[8] = {};
+  for (int k0 = from + 4 * first; k0 < keys; k0 += 4 * U * step) {
+    float old[U][4], p[U][4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int k = (i < 4 ? k0 : k1 - 4) + i;
-      old[i] = k < keys ? w[k] : 0.f;
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = k0 + 4 * u * step + i;
+        old[u][i] = k < keys ? w[k] : 0.f;
+        p[u][i] = 0.f;
+      }
     }
     for (int g0 = 0; g0 < G; g0 += 4) {
-      float4 s[2][4];
+      float4 s[U][4];
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const float* row = s0 + static_cast<long long>(g0 + g) * a.S;
-        const float4 none = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        s[0][g] = g0 + g < G ? *reinterpret_cast<const float4*>(row + k0) : none;
-        s[1][g] = g0 + g < G && k1 < keys ? *reinterpret_cast<const float4*>(row + k1) : none;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int k = k0 + 4 * u * step;
+          s[u][g] = g0 + g < G && (u == 0 || k < keys) ? *reinterpret_cast<const float4*>(row + k) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        }
       }
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const float m = top[(g0 + g) & 15], f = g0 + g < G ? inv[(g0 + g) & 15] : 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float4& v = s[i >> 2][g];
-          const float x = (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
-          float e;
-          asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((x - m) * 1.44269504088896341f));
-          p[i] = fmaf(e, f, p[i]);
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float4& v = s[u][g];
+            const float x = i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+            float e;
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((x - m) * 1.44269504088896341f));
+            p[u][i] = fmaf(e, f, p[u][i]);
+          }
         }
       }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int k = (i < 4 ? k0 : k1 - 4) + i;
-      if (k < keys) w[k] = old[i] + p[i];
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = k0 + 4 * u * step + i;
+        if (k < keys) w[k] = old[u][i] + p[u][i];
+      }
     }
   }
 }
@@ -1050,7 +1062,7 @@ __global__ void __launch_bounds__(NW * 32, (WEIGH && D <= 64 ? 4 : D <= 128 && N
         top[tid] = inv[tid] = 0.f;
       }
       __syncthreads();
-      weigh_keys(weigh, b, kvh, ctx, tid, NW * 32, top, inv);
+      weigh_keys<D <= 64 ? 2 : 5>(weigh, b, kvh, ctx, tid, NW * 32, top, inv);
     }
     return;
   }
@@ -1195,7 +1207,7 @@ int launch_decode_attention_rope(const void* qkv, long long pitch, const DecodeR
 
 // What follows weighed decode attention where sequences are split: the keys' weights (even blocks of a pair) and the outputs from the splits' partials (odd ones).
 // grid (B * KV, 2 * parts): a part takes every parts-th 256 outputs or groups of four keys.
-__global__ void __launch_bounds__(256) weigh_kernel(const __grid_constant__ WeighArgs a) {
+__global__ void __launch_bounds__(256, 4) weigh_kernel(const __grid_constant__ WeighArgs a) {
   pdl_trigger();
   __shared__ float top[16], inv[16], factor[16][kWeighMaxSplits];
   const int b = blockIdx.x / a.KV, kvh = blockIdx.x % a.KV, t = threadIdx.x, lane = t & 31, warp = t >> 5, G = a.H / a.KV;
@@ -1236,7 +1248,7 @@ __global__ void __launch_bounds__(256) weigh_kernel(const __grid_constant__ Weig
     }
   }
   if (weights) {
-    if (weigh_slot(a, b)) weigh_keys(a, b, kvh, ctx, first, step, top, inv);  // (a barrier in weigh_slot where it is true)
+    if (weigh_slot(a, b)) weigh_keys<2>(a, b, kvh, ctx, first, step, top, inv);  // (a barrier in weigh_slot where it is true)
     return;
   }
   __syncthreads();

@@ -508,7 +508,7 @@ struct MoveUnit<2> {
 
 // grid (parts of a slot, tensors, requests): a part takes every gridDim.x-th 256 units
 template <int UNIT, int MAXW>
-__global__ void __launch_bounds__(256) beam_move_kernel(const __grid_constant__ BeamMoveArgs a) {
+__global__ void __launch_bounds__(256, MAXW <= 4 ? 5 : MAXW <= 8 ? 4 : MAXW <= 16 ? 2 : 1) beam_move_kernel(const __grid_constant__ BeamMoveArgs a) {
   using U = typename MoveUnit<UNIT>::type;
   pdl_trigger();
   pdl_wait();
