@@ -553,7 +553,9 @@ struct DecodeRope {};
 template <>
 struct DecodeRope<true> : DecodeRopeArgs {};
 // WEIGH: every score goes to fp32 [B, H, S] as well, so that what is behind a sequence's last key (this CTA where it is the only split, weigh_kernel where not) can
-// add the probabilities to the keys' weights: 4 bytes per key and query head written and read again, out of L2, for no second product of queries and keys.
+// add the probabilities to the keys' weights: 4 bytes per key and query head written and read again, out of L2, for no second product of queries and keys. Keys and values are the
+// first to leave L2 here, so that the scores stay (64 x 2176 keys 96 us, 104 without). 64 x 2176 keys, 32 heads on 8: 94 us (87.4 for decode attention that weighs nothing), one sequence of 4,000 9.8 (8.4),
+// 128 of 100 to 600 keys, 16 heads of 64 per KV head 22 (17): what is left is the tail of every CTA, which waits for its scores. (The weights by a kernel of their own: 104 and 28 us where this was 104 and 25.)
 // This form looks at what it is given: lengths end with the block table, pages outside the cache are read as page 0 and reported.
 template <bool WEIGH>
 struct DecodeWeigh {};

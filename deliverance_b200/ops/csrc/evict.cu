@@ -68,7 +68,7 @@ struct EvictTask {
     const bool ok = n == 0 || slot_ok(a.slots, b, a.num_slots);
     if (layer == 0 && kvh == 0 && t == 0) {
       a.lens[b] = ok ? min(n, a.keep) : n;
-      if (!ok) atomicCAS(a.status, kStatusOk, kStatusBadArgs);
+      if (!ok || a.ctx[b] != n) atomicCAS(a.status, kStatusOk, kStatusBadArgs);
     }
     if (!ok || n <= a.keep) {
       for (int j = t; j < a.keep; j += blockDim.x) kept[j] = ok && j < n ? j : -1;
@@ -249,7 +249,9 @@ struct RowUnit<2> {
 
 // grid (2 * slices, B * KV, layers): a CTA moves a range of columns of all rows of K or V of one head, in ascending batches of rows that are read as a
 // whole before they are written. Sources lie at or behind their targets, so no batch reads what an earlier one wrote, and in place is safe. The places of a
-// batch's rows are looked up once per row, while the rows of the batch in front are on their way.
+// batch's rows are looked up once per row, while the rows of the batch in front are on their way (looked up by every thread for itself: 16 sequences of 2,304 rows in
+// 36 layers 2,509 us instead of 1,590). 9.6 GB in 1,470 us, the copy rate; 288 heads of 1,024 rows 50 us, 47 at the copy rate. (Selection and move in one kernel: 1,850 us. Registers
+// spill, and while one CTA of an SM selects, only the other moves.)
 constexpr int kMoveThreads = 512, kMoveBatch = 8;
 template <int UNIT>
 __global__ void __launch_bounds__(kMoveThreads, 2) evict_move_kernel(const __grid_constant__ EvictArgs a, int slices, int most_lines) {

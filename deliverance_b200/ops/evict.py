@@ -47,7 +47,9 @@ def evict_keys(k_caches, v_caches, weights, block_tables, ctx_lens, slots, keep:
     ``weights[layer][slots[b]]``; the weights behind them, up to the old length, become zero. Sequences that are short enough keep everything, and with ``out_tables`` move too.
 
     ``k_caches`` / ``v_caches``: per layer ``[pages, KV, page, D]`` (widths may differ); ``weights``: per layer fp32 ``[slots, KV, capacity]``; ``block_tables`` / ``out_tables`` int32 ``[B, pages]``,
-    ``ctx_lens`` int32 ``[B]``, ``slots`` int64 ``[B]``, all different (0, the scratch slot: only for sequences of length 0). An entry of ``out_tables`` is either the page that ``block_tables`` has in the same place or a page that no sequence of the call reads.
+    ``ctx_lens`` int32 ``[B]``, ``slots`` int64 ``[B]``, all different (0, the scratch slot: only for sequences of length 0). An entry of ``out_tables`` is either the page that ``block_tables`` has in the same place, if no other sequence has it, or a page that no sequence of the
+    call reads: what sequences share (a cached prefix, beams) is replaced, not changed. A sequence on a slot that another one has, or outside the weights, is left as it is; that, pages
+    outside the caches and lengths beyond the table are reported by :func:`ops.check_status` (on the CPU: raised).
     Returns the rows that were kept, int32 ``[layers, B, KV, keep]`` (-1 behind a sequence's end), and the new lengths, int32 ``[B]``."""
     if ctx_lens.is_cuda:  # (the extension checks: a loop over the layers here takes longer than the kernels)
         kept, lens, launches = ops.require_ext().evict_keys(k_caches, v_caches, weights, block_tables, ctx_lens, slots, keep, recent, block_tables if out_tables is None else out_tables)

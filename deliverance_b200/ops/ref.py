@@ -467,6 +467,8 @@ def evict_keys(k_caches, v_caches, weights, block_tables, ctx_lens, slots, keep:
     used = [int(s) for s, n in zip(slots.tolist(), ctx_lens.tolist()) if n > 0]
     if len(set(used)) < len(used) or any(not 0 < s < weights[0].shape[0] for s in used):
         raise IndexError("weight slots must be different ones inside the weights")
+    if any(not 0 <= n <= block_tables.shape[1] * P for n in ctx_lens.tolist()):
+        raise IndexError("a length beyond the block table")
     for b in range(B):
         n, slot = int(ctx_lens[b]), int(slots[b])
         m = min(n, keep)

@@ -118,6 +118,21 @@ def test_select_ties_go_to_the_lowest(device):
     assert beam_select(zeros.to(device), torch.zeros(1, 1).to(device), 4)[2][0].tolist() == [1, 2, 3, 4]
 
 
+@pytest.mark.gpu
+def test_select_ties_over_many_groups():
+    """One value everywhere, in more groups than are listed; the same with a masked start; two beams of which the second is behind."""
+    for W, V, dtype in ((8, 20000, F32), (5, 60001, BF16)):
+        rows = torch.full((W, V), 3.25, dtype=dtype).cuda()
+        _, p, t = (x.cpu() for x in beam_select(rows, torch.zeros(1, W).cuda(), 64))
+        assert (p == 0).all() and t[0].tolist() == list(range(64))
+        bits = torch.ones(W, V, dtype=torch.bool)
+        bits[0] = False
+        bits[1, : V - 10] = False
+        _, p, t = (x.cpu() for x in beam_select(rows, torch.tensor([[0.0, -12.0] + [-1.0] * (W - 2)]).cuda(), 64, pack(bits).cuda()))
+        # ten tokens of the second beam at a tenth each beat V of the others only if -12 - log 10 > -1 - log V, which it does not
+        assert (p == 2).all() and t[0].tolist() == list(range(64))
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("order", ["rising", "falling"])
 def test_select_sorted_rows(device, order):
@@ -371,6 +386,25 @@ def test_engine_beams_in_batches_and_repeats(tmp_path):
     assert [engine_of(model).generate(q, p).token_ids for q in prompts] == [a[0].token_ids for a in alone]
     assert [r.token_ids for r in engine_of(model).generate_batch(prompts, p)] == [a[0].token_ids for a in alone]
     assert len(greedy) == 5
+
+
+def test_beam_search_through_the_model_api(tmp_path):
+    """Text in, ranked texts out; the first one is what ``generate`` answers."""
+    from deliverance_b200.api import CausalLanguageModel
+    from deliverance_b200.tokenizer.auto import AutoTokenizer
+
+    model = tiny_model(tmp_path, "llama")
+    clm = CausalLanguageModel(model, engine_of(model), AutoTokenizer.from_pretrained(str(tmp_path / "llama")), "t")
+    p = params_of(num_beams=3, max_tokens=8)
+    hyps = clm.generate_beams("Why is the sky blue?", p)
+    best = clm.generate("Why is the sky blue?", p)
+    assert best.token_ids == hyps[0].token_ids and best.text == hyps[0].text and best.score == hyps[0].score
+    assert [r.score for r in hyps] == sorted([r.score for r in hyps], reverse=True) and all(isinstance(r.text, str) for r in hyps)
+    assert [r.token_ids for r in clm.generate_many(["Why is the sky blue?", "Hi"], p)][0] == best.token_ids
+    with pytest.raises(ValueError):
+        clm.generate("Hi", p, on_event=lambda *a: None)
+    with pytest.raises(ValueError):
+        clm.submit("Hi", p)
 
 
 def test_engine_beams_refusals(tmp_path):

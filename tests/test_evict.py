@@ -286,6 +286,165 @@ def test_refusals(device):
         ops.check_status(0)
 
 
+# ---------------------------------------------------------------------------------------------------------------- together
+def run_together(device, steps=24, W=3, L=2, KV=2, G=4, D=64, keep=40, recent=10):
+    """Beams of one request on a bounded cache, operator by operator: every step writes a row per beam, attends and adds weights in all layers, selects, reorders pages, weights
+    and a recurrent state; every eight steps all beams are shortened into pages of their own. Returns everything that can be compared."""
+    from deliverance_b200.ops.beam import beam_reorder, beam_select
+
+    g = torch.Generator().manual_seed(3)
+    rnd = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    to = lambda t: t.to(device)  # noqa: E731
+    pool = 64
+    k, v = ([to(rnd(pool, KV, P, D).to(BF16)) for _ in range(L)] for _ in range(2))
+    weights = [to(torch.zeros(W + 1, KV, 160)) for _ in range(L)]
+    state = to(rnd(W + 1, 50))
+    n, free = 70, list(range(pool - 1, 0, -1))
+    shared = [free.pop() for _ in range(n // P)]
+    pages = [shared + [free.pop()] for _ in range(W)]
+    slots = to(torch.arange(1, W + 1))
+    for layer in range(L):  # all beams start with the same rows
+        for j in range(1, W):
+            k[layer][pages[j][-1]] = k[layer][pages[0][-1]]
+            v[layer][pages[j][-1]] = v[layer][pages[0][-1]]
+    scores, picked, kept_rows = torch.tensor([[0.0, -0.5, -1.0]]), [], []
+    for step in range(steps):
+        if n % P == 0:
+            for pg in pages:
+                pg.append(free.pop())
+        for layer in range(L):
+            for pg in pages:
+                k[layer][pg[n // P], :, n % P] = to(rnd(KV, D).to(BF16))
+                v[layer][pg[n // P], :, n % P] = to(rnd(KV, D).to(BF16))
+        n += 1
+        table = torch.zeros(W, 8, dtype=torch.int32)
+        for j, pg in enumerate(pages):
+            table[j, : len(pg)] = torch.tensor(pg)
+        ctx = torch.full((W,), n, dtype=torch.int32)
+        outs = [decode_attention_weighted(to(rnd(W, KV * G * D).to(BF16)), k[i], v[i], to(table), to(ctx), KV * G, D**-0.5, weights[i], slots, splits=1 + step % 5) for i in range(L)]
+        values, parents, tokens = beam_select(to(rnd(W, 1000) * 3), to(scores), 2 * W)
+        picked.append((parents.cpu(), tokens.cpu()))
+        par = parents[:, :W].contiguous()
+        full = n // P
+        lists = [pages[p][:full] for p in par[0].tolist()]
+        tails = torch.tensor([[pg[full] if n % P else 0 for pg in pages]])
+        beam_reorder(par, states=weights + [state], slots=slots.view(1, -1), caches=k + v if n % P else (), pages=to(tails) if n % P else None,
+                     rows=to(torch.tensor([n % P], dtype=torch.int32)) if n % P else None)
+        pages = [a + pg[full:] for a, pg in zip(lists, pages)]
+        scores = values[:, :W].cpu()
+        if step % 8 == 7:
+            table = torch.zeros(W, 8, dtype=torch.int32)
+            out = torch.zeros(W, 2, dtype=torch.int32)
+            fresh = [[free.pop(), free.pop()] for _ in range(W)]
+            for j, pg in enumerate(pages):
+                table[j, : len(pg)] = torch.tensor(pg)
+                out[j] = torch.tensor(fresh[j])
+            kept, lens = evict_keys(k, v, weights, to(table), to(ctx), slots, keep, recent, to(out))
+            assert lens.tolist() == [keep] * W
+            kept_rows.append(kept.cpu())
+            pages, n = fresh, keep
+    if device == "cuda":
+        ops.check_status(0)
+    return picked, kept_rows, [t.cpu() for t in weights], state.cpu(), [dense(t.cpu(), torch.tensor(pg), n) for t in k + v for pg in pages], [o.cpu().float() for o in outs]
+
+
+def test_operators_together_on_the_cpu():
+    picked, kept, weights, state, rows, outs = run_together("cpu")
+    assert len(kept) == 3 and all((r[:, :, :, 1:] > r[:, :, :, :-1]).all() for r in kept)
+    # what a row has gathered since it came is at most one per query head and step
+    assert all(float(w.max()) <= 4 * 24 and float(w[:, :, 40:].abs().max()) == 0 for w in weights)
+
+
+@pytest.mark.gpu
+def test_operators_together():
+    a, b = run_together("cpu"), run_together("cuda")
+    for (p, t), (q, u) in zip(a[0], b[0]):
+        assert torch.equal(p, q) and torch.equal(t, u)
+    assert all(torch.equal(x, y) for x, y in zip(a[1], b[1]))
+    for x, y in zip(a[2], b[2]):
+        # (24 steps of the tolerance that a step has against 64 bits, on either side)
+        assert (x - y).abs().max() <= 2 * 24 * 4 * (5 * 8 * 66 * 2**-24 + 64 * 2**-23 + 100 * 2**-24)
+    assert torch.equal(a[3], b[3]) and all(torch.equal(x, y) for x, y in zip(a[4], b[4]))
+    assert all((x - y).abs().max() <= 2**-8 * (x.abs().max() + 6) + 2**-8 * x.abs().max() for x, y in zip(a[5], b[5]))
+
+
+@pytest.mark.gpu
+def test_captured_and_replayed():
+    """Attention, eviction and reordering in two captured graphs, replayed in turn, against the same calls made one by one; on a stream of their own too."""
+    from deliverance_b200.ops.beam import beam_reorder
+
+    def world(seed):
+        g = torch.Generator().manual_seed(seed)
+        rnd = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+        table, pages = tables_for([100, 77])
+        s = dict(k=rnd(pages, 2, P, 64).to(BF16).cuda(), v=rnd(pages, 2, P, 64).to(BF16).cuda(), w=torch.rand(3, 2, 128, generator=g).cuda(), q=rnd(2, 512).to(BF16).cuda(),
+                 table=table.cuda(), ctx=torch.tensor([100, 77], dtype=torch.int32).cuda(), short=torch.tensor([50, 50], dtype=torch.int32).cuda(), slots=torch.tensor([2, 1]).cuda(),
+                 parents=torch.tensor([[1, 1]]).cuda(), rows=torch.tensor([18], dtype=torch.int32).cuda())
+        s["tails"] = s["table"][:, 1].long().view(1, 2).contiguous()
+        return s
+
+    def work(s):
+        o = decode_attention_weighted(s["q"], s["k"], s["v"], s["table"], s["ctx"], 8, 0.125, s["w"], s["slots"], splits=4)
+        kept, _ = evict_keys([s["k"]], [s["v"]], [s["w"]], s["table"], s["ctx"], s["slots"], 50, 9)
+        beam_reorder(s["parents"], [s["w"]], s["slots"].view(1, 2), [s["k"], s["v"]], s["tails"], s["rows"])
+        return [o, kept, s["k"], s["v"], s["w"]]
+
+    want, graphs = [], []
+    for seed in (1, 2):
+        torch.manual_seed(seed)
+        a = world(seed)
+        torch.manual_seed(seed)
+        b = world(seed)
+        steps = [[t.clone() for t in work(a)] for _ in range(3)]
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            got = work(b)
+        want.append(steps)
+        graphs.append((g, got, b))  # (a graph reads its inputs where they are)
+    for i in range(3):
+        for (g, got, _), steps in zip(graphs, want):
+            g.replay()
+            torch.cuda.synchronize()
+            for x, y in zip(got, steps[i]):
+                assert torch.equal(x, y)
+    side = torch.cuda.Stream()
+    torch.manual_seed(1)
+    c = world(1)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = work(c)
+    side.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, want[0][0]))
+    ops.check_status(0)
+
+
+@pytest.mark.gpu
+def test_outputs_and_workspaces_stay_inside_their_guards():
+    from deliverance_b200.ops.beam import beam_select
+
+    ops.set_bounds_check(True)
+    try:
+        for lens, splits, D, KV, G in (([700, 31, 32, 0], 8, 64, 2, 5), ([64] * 40, 1, 128, 1, 16), ([500], 40, 256, 2, 1)):
+            run_attention("cuda", D, KV, G, lens, splits, 0.0, 0)
+        run_evict("cuda", [513, 512, 3], 200, 31)
+        run_evict("cuda", [9000, 40], 4000, 31, L=1, KV=1, D=8)
+        for B, W, V, k in ((1, 1, 7, 7), (2, 3, 4097, 6), (3, 5, 50257, 64)):
+            beam_select(torch.randn(B * W, V).cuda(), torch.zeros(B, W).cuda(), k)
+        torch.cuda.synchronize()
+        ops.check_guards()
+    finally:
+        ops.set_bounds_check(False)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_evict_length_beyond_the_table(device):
+    k, w = torch.zeros(4, 1, P, 8, dtype=BF16, device=device), torch.zeros(3, 1, 64, device=device)
+    with pytest.raises((IndexError, RuntimeError)):
+        evict_keys([k], [k.clone()], [w], torch.ones(1, 1, dtype=torch.int32, device=device), torch.tensor([40], dtype=torch.int32, device=device), torch.ones(1, dtype=torch.int64, device=device), 8, 2)
+        ops.check_status(0)
+
+
 # ---------------------------------------------------------------------------------------------------------------- engine
 def tiny_model(tmp, device="cpu", family="llama", **over):
     from deliverance_b200.ckpt.loader import WeightLoader
@@ -443,11 +602,13 @@ def test_engine_bounded_cache_refusals(tmp_path):
             engine_of(tiny_model(tmp_path, family=family), 64)
 
 
-def test_engine_beams_on_a_bounded_cache(tmp_path):
+@pytest.mark.parametrize("device", DEVICES)
+def test_engine_beams_on_a_bounded_cache(tmp_path, device):
     """Beam search keeps whole caches; requests before and after it are shortened."""
     from deliverance_b200.params import GeneratorParameters
 
-    model = tiny_model(tmp_path)
+    over = dict(hidden_size=256, num_attention_heads=4, num_key_value_heads=2, head_dim=64) if device == "cuda" else {}
+    model = tiny_model(tmp_path, device, "qwen3" if over else "llama", **over)
     prompt = [(7 * i * i + 3 * i + 11) % 200 + 3 for i in range(50)]
     p = GeneratorParameters(max_tokens=30, num_beams=3)
     want = [r.token_ids for r in engine_of(model).generate_beams([prompt], p)[0]]
@@ -456,6 +617,36 @@ def test_engine_beams_on_a_bounded_cache(tmp_path):
     assert [r.token_ids for r in e.generate_beams([prompt], p)[0]] == want
     assert e.generate(prompt, params_of(40)).token_ids == first
     e.kv.audit([])
+
+
+def test_engine_bounded_cache_and_beams_under_tensor_parallelism(tmp_path):
+    """Two ranks as threads: each shortens its own KV heads and takes the same beams; the tokens are those of one rank."""
+    import threading
+
+    from deliverance_b200.ckpt.loader import WeightLoader
+    from deliverance_b200.ckpt.tiny import write_tiny_model
+    from deliverance_b200.config import load_config
+    from deliverance_b200.models.transformer import DecoderModel
+    from deliverance_b200.parallel.context import InProcessCollectives, InProcessGroup, TensorParallelContext
+
+    d = str(tmp_path / "tp")
+    write_tiny_model(d, "llama", seed=5, std=0.25)
+    prompt = [(7 * i * i + 3 * i + 11) % 200 + 3 for i in range(50)]
+
+    def run(ctx, out, i):
+        try:
+            e = engine_of(DecoderModel(load_config(d), "cpu", tp=ctx).load(WeightLoader(d)), 30, 8, 9)
+            out[i] = (e.generate(prompt, params_of(40)).token_ids, [r.token_ids for r in e.generate_beams([prompt], params_of(12, num_beams=3))[0]], e.metrics["evictions"])
+        except Exception as x:  # noqa: BLE001
+            out[i] = x
+
+    single, out, group = [None], [None, None], InProcessGroup(2, timeout=60)
+    run(TensorParallelContext(), single, 0)
+    ts = [threading.Thread(target=run, args=(TensorParallelContext(r, 2, InProcessCollectives(group, r)), out, r)) for r in range(2)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    assert not isinstance(out[0], Exception), out[0]
+    assert out[0] == out[1] == single[0] and single[0][2] > 2
 
 
 @pytest.mark.gpu
