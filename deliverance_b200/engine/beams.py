@@ -59,6 +59,8 @@ class BeamSearch:
 
     def run(self, prompts: list) -> list:
         e = self.e
+        if not (e.waiting or e.running):
+            e._drain()  # the step that was launched ahead of a request's last token
         if e.has_work():
             raise RuntimeError("beam search and scheduled requests do not share an engine at the same time")
         most = max(1, e.config.max_seqs // self.W)
