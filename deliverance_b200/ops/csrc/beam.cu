@@ -14,7 +14,7 @@ namespace dlv {
 
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr int kPerLane = 16;                      // logits per lane and tile
 constexpr int kTile = kThreads * kPerLane;        // logits of a CTA's tile
 constexpr int kMergeThreads = 512, kMergeWarps = kMergeThreads / 32;
@@ -84,12 +84,14 @@ __device__ __forceinline__ float redux_max(float v) {
 }
 
 // grid: B * W * splits. A tile is 16 logits per thread, 16 bytes of a warp's lanes side by side: one group per load. The next tile is on its way while a tile is
-// worked on; a running maximum and sum per thread, joined at the end in a fixed order. What bounds it: the loads in flight. 256 rows of 151,936: 29 us, 24 at the copy rate (5.3 TB/s; 9
-// instructions per logit, which are not it: with 14 the same time, with expf and 20 instructions 35 us; 32 logits per thread 37 for the whole selection instead of 36, 8 logits 38 to 45).
+// worked on; a running maximum per warp (the groups' maxima are there anyway; one per lane moves in nearly every tile of some lane) and a sum per thread, joined at the end in a fixed
+// order. 256 rows of 151,936, the whole selection: 34.7 us, 24 at the copy rate of fp32 (29.0 and 12 in bf16, where some ten instructions per logit and one exponential
+// in 16 a cycle hold it). With expf 42; 32 logits per thread 37, 8 logits 38 to 45; two more tiles on their way through shared memory 46 (16-byte asynchronous copies per thread) and
+// 57 (bulk copies per warp).
 // (Candidates listed in this kernel instead of groups' maxima were 33 of 74 us: every tile has one in some warp, and all lanes wait while it is listed.)
 // PLAIN: neither scale nor cap.
 template <typename T, bool MASK, bool ALIGNED, bool PLAIN>
-__global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_constant__ BeamSelectArgs a) {
+__global__ void __launch_bounds__(kThreads, 8) beam_part_kernel(const __grid_constant__ BeamSelectArgs a) {
   pdl_trigger();
   pdl_wait();
   __shared__ double sums[kWarps];
@@ -101,7 +103,7 @@ __global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_con
   const T* x_row = static_cast<const T*>(a.logits) + static_cast<long long>(row) * a.ld;
   const uint32_t* bits = MASK ? a.mask + static_cast<long long>(row) * a.mask_ld : nullptr;
   float* group_max = a.group_max + static_cast<long long>(row) * a.groups;
-  float m = -FLT_MAX;
+  float m = -FLT_MAX;  // (the warp's)
   double sum = 0.0;
   uint4 raw[NV];
   uint32_t word[NV];
@@ -140,14 +142,14 @@ __global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_con
       float g = x[v][0];
 #pragma unroll
       for (int e = 1; e < N; ++e) g = fmaxf(g, x[v][e]);
-      top = fmaxf(top, g);
       g = redux_max(g);
+      top = fmaxf(top, g);
       if (lane == v) mine = g;
     }
     const int group = at / (32 * N) + warp * NV + lane;
     if (lane < NV && group * 32 * N < hi) group_max[group] = mine;
     const float top_z = PLAIN ? top : post(top, a.softcap, a.inv_scale);
-    if (top_z > m) {
+    if (top_z > m) {  // (the same for the whole warp)
       sum *= static_cast<double>(expf(m - top_z));
       m = top_z;
     }
@@ -162,12 +164,10 @@ __global__ void __launch_bounds__(kThreads, 4) beam_part_kernel(const __grid_con
     const float part = __uint_as_float(static_cast<uint32_t>(part2)) + __uint_as_float(static_cast<uint32_t>(part2 >> 32));
     sum += static_cast<double>(part);
   }
-  const float wm = warp_max(m);
-  sum *= static_cast<double>(expf(m - wm));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) {
-    tops[warp] = wm;
+    tops[warp] = m;
     sums[warp] = sum;
   }
   __syncthreads();
@@ -255,9 +255,13 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
   const int K = a.K, W = a.W, n = W * a.groups;
   const float* maxima = a.group_max + static_cast<long long>(b) * n;
   constexpr int AHEAD = 12;
+  // Of few groups a cluster has every 64th, so that those of one beam are spread over all clusters: neighbours in one cluster made bounds that thousands of candidates
+  // reach (3 requests of 12 beams and 1,300 tokens 33 us instead of 12, 20 of 16 guided beams and 3,000 tokens 54 instead of 19). Many groups spread by themselves, and
+  // are read side by side (4 x 16 beams of 151,936 tokens 30 us instead of 32).
+  const int own = n <= 8 * kMergeThreads ? (t & 7) * kClusters + (t >> 3) : t;
   float x[AHEAD];  // (on their way while the sums are joined)
 #pragma unroll
-  for (int j = 0; j < AHEAD; ++j) x[j] = j * kMergeThreads + t < n ? maxima[j * kMergeThreads + t] : -INFINITY;
+  for (int j = 0; j < AHEAD; ++j) x[j] = j * kMergeThreads + own < n ? maxima[j * kMergeThreads + own] : -INFINITY;
   if (t == 0) listed = n_groups = 0;
   for (int w = warp; w < W; w += kMergeWarps) {
     const long long at = (static_cast<long long>(b) * W + w) * a.splits;
@@ -293,11 +297,11 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
   float best = -INFINITY;
 #pragma unroll
   for (int j = 0; j < AHEAD; ++j) {
-    const int i = j * kMergeThreads + t;
+    const int i = j * kMergeThreads + own;
     x[j] = i < n ? rough_of(x[j], i) : -INFINITY;
     best = fmaxf(best, x[j]);
   }
-  for (int i0 = AHEAD * kMergeThreads + t; i0 < n; i0 += 8 * kMergeThreads) {
+  for (int i0 = AHEAD * kMergeThreads + own; i0 < n; i0 += 8 * kMergeThreads) {
     float y[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[j] = i0 + j * kMergeThreads < n ? maxima[i0 + j * kMergeThreads] : -INFINITY;
@@ -338,8 +342,8 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
   };
 #pragma unroll
   for (int j = 0; j < AHEAD; ++j)
-    if (x[j] > -INFINITY && x[j] >= bound) list_group(j * kMergeThreads + t);
-  for (int i0 = AHEAD * kMergeThreads + t; i0 < n; i0 += 8 * kMergeThreads) {
+    if (x[j] > -INFINITY && x[j] >= bound) list_group(j * kMergeThreads + own);
+  for (int i0 = AHEAD * kMergeThreads + own; i0 < n; i0 += 8 * kMergeThreads) {
     float y[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[j] = i0 + j * kMergeThreads < n ? maxima[i0 + j * kMergeThreads] : -INFINITY;
@@ -450,9 +454,12 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
 
 int beam_select_group(bool f32) { return f32 ? 32 * Vec<float>::N : 32 * Vec<__nv_bfloat16>::N; }
 
-// CTAs per row: the fewest that keep the GPU about evenly busy (four resident per SM), each with a tile at least.
+// CTAs per row. Much work: four units each, which end at different times and so keep the GPU full (256 rows of 151,936 with 4 / 10 / 13 CTAs each: 36.7 / 34.7 / 35.9 us, in bf16 33.3 / 29.0 / 29.3).
+// Otherwise the fewest that keep the GPU about evenly busy (eight resident per SM), each with a unit at least (256 rows of 32,000 with 4 / 8: 14.4 / 14.7).
 int beam_select_splits(int rows, int V) {
-  const int tiles = (V + kTile - 1) / kTile, slots = 4 * 148;
+  const int tiles = (V + kBeamSplitUnit - 1) / kBeamSplitUnit, slots = 8 * 148;
+  const long long quarters = (tiles + 3) / 4;
+  if (rows * quarters >= 2 * slots) return static_cast<int>(quarters);
   int best = 1;
   double most = 0.0;
   for (int s = 1; s <= tiles && s <= 64; ++s) {
