@@ -10,14 +10,13 @@ namespace dlv {
 
 namespace {
 
-constexpr size_t kSelectShared = 220 * 1024;
-
 // larger = heavier; NaN is the smallest, -0 equals 0
 __device__ __forceinline__ uint32_t weight_order(float w) {
   if (w != w) return 0u;
   const uint32_t u = __float_as_uint(w + 0.f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float weight_of(uint32_t order) { return __uint_as_float(order & 0x80000000u ? order ^ 0x80000000u : ~order); }
 
 // sum over the CTA's NT threads; `red`: two buffers used in turn, one barrier per call
 template <int NT>
@@ -82,32 +81,31 @@ struct EvictTask {
   }
 };
 
-// grid (KV, B, layers). Up to R * NT rows: the weights go through shared memory, every thread holds R neighbouring ones as ordered integers in registers.
-// The edge (what the want-th heaviest weighs) is found bit by bit, a count over the CTA each, until exactly `want` keys reach it. Shared: R * NT weights, keep rows.
-template <int NT, int R>
-__global__ void __launch_bounds__(NT) evict_select_kernel(const __grid_constant__ EvictArgs a) {
+// grid (KV, B, layers). Up to R * NT rows, `rounds` per thread: a warp has neighbouring rows, 32 at a time, and every thread its rows' weights as ordered integers in registers.
+// The edge (what the want-th heaviest weighs) is found bit by bit, a count over the CTA each, until exactly `want` keys reach it. Places are counted by ballots,
+// and the weights that stay are written from the registers. What bounds it: issue (some 80 instructions per row) and, with 1,024 threads, the barriers of the search.
+// 4,608 heads of 2,304 rows 63 us with 256 threads of 10 rows and four CTAs per SM (five 63, six 66; 512 of 5 83; 128 of 20 71; with rows side by side in a thread, by way of shared memory, 109),
+// 256 heads of 30,000 rows 44 to 71 us with 1,024 of 36 (512 of 72 76 to 101), 1,024 of 9,000 rows 64 with 512 of 20 (one CTA per SM 76; 1,024 of 10 76; 256 of 40 92).
+template <int NT, int R, int CTAS>
+__global__ void __launch_bounds__(NT, CTAS) evict_select_kernel(const __grid_constant__ EvictArgs a) {
   pdl_trigger();
   pdl_wait();
-  extern __shared__ float weight[];  // padded by one per 32: threads read R neighbours each
-  __shared__ int red[2 * (NT / 32)];
-  const int t = threadIdx.x;
+  constexpr int WARPS = NT / 32;
+  __shared__ int red[2 * WARPS];
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   EvictTask k;
   if (!k.open(a)) return;
-  auto at = [](int i) { return i + (i >> 5); };
-  int* list = reinterpret_cast<int*>(weight + at(R * NT));
-  constexpr int BATCH = R < 16 ? R : 18;
-  for (int i0 = t; i0 < k.n; i0 += BATCH * NT) {
-    float v[BATCH];
+  const int rounds = (k.n + NT - 1) / NT;  // (at most R: the launcher's choice)
+  const int first = warp * rounds * 32 + lane, end = (warp + 1) * rounds * 32;
+  // row first + 32 r is one of this thread's, has a weight, can go: for 32 r below
+  const int mine = min(k.n, end) - first, weighed = min(k.counted, end) - first, open = min(k.old, end) - first;
+  const uint32_t before = (1u << lane) - 1u;
+  const float* w = k.w + first;
+  uint32_t key[R];  // of the rows that can go, 0 for the others
 #pragma unroll
-    for (int r = 0; r < BATCH; ++r) v[r] = i0 + r * NT < k.counted ? k.w[i0 + r * NT] : 0.f;
+  for (int r = 0; r < R; ++r) key[r] = r * 32 < min(open, weighed) ? __float_as_uint(w[r * 32]) : 0u;  // (a row without a weight: 0.0)
 #pragma unroll
-    for (int r = 0; r < BATCH; ++r)
-      if (i0 + r * NT < R * NT) weight[at(i0 + r * NT)] = v[r];
-  }
-  __syncthreads();
-  uint32_t key[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) key[r] = t * R + r < k.old ? weight_order(weight[at(t * R + r)]) : 0u;
+  for (int r = 0; r < R; ++r) key[r] = r * 32 < open ? weight_order(__uint_as_float(key[r])) : 0u;
   uint32_t edge = 0xffffffffu;  // keys above the edge stay, and `spare` of those that equal it
   int spare = 0, turn = 0;
   if (k.want > 0) {
@@ -129,16 +127,29 @@ __global__ void __launch_bounds__(NT) evict_select_kernel(const __grid_constant_
       exact = c == k.want;
     }
     if (bit >= 0 && !exact) {  // one open key per thread from here on
-      __syncthreads();
+      const uint32_t range = bit == 31 ? 0xffffffffu : (2u << bit) - 1u;  // keys from edge to edge + range
+      int c = 0;
+#pragma unroll
+      for (int r = 0; r < R; ++r) c += r * 32 < open && key[r] - edge <= range ? 1 : 0;
+      int at = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, at, o);
+        at += lane >= o ? u : 0;
+      }
+      __syncthreads();  // (n_few is 0)
+      int base = 0;
+      if (lane == 31) base = atomicAdd(&n_few, at);
+      at += __shfl_sync(0xffffffffu, base, 31) - c;
 #pragma unroll
       for (int r = 0; r < R; ++r)
-        if (t * R + r < k.old && (static_cast<unsigned long long>(key[r]) >> (bit + 1)) == (static_cast<unsigned long long>(edge) >> (bit + 1))) few[atomicAdd(&n_few, 1)] = key[r];
+        if (r * 32 < open && key[r] - edge <= range) few[at++] = key[r];
       __syncthreads();
-      const uint32_t mine = t < n_few ? few[t] : 0u;
+      const uint32_t own = t < n_few ? few[t] : 0u;
       const int beyond = above;
       for (; bit >= 0 && !exact; --bit) {
         const uint32_t probe = edge | (1u << bit);
-        const int c = beyond + __syncthreads_count(mine >= probe);
+        const int c = beyond + __syncthreads_count(own >= probe);
         if (c >= k.want) edge = probe;
         exact = c == k.want;
         if (c < k.want) above = c;
@@ -147,34 +158,57 @@ __global__ void __launch_bounds__(NT) evict_select_kernel(const __grid_constant_
     if (exact) edge -= 1;  // (all that reach the probe: above probe - 1; a probe is not 0)
     else spare = k.want - above;
   }
-  // how many ties lie in front of a thread's rows, then how many rows that stay
-  int ties = 0, total;
+  // sum over the warps in front of this one of a number that a warp's lanes share
+  auto in_front = [&](int v) {
+    int* q = red + turn * WARPS;
+    turn ^= 1;
+    if (lane == 0) q[warp] = v;
+    __syncthreads();
+    return __reduce_add_sync(0xffffffffu, lane < warp ? q[lane] : 0);
+  };
+  int tie = 0;  // keys that equal the edge in front of a round
   if (spare > 0) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) ties += t * R + r < k.old && key[r] == edge ? 1 : 0;
-    ties = block_scan<NT>(ties, red, turn, total);
-    turn ^= 1;
+    for (int r = 0; r < R; ++r) {
+      if (r >= rounds) break;
+      tie += __popc(__ballot_sync(0xffffffffu, r * 32 < open && key[r] == edge));
+    }
+    tie = in_front(tie);
   }
-  int takes = 0, tie = ties;
+  uint32_t takes[(R + 31) / 32] = {};
+  int place = 0;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int i = t * R + r;
-    const bool even = i < k.old && key[r] == edge;
-    takes += i < k.n && (i >= k.old || key[r] > edge || (even && tie < spare)) ? 1 : 0;
-    tie += even ? 1 : 0;
+    if (r >= rounds) break;
+    bool take = r * 32 < mine && (r * 32 >= open || key[r] > edge);
+    if (spare > 0) {
+      const bool even = r * 32 < open && key[r] == edge;
+      const uint32_t all = __ballot_sync(0xffffffffu, even);
+      take = take || (even && tie + __popc(all & before) < spare);
+      tie += __popc(all);
+    }
+    takes[r / 32] |= (take ? 1u : 0u) << (r % 32);
+    place += __popc(__ballot_sync(0xffffffffu, take));
   }
-  takes = block_scan<NT>(takes, red, turn, total);
-  tie = ties;
+  if (open < mine) {  // the weights of the recent rows, as they are
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (r * 32 >= open && r * 32 < weighed) key[r] = __float_as_uint(w[r * 32]);
+  }
+  place = in_front(place);  // (with the barrier behind which all weights are in registers)
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int i = t * R + r;
-    const bool even = i < k.old && key[r] == edge;
-    if (i < k.n && (i >= k.old || key[r] > edge || (even && tie < spare)) && takes < a.keep) list[takes++] = i;
-    tie += even ? 1 : 0;
+    if (r >= rounds) break;
+    const bool take = (takes[r / 32] >> (r % 32)) & 1u;
+    const uint32_t all = __ballot_sync(0xffffffffu, take);
+    const int j = place + __popc(all & before);
+    if (take && j < a.keep) {
+      k.kept[j] = first + r * 32;
+      if (j < k.counted) k.w[j] = r * 32 < open ? weight_of(key[r]) : __uint_as_float(key[r]);
+    }
+    place += __popc(all);
   }
-  __syncthreads();
-  for (int j = t; j < a.keep; j += NT) k.kept[j] = list[j];
-  for (int j = t; j < k.counted; j += NT) k.w[j] = j < a.keep ? weight[at(list[j])] : 0.f;
+  for (int j = a.keep + t; j < k.counted; j += NT) k.w[j] = 0.f;
 }
 
 // The same for any length, with the weights read again for every count and the list in global memory.
@@ -316,18 +350,10 @@ void launch_evict(const EvictArgs& a, int unit, cudaStream_t st) {
   if (a.B == 0 || a.layers == 0 || a.KV == 0) return;
   const dim3 heads(a.KV, a.B, a.layers);
   const long long most = static_cast<long long>(a.table_width) * a.page;  // rows of a sequence
-  const auto shared = [&](int rows) { return (static_cast<size_t>(rows) * 33 / 32 + 1 + static_cast<size_t>(a.keep < most ? a.keep : most)) * 4; };
-#define DLV_EVICT_SELECT(NT, RR)                                                                                                          \
-  do {                                                                                                                                    \
-    static PerDeviceOnce once;                                                                                                            \
-    if (once.first()) cudaFuncSetAttribute(evict_select_kernel<NT, RR>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelectShared);      \
-    launch_pdl(evict_select_kernel<NT, RR>, heads, dim3(NT), shared(NT * RR), st, a);                                                     \
-  } while (0)
-  if (most <= 512 * 5 && shared(512 * 5) <= kSelectShared) DLV_EVICT_SELECT(512, 5);
-  else if (most <= 512 * 20 && shared(512 * 20) <= kSelectShared) DLV_EVICT_SELECT(512, 20);
-  else if (most <= 1024 * 36 && shared(1024 * 36) <= kSelectShared) DLV_EVICT_SELECT(1024, 36);
+  if (most <= 256 * 10) launch_pdl(evict_select_kernel<256, 10, 4>, heads, dim3(256), 0, st, a);
+  else if (most <= 512 * 20) launch_pdl(evict_select_kernel<512, 20, 2>, heads, dim3(512), 0, st, a);
+  else if (most <= 1024 * 36) launch_pdl(evict_select_kernel<1024, 36, 1>, heads, dim3(1024), 0, st, a);
   else launch_pdl(evict_select_long_kernel, heads, dim3(512), 0, st, a);
-#undef DLV_EVICT_SELECT
   // columns are cut (to 64 bytes at least) where there are too few heads to fill the GPU
   int wide = 0;
   for (int i = 0; i < a.layers; ++i) wide = a.layer[i].k_bytes > wide ? a.layer[i].k_bytes : wide;
