@@ -260,6 +260,10 @@ def test_evict_long_sequences():
     run_evict("cuda", [10241, 20000], 5000, 4999, L=1, KV=1, D=8)
     run_evict("cuda", [40000, 100], 10000, 17, L=1, KV=1, D=8)
     run_evict("cuda", [40000], 39999, 17, L=1, KV=1, D=8, weights=[torch.zeros(3, 1, 40000)])
+    for n in (2560, 9000, 30001):  # ties over many rows of a thread: few values, one value
+        run_evict("cuda", [n], n // 3, n // 7, L=1, KV=2, D=8, weights=[torch.randint(0, 3, (3, 2, n)).float()])
+        run_evict("cuda", [n], n - 1, 0, L=1, KV=1, D=8, weights=[torch.full((3, 1, n), 0.25)])
+        run_evict("cuda", [n], n // 2, 5, L=1, KV=1, D=8, capacity=n // 2 + 77)
 
 
 @pytest.mark.parametrize("device", DEVICES)
