@@ -455,9 +455,10 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
 int beam_select_group(bool f32) { return f32 ? 32 * Vec<float>::N : 32 * Vec<__nv_bfloat16>::N; }
 
 // CTAs per row. Much work: four units each, which end at different times and so keep the GPU full (256 rows of 151,936 with 4 / 10 / 13 CTAs each: 36.7 / 34.7 / 35.9 us, in bf16 33.3 / 29.0 / 29.3).
-// Otherwise the fewest that keep the GPU about evenly busy (eight resident per SM), each with a unit at least (256 rows of 32,000 with 4 / 8: 14.4 / 14.7).
+// Little work: a unit each (4 rows of 83,308 with 1 / 21 CTAs each: 17.9 / 9.2 us). Otherwise the fewest that keep the GPU about evenly busy (eight resident per SM), each with a unit at least (256 rows of 32,000 with 4 / 8: 14.4 / 14.7).
 int beam_select_splits(int rows, int V) {
   const int tiles = (V + kBeamSplitUnit - 1) / kBeamSplitUnit, slots = 8 * 148;
+  if (static_cast<long long>(rows) * tiles <= slots) return tiles;
   const long long quarters = (tiles + 3) / 4;
   if (rows * quarters >= 2 * slots) return static_cast<int>(quarters);
   int best = 1;
