@@ -23,14 +23,20 @@ def decode_attention_weighted(q, k_cache, v_cache, block_tables, ctx_lens, H, sc
     slots of a call are different ones; a second sequence on a slot, or a slot outside ``weights``, adds nothing and is reported by :func:`ops.check_status` (on the CPU:
     raised)."""
     if q.is_cuda:  # (the extension checks)
-        if not even:
+        B, (_, KV, page, D) = q.shape[0], k_cache.shape
+        if even:
+            # Of heads of 64 four CTAs are resident per SM, and parts are longer here (us, as many as the engine asks for / this: 6 sequences of 23,000 keys 48.7 / 38.6; 2 of 8,000 18.0 / 16.0;
+            # 1 of 60,000 28.7 / 19.5; 4 of 4,000 13.3 / 13.0). Of heads of 128 two are: 1 of 4,000 9.9 / 11.4, 3 of 20,000 49.3 / 49.5.
+            if D <= 64 and splits > 1:
+                splits = max(splits, min(ops.decode_room(B, H, KV, D), 128, block_tables.shape[1] * page // 128))
+        elif splits <= 32 and (plan is not None or block_tables.shape[1] * page >= 4096):
             # Splits by length pay here where splits by number do not, because every part's tail is longer: twice as many as the batch has use for, given to the long sequences
             # (us, as many as the engine asks for / this, plan kept by the caller: 16 sequences of 500 to 16,000 keys, heads of 64, 47.3 / 41.3; 24 of 100 to 6,000 25.6 / 19.1; 8 of 1,000 to 32,000, heads of
             # 128, 69.7 / 66.8; 12 of 50 to 500 11.8 / 11.9, and 13.3 with a plan of its own; 3 sequences, with room for 98, 19.1 / 22.8).
-            room = ops.decode_room(q.shape[0], H, k_cache.shape[1], k_cache.shape[3])
-            if splits <= room <= 32 and (plan is not None or block_tables.shape[1] * k_cache.shape[2] >= 4096):
+            room = ops.decode_room(B, H, KV, D)
+            if splits <= room <= 32:
                 splits = 2 * room
-        splits, used = ops.decode_launch(splits, even, plan, ctx_lens, q.shape[0], H, k_cache.shape[1], k_cache.shape[3], int(window))
+        splits, used = ops.decode_launch(splits, even, plan, ctx_lens, B, H, KV, D, int(window))
         out, launches = ops.require_ext().decode_attention_weighted(q, k_cache, v_cache, block_tables, ctx_lens, H, scale, softcap, window, splits, weights, slots, used)
         ops._count(launches)
         return out

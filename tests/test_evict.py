@@ -62,7 +62,7 @@ def test_weighted_attention_softcap_window(device, D, softcap, window):
     run_attention(device, D, 2, 2, [777, 16, 100, 101], 6, softcap, window)
 
 
-def run_attention(device, D, KV, G, lens, splits, softcap, window, capacity=None, extra=1):
+def run_attention(device, D, KV, G, lens, splits, softcap, window, capacity=None, extra=1, even=False):
     B, H = len(lens), KV * G
     table, pages = tables_for(lens, extra=extra)
     q = torch.randn(B, H * D).to(BF16)
@@ -79,7 +79,7 @@ def run_attention(device, D, KV, G, lens, splits, softcap, window, capacity=None
     w = to(start.clone())
     ctx = torch.tensor(lens, dtype=torch.int32)
     scale = D**-0.5
-    out = decode_attention_weighted(to(q), to(k), to(v), to(table), to(ctx), H, scale, w, to(slots), softcap, window, splits)
+    out = decode_attention_weighted(to(q), to(k), to(v), to(table), to(ctx), H, scale, w, to(slots), softcap, window, splits, even)
     if device == "cuda":
         ops.check_status(0)
     want, sums = plain_attention(q, k, v, table, lens, KV, scale, softcap, window)
@@ -103,6 +103,14 @@ def run_attention(device, D, KV, G, lens, splits, softcap, window, capacity=None
     for s in range(B + 2):
         if s not in slots.tolist():
             assert torch.equal(w[s], start[s].double())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens,splits", [([9000], 30), ([4001, 4000], 18), ([40, 33], 5), ([1], 2), ([0, 0], 3)])
+def test_weighted_attention_of_like_lengths(device, D, lens, splits):
+    run_attention(device, D, 2, 4, lens, splits, 0.0, 0, even=True)
+    run_attention(device, D, 1, 3, lens, splits, 30.0, 700, even=True)
 
 
 @pytest.mark.parametrize("device", DEVICES)
