@@ -324,17 +324,32 @@ class Engine:
         self.kv.ensure_pages(r.pages, n_tokens)
         return True
 
+    def _step_pages(self, reqs: list[Request]) -> int:
+        """Pages that the coming decode step takes from the pool: for new rows, less what the sequences that are shortened in front of it give back, and,
+        before anything is given back, for the pages that they replace because others hold them too."""
+        ref, keep = self.kv.allocator.ref, (self.config.kv.keep_tokens + self.page_size - 1) // self.page_size
+        replaced = grown = 0
+        for r in reqs:
+            if self.bounded and self._due(r):
+                replaced += sum(ref[p] > 1 for p in r.pages[:keep])
+                grown += self.config.kv.keep_tokens // self.page_size + 1 - keep - sum(ref[p] == 1 for p in r.pages[keep:])
+            else:
+                grown += self._new_pages(r, r.total_len + r.pending)
+        return replaced + max(0, grown)
+
     def _make_room_for_decode(self, reqs: list[Request]) -> tuple:
-        """Before a decode step: every sequence needs room for one more position (two with a token in flight). When the
-        pool cannot supply that, the step in flight is settled and the youngest sequences are preempted until it can."""
-        need = sum(self._new_pages(r, r.total_len + r.pending) for r in reqs)
+        """Before a decode step: every sequence needs room for one more position (two with a token in flight), a shared one that is to be shortened for pages of
+        its own. When the pool cannot supply that, the step in flight is settled and the youngest sequences are preempted until it can."""
+        need = self._step_pages(reqs)
         if need == 0 or self.kv.can_allocate(need):
             return reqs, []
         finished = self._drain()
         reqs = [r for r in reqs if r.state == RUNNING]
-        while reqs and not self.kv.can_allocate(sum(self._new_pages(r, r.total_len) for r in reqs)):
+        while reqs and not self.kv.can_allocate(self._step_pages(reqs)):
             v = self.running[-1]  # youngest first; that may be a request whose prefill is waiting for pages
-            if v is reqs[0]:
+            if v is reqs[0] and self.bounded and self._due(v) and self.kv.prefix.evict_one():
+                continue  # (a page that only cached prefixes share need not be replaced)
+            if v is reqs[0] and not (self.bounded and v is not self.running[0]):
                 self._fail_oom(v)
                 reqs.remove(v)
                 continue
@@ -532,21 +547,25 @@ class Engine:
                 seqs[-1]["prev"] = r.output[before - 1] if before > 0 else r.prompt[-1]
         return seqs
 
+    def _due(self, r: Request) -> int:
+        """Bounded cache: the rows that ``r`` holds if it is shortened in front of the coming decode step, else 0. That depends on the sequence alone, not on
+        what else runs."""
+        s, rows = self.config.kv, r.total_len - 1 + r.pending - r.evicted
+        return rows if rows > s.keep_tokens and (r.observed >= s.keep_every or rows >= self.kv.key_weights[0].shape[2]) else 0
+
     def _shorten(self, reqs: list[Request]) -> None:
         """Bounded cache: sequences that hold more than ``keep_tokens`` rows and have been observed long enough (or have no weights left) drop the rows that had the
-        least attention. Their own pages are filled from the front; a page that others hold too (cached prefixes) is replaced by a new one, or, where
-        there is none, the sequence waits. Launched behind the step in flight and in front of the next one."""
+        least attention. Their own pages are filled from the front; a page that others hold too (cached prefixes) is replaced by a new one
+        (``_make_room_for_decode`` has seen to it that there is one). Launched behind the step in flight and in front of the next one."""
         s, ps = self.config.kv, self.page_size
-        keep, cap = s.keep_tokens, self.kv.key_weights[0].shape[2]
+        keep = s.keep_tokens
         due, targets = [], []
         for r in reqs:
-            rows = r.total_len - 1 + r.pending - r.evicted
-            if rows <= keep or (r.observed < s.keep_every and rows < cap):
+            rows = self._due(r)
+            if not rows:
                 continue
             n = (keep + ps - 1) // ps
             shared = [i for i in range(n) if self.kv.allocator.ref[r.pages[i]] > 1]
-            if shared and not self.kv.can_allocate(len(shared)):
-                continue
             fresh: list[int] = []
             self.kv.ensure_pages(fresh, len(shared) * ps)
             target = r.pages[:n]

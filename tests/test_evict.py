@@ -681,3 +681,35 @@ def test_engine_bounded_cache_on_the_gpu(tmp_path, D, KV):
     # (batches of other sizes run other kernels, whose roundings differ: the schedules here are the same but for the step that lookahead settles late)
     assert outs[1] == outs[2]
     assert sum(a == b for x, y in zip(outs[0], outs[1]) for a, b in zip(x, y)) >= 0.5 * sum(map(len, outs[1]))
+
+
+def shared_head(lens, head=64):
+    """Prompts that begin alike."""
+    h = [(3 * i * i + 5) % 200 + 3 for i in range(head)]
+    return [h + [(7 * i + 11 * k) % 200 + 3 for i in range(n - head)] for k, n in enumerate(lens)]
+
+
+@pytest.mark.parametrize("lookahead", [False, "force"])
+@pytest.mark.parametrize("lens,keep,every,pages,steps", [([92, 84, 81], 83, 8, 8, 60), ([80, 68, 85], 92, 11, 7, 120), ([75, 81, 86], 86, 10, 7, 40), ([66, 95, 95, 70], 64, 3, 9, 40)])
+def test_engine_bounded_cache_replaces_shared_pages_in_a_small_pool(tmp_path, lens, keep, every, pages, steps, lookahead):
+    """The pages that replace shared ones come out of the pool that the step's new rows need too: both are counted before the step, and younger sequences make room."""
+    model = tiny_model(tmp_path)
+    e = engine_of(model, keep, 8, every, pages=pages, lookahead=lookahead)
+    rs = [e.add_request(p, params_of(steps)) for p in shared_head(lens)]
+    e.run()
+    assert [(len(r.output), r.error) for r in rs] == [(steps, None)] * len(rs)
+    e.kv.audit([])
+    assert e.metrics["evictions"] > 2 and len(e.kv.free_weight_slots) == 8
+
+
+def test_engine_bounded_cache_one_sequence_fills_the_pool(tmp_path):
+    """Shared with nothing but cached prefixes, in a pool that its rows fill: cached prefixes give way."""
+    model = tiny_model(tmp_path)
+    for lookahead in (False, "force"):
+        e = engine_of(model, 90, 8, 6, pages=4, lookahead=lookahead)  # three pages for 90 to 96 rows
+        prompt = shared_head([80])[0]
+        first = e.generate(prompt, params_of(60))
+        assert len(first.token_ids) == 60 and e.metrics["evictions"] > 5
+        e.kv.audit([])
+        assert e.generate(prompt, params_of(60)).token_ids == first.token_ids
+        assert first.token_ids == engine_of(model, 90, 8, 6).generate(prompt, params_of(60)).token_ids
