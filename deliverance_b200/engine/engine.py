@@ -62,6 +62,7 @@ class Request:
     evicted: int = 0  # rows dropped from a bounded cache: the cache row of position p is p - evicted
     weight_slot: int = -1  # its row of key weights
     observed: int = 0  # decode steps whose attention its weights hold
+    saved: Optional[tuple] = None  # preempted from a bounded cache: its rows and weights on the host
     t_progress: float = 0.0
 
     def __post_init__(self):
@@ -221,7 +222,8 @@ class Engine:
         """Prefix lookup + page reservation for a waiting request."""
         if len(self.running) >= self.config.max_seqs:
             return False
-        need_pages = (len(r.fill) + 1 + self.page_size - 1) // self.page_size
+        rows = len(r.fill) if r.saved is None else r.total_len - 1 - r.evicted
+        need_pages = (rows + 1 + self.page_size - 1) // self.page_size
         # one page of headroom per running sequence: a request admitted into a nearly full pool would be preempted at once
         if not self.kv.can_allocate(need_pages + len(self.running)):
             return False
@@ -230,7 +232,13 @@ class Engine:
                 return False
             r.state_slot = self.kv.alloc_state_slot()
         if self.bounded:  # (as many rows as places)
-            r.weight_slot, r.observed = self.kv.alloc_weight_slot(), 0
+            r.weight_slot = self.kv.alloc_weight_slot()
+        if r.saved is not None:
+            self.kv.ensure_pages(r.pages, rows)
+            self.kv.load_rows(r.saved, r.pages, r.weight_slot)
+            r.saved, r.computed, r.state = None, len(r.fill), RUNNING
+            self.running.append(r)
+            return True
         # Recurrent (conv / SSM) state is not idempotent: a snapshot taken after L tokens may only be resumed at token L. A hit
         # that covers the whole prompt would have to replay the last token on a state that already absorbed it, so hybrid
         # models only take checkpoints strictly shorter than the prompt and prefill the remainder from the restored state.
@@ -251,6 +259,7 @@ class Engine:
         r.finish_reason = reason
         r.state = FINISHED
         r.t_done = time.perf_counter()
+        r.saved = None
         if r in self.running:
             self.running.remove(r)
         self._release(r)
@@ -269,11 +278,14 @@ class Engine:
     def _preempt(self, v: Request) -> None:
         """Take a running request out of the batch and give its pages back; it re-enters at the head of the waiting queue and
         rebuilds its cache by prefilling prompt + generated tokens (recompute; its own prompt is usually a prefix-cache hit).
-        Sampling state, guide, stop detector and the tokens produced so far stay with the request, so its output is unchanged."""
+        Sampling state, guide, stop detector and the tokens produced so far stay with the request, so its output is unchanged. What a bounded cache has weighed
+        or dropped cannot be rebuilt from tokens: a sequence that has taken decode steps keeps its rows and weights on the host meanwhile."""
         self.running.remove(v)
+        if self.bounded and (v.observed or v.evicted):
+            v.saved = self.kv.save_rows(v.pages, v.total_len - 1 - v.evicted, v.weight_slot)
         self._release(v)
-        v.state, v.computed, v.state_snapshots, v.evicted = WAITING, 0, {}, 0
-        v.resumed = bool(v.output)
+        v.state, v.computed, v.state_snapshots = WAITING, 0, {}
+        v.resumed = bool(v.output) and v.saved is None
         v.fill = v.prompt + v.output[:-1] if v.output else v.prompt
         v.preemptions += 1
         self.metrics["preemptions"] = self.metrics.get("preemptions", 0) + 1

@@ -378,6 +378,19 @@ class PagedKVCache:
             raise RuntimeError(f"key weight slot {s} is not in use")
         self.free_weight_slots.append(s)
 
+    def save_rows(self, pages: list[int], rows: int, weight_slot: int) -> tuple:
+        """Host copies of a bounded sequence's pages in all layers and of its ``rows`` weights."""
+        idx = torch.tensor(pages[: (rows + self.page_size - 1) // self.page_size], dtype=torch.int64).to(self.device)
+        return [t.index_select(0, idx).cpu() for t in self.k + self.v], self._weights[:, weight_slot, :, :rows].to("cpu", copy=True)
+
+    def load_rows(self, saved: tuple, pages: list[int], weight_slot: int) -> None:
+        """The inverse of :meth:`save_rows`, into other pages and another, cleared slot."""
+        caches, weights = saved
+        idx = torch.tensor(pages[: caches[0].shape[0]], dtype=torch.int64).to(self.device)
+        for t, rows in zip(self.k + self.v, caches):
+            t.index_copy_(0, idx, rows.to(self.device))
+        self._weights[:, weight_slot, :, : weights.shape[2]] = weights.to(self.device)
+
     def snapshot_state(self, slot: int) -> dict:
         return {name: {i: t[slot].clone() for i, t in layers.items()} for name, layers in self.state.items()}
 

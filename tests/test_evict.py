@@ -713,3 +713,61 @@ def test_engine_bounded_cache_one_sequence_fills_the_pool(tmp_path):
         e.kv.audit([])
         assert e.generate(prompt, params_of(60)).token_ids == first.token_ids
         assert first.token_ids == engine_of(model, 90, 8, 6).generate(prompt, params_of(60)).token_ids
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("at", [2, 23, 60, 61, 66])
+def test_engine_bounded_cache_preempted_and_resumed(tmp_path, device, at):
+    """A preempted sequence goes on as if nothing had happened: what was weighed and dropped cannot be rebuilt from its tokens. Where decoding fits, resuming fits."""
+    over = dict(hidden_size=256, num_attention_heads=4, num_key_value_heads=2, head_dim=64) if device == "cuda" else {}
+    model = tiny_model(tmp_path, device, "qwen3" if over else "llama", **over)
+    prompt = shared_head([60])[0]
+    lookahead = True if device == "cuda" else "force"
+    for la, pages in ((False, 256), (lookahead, 256), (False, 4), (lookahead, 4)):
+        alone = engine_of(model, 40, 8, 5, lookahead=la).generate(prompt, params_of(120)).token_ids
+        e = engine_of(model, 40, 8, 5, lookahead=la, pages=pages)
+        r = e.add_request(prompt, params_of(120))
+        while len(r.output) < at:
+            e.step()
+        e._drain()
+        e._preempt(r)
+        assert not r.pages and r.weight_slot == -1
+        e.kv._weights.fill_(7.0), [t.fill_(3.0) for t in e.kv.k + e.kv.v]
+        e.kv.prefix.clear()
+        e.run()
+        assert r.output == alone and r.error is None and r.saved is None
+        e.kv.audit([])
+        r = e.add_request(prompt, params_of(120))
+        while len(r.output) < at:
+            e.step()
+        e._drain()
+        e._preempt(r)
+        e.abort(r)
+        assert r.saved is None and len(e.kv.free_weight_slots) == 8
+        e.run()
+
+
+def pressed(seed):
+    import random
+
+    rng = random.Random(seed)
+    lens = [rng.choice([64, 96]) + rng.randint(1, 40) for _ in range(rng.randint(2, 4))]
+    every, steps = rng.randint(3, 16), rng.randint(30, 80)
+    keep = rng.randint(33, 100)
+    recent = rng.randint(0, keep)
+    # a sequence holds what its prompt and its first steps make or what it keeps and is weighed on, and a page more
+    pages = 2 + max(-(-(max(max(lens), keep) + every + 1) // P) + 1, -(-(max(lens) + 1) // P) + 1) + rng.randint(0, 4)
+    return shared_head(lens), keep, recent, every, steps, pages, rng.choice([False, "force"]), rng.choice([0, 0, 2])
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_engine_bounded_cache_answers_do_not_depend_on_the_pool(tmp_path, seed):
+    prompts, keep, recent, every, steps, pages, lookahead, interleave = pressed(seed)
+    model = tiny_model(tmp_path)
+    alone = [engine_of(model, keep, recent, every).generate(p, params_of(steps)).token_ids for p in prompts]
+    e = engine_of(model, keep, recent, every, pages=pages, lookahead=lookahead, decode_interleave=interleave)
+    rs = [e.add_request(p, params_of(steps)) for p in prompts]
+    e.run()
+    assert [r.error for r in rs] == [None] * len(rs) and [r.output for r in rs] == alone
+    e.kv.audit([])
+    assert len(e.kv.free_weight_slots) == 8
