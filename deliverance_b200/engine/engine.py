@@ -20,7 +20,7 @@ import torch
 from .. import ops
 from ..kv.paged import KvCacheSettings, PagedKVCache, compose_salt
 from ..models.batch import ForwardBatch, make_batch
-from ..ops.evict import evict_keys
+from ..ops.evict import by_length, evict_keys
 from ..params import FinishReason, GeneratorParameters, Response, TokenLogProb
 from .sampler import Sampler, SamplingState
 
@@ -732,7 +732,9 @@ class Engine:
         """Which of two captured steps a decode batch takes: the one for sequences of like length or the other. Batches whose attention is launched alike
         in both cases have one only."""
         kv, splits = self.model.n_kv, self._splits(len(lens))
-        return splits <= ops.decode_room(len(lens), getattr(self.model, "n_heads", kv), kv, getattr(self.cfg, "head_dim", 0) or 128) or ops.even_lengths(lens)
+        shape = len(lens), getattr(self.model, "n_heads", kv), kv, getattr(self.cfg, "head_dim", 0) or 128
+        alike = not by_length(splits, *shape) if self.bounded else splits <= ops.decode_room(*shape)
+        return alike or ops.even_lengths(lens)
 
     def _graph_decode(self, seqs: list[dict], dev_tokens: Optional[torch.Tensor] = None) -> torch.Tensor:
         B = len(seqs)

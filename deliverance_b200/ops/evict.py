@@ -17,6 +17,14 @@ from .. import ops
 from . import ref
 
 
+def by_length(splits: int, B: int, H: int, KV: int, D: int) -> bool:
+    """Whether weighted attention of ``B`` sequences of unlike lengths is launched otherwise than of like ones, ``splits`` being what the caller allows (us per layer, launched as of like
+    lengths / as of their own, plan shared by four layers, heads of 128 on 8 KV heads: 8 sequences of 1,000 to 32,000 keys 86.0 / 73.2, 16 of 500 to 16,000 90.6 / 70.1, 64 of 100 to 2,176 52.2 / 47.1;
+    heads of 64 on 4: 16 of 500 to 16,000 41.0 / 31.2; 2 of 200 to 2,000, with room for 74, the same)."""
+    room = ops.decode_room(B, H, KV, D)
+    return splits > room or room <= 32
+
+
 def decode_attention_weighted(q, k_cache, v_cache, block_tables, ctx_lens, H, scale, weights, slots, softcap=0.0, window=0, splits=1, even=False, plan=None):
     """:func:`ops.decode_attention`, which also adds every key's probabilities to ``weights[slots[b], kv head, row]`` (fp32 ``[slots, KV, capacity]``, in place;
     ``slots`` int64 ``[B]``). Rows of a sequence at or behind the capacity are attended to and not counted. Slot 0 is the scratch slot: a sequence with slot 0 adds nothing. The other

@@ -771,3 +771,39 @@ def test_engine_bounded_cache_answers_do_not_depend_on_the_pool(tmp_path, seed):
     assert [r.error for r in rs] == [None] * len(rs) and [r.output for r in rs] == alone
     e.kv.audit([])
     assert len(e.kv.free_weight_slots) == 8
+
+
+def test_engine_bounded_cache_knows_unlike_lengths(tmp_path):
+    """A captured step of a bounded cache is one for unlike lengths where weighted attention is launched otherwise for them, which is also where plain attention is not."""
+    from deliverance_b200.ops.evict import by_length
+
+    model = tiny_model(tmp_path)
+    e, plain = engine_of(model, 64), engine_of(model)
+    ragged = lambda n: [1000] * (n - 1) + [30000]  # noqa: E731
+    seen = set()
+    for B in (1, 2, 4, 8, 16, 32, 64, 128):
+        room, splits = ops.decode_room(B, model.n_heads, model.n_kv, model.cfg.head_dim), e._splits(B)
+        matters = by_length(splits, B, model.n_heads, model.n_kv, model.cfg.head_dim)
+        assert e._even([700] * B) and (B < 4 or e._even(ragged(B)) == (not matters))
+        assert matters == (room <= 32 or splits > room) and (B < 4 or plain._even(ragged(B)) == (splits <= room))
+        seen.add((matters, splits <= room))
+    assert (True, True) in seen and (False, True) in seen
+
+
+@pytest.mark.gpu
+def test_engine_bounded_cache_captures_unlike_lengths(tmp_path):
+    """Sixteen sequences, one much longer: the step of that bucket is launched by a plan, and answers as plain launches do."""
+    from deliverance_b200.ops.evict import by_length
+
+    model = tiny_model(tmp_path, "cuda", "qwen3", hidden_size=256, num_attention_heads=8, num_key_value_heads=4, head_dim=64, vocab_size=512)
+    assert by_length(9, 16, 8, 4, 64)
+    prompts = [shared_head([40 + k])[0] for k in range(15)] + shared_head([215])
+    outs = []
+    for kw in (dict(lookahead=False), dict(cuda_graphs=False)):
+        e = engine_of(model, 200, 16, 10, max_seqs=16, **kw)
+        outs.append([r.token_ids for r in e.generate_batch(prompts, params_of(30))])
+        ops.check_status(0)
+    assert outs[0] == outs[1] and e.metrics["evictions"] > 1
+    e = engine_of(model, 200, 16, 10, max_seqs=16)
+    e.generate_batch(prompts, params_of(30))
+    assert -16 in e._graphs
