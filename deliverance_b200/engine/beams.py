@@ -82,6 +82,9 @@ class BeamSearch:
             out += self._search(group)
         if e.device.type == "cuda":
             ops.check_status(e.device.index)
+        for i, hypotheses in enumerate(out):
+            if not hypotheses:
+                raise RuntimeError(f"beam search found no continuation of prompt {i} that has a finite log-probability: the model's logits are NaN or infinite")
         return out
 
     def _search(self, group: list) -> list:

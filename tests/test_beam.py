@@ -455,3 +455,33 @@ def test_engine_beams_on_the_gpu(tmp_path, family, over):
         want = float(z.gather(1, torch.tensor(hyps[0].token_ids).view(-1, 1)).sum()) / len(hyps[0].token_ids)
         # bf16 activations over a few layers: a log-probability is off by some hundredths, here their mean over 40 tokens
         assert abs(hyps[0].score - want) < 0.1
+
+
+@pytest.mark.parametrize("bad", [math.nan, INF])
+def test_engine_beams_without_a_finite_continuation(tmp_path, bad):
+    """A model that returns no numbers: the error says so, and nothing is lost. Hypotheses that ended before stand."""
+    model = tiny_model(tmp_path, "llama")
+    e, prompt = engine_of(model), list(range(3, 40))
+    p = params_of(num_beams=3, max_tokens=6)
+    want = e.generate_beams([prompt], p)[0]
+    forward, calls = model.forward, []
+
+    def broken(batch, kv):
+        calls.append(1)
+        z = forward(batch, kv)
+        return torch.full_like(z, bad) if len(calls) > good else z
+
+    model.forward = broken
+    for good in (0, 1, 3):
+        for call in (lambda: e.generate(prompt, p), lambda: e.generate_batch([prompt], p), lambda: e.generate_beams([prompt], p)):
+            calls.clear()
+            with pytest.raises(RuntimeError, match="logits are NaN"):
+                call()
+            assert not e.has_work()
+            e.kv.audit([])
+    first = want[0].token_ids[0]  # ends at the first step, as the others of its candidates do not
+    e.eos_ids, good = frozenset([first]), 1
+    calls.clear()
+    assert [r.token_ids for r in e.generate_beams([prompt], p)[0]] == [[first]]
+    model.forward, e.eos_ids = forward, frozenset()
+    assert [r.token_ids for r in e.generate_beams([prompt], p)[0]] == [r.token_ids for r in want]
