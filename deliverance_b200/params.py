@@ -6,7 +6,6 @@
 from __future__ import annotations
 
 import enum
-import math
 from dataclasses import dataclass, field
 from typing import Any, Callable, Optional
 
@@ -46,7 +45,7 @@ class GeneratorParameters:
     uniform_top_p: Optional[float] = None
     lora_adapter: Optional[str] = None
     num_beams: int = 1  # > 1: beam search (Engine.generate_beams); deterministic, without guides, stop strings and log-probabilities
-    length_penalty: float = 1.0  # a hypothesis of n tokens ranks by its log-probability / n ** length_penalty
+    length_penalty: float = 1.0  # a hypothesis of n tokens ranks by its log-probability / n ** length_penalty; -32 to 32
 
     def validate(self) -> None:
         if not 1 <= self.num_beams <= 32:
@@ -54,8 +53,8 @@ class GeneratorParameters:
         if self.num_beams > 1 and (self.temperature != 0 or self.xtc_threshold or self.logprobs or self.stop_words or
                                    any(x is not None for x in (self.guided_choice, self.guided_regex, self.guided_json, self.top_k, self.top_p, self.uniform_top_p))):
             raise ValueError("beam search does not combine with sampling, guides, stop strings or log-probabilities")
-        if not math.isfinite(self.length_penalty):
-            raise ValueError("length_penalty must be finite")
+        if not -32 <= self.length_penalty <= 32:  # (a power of any context's length within the range of 64 bits)
+            raise ValueError("length_penalty must lie in [-32, 32]")
         modes = sum(x is not None for x in (self.guided_choice, self.guided_regex, self.guided_json))
         if modes > 1:
             raise ValueError("only one of guided_choice, guided_regex, guided_json may be set")

@@ -485,3 +485,23 @@ def test_engine_beams_without_a_finite_continuation(tmp_path, bad):
     assert [r.token_ids for r in e.generate_beams([prompt], p)[0]] == [[first]]
     model.forward, e.eos_ids = forward, frozenset()
     assert [r.token_ids for r in e.generate_beams([prompt], p)[0]] == [r.token_ids for r in want]
+
+
+@pytest.mark.parametrize("lp", [1000.0, -2000.0, 33.0, math.nan, -INF])
+def test_length_penalty_out_of_range_is_refused_at_once(tmp_path, lp):
+    e = engine_of(tiny_model(tmp_path, "llama"))
+    with pytest.raises(ValueError, match="length_penalty"):
+        e.generate_beams([list(range(3, 40))], params_of(num_beams=2, max_tokens=9, length_penalty=lp))
+    assert e.metrics["prefill_steps"] == 0
+
+
+@pytest.mark.parametrize("lp", [32.0, -32.0])
+def test_length_penalty_at_its_ends(tmp_path, lp):
+    """The longest hypotheses, or the shortest, rank first, with finite scores; powers of the longest contexts are in range too."""
+    model = tiny_model(tmp_path, "llama")
+    e, prompt = engine_of(model), [(7 * i * i + 3 * i + 11) % 200 + 3 for i in range(31)]
+    p = params_of(num_beams=4, max_tokens=5, length_penalty=lp)
+    e.eos_ids = frozenset({h[1][2] for h in plain_beams(model, prompt, 4, 5, (), 0.0)[:2]})
+    got = e.generate_beams([prompt], p)[0]
+    assert [(r.score, r.token_ids) for r in got] == sorted([(r.score, r.token_ids) for r in got], key=lambda h: -h[0]) and all(math.isfinite(r.score) and r.score < 0 for r in got)
+    assert (1 << 20) ** lp > 0 and math.isfinite(1e9 / (1 << 20) ** lp)
