@@ -221,27 +221,32 @@ class CausalLanguageModel:
         import copy
 
         if params is not None and params.num_beams > 1:
-            return [self.generate(p, params) for p in prompts]
+            return [answers[0] for answers in self._search_beams(prompts, params)]
         gens = [self.submit(p, copy.deepcopy(params) if params else None) for p in prompts]
         self.engine.run([g.request for g in gens])
         return [g.finish() for g in gens]
 
     def generate_beams(self, prompt, params: GeneratorParameters) -> list[Response]:
         """``params.num_beams`` answers of a beam search, best first (``Response.score``)."""
-        if getattr(prompt, "has_tools", False):
+        return self._search_beams([prompt], params)[0]
+
+    def _search_beams(self, prompts: list, params: GeneratorParameters) -> list[list[Response]]:
+        """One search over all prompts, whose beams decode in common steps."""
+        if any(getattr(p, "has_tools", False) for p in prompts):
             raise ValueError("beam search does not combine with tools")
-        if isinstance(prompt, PromptContext):
-            prompt = prompt.prompt
-        ids = self.encode_prompt(prompt) if isinstance(prompt, str) else [int(t) for t in prompt]
+        prompts = [p.prompt if isinstance(p, PromptContext) else p for p in prompts]
+        ids = [self.encode_prompt(p) if isinstance(p, str) else [int(t) for t in p] for p in prompts]
         out = []
-        for r in self.engine.generate_beams([ids], params)[0]:
-            gen = Generation(self, params, None, "", False)
-            gen.starts_in_reasoning = isinstance(prompt, str) and prompt_ends_inside_reasoning(prompt)
-            for token in r.token_ids:
-                gen.detok_special.push(token)
-                gen.detok_plain.push(token)
-            gen.request = SimpleNamespace(response=lambda r=r: r)
-            out.append(gen.finish())
+        for prompt, hypotheses in zip(prompts, self.engine.generate_beams(ids, params)):
+            out.append([])
+            for r in hypotheses:
+                gen = Generation(self, params, None, "", False)
+                gen.starts_in_reasoning = isinstance(prompt, str) and prompt_ends_inside_reasoning(prompt)
+                for token in r.token_ids:
+                    gen.detok_special.push(token)
+                    gen.detok_plain.push(token)
+                gen.request = SimpleNamespace(response=lambda r=r: r)
+                out[-1].append(gen.finish())
         return out
 
     def close(self) -> None:

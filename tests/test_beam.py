@@ -505,3 +505,21 @@ def test_length_penalty_at_its_ends(tmp_path, lp):
     got = e.generate_beams([prompt], p)[0]
     assert [(r.score, r.token_ids) for r in got] == sorted([(r.score, r.token_ids) for r in got], key=lambda h: -h[0]) and all(math.isfinite(r.score) and r.score < 0 for r in got)
     assert (1 << 20) ** lp > 0 and math.isfinite(1e9 / (1 << 20) ** lp)
+
+
+def test_beam_search_over_many_prompts_shares_its_steps(tmp_path):
+    """``generate_many`` is one search over all prompts: as many decode steps as the longest takes, and the answers of one prompt after another."""
+    from deliverance_b200.api import CausalLanguageModel
+    from deliverance_b200.tokenizer.auto import AutoTokenizer
+
+    model = tiny_model(tmp_path, "llama")
+    tok = AutoTokenizer.from_pretrained(str(tmp_path / "llama"))
+    prompts, p = ["Why is the sky blue?", "Hi", list(range(3, 40))], params_of(num_beams=3, max_tokens=8)
+    one, many = (CausalLanguageModel(model, engine_of(model), tok, "t") for _ in range(2))
+    one.engine.eos_ids = many.engine.eos_ids = frozenset()
+    alone = [one.generate(q, p) for q in prompts]
+    got = many.generate_many(prompts, p)
+    assert [(r.token_ids, r.text) for r in got] == [(r.token_ids, r.text) for r in alone]
+    assert max(abs(r.score - a.score) for r, a in zip(got, alone)) < 1e-3  # (fp32 in other orders)
+    assert many.engine.metrics["decode_steps"] == 7 and one.engine.metrics["decode_steps"] == 21
+    assert many.generate_many([], p) == []
