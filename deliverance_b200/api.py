@@ -210,8 +210,8 @@ class CausalLanguageModel:
 
     def generate(self, prompt, params: Optional[GeneratorParameters] = None, on_event=None, session: Optional[str] = None) -> Response:
         if params is not None and params.num_beams > 1:
-            if on_event is not None:
-                raise ValueError("beam search has no token events")
+            if on_event is not None or session is not None:
+                raise ValueError("beam search has no token events and no sessions")
             return self.generate_beams(prompt, params)[0]
         gen = self.submit(prompt, params, on_event, session)
         self.engine.run([gen.request])

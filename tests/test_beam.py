@@ -523,3 +523,16 @@ def test_beam_search_over_many_prompts_shares_its_steps(tmp_path):
     assert max(abs(r.score - a.score) for r, a in zip(got, alone)) < 1e-3  # (fp32 in other orders)
     assert many.engine.metrics["decode_steps"] == 7 and one.engine.metrics["decode_steps"] == 21
     assert many.generate_many([], p) == []
+
+
+def test_beam_search_has_no_session(tmp_path):
+    """A session names a request's events, of which a search has none: refused like a callback for them, not left aside."""
+    from deliverance_b200.api import CausalLanguageModel
+    from deliverance_b200.tokenizer.auto import AutoTokenizer
+
+    model = tiny_model(tmp_path, "llama")
+    clm = CausalLanguageModel(model, engine_of(model), AutoTokenizer.from_pretrained(str(tmp_path / "llama")), "t")
+    for kw in (dict(session="s"), dict(on_event=lambda *a: None)):
+        with pytest.raises(ValueError):
+            clm.generate("Hi", params_of(num_beams=3, max_tokens=8), **kw)
+    assert clm.engine.metrics["prefill_steps"] == 0 and clm.generate("Hi", params_of(max_tokens=2), session="s").generated_tokens == 2
