@@ -68,14 +68,17 @@ class BeamSearch:
             most = max(1, len(e.kv.free_slots) // self.W)
             if len(e.kv.free_slots) < self.W:
                 raise MemoryError(f"{self.W} beams need as many recurrent-state slots")
+        for prompt in prompts:  # (all of them before the first search: an error in the last one costs no answers)
+            e._limit_of(prompt, self.params)
+            need = self._limits(prompt)[1]
+            if not e.kv.can_allocate(need):
+                raise MemoryError(f"{self.W} beams of this prompt may need {need} pages, which the KV cache does not have")
         out, group, pages = [], [], 0
         for prompt in prompts:
             steps, need = self._limits(prompt)
             if group and (len(group) >= most or not e.kv.can_allocate(pages + need)):
                 out += self._search(group)
                 group, pages = [], 0
-            if not e.kv.can_allocate(need):
-                raise MemoryError(f"{self.W} beams of this prompt may need {need} pages, which the KV cache does not have")
             group.append((prompt, steps))
             pages += need
         if group:

@@ -188,7 +188,8 @@ class Engine:
         self.waiting.append(r)
         return r
 
-    def _new_request(self, prompt: list[int], params: GeneratorParameters, on_token=None) -> Request:
+    def _limit_of(self, prompt: list[int], params: GeneratorParameters) -> int:
+        """Position limit of a request, or an error where the prompt cannot be one."""
         ctx = self.cfg.max_position_embeddings
         limit = min(params.ntokens or ctx, ctx)
         if len(prompt) == 0:
@@ -199,6 +200,10 @@ class Engine:
             raise ValueError(f"prompt has {len(prompt)} tokens, which does not fit ntokens={limit}")
         if min(prompt) < 0 or max(prompt) >= self.cfg.vocab_size:
             raise ValueError(f"token ids must lie in [0, {self.cfg.vocab_size})")
+        return limit
+
+    def _new_request(self, prompt: list[int], params: GeneratorParameters, on_token=None) -> Request:
+        limit = self._limit_of(prompt, params)
         r = Request(self._next_id, [int(t) for t in prompt], params, on_token)
         self._next_id += 1
         r.sampling = SamplingState.create(params, self.special_ids)

@@ -536,3 +536,15 @@ def test_beam_search_has_no_session(tmp_path):
         with pytest.raises(ValueError):
             clm.generate("Hi", params_of(num_beams=3, max_tokens=8), **kw)
     assert clm.engine.metrics["prefill_steps"] == 0 and clm.generate("Hi", params_of(max_tokens=2), session="s").generated_tokens == 2
+
+
+def test_all_prompts_are_checked_before_the_first_search(tmp_path):
+    model = tiny_model(tmp_path, "llama")
+    e, good = engine_of(model, pages=16, max_seqs=4), list(range(3, 40))
+    p = params_of(num_beams=4, max_tokens=4)
+    for bad, error in (([], ValueError), ([5, 10**6], ValueError), ([5] * 300, ValueError), (list(range(3, 163)), MemoryError)):
+        with pytest.raises(error):
+            e.generate_beams([good, bad], p if error is ValueError else params_of(num_beams=4, max_tokens=90))
+        assert e.metrics["prefill_steps"] == 0 and not e.has_work()
+        e.kv.audit([])
+    assert len(e.generate_beams([good, good[:9]], p)) == 2
