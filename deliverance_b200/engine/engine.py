@@ -20,7 +20,7 @@ import torch
 from .. import ops
 from ..kv.paged import KvCacheSettings, PagedKVCache, compose_salt
 from ..models.batch import ForwardBatch, make_batch
-from ..ops.evict import by_length, evict_keys
+from ..ops.evict import by_length, evict_keys, score_room
 from ..params import FinishReason, GeneratorParameters, Response, TokenLogProb
 from .sampler import Sampler, SamplingState
 
@@ -133,6 +133,8 @@ class Engine:
         self.hybrid = any(layout.get("state_shapes") or [])  # recurrent layers: every sequence holds a state slot
         self.kv = PagedKVCache(layout, pages, self.device, model.dtype, self.config.kv, self._state_slots(layout), self.config.max_seqs if self.bounded else 0,
                                self._weight_capacity())
+        if self.bounded and self.device.type == "cuda":
+            self.kv.key_scores = torch.empty(self._score_room(), dtype=torch.float32, device=self.device)
         self.page_size = self.kv.page_size
         self.max_pages_per_seq = (self.cfg.max_position_embeddings + self.page_size - 1) // self.page_size
         self.waiting: list[Request] = []
@@ -162,13 +164,19 @@ class Engine:
         n = self.config.kv.keep_capacity or self.cfg.max_position_embeddings
         return (min(n, self.cfg.max_position_embeddings) + 31) // 32 * 32 if self.bounded else 0
 
+    def _score_room(self) -> int:
+        """Numbers that the largest decode step of a bounded cache keeps for a while: every captured step, and steps launched one by one, use the same ones."""
+        n, ps = self.config.max_seqs, self.config.kv.block_size
+        rows = (self.cfg.max_position_embeddings + ps - 1) // ps * ps
+        return score_room(next((b for b in _BUCKETS if b >= n), n), self.model.n_heads, rows, self._weight_capacity())
+
     def _auto_pages(self, layout) -> int:
         per = max(1, PagedKVCache.bytes_per_page(layout, self.config.kv.block_size, self.model.dtype))
         if self.device.type == "cuda":
             free, _ = torch.cuda.mem_get_info(self.device)
             free -= (1 + self._state_slots(layout)) * PagedKVCache.bytes_per_state_slot(layout)
             if self.bounded:
-                free -= 4 * len(layout["layer_kinds"]) * (1 + self.config.max_seqs) * layout["kv_heads"] * self._weight_capacity()
+                free -= 4 * len(layout["layer_kinds"]) * (1 + self.config.max_seqs) * layout["kv_heads"] * self._weight_capacity() + 4 * self._score_room()
             budget = int(max(0, free) * self.config.kv_memory_fraction)
             # enough for max_seqs full contexts, never more than the budget
             want = self.config.max_seqs * ((self.cfg.max_position_embeddings + self.config.kv.block_size - 1) // self.config.kv.block_size) + 1

@@ -281,6 +281,7 @@ class PagedKVCache:
 
         # attention weights of a bounded cache: per layer fp32 [1 + slots, KV, capacity] (slot 0 is scratch), one allocation
         self.key_weights: Optional[list] = None
+        self.key_scores: Optional[torch.Tensor] = None  # what decode steps keep of their scores until the weights are added, one for all steps (set by the engine)
         self.free_weight_slots = list(range(weight_slots, 0, -1))
         if weight_slots > 0:
             self._weights = torch.zeros(len(kinds), 1 + weight_slots, heads[0], weight_capacity, dtype=torch.float32, device=self.device)

@@ -389,7 +389,7 @@ class DecoderModel:
                                               batch.decode_even, lambda *a: batch.decode_plan(i, *a))
             elif batch.is_decode and batch.key_slots is not None:  # bounded cache
                 a = decode_attention_weighted(q, k_cache, v_cache, batch.block_tables, batch.ctx_len, self.n_heads, cfg.scale, kv.key_weights[i], batch.key_slots,
-                                              cfg.attn_softcap, 0, batch.decode_splits, batch.decode_even, lambda *a: batch.decode_plan(i, *a))
+                                              cfg.attn_softcap, 0, batch.decode_splits, batch.decode_even, lambda *a: batch.decode_plan(i, *a), kv.key_scores)
             elif batch.is_decode:
                 a = ops.decode_attention(q, k_cache, v_cache, batch.block_tables, batch.ctx_len, self.n_heads, cfg.scale,
                                          cfg.attn_softcap, window, batch.decode_splits, even=batch.decode_even,

@@ -25,11 +25,16 @@ def by_length(splits: int, B: int, H: int, KV: int, D: int) -> bool:
     return splits > room or room <= 32
 
 
-def decode_attention_weighted(q, k_cache, v_cache, block_tables, ctx_lens, H, scale, weights, slots, softcap=0.0, window=0, splits=1, even=False, plan=None):
+def score_room(B: int, H: int, rows: int, capacity: int) -> int:
+    """Scores that weighted attention of ``B`` sequences keeps for a while, with block tables of ``rows`` rows and weights of ``capacity``."""
+    return B * H * max(16, (min(rows, capacity) + 15) // 16 * 16)
+
+
+def decode_attention_weighted(q, k_cache, v_cache, block_tables, ctx_lens, H, scale, weights, slots, softcap=0.0, window=0, splits=1, even=False, plan=None, scores=None):
     """:func:`ops.decode_attention`, which also adds every key's probabilities to ``weights[slots[b], kv head, row]`` (fp32 ``[slots, KV, capacity]``, in place;
     ``slots`` int64 ``[B]``). Rows of a sequence at or behind the capacity are attended to and not counted. Slot 0 is the scratch slot: a sequence with slot 0 adds nothing. The other
     slots of a call are different ones; a second sequence on a slot, or a slot outside ``weights``, adds nothing and is reported by :func:`ops.check_status` (on the CPU:
-    raised)."""
+    raised). ``scores``: fp32 workspace of :func:`score_room` numbers, for calls that follow one another on a stream (captured ones would else keep one each); default: the call's own."""
     if q.is_cuda:  # (the extension checks)
         B, (_, KV, page, D) = q.shape[0], k_cache.shape
         if even:
@@ -45,7 +50,7 @@ def decode_attention_weighted(q, k_cache, v_cache, block_tables, ctx_lens, H, sc
             if splits <= room <= 32:
                 splits = 2 * room
         splits, used = ops.decode_launch(splits, even, plan, ctx_lens, B, H, KV, D, int(window))
-        out, launches = ops.require_ext().decode_attention_weighted(q, k_cache, v_cache, block_tables, ctx_lens, H, scale, softcap, window, splits, weights, slots, used)
+        out, launches = ops.require_ext().decode_attention_weighted(q, k_cache, v_cache, block_tables, ctx_lens, H, scale, softcap, window, splits, weights, slots, used, scores)
         ops._count(launches)
         return out
     if weights.dim() != 3 or weights.dtype != torch.float32 or weights.shape[1] != k_cache.shape[1]:

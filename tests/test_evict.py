@@ -807,3 +807,43 @@ def test_engine_bounded_cache_captures_unlike_lengths(tmp_path):
     e = engine_of(model, 200, 16, 10, max_seqs=16)
     e.generate_batch(prompts, params_of(30))
     assert -16 in e._graphs
+
+
+@pytest.mark.gpu
+def test_weighted_attention_on_a_given_workspace():
+    """Scores in a workspace of the caller's, used by one call after another: the same bits as with the call's own; one that is too small is refused."""
+    from deliverance_b200.ops.evict import score_room
+
+    table, pages = tables_for([700, 33, 500], extra=3)
+    k, v = torch.randn(pages, 2, P, 64).to(BF16).cuda(), torch.randn(pages, 2, P, 64).to(BF16).cuda()
+    ctx, slots, table = torch.tensor([700, 33, 500], dtype=torch.int32).cuda(), torch.tensor([3, 1, 2]).cuda(), table.cuda()
+    room = score_room(3, 8, table.shape[1] * P, 650)
+    assert room == 3 * 8 * 656
+    scores = torch.full((room + 64,), math.nan, device="cuda")
+    a, b = torch.rand(4, 2, 650).cuda(), None
+    b = a.clone()
+    for splits in (1, 6, 3):
+        q = torch.randn(3, 512).to(BF16).cuda()
+        x = decode_attention_weighted(q, k, v, table, ctx, 8, 0.125, a, slots, splits=splits)
+        y = decode_attention_weighted(q, k, v, table, ctx, 8, 0.125, b, slots, splits=splits, scores=scores)
+        assert torch.equal(x, y) and torch.equal(a, b) and scores[room:].isnan().all()
+    for bad in (scores[: room - 1], scores.half(), scores.cpu(), scores[1:]):
+        with pytest.raises(RuntimeError):
+            decode_attention_weighted(q, k, v, table, ctx, 8, 0.125, b, slots, scores=bad)
+    ops.check_status(0)
+
+
+@pytest.mark.gpu
+def test_engine_bounded_cache_keeps_one_workspace(tmp_path):
+    """Steps captured for several batch sizes, of like and unlike lengths, over a context of 131,072: one workspace of 268 MB for all of them, allocated with the cache."""
+    model = tiny_model(tmp_path, "cuda", "qwen3", hidden_size=256, num_attention_heads=8, num_key_value_heads=4, head_dim=64, vocab_size=512, max_position_embeddings=131072)
+    e = engine_of(model, 200, 16, 10, max_seqs=64, capacity=131072)
+    assert e.kv.key_scores.numel() * 4 == 64 * 8 * 131072 * 4
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_reserved()
+    e.generate_batch([shared_head([40 + k % 8])[0] for k in range(60)] + shared_head([400]), params_of(12))
+    e.generate_batch([shared_head([40 + k])[0] for k in range(30)], params_of(4))
+    assert {64, 32} <= {abs(b) for b in e._graphs}
+    torch.cuda.synchronize()
+    # (what the steps keep for themselves: activations, split outputs, block tables of 4,096 pages per row)
+    assert torch.cuda.memory_reserved() - before < 200 << 20
