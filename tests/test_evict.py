@@ -847,3 +847,12 @@ def test_engine_bounded_cache_keeps_one_workspace(tmp_path):
     torch.cuda.synchronize()
     # (what the steps keep for themselves: activations, split outputs, block tables of 4,096 pages per row)
     assert torch.cuda.memory_reserved() - before < 200 << 20
+
+
+@pytest.mark.gpu
+def test_weights_of_more_rows_than_an_int_counts_are_refused():
+    k = torch.zeros(2, 1, P, 64, dtype=BF16, device="cuda")
+    w = torch.empty(1, 1, 2**31, device="cuda")  # (never touched)
+    with pytest.raises(RuntimeError, match="out of range"):
+        decode_attention_weighted(torch.zeros(1, 64, dtype=BF16, device="cuda"), k, k.clone(), torch.ones(1, 1, dtype=torch.int32, device="cuda"), torch.tensor([5], dtype=torch.int32, device="cuda"), 1, 0.1, w,
+                                  torch.zeros(1, dtype=torch.int64, device="cuda"))
