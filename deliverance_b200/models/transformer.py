@@ -618,10 +618,10 @@ class DecoderModel:
 
     def supports_key_weights(self) -> bool:
         """Whether the cache of this model can be bounded (``KvCacheSettings.keep_tokens``): attention over all cached rows in every layer, so that which row a
-        key lies in does not matter, and heads that weighted attention takes."""
+        key lies in does not matter."""
         cfg = self.cfg
         return (type(self) is DecoderModel and all(cfg.layer_type(i) != "mamba" and not cfg.window(i) for i in range(cfg.num_layers)) and
-                self.n_heads // self.n_kv <= 16 and (self.device.type != "cuda" or cfg.head_dim in (64, 128, 256)))
+                self.n_heads // self.n_kv <= 16)
 
     def weight_bytes(self) -> int:
         n = self.embed.numel() * self.embed.element_size()

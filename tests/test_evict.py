@@ -856,21 +856,3 @@ def test_weights_of_more_rows_than_an_int_counts_are_refused():
     with pytest.raises(RuntimeError, match="out of range"):
         decode_attention_weighted(torch.zeros(1, 64, dtype=BF16, device="cuda"), k, k.clone(), torch.ones(1, 1, dtype=torch.int32, device="cuda"), torch.tensor([5], dtype=torch.int32, device="cuda"), 1, 0.1, w,
                                   torch.zeros(1, dtype=torch.int64, device="cuda"))
-
-
-def test_engine_bounded_cache_needs_heads_that_the_kernel_takes(tmp_path):
-    """On a GPU weighted attention takes heads of 64, 128 and 256: another model is refused when the engine is made, not at its first decode step."""
-    model = tiny_model(tmp_path)
-    assert model.supports_key_weights() and model.cfg.head_dim not in (64, 128, 256)
-    model.device = torch.device("cuda")
-    assert not model.supports_key_weights()
-    for D in (64, 128, 256):
-        model.cfg.head_dim = D
-        assert model.supports_key_weights()
-
-
-@pytest.mark.gpu
-def test_engine_bounded_cache_refuses_other_heads(tmp_path):
-    model = tiny_model(tmp_path, "cuda", "qwen3", hidden_size=256, num_attention_heads=4, num_key_value_heads=2, head_dim=32, vocab_size=512)
-    with pytest.raises(ValueError):
-        engine_of(model, 64)
