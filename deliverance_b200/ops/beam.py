@@ -21,7 +21,7 @@ MAX_CANDIDATES = 64
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, mask: Optional[torch.Tensor] = None, softcap: float = 0.0, inv_scale: float = 1.0):
     """The ``k`` best continuations of every request: ``(values [B, k] fp32, parents [B, k], tokens [B, k])``, best first, equal values in the order of
     beam and token. ``logits [B * W, V]`` (fp32 or bf16, post-processed like :func:`ops.logits_post`: ``softcap(logits * inv_scale)``, tokens outside the int32
-    allow-bitmask ``mask`` left out), ``scores [B, W]`` fp32, the beams' sums so far; -inf for a beam that is not in use. A candidate's value is finite: a logit of
+    allow-bitmask ``mask`` left out), ``scores [B, W]`` fp32, the beams' sums so far; -inf for a beam that is not in use. A candidate's value is finite in fp32: a logit of
     -inf is a masked token, a row with a NaN (or +inf, without a softcap) and a beam whose score is not finite give none. Places that no candidate is left for have value
     -inf, parent and token -1."""
     if logits.is_cuda:  # (the extension checks)

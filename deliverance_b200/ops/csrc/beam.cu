@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
     double z = static_cast<double>(y) * static_cast<double>(a.inv_scale);
     if (a.softcap > 0.f) z = capped(z, static_cast<double>(a.softcap));
     const double v = base[w] + (z - static_cast<double>(top[w]));
-    return isfinite(v) ? v : -static_cast<double>(INFINITY);
+    return isfinite(static_cast<float>(v)) ? v : -static_cast<double>(INFINITY);  // (as it is returned)
   };
   // in 32 bits: off by less than half of `slack` (roundings of the row's constant, of the sum and of scale and cap)
   auto rough_post = [&](float y) {

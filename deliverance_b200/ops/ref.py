@@ -409,7 +409,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, allowed: Opt
     top = torch.where(z.isnan(), -math.inf, z).amax(dim=-1, keepdim=True).clamp_min(torch.finfo(torch.float32).min)
     logp = z - top - (z - top).exp().sum(dim=-1, keepdim=True).log()
     value = (scores.double().reshape(B * W, 1) + logp).reshape(B, W * V)
-    value, at = torch.sort(torch.where(value.isfinite(), value, -math.inf), dim=-1, descending=True, stable=True)
+    value, at = torch.sort(torch.where(value.float().isfinite(), value, -math.inf), dim=-1, descending=True, stable=True)
     value, at = value[:, :k], at[:, :k]
     none = value == -math.inf
     return value.float(), torch.where(none, -1, at // V), torch.where(none, -1, at % V)

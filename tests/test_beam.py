@@ -548,3 +548,22 @@ def test_all_prompts_are_checked_before_the_first_search(tmp_path):
         assert e.metrics["prefill_steps"] == 0 and not e.has_work()
         e.kv.audit([])
     assert len(e.generate_beams([good, good[:9]], p)) == 2
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_select_values_beyond_fp32_are_no_candidates(device):
+    """A masked place of the type's lowest value, scaled out of its range: a value that fp32 does not hold is none, and its place has no parent."""
+    low = torch.finfo(F32).min
+    for V, k in ((100, 8), (9000, 64)):
+        logits = torch.full((2, V), low)
+        logits[0, [3, V - 2]] = torch.tensor([2.0, 1.5])
+        logits[1, 7] = 0.0
+        scores = torch.tensor([[-1.0, -3.0]])
+        # (the second token of the first beam: -1 - 2 - log(1 + e^-2) = -3.13 at a scale of 4, behind the second beam's -3; -1 - 0.75 - log(1 + e^-0.75) = -2.14 at 1.5)
+        for inv_scale, parents, tokens in ((4.0, [0, 1, 0], [3, 7, V - 2]), (1.5, [0, 0, 1], [3, V - 2, 7])):
+            v, p, t = (x.cpu()[0] for x in beam_select(logits.to(device), scores.to(device), k, inv_scale=inv_scale))
+            assert p.tolist() == parents + [-1] * (k - 3) and t.tolist() == tokens + [-1] * (k - 3)
+            assert v[:3].isfinite().all() and (v[3:] == -INF).all()
+        # within the range they are candidates like any other
+        v, p, t = (x.cpu()[0] for x in beam_select(logits.to(device), scores.to(device), k, inv_scale=0.5))
+        assert t[:3].tolist() == [3, V - 2, 7] and p[3:].tolist() == [0] * (k - 3) and t[3:].tolist() == [j for j in range(V) if j not in (3, V - 2)][: k - 3] and v.isfinite().all()
