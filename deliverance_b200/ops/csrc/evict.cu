@@ -195,7 +195,9 @@ __global__ void __launch_bounds__(NT, CTAS) evict_select_kernel(const __grid_con
     for (int r = 0; r < R; ++r)
       if (r * 32 >= open && r * 32 < weighed) key[r] = __float_as_uint(w[r * 32]);
   }
+  const int own_places = place;
   place = in_front(place);  // (with the barrier behind which all weights are in registers)
+  if (t == NT - 1 && place + own_places != a.keep) atomicCAS(a.status, kStatusOk, kStatusBadArgs);  // (a wrong edge would be said; the list never overruns)
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     if (r >= rounds) break;
@@ -250,8 +252,9 @@ __global__ void __launch_bounds__(512) evict_select_long_kernel(const __grid_con
     const int place = take_base + block_scan<NT>(take ? 1 : 0, red, turn, all);
     turn ^= 1;
     take_base += all;
-    if (take) k.kept[place] = i;
+    if (take && place < a.keep) k.kept[place] = i;
   }
+  if (t == 0 && take_base != a.keep) atomicCAS(a.status, kStatusOk, kStatusBadArgs);
   __syncthreads();
   // entry j takes over entry kept[j] >= j: a tile is read as a whole before it is written
   for (int j0 = 0; j0 < k.counted; j0 += NT) {
