@@ -503,25 +503,10 @@ void launch_beam_select(const BeamSelectArgs& a, bool f32, cudaStream_t st) {
 // slot[j] takes over what slot[parent[j]] held, in place: a thread owns the same few bytes of all of a request's slots, reads what every moved beam will
 // hold before it writes any of it, and nobody else touches them. No second buffer, one launch for all tensors. Parents outside 0 .. W - 1 leave their
 // beam as it is. What bounds it: the bytes of distinct parents read and of moved beams written (a parent that several beams read comes from L1).
-template <int UNIT>
-struct MoveUnit;
-template <>
-struct MoveUnit<16> {
-  using type = uint4;
-};
-template <>
-struct MoveUnit<4> {
-  using type = uint32_t;
-};
-template <>
-struct MoveUnit<2> {
-  using type = unsigned short;
-};
-
 // grid (parts of a slot, tensors, requests): a part takes every gridDim.x-th 256 units
 template <int UNIT, int MAXW>
 __global__ void __launch_bounds__(256, MAXW <= 4 ? 5 : MAXW <= 8 ? 4 : MAXW <= 16 ? 2 : 1) beam_move_kernel(const __grid_constant__ BeamMoveArgs a) {
-  using U = typename MoveUnit<UNIT>::type;
+  using U = typename CopyUnit<UNIT>::type;
   pdl_trigger();
   pdl_wait();
   __shared__ long long from[MAXW], to[MAXW];  // byte offsets of slots; to < 0: the beam stays

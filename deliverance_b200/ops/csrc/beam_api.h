@@ -34,6 +34,22 @@ int beam_select_group(bool f32);              // neighbouring logits of a group
 int beam_select_splits(int rows, int V);      // CTAs per row of V logits, when there are `rows` rows
 constexpr int kBeamSplitUnit = 4096;
 
+// what one access of a copying kernel moves: 16, 4 or 2 bytes
+template <int UNIT>
+struct CopyUnit;
+template <>
+struct CopyUnit<16> {
+  using type = uint4;
+};
+template <>
+struct CopyUnit<4> {
+  using type = uint32_t;
+};
+template <>
+struct CopyUnit<2> {
+  using type = unsigned short;
+};
+
 struct BeamMoveTensor {
   void* base;
   long long slot_bytes;  // bytes from one slot (page) to the next

@@ -269,21 +269,6 @@ __global__ void __launch_bounds__(512) evict_select_long_kernel(const __grid_con
   }
 }
 
-template <int UNIT>
-struct RowUnit;
-template <>
-struct RowUnit<16> {
-  using type = uint4;
-};
-template <>
-struct RowUnit<4> {
-  using type = uint32_t;
-};
-template <>
-struct RowUnit<2> {
-  using type = unsigned short;
-};
-
 // grid (2 * slices, B * KV, layers): a CTA moves a range of columns of all rows of K or V of one head, in ascending batches of rows that are read as a
 // whole before they are written. Sources lie at or behind their targets, so no batch reads what an earlier one wrote, and in place is safe. The places of a
 // batch's rows are looked up once per row, while the rows of the batch in front are on their way (looked up by every thread for itself: 16 sequences of 2,304 rows in
@@ -292,7 +277,7 @@ struct RowUnit<2> {
 constexpr int kMoveThreads = 512, kMoveBatch = 8;
 template <int UNIT>
 __global__ void __launch_bounds__(kMoveThreads, 2) evict_move_kernel(const __grid_constant__ EvictArgs a, int slices, int most_lines) {
-  using U = typename RowUnit<UNIT>::type;
+  using U = typename CopyUnit<UNIT>::type;
   pdl_trigger();
   pdl_wait();
   extern __shared__ int2 place[];  // [2][rows of a batch]: source and target row in the cache; target -1: the row stays
