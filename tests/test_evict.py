@@ -856,3 +856,132 @@ def test_weights_of_more_rows_than_an_int_counts_are_refused():
     with pytest.raises(RuntimeError, match="out of range"):
         decode_attention_weighted(torch.zeros(1, 64, dtype=BF16, device="cuda"), k, k.clone(), torch.ones(1, 1, dtype=torch.int32, device="cuda"), torch.tensor([5], dtype=torch.int32, device="cuda"), 1, 0.1, w,
                                   torch.zeros(1, dtype=torch.int64, device="cuda"))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D,KV,G", [(64, 2, 4), (128, 2, 4), (256, 1, 2), (64, 1, 16)])
+@pytest.mark.parametrize("lens,splits,even,extra", [([3001, 2, 700], 32, False, 1), ([9000], 30, True, 1), ([4001, 4000], 18, True, 60), ([40, 2500, 300], 1, False, 1), ([9000, 31, 5], 32, False, 200)])
+def test_weighted_attention_outputs_value_by_value(device, D, KV, G, lens, splits, even, extra):
+    """Long sequences of like keys have outputs far smaller than their values, so each output is held to its own sum of p |v|. A probability is rounded to bf16 (2^-8 of it) and is off by
+    what its score is (as a weight is, numerator and denominator: twice), the result is rounded once more (2^-8 of it); sums in fp32 add n * 2^-24 of the sum of magnitudes."""
+    if device == "cpu" and sum(lens) * KV * G * D > 3e7:
+        pytest.skip("large for the CPU")
+    B, H, n = len(lens), KV * G, max(lens)
+    table, pages = tables_for(lens, extra=extra)
+    q, k, v = torch.randn(B, H * D).to(BF16), torch.randn(pages, KV, P, D).to(BF16), torch.randn(pages, KV, P, D).to(BF16)
+    to = lambda t: t.to(device)  # noqa: E731
+    ctx = torch.tensor(lens, dtype=torch.int32)
+    out = decode_attention_weighted(to(q), to(k), to(v), to(table), to(ctx), H, D**-0.5, torch.zeros(B + 1, KV, n, device=device), to(torch.arange(1, B + 1)), 0.0, 0, splits, even).cpu().double()
+    want, _ = plain_attention(q, k, v, table, lens, KV, D**-0.5, 0.0, 0)
+    size, _ = plain_attention(q, k, v.abs(), table, lens, KV, D**-0.5, 0.0, 0)
+    # (D + 2 roundings of a score, each 2^-24 of the sum of its magnitudes at most; the exponential as in run_attention)
+    heads = k.abs().float().permute(1, 0, 2, 3).reshape(KV, -1, D).transpose(1, 2)
+    score = float((q.abs().float().view(B, KV, G, D).permute(1, 0, 2, 3).reshape(KV, -1, D) @ heads).max()) * D**-0.5 * (D + 2) * 2**-24 + 64 * 2**-23
+    bound = (2**-8 + 2 * score + 2 * n * 2**-24) * size + 2**-8 * want.abs()
+    assert ((out - want).abs() <= bound).all(), float(((out - want).abs() / bound).max())
+    long = lens.index(n)
+    assert bound[long].mean() < 0.4 * want[long].abs().mean()  # (an output of zeros is found)
+
+
+def bounded_logits(model, prompt, tokens, recorded, keep, recent, every, rounded=False):
+    """64-bit decoding of given tokens on a bounded cache that keeps, at its own times, the rows that were recorded ([layers, KV, keep] each); "own": those that its weights say, None: all.
+    Returns the logits after the prompt and after every token, the rows kept and, for each eviction, what their old rows weigh, as a part of what the heaviest ones would. ``model``: of the CPU,
+    its weights rounded to bf16 as the GPU's are. ``rounded``: every vector between two products is rounded to bf16 as well."""
+    c = model.cfg
+    H, KV, D = c.num_heads, c.num_kv_heads, c.head_dim
+    w16 = lambda t: t.to(BF16).double()  # noqa: E731
+    r16 = w16 if rounded else lambda t: t
+    cos, sin = model.cos.double(), model.sin.double()
+    layers = [(w16(lw.qkv.w), w16(lw.o.w), w16(lw.gate_up.w), w16(lw.down.w), w16(lw.input_norm), w16(lw.pre_ff_norm)) for lw in model.layers]
+    rows = [[[torch.zeros(0, D, dtype=torch.float64), torch.zeros(0, D, dtype=torch.float64), torch.zeros(0, dtype=torch.float64)] for _ in range(KV)] for _ in layers]
+    norm = lambda x, w: r16(x * torch.rsqrt(x.pow(2).mean() + c.norm_eps) * w)  # noqa: E731
+    embed, head, last = w16(model.embed), w16(model.lm_head.w), w16(model.final_norm)
+
+    def rotate(x, pos):
+        a, b = x[..., : D // 2], x[..., D // 2 :]
+        return r16(torch.cat([a * cos[pos] - b * sin[pos], b * cos[pos] + a * sin[pos]], -1))
+
+    def feed(token, pos, weigh):
+        h = embed[token]
+        for i, (qkv_w, o_w, gu_w, down_w, n1, n2) in enumerate(layers):
+            qkv = r16(qkv_w @ norm(h, n1))
+            q, k, v = rotate(qkv[: H * D].view(KV, H // KV, D), pos), rotate(qkv[H * D : (H + KV) * D].view(KV, D), pos), qkv[(H + KV) * D :].view(KV, D)
+            out = []
+            for j in range(KV):
+                r = rows[i][j]
+                r[0], r[1], r[2] = torch.cat([r[0], k[j : j + 1]]), torch.cat([r[1], v[j : j + 1]]), torch.cat([r[2], torch.zeros(1, dtype=torch.float64)])
+                p = torch.softmax(q[j] @ r[0].T * c.scale, -1)
+                out.append(r16(r16(p) @ r[1]))
+                if weigh:
+                    r[2] += p.sum(0)
+            h = r16(h + r16(o_w @ torch.stack(out).flatten()))
+            g, u = r16(gu_w @ norm(h, n2)).chunk(2)
+            h = r16(h + r16(down_w @ r16(torch.nn.functional.silu(g) * u)))
+        return head @ norm(h, last)
+
+    for pos, token in enumerate(prompt):
+        z = feed(token, pos, False)
+    logits, parts, kept, seen = [z], [], [], 0
+    for i, token in enumerate(tokens):
+        n = rows[0][0][0].shape[0]
+        if recorded is not None and n > keep and seen >= every:
+            best = [[plain_evict(r[2].tolist(), n, keep, recent) for r in layer] for layer in rows]
+            kept.append(best if recorded == "own" else recorded[len(kept)].tolist())
+            part = 1.0
+            for layer, mine, heaviest in zip(rows, kept[-1], best):
+                for r, stay, most in zip(layer, mine, heaviest):
+                    assert len(stay) == keep and sorted(set(stay)) == stay and stay[keep - recent :] == list(range(n - recent, n))
+                    part = min(part, float(r[2][stay[: keep - recent]].sum() / r[2][most[: keep - recent]].sum()))
+                    r[:] = [x[stay] for x in r]
+            parts.append(part)
+            seen = 0
+        logits.append(feed(token, len(prompt) + i, True))
+        seen += 1
+    return torch.stack(logits), [torch.tensor(x) for x in kept], parts
+
+
+def away(a, b):
+    return ((a - b).norm(dim=1) / b.norm(dim=1)).max().item()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,KV", [(4, 2), (4, 4), (2, 1)])
+@pytest.mark.parametrize("lookahead", [False, True])
+def test_engine_bounded_cache_logits_against_64_bits(tmp_path, monkeypatch, H, KV, lookahead):
+    """The logits of every decode step on the GPU against a 64-bit decoder that is fed the same tokens and drops the same rows, which are held to be the heaviest by its own weights. How far
+    roundings to bf16 carry is computed, not guessed: the same decoder with every vector between two products rounded, dropping what its own weights say, against the exact one that drops
+    the same. The GPU rounds in other places of the same kind: three times that is allowed. What is kept weighs 95 % of the heaviest rows at least: the rounded decoder loses 0 to 1.5 % here,
+    keeping the oldest rows instead 28 to 56 % in the worst eviction."""
+    from deliverance_b200.engine import engine as module
+
+    over = dict(hidden_size=256, num_attention_heads=H, num_key_value_heads=KV, vocab_size=512)
+    gpu, cpu = tiny_model(tmp_path, "cuda", **over), tiny_model(tmp_path, "cpu", **over)
+    keep, recent, every, steps = 48, 16, 10, 70
+    e = engine_of(gpu, keep, recent, every, lookahead=lookahead)
+    recorded, seen = [], []
+    evict, greedy = module.evict_keys, e._greedy
+
+    def record_evict(*a):
+        got = evict(*a)
+        recorded.append(got[0][:, 0].cpu())
+        return got
+
+    def record_logits(z):
+        seen.append(z.float().cpu().double())
+        return greedy(z)
+
+    monkeypatch.setattr(module, "evict_keys", record_evict)
+    e._greedy = record_logits
+    prompt = [(7 * i * i + 3 * i + 11) % 200 + 3 for i in range(40)]
+    tokens = e.generate(prompt, params_of(steps)).token_ids
+    got = torch.cat(seen)[:steps]  # (a step ahead of the last token computes one more)
+    run = lambda rows, **kw: bounded_logits(cpu, prompt, tokens[:-1], rows, keep, recent, every, **kw)  # noqa: E731
+    want, kept, parts = run(recorded)
+    assert len(kept) == len(recorded) >= 5
+    bits16, own, _ = run("own", rounded=True)
+    exact, _, own_parts = run(own)
+    noise = away(bits16, exact)
+    assert away(got, want) <= 3 * noise, (away(got, want), noise)
+    assert min(parts) >= 0.95 and min(own_parts) >= 0.95, (parts, own_parts)
+    whole, _, _ = run(None)
+    assert away(whole, want) > 3 * noise  # (what was dropped shows)
