@@ -23,7 +23,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, mask: Option
     beam and token. ``logits [B * W, V]`` (fp32 or bf16, post-processed like :func:`ops.logits_post`: ``softcap(logits * inv_scale)``, tokens outside the int32
     allow-bitmask ``mask`` left out), ``scores [B, W]`` fp32, the beams' sums so far; -inf for a beam that is not in use. A candidate's value is finite in fp32: a logit of
     -inf is a masked token, a row with a NaN (or +inf, without a softcap) and a beam whose score is not finite give none. Places that no candidate is left for have value
-    -inf, parent and token -1."""
+    -inf, parent and token -1. On the GPU a beam's log-sum-exp is off by 4e-6 at most (32-bit exponentials), the same for all of its tokens: candidates of different beams that are closer than twice that
+    may come in either order, candidates of one beam come in the order of their logits."""
     if logits.is_cuda:  # (the extension checks)
         ops._count(2)
         return ops.require_ext().beam_select(logits, scores, k, mask, softcap, inv_scale)

@@ -554,8 +554,9 @@ template <>
 struct DecodeRope<true> : DecodeRopeArgs {};
 // WEIGH: every score goes to fp32 [B, H, S] as well, so that what is behind a sequence's last key (this CTA where it is the only split, weigh_kernel where not) can
 // add the probabilities to the keys' weights: 4 bytes per key and query head written and read again, out of L2, for no second product of queries and keys. Keys and values are the
-// first to leave L2 here, so that the scores stay (64 x 2176 keys 96 us, 104 without). 64 x 2176 keys, 32 heads on 8: 94 us (87.4 for decode attention that weighs nothing), one sequence of 4,000 9.8 (8.4),
-// 128 of 100 to 600 keys, 16 heads of 64 per KV head 22 (17): what is left is the tail of every CTA, which waits for its scores. (The weights by a kernel of their own: 104 and 28 us where this was 104 and 25.)
+// first to leave L2 here, so that the scores stay (8 us less in the first case). In a stream of calls, in parentheses decode attention that weighs nothing: 64 x 2176 keys, 32 heads on 8, 92.9 us (85.8), 95.1 (86.0) with
+// block tables of 1,280 pages, as a captured step has them; one sequence of 4,000 10.8 (9.4) and 11.3 (9.3); 64 x 2176 with 16 heads of 256 on 4 97.9 (89.5); 128 of 100 to 600 keys, 16 heads of 64 per KV head,
+// 22.5 (14.0): what is left is the tail of every CTA, which waits for its scores. (The weights of unsplit sequences by a kernel of their own: the first case the same, the last 3 us slower.)
 // This form looks at what it is given: lengths end with the block table, pages outside the cache are read as page 0 and reported.
 template <bool WEIGH>
 struct DecodeWeigh {};

@@ -4,7 +4,8 @@
 // The order inside a row is the order of the raw logits (soft-capping and positive scaling are monotone). The first kernel reads every logit once and leaves, per
 // row, maxima and sums of exponentials, and the largest logit of every group of 128 (bf16: 256) neighbours. The K best candidates lie in the K groups with the largest
 // maxima (equal ones: the first), so the second kernel compares those maxima over all rows, in 64 bits because rows differ by their log-sum-exp, and reads only
-// the few groups that can matter again. What bounds it: the logits, read once.
+// the few groups that can matter again. Inside a row the order is exact. What is compared across rows is exact but for the log-sum-exps, sums of 32-bit exponentials (each off by 2^-22 + 1.5 * 2^-23 times its
+// distance from the maximum, 16 at a time added in 32 bits, the rest in 64): candidates of different beams within 8e-6 of each other may change places. What bounds it: the logits, read once.
 #include <cfloat>
 
 #include "beam_api.h"
