@@ -133,6 +133,7 @@ class Engine:
         self.hybrid = any(layout.get("state_shapes") or [])  # recurrent layers: every sequence holds a state slot
         self.kv = PagedKVCache(layout, pages, self.device, model.dtype, self.config.kv, self._state_slots(layout), self.config.max_seqs if self.bounded else 0,
                                self._weight_capacity())
+        self._weighed = self._weight_capacity()
         if self.bounded and self.device.type == "cuda":
             self.kv.key_scores = torch.empty(self._score_room(), dtype=torch.float32, device=self.device)
         self.page_size = self.kv.page_size
@@ -576,7 +577,7 @@ class Engine:
         """Bounded cache: the rows that ``r`` holds if it is shortened in front of the coming decode step, else 0. That depends on the sequence alone, not on
         what else runs."""
         s, rows = self.config.kv, r.total_len - 1 + r.pending - r.evicted
-        return rows if rows > s.keep_tokens and (r.observed >= s.keep_every or rows >= self.kv.key_weights[0].shape[2]) else 0
+        return rows if rows > s.keep_tokens and (r.observed >= s.keep_every or rows >= self._weighed) else 0
 
     def _shorten(self, reqs: list[Request]) -> None:
         """Bounded cache: sequences that hold more than ``keep_tokens`` rows and have been observed long enough (or have no weights left) drop the rows that had the
