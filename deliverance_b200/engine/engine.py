@@ -747,8 +747,10 @@ class Engine:
         in both cases have one only."""
         kv, splits = self.model.n_kv, self._splits(len(lens))
         shape = len(lens), getattr(self.model, "n_heads", kv), kv, getattr(self.cfg, "head_dim", 0) or 128
-        alike = not by_length(splits, *shape) if self.bounded else splits <= ops.decode_room(*shape)
-        return alike or ops.even_lengths(lens)
+        if splits > ops.decode_room(*shape):
+            return ops.even_lengths(lens)
+        # (here the rows of one key that fill a bucket up do not make it unlike: 5 sequences of 1,088 keys in a bucket of 8, heads of 128, 14.8 us as alike, 17.4 as unlike)
+        return not (self.bounded and by_length(splits, *shape)) or ops.even_lengths([n for n in lens if n > 1])
 
     def _graph_decode(self, seqs: list[dict], dev_tokens: Optional[torch.Tensor] = None) -> torch.Tensor:
         B = len(seqs)

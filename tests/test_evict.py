@@ -985,3 +985,17 @@ def test_engine_bounded_cache_logits_against_64_bits(tmp_path, monkeypatch, H, K
     assert min(parts) >= 0.95 and min(own_parts) >= 0.95, (parts, own_parts)
     whole, _, _ = run(None)
     assert away(whole, want) > 3 * noise  # (what was dropped shows)
+
+
+def test_engine_bounded_cache_padding_is_not_unlike(tmp_path):
+    """Like sequences in a bucket that is not full take the step for like ones, where the split is by number in both; an unlike one among them does not."""
+    from deliverance_b200.ops.evict import by_length
+
+    model = tiny_model(tmp_path)
+    e, seen = engine_of(model, 64), 0
+    for B in (8, 16, 32, 64):
+        room, splits = ops.decode_room(B, model.n_heads, model.n_kv, model.cfg.head_dim), e._splits(B)
+        if splits <= room and by_length(splits, B, model.n_heads, model.n_kv, model.cfg.head_dim):
+            n, seen = B // 2 + 1, seen + 1
+            assert e._even([700] * n + [1] * (B - n)) and not e._even([700] * (n - 1) + [20000] + [1] * (B - n))
+    assert seen
