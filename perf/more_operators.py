@@ -198,6 +198,8 @@ def prepare(case, seed):
         rows = sum(new)
         s["q_start"], s["q_len"] = _ints([sum(new[:i]) for i in range(len(new))]), _ints(new)
         s["q_len_host"] = new
+        # (a step's query tiles are made once for all its layers)
+        s["tiles"] = {n: (_ints([i for i, m in enumerate(new) for _ in range(0, m, n)]), _ints([t for m in new for t in range(0, m, n)])) for n in (64, 128, 256)}
     s["lens"] = lens
     s["tables"], pages = _block_tables(lens, g)
     s["ctx"] = _ints(lens)
@@ -324,7 +326,7 @@ def run(state):
             return decode_attention4(s["q"], s["k"], s["v"], s["tables"], s["ctx"], case["kv"] * case["group"], case["dim"] ** -0.5, softcap=case["softcap"], window=case["window"])
         if op == "prompt":
             return prefill_attention4(s["q"], s["k"], s["v"], s["tables"], s["q_start"], s["q_len"], s["ctx"], case["kv"] * case["group"], case["dim"] ** -0.5,
-                                      softcap=case["softcap"], window=case["window"], q_len_host=s["q_len_host"], ctx_len_host=s["lens"])
+                                      softcap=case["softcap"], window=case["window"], q_len_host=s["q_len_host"], ctx_len_host=s["lens"], tiles_for=s["tiles"].get)
         t = step_tables(s["pages"], s["page_start"], s["cached"], s["start"], s["new"], s["tokens"], case["width"], PAGE, TILE, s["tiles"])
         return {n: getattr(t, n) for n in ("positions", "slots", "q_start", "ctx_len", "block_tables", "logits_rows", "tile_seq", "tile_q0")}
     return {"write": _plain_write, "decode": _plain_decode, "prompt": _plain_prompt, "tables": _plain_tables}[op](s)
