@@ -12,6 +12,7 @@
 #include "chain_api.h"
 #include "divisor.h"
 #include "gemm_api.h"
+#include "kv4_api.h"
 
 namespace {
 
@@ -1079,6 +1080,7 @@ Tensor prefill_attention_tc(const Tensor& q, const Tensor& k_cache, const Tensor
 #include "bindings_recurrent.inc"
 #include "bindings_mixed.inc"
 #include "bindings_beam.inc"
+#include "bindings_kv4.inc"
 
 // ---- sampling ---------------------------------------------------------------------------------------------------------
 std::vector<Tensor> argmax(const Tensor& logits, c10::optional<Tensor> mask, double softcap, double inv_scale) {
@@ -1881,6 +1883,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("decode_attention_weighted", &decode_attention_weighted);
   m.def("evict_keys", &evict_keys);
   m.def("beam_move", &beam_move, py::arg("tensors"), py::arg("slots"), py::arg("parents"), py::arg("rows") = py::none(), py::arg("paged") = false);
+  m.def("kv4_write", &kv4_write);
+  m.def("kv4_expand", &kv4_expand);
+  m.def("kv4_expand_seqs", &kv4_expand_seqs);
+  m.def("kv4_decode", &kv4_decode);
+  m.def("step_tables", &step_tables);
   m.def("q4_quantize", &q4_quantize);
   m.def("q4_dequantize", &q4_dequantize, py::arg("packed"), py::arg("scales"), py::arg("to_bf16") = false);
 }

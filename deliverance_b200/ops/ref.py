@@ -497,3 +497,85 @@ def evict_keys(k_caches, v_caches, weights, block_tables, ctx_lens, slots, keep:
                 for h in range(KV):
                     t[dst[j // P], h, j % P] = new[h]
     return kept, lens
+
+
+# ---------------------------------------------------------------------------------------------------------- cache in 4 bits
+KV4_LIMIT = 472.0
+
+
+def kv4_pack(x):
+    """``[..., D]`` -> uint8 rows ``[..., D / 2 + D / 8]`` (``ops.kv4``). Every operation rounds to fp32 by itself, as in the kernels."""
+    b = x.float().unflatten(-1, (-1, 32))
+    nan = torch.isnan(b).any(-1)
+    b = b.clamp(-KV4_LIMIT, KV4_LIMIT)
+    low = (b.amin(-1) + 0.0).half()
+    step = (b.amax(-1) - low.float()).clamp_min(0.0) * (1.0 / 15.0) + 0.0  # (no negative zero)
+    up = ((step.view(torch.int32) + 0x1FFFF) & ~0x1FFFF).view(torch.float32)
+    step = torch.where(step < 2.0**-14, torch.ceil(step * 2.0**20) * 2.0**-20, up)
+    step = torch.where(nan, 0.0, step)
+    low = torch.where(nan, math.nan, low)
+    codes = (b - low.float().unsqueeze(-1)) * (1.0 / step).unsqueeze(-1)
+    codes = torch.where(step.unsqueeze(-1) > 0, codes, 0.0).round().clamp(0.0, 15.0).to(torch.uint8).flatten(-2)
+    side = torch.stack((step.half(), low), -1).flatten(-2).contiguous().view(torch.uint8)
+    return torch.cat((codes[..., 0::2] | (codes[..., 1::2] << 4), side), -1)
+
+
+def kv4_unpack(rows, dtype=torch.float32):
+    """The values of uint8 rows."""
+    D = rows.shape[-1] * 8 // 5
+    codes = rows[..., : D // 2]
+    c = torch.stack((codes & 15, codes >> 4), -1).flatten(-2).unflatten(-1, (-1, 32)).float()
+    side = rows[..., D // 2 :].contiguous().view(torch.float16).float().unflatten(-1, (-1, 2))
+    return (c * side[..., :1] + side[..., 1:]).flatten(-2).to(dtype)
+
+
+def rotate_columns(x, cos, sin, pairs: bool):
+    """fp32 ``[T, heads, D]``: the first ``2 * half`` columns rotated by ``cos`` / ``sin [T, half]``; ``pairs``: column 2 i with 2 i + 1, else i with i + half."""
+    half = cos.shape[-1]
+    c, n, x = cos.unsqueeze(1), sin.unsqueeze(1), x.clone()
+    a, b = (x[..., 0 : 2 * half : 2], x[..., 1 : 2 * half : 2]) if pairs else (x[..., :half], x[..., half : 2 * half])
+    turned = a * c - b * n, b * c + a * n
+    a.copy_(turned[0])
+    b.copy_(turned[1])
+    return x
+
+
+def rope_kv4(qkv, positions, slots, q_norm_w, k_norm_w, cos, sin, k_cache, v_cache, H, KV, D, eps, norm_offset, pairs):
+    T = qkv.shape[0]
+    q, k, v = qkv.float().reshape(T, H + 2 * KV, D).split((H, KV, KV), 1)
+    if q_norm_w is not None:
+        norm = lambda x, w: x * (1.0 / torch.sqrt(x.double().square().mean(-1, keepdim=True) + eps)).float() * (w.float() + norm_offset)  # noqa: E731
+        q, k = norm(q, q_norm_w), norm(k, k_norm_w)
+    if cos is not None:
+        at = positions.long().clamp(0, cos.shape[0] - 1)
+        q, k = (rotate_columns(x, cos[at], sin[at], pairs) for x in (q, k))
+    keep = slots >= 0
+    page = k_cache.shape[2]
+    block, row = torch.div(slots[keep], page, rounding_mode="floor"), slots[keep] % page
+    k_cache[block, :, row] = kv4_pack(k[keep])
+    v_cache[block, :, row] = kv4_pack(v[keep])
+    return q.to(qkv.dtype).reshape(T, H * D)
+
+
+def step_tables(pages, page_start, cached, start, new, tokens, width, page, tile, tiles):
+    S = new.shape[0]
+    new, cached, start, first, pages = (t.long() for t in (new, cached, start, page_start, pages))
+    have = first[1:] - first[:-1]
+    count = torch.div(new + tile - 1, tile, rounding_mode="floor")
+    need = torch.where(new > 0, torch.div(cached + new + page - 1, page, rounding_mode="floor"), 0)
+    if bool((new < 0).any()) or int(new.sum()) != tokens or (tiles and int(count.sum()) != tiles):
+        raise ValueError("lengths do not add up to the number of tokens or tiles")
+    if bool((have < 0).any()) or bool((have > width).any()) or bool((need > have).any()) or bool((cached < 0).any()) or int(first[0]) < 0 or int(first[-1]) > pages.shape[0]:
+        raise ValueError("rows without a page, or tables too narrow")
+    q_start = new.cumsum(0) - new
+    b = torch.repeat_interleave(torch.arange(S), new)
+    off = torch.arange(tokens) - q_start[b]
+    row = cached[b] + off
+    slots = pages[first[b] + torch.div(row, page, rounding_mode="floor")] * page + row % page
+    table = torch.zeros(S, width, dtype=torch.int32)
+    for i in range(S):
+        table[i, : int(have[i])] = pages[int(first[i]) : int(first[i + 1])]
+    b_tile = torch.repeat_interleave(torch.arange(S), count) if tiles else torch.zeros(0, dtype=torch.long)
+    q0 = (torch.arange(tiles) - (count.cumsum(0) - count)[b_tile]) * tile
+    i32 = torch.int32
+    return (start[b] + off).to(i32), slots, q_start.to(i32), (cached + new).to(i32), table, q_start + new - 1, b_tile.to(i32), q0.to(i32)

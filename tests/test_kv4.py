@@ -1,0 +1,531 @@
+"""The KV cache in 4 bits (quantising write, unpacking, decode and prompt attention) and step tables against plain statements in 64 bits, on the CPU and, on a GPU box, on the CUDA kernels."""
+import math
+
+import pytest
+import torch
+
+from deliverance_b200 import ops
+from deliverance_b200.ops import ref
+from deliverance_b200.ops.kv4 import decode_attention4, expand4, prefill_attention4, rope_kv4, row_bytes
+from deliverance_b200.ops.tables import step_tables
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+GPU = [pytest.param("cuda", marks=pytest.mark.gpu)]
+BF16 = torch.bfloat16
+HALF_STEP = torch.finfo(BF16).eps / 2
+
+
+def done(device):
+    if device == "cuda":
+        ops.check_status()
+
+
+def plain_block(x):
+    """One block of 32 numbers by the definition, in Python: (codes, step, minimum)."""
+    f32 = lambda v: torch.tensor(v, dtype=torch.float64).float().item()  # noqa: E731
+    x = [min(max(float(v), -472.0), 472.0) for v in x]
+    m = torch.tensor(min(x)).half().item()
+    s0 = f32(max(f32(max(x) - m), 0.0) * f32(1 / 15))
+    if s0 < 2.0**-14:
+        s = math.ceil(s0 * 2**20) / 2**20
+    else:
+        frac, e = math.frexp(s0)
+        s = math.ldexp(math.ceil(frac * 128), e - 7)
+    codes = []
+    for v in x:
+        c = f32(f32(v - m) * f32(1 / s)) if s > 0 else 0.0
+        codes.append(int(min(max(round(c), 0), 15)))  # (Python rounds halves to even, as rint does)
+    return codes, s, m
+
+
+def test_block_definition():
+    for scale in (1e-6, 1e-5, 3e-4, 0.02, 1.0, 31.0, 2000.0):
+        x = (torch.randn(40, 32) * scale).float()
+        x[0] = 0.0
+        x[1] = scale
+        x[2, :16], x[2, 16:] = -0.0, 0.0
+        x[3] = scale * torch.arange(32) / 31
+        x[4, 0], x[4, 1] = math.inf, -math.inf
+        rows = ref.kv4_pack(x)
+        assert rows.shape == (40, row_bytes(32)) and row_bytes(128) == 80
+        for r in range(40):
+            codes, s, m = plain_block(x[r].tolist())
+            packed = bytes(rows[r, :16].tolist())
+            assert [packed[i // 2] >> (4 * (i % 2)) & 15 for i in range(32)] == codes
+            side = rows[r, 16:].view(torch.float16)
+            assert side[0].item() == s and side[1].item() == m and math.copysign(1.0, m or 1.0) == math.copysign(1.0, side[1].item() or 1.0)
+        back = ref.kv4_unpack(rows)
+        lo = x.clamp(-472, 472).amin(1, keepdim=True)
+        step = rows[:, 16:18].view(torch.float16).float()
+        # half a step, half a step of fp16 of the minimum (or of its smallest numbers), and the fp32 roundings of (x - m) / s, some 2^-22 of 15 steps
+        assert ((back - x.clamp(-472, 472)).abs() <= step * (0.5 + 2.0**-18) + lo.abs() * 2.0**-11 + 2.0**-25).all()
+
+
+def test_nan_makes_its_block_nan():
+    x = torch.randn(3, 128)
+    x[1, 70] = math.nan
+    back = ref.kv4_unpack(ref.kv4_pack(x))
+    assert torch.isnan(back[1, 64:96]).all() and not torch.isnan(back[1, :64]).any() and not torch.isnan(back[1, 96:]).any() and not torch.isnan(back[[0, 2]]).any()
+
+
+def rotary(positions, half, far, mult=1.0):
+    turn = torch.arange(far, dtype=torch.float64).view(-1, 1) * (1e4 ** (-torch.arange(half, dtype=torch.float64) / max(half, 1)))
+    return (torch.cos(turn) * mult).float(), (torch.sin(turn) * mult).float()
+
+
+def exact_heads(x, w, eps, offset, cos, sin, positions, pairs):
+    """fp64 [T, heads, D], element by element of a head."""
+    x = x.double().clone()
+    if w is not None:
+        x = x / torch.sqrt((x * x).sum(-1, keepdim=True) / x.shape[-1] + eps) * (w.double() + offset)
+    if cos is not None:
+        y = x.clone()
+        at = positions.clamp(0, cos.shape[0] - 1).long()
+        for i in range(cos.shape[1]):
+            a, b = (2 * i, 2 * i + 1) if pairs else (i, i + cos.shape[1])
+            c, s = cos[at, i].double().view(-1, 1), sin[at, i].double().view(-1, 1)
+            y[..., a] = x[..., a] * c - x[..., b] * s
+            y[..., b] = x[..., b] * c + x[..., a] * s
+        x = y
+    return x
+
+
+WRITES = [(D, H, KV, T, rotate, half, norm) for D, half in ((64, 32), (128, 64), (256, 128)) for H, KV, T in ((1, 1, 1), (6, 2, 37), (12, 3, 5))
+          for rotate, norm in (("halves", True), ("pairs", False))] + [
+    (64, 4, 1, 9, "halves", 5, True), (64, 4, 1, 9, "pairs", 5, False), (128, 4, 2, 9, "halves", 16, False), (128, 4, 2, 9, "halves", 20, True), (256, 2, 1, 9, "pairs", 33, True),
+    (128, 4, 2, 9, "halves", 0, True), (128, 32, 8, 130, "halves", 64, True)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D,H,KV,T,rotate,half,norm", WRITES)
+def test_write_matches_plain(device, D, H, KV, T, rotate, half, norm):
+    page, pages, eps, offset = 32 if D < 256 else 64, 2 + T // 16, 1e-5, 1.0 if T % 2 else 0.0
+    wide = torch.randn(T, (H + 2 * KV) * D + 24).to(BF16)  # (rows further apart than they are long)
+    wide[:, : H * D] *= 3
+    qn, kn = (torch.randn(D).to(BF16), torch.randn(D).to(BF16)) if norm else (None, None)
+    far = 300
+    cos, sin = rotary(None, half, far, 1.2) if half else (None, None)
+    positions = torch.randint(-2, far + 2, (T,), dtype=torch.int32)
+    slots = torch.randperm(pages * page)[:T]
+    if T > 3:
+        slots[2] = -1
+    start = torch.randint(0, 256, (2, pages, KV, page, row_bytes(D)), dtype=torch.uint8)
+    to = lambda t: None if t is None else t.to(device)  # noqa: E731
+    x = to(wide)[:, : (H + 2 * KV) * D]
+    before = x.clone()
+    kc, vc = to(start[0].clone()), to(start[1].clone())
+    q = rope_kv4(x, to(positions), to(slots), to(qn), to(kn), to(cos), to(sin), kc, vc, H, KV, D, eps, offset, rotate)
+    done(device)
+    assert torch.equal(x, before) and q.shape == (T, H * D) and q.dtype == BF16
+    heads = wide[:, : (H + 2 * KV) * D].reshape(T, H + 2 * KV, D)
+    want = exact_heads(heads[:, :H], qn, eps, offset, cos, sin, positions, rotate == "pairs").flatten(1)
+    # one rounding to bf16, and before it fp32 roundings of some six products and sums no larger than 1.2 (|a| + |b|) of a pair
+    size = 2.4 * exact_heads(heads[:, :H], qn, eps, offset, None, None, None, False).abs().amax(-1, keepdim=True).expand(T, H, D).flatten(1)
+    assert ((q.cpu().double() - want).abs() <= want.abs() * HALF_STEP + size * 2.0**-21).all()
+    # the cache: the same bytes as the plain statement, everything else as it was
+    k64 = exact_heads(heads[:, H : H + KV], kn, eps, offset, cos, sin, positions, rotate == "pairs")
+    k2, v2 = start[0].clone(), start[1].clone()
+    ref.rope_kv4(wide[:, : (H + 2 * KV) * D], positions, slots, qn, kn, cos, sin, k2, v2, H, KV, D, eps, offset, rotate == "pairs")
+    assert torch.equal(kc.cpu(), k2) and torch.equal(vc.cpu(), v2)
+    for cache, old, fresh in ((kc, start[0], k64), (vc, start[1], heads[:, H + KV :].double())):
+        flat, was = cache.cpu().transpose(1, 2).flatten(0, 1), old.transpose(1, 2).flatten(0, 1)
+        written = slots[slots >= 0]
+        rest = torch.ones(flat.shape[0], dtype=torch.bool)
+        rest[written] = False
+        assert torch.equal(flat[rest], was[rest])
+        rows = flat[written]
+        step = rows[..., D // 2 :].contiguous().view(torch.float16).float().unflatten(-1, (-1, 2))[..., 0].repeat_interleave(32, -1)
+        x64 = fresh[slots >= 0].clamp(-472, 472)
+        lo = x64.unflatten(-1, (-1, 32)).amin(-1).abs().repeat_interleave(32, -1)
+        assert ((ref.kv4_unpack(rows).double() - x64).abs() <= step * (0.5 + 2.0**-18) + lo * 2.0**-11 + x64.abs().amax() * 2.0**-20).all()
+
+
+@pytest.mark.parametrize("device", GPU)
+def test_write_of_extremes_has_the_plain_bytes(device):
+    D, H, KV, T = 128, 2, 2, 64
+    x = torch.randn(T, H + 2 * KV, D) * 10.0 ** torch.randint(-7, 4, (T, 1, 1))
+    x[5, 2:, 3], x[6, 2:, 9], x[7, 2:, 40], x[8], x[9] = math.nan, math.inf, -math.inf, 0.0, -0.0
+    x = x.to(BF16).flatten(1)
+    k, v = (torch.zeros(2, KV, 32, row_bytes(D), dtype=torch.uint8) for _ in range(2))
+    kc, vc = k.to(device), v.to(device)
+    slots, positions = torch.arange(T), torch.zeros(T, dtype=torch.int32)
+    ref.rope_kv4(x, positions, slots, None, None, None, None, k, v, H, KV, D, 1e-6, 0.0, False)
+    rope_kv4(x.to(device), positions.to(device), slots.to(device), None, None, None, None, kc, vc, H, KV, D, 1e-6)
+    done(device)
+    assert torch.equal(kc.cpu(), k) and torch.equal(vc.cpu(), v)
+
+
+def random_cache(pages, KV, page, D, loud=True):
+    x = torch.randn(pages, KV, page, D)
+    if loud:
+        x[..., :: 17] *= 6
+    return ref.kv4_pack(x)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D,KV,page", [(64, 3, 32), (128, 1, 96), (256, 2, 64)])
+def test_expand_matches_plain(device, D, KV, page):
+    k, v = random_cache(7, KV, page, D), random_cache(7, KV, page, D)
+    for pages in ([3], [6, 0, 6, 1], []):
+        want = [ref.kv4_unpack(t)[torch.tensor(pages, dtype=torch.long)] for t in (k, v)]
+        for dtype in (torch.float32, BF16):
+            got = expand4(k.to(device), v.to(device), torch.tensor(pages, dtype=torch.int32, device=device), dtype)
+            done(device)
+            for g, w in zip(got, want):
+                assert g.dtype == dtype and torch.equal(g.cpu(), w.to(dtype))
+
+
+def tables_for(lens, page, first=1, extra=0):
+    need = [-(-n // page) for n in lens]
+    order = (torch.randperm(sum(need)) + first).to(torch.int32)
+    t = torch.zeros(len(lens), max(max(need), 1) + extra, dtype=torch.int32)
+    at = 0
+    for i, n in enumerate(need):
+        t[i, :n] = order[at : at + n]
+        at += n
+    return t, first + sum(need)
+
+
+def plain_attention(q, k, v, table, lens, news, KV, scale, softcap, window, values=ref.kv4_unpack):
+    """fp64 outputs, and what errors are measured by: sum of p |v|, and the largest sum of |q| |k| of a row."""
+    D = k.shape[3] * 8 // 5
+    out, mass, reach = torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64)
+    row = 0
+    for b, (n, m) in enumerate(zip(lens, news)):
+        if m == 0:
+            continue
+        pages = table[b, : -(-n // k.shape[2])].long()
+        K, V = (values(t[pages]).transpose(0, 1).flatten(1, 2)[:, :n].double() for t in (k, v))
+        Q = q[row : row + m].double().view(m, KV, -1, D).permute(1, 2, 0, 3)
+        x = torch.einsum("kgtd,knd->kgtn", Q, K) * scale
+        if softcap:
+            x = softcap * torch.tanh(x / softcap)
+        last, j = torch.arange(n - m, n).view(-1, 1), torch.arange(n)
+        hidden = j > last
+        if window:
+            hidden = hidden | (j <= last - window)
+        if n:  # (without keys: zeros)
+            p = torch.softmax(x.masked_fill(hidden, -math.inf), -1)
+            flat = lambda y: y.permute(2, 0, 1, 3).reshape(m, -1)  # noqa: E731
+            out[row : row + m] = flat(torch.einsum("kgtn,knd->kgtd", p, torch.where(torch.isfinite(V), V, 0.0)))
+            mass[row : row + m] = flat(torch.einsum("kgtn,knd->kgtd", p, torch.where(torch.isfinite(V), V, 0.0).abs()))
+            size = torch.einsum("kgtd,knd->kgtn", Q.abs(), K.abs()).masked_fill(hidden, 0.0).amax(-1, keepdim=True) * scale
+            reach[row : row + m] = flat(size.expand(*size.shape[:-1], D))
+        row += m
+    return out, mass, reach
+
+
+def check_decode(got, q, k, v, table, lens, KV, scale, softcap, window):
+    want, mass, reach = plain_attention(q, k, v, table, lens, [1] * len(lens), KV, scale, softcap, window)
+    got = got.cpu().double()
+    assert torch.isfinite(got).all()
+    # the result's rounding to bf16; of every probability one rounding to fp16 and the exponential's 2^-21 and 2^-22 of its argument, numerator and denominator; of a score, whose codes, steps and minima are exact, fp32 sums of 256 numbers
+    # (products of tensor cores are cut off, not rounded: 2^-22 of the sum of magnitudes per addition would be 2^-14 at worst, and errs one way for all keys alike; 2^-17 is allowed)
+    tol = want.abs() * HALF_STEP + mass * (2.0**-10 + reach * (2.0**-16 + 2.0**-20)) + 1e-30
+    assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
+
+
+def run_decode(device, D, KV, G, lens, softcap=0.0, window=0, page=32, extra=1, spoil=True, scale=None, mult=1.0):
+    B, H = len(lens), KV * G
+    table, pages = tables_for(lens, page, extra=extra)
+    q = (torch.randn(B, H * D) * mult).to(BF16)
+    k, v = random_cache(pages, KV, page, D), random_cache(pages, KV, page, D, False)
+    if spoil:  # what lies behind a sequence's end or in front of its window must not matter, not even infinities and NaN
+        for b, n in enumerate(lens):
+            if n % page:
+                k[table[b, n // page].long(), :, n % page :] = v[table[b, n // page].long(), :, n % page :] = 0xFE
+            if window and n > window:
+                for j in range(n - window):
+                    k[table[b, j // page].long(), :, j % page] = v[table[b, j // page].long(), :, j % page] = 0x7D if j % 2 else 0xFE
+    scale = scale or D**-0.5
+    to = lambda t: t.to(device)  # noqa: E731
+    got = decode_attention4(to(q), to(k), to(v), to(table), to(torch.tensor(lens, dtype=torch.int32)), H, scale, softcap, window)
+    done(device)
+    assert got.shape == q.shape and got.dtype == BF16
+    check_decode(got, q, k, v, table, lens, KV, scale, softcap, window)
+    for b, n in enumerate(lens):
+        if n == 0:
+            assert (got[b] == 0).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("KV,G", [(1, 1), (2, 4), (3, 5), (1, 16), (8, 8), (2, 9)])
+@pytest.mark.parametrize("lens", [[1], [33, 0, 1, 500], [700, 31, 32], [3001, 2], [64] * 70, [0]])
+def test_decode_matches_plain(device, D, KV, G, lens):
+    if device == "cpu" and sum(lens) * KV * G * D > 3e7:
+        pytest.skip("large for the CPU")
+    run_decode(device, D, KV, G, lens)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("G,softcap,window", [(2, 50.0, 0), (12, 0.5, 0), (2, 0.0, 100), (8, 50.0, 17), (3, 0.0, 1)])
+def test_decode_softcap_window(device, D, G, softcap, window):
+    run_decode(device, D, 2, G, [777, 16, 100, 101, 0, 1], softcap, window)
+
+
+@pytest.mark.parametrize("device", GPU)
+@pytest.mark.parametrize("lens", [[40000], [20000, 1, 3, 500, 9000], [100 + 7 * i for i in range(130)], [1] * 300, [32] * 128, [5000] * 9, [31, 33] * 40])
+@pytest.mark.parametrize("D,KV,G", [(128, 8, 4), (64, 1, 2), (256, 2, 16)])
+def test_decode_work_split(device, lens, D, KV, G):
+    run_decode(device, D, KV, G, lens, page=64 if len(lens) == 5 else 32, extra=0, spoil=len(lens) < 200)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_decode_sharp_and_large(device):
+    run_decode(device, 128, 2, 4, [300, 65], mult=60.0)  # single keys take all the weight, scores of thousands
+    run_decode(device, 128, 2, 4, [300, 65], mult=3e4, scale=1e-6)
+    run_decode(device, 64, 1, 8, [200], mult=1e-30, scale=1e30)
+    run_decode(device, 64, 1, 8, [200], mult=0.0)
+
+
+def run_prefill(device, D, KV, G, news, befores, softcap=0.0, window=0, page=32):
+    lens = [a + b for a, b in zip(news, befores)]
+    H, T = KV * G, sum(news)
+    table, pages = tables_for(lens, page, extra=1)
+    q = torch.randn(T, H * D).to(BF16)
+    k, v = random_cache(pages, KV, page, D, False), random_cache(pages, KV, page, D, False)
+    for b, n in enumerate(lens):
+        if n % page:
+            k[table[b, n // page].long(), :, n % page :] = v[table[b, n // page].long(), :, n % page :] = 0xFE
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    start = [sum(news[:i]) for i in range(len(news))]
+    got = prefill_attention4(q.to(device), k.to(device), v.to(device), table.to(device), i32(start), i32(news), i32(lens), H, D**-0.5, softcap, window)
+    done(device)
+    if device == "cpu":
+        want, mass, reach = plain_attention(q, k, v, table, lens, news, KV, D**-0.5, softcap, window)
+        tol = want.abs() * HALF_STEP + mass * (2.0**-16 + reach * 2.0**-16)
+    else:  # keys and values in bf16, as the kernel behind reads them (unpacking is tested by itself): probabilities in bf16, numerator and denominator, the result in bf16
+        want, mass, reach = plain_attention(q, k, v, table, lens, news, KV, D**-0.5, softcap, window, lambda t: ref.kv4_unpack(t, BF16))
+        tol = want.abs() * HALF_STEP + mass * (2 * HALF_STEP + reach * 2.0**-16)
+    assert ((got.cpu().double() - want).abs() <= tol + 1e-30).all(), ((got.cpu().double() - want).abs() / (tol + 1e-30)).max()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D,KV,G", [(64, 2, 3), (128, 1, 4), (256, 2, 1)])
+@pytest.mark.parametrize("news,befores", [([1], [0]), ([33, 5], [0, 70]), ([130, 1, 64], [3, 31, 0]), ([3, 0, 2], [0, 40, 9])])
+def test_prefill_matches_plain(device, D, KV, G, news, befores):
+    run_prefill(device, D, KV, G, news, befores)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("softcap,window,page", [(30.0, 0, 32), (0.0, 40, 64), (50.0, 7, 32), (0.0, 0, 96)])
+def test_prefill_options(device, softcap, window, page):
+    run_prefill(device, 64, 2, 2, [70, 40], [100, 0], softcap, window, page)
+
+
+@pytest.mark.parametrize("device", GPU)
+def test_prefill_in_portions(device, monkeypatch):
+    from deliverance_b200.ops import kv4
+
+    monkeypatch.setattr(kv4, "EXPAND_PAGES_BYTES", 5 * 2 * 32 * 64 * 4)
+    run_prefill(device, 64, 2, 2, [70, 40, 1, 9, 300], [100, 0, 20, 3, 0])
+
+
+def plain_tables(pages, cached, start, new, width, page, tile):
+    out = {n: [] for n in ("positions", "slots", "q_start", "ctx_len", "block_tables", "logits_rows", "tile_seq", "tile_q0")}
+    row = 0
+    for i, n in enumerate(new):
+        out["q_start"].append(row)
+        out["ctx_len"].append(cached[i] + n)
+        out["logits_rows"].append(row + n - 1)
+        out["block_tables"].append(pages[i] + [0] * (width - len(pages[i])))
+        for j in range(n):
+            out["positions"].append(start[i] + j)
+            out["slots"].append(pages[i][(cached[i] + j) // page] * page + (cached[i] + j) % page)
+        for t in range(0, n, tile):
+            out["tile_seq"].append(i)
+            out["tile_q0"].append(t)
+        row += n
+    return out
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("new,page,tile", [([1], 32, 64), ([1] * 70, 32, 64), ([333, 1, 64, 65], 32, 64), ([5, 0, 0, 129, 0], 64, 32), ([0], 32, 64), ([3] * 1000, 96, 64), ([], 32, 64)])
+def test_step_tables(device, new, page, tile):
+    cached = [int(torch.randint(0, 200, ())) for _ in new]
+    start = [c + int(torch.randint(0, 50, ())) for c in cached]
+    need = [-(-(c + n) // page) + i % 3 for i, (c, n) in enumerate(zip(cached, new))]  # (some hold pages in reserve)
+    order = (torch.randperm(sum(need)) + 1 + (1 << 28 if page == 96 else 0)).tolist()  # (slots beyond 32 bits)
+    pages = [order[sum(need[:i]) : sum(need[: i + 1])] for i in range(len(new))]
+    width, tiles = max(need + [0]) + 2, sum(-(-n // tile) for n in new)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    got = step_tables(i32(order), i32([sum(need[:i]) for i in range(len(new) + 1)]), i32(cached), i32(start), i32(new), sum(new), width, page, tile, tiles)
+    done(device)
+    want = plain_tables(pages, cached, start, new, width, page, tile)
+    for name, t in got._asdict().items():
+        dtype = torch.int64 if name in ("slots", "logits_rows") else torch.int32
+        assert t.dtype == dtype and t.device.type == device
+        assert torch.equal(t.cpu(), torch.tensor(want[name], dtype=dtype).reshape(t.shape)), name
+    assert step_tables(i32(order), i32([sum(need[:i]) for i in range(len(new) + 1)]), i32(cached), i32(start), i32(new), sum(new), width, page).tile_seq.numel() == 0
+
+
+BAD_TABLES = [
+    dict(tokens=4),  # five rows
+    dict(new=[2, -3]),
+    dict(tiles=3),
+    dict(width=1),
+    dict(cached=[31, 33]),  # row 64 has no page
+    dict(cached=[-1, 0]),
+    dict(page_start=[0, 2, 9]),
+    dict(page_start=[0, 3, 2]),
+    dict(page_start=[-1, 1, 3]),
+]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("change", BAD_TABLES)
+def test_step_tables_reports(device, change):
+    a = dict(pages=[4, 5, 6], page_start=[0, 1, 3], cached=[0, 30], start=[0, 30], new=[2, 3], tokens=5, width=2, tiles=2)
+    a.update(change)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    call = lambda: step_tables(i32(a["pages"]), i32(a["page_start"]), i32(a["cached"]), i32(a["start"]), i32(a["new"]), a["tokens"], a["width"], 32, 64, a["tiles"])  # noqa: E731
+    if device == "cpu":
+        with pytest.raises(ValueError):
+            call()
+    else:
+        got = call()
+        with pytest.raises(RuntimeError, match="bad kernel arguments"):
+            ops.check_status()
+        ops.check_status()
+        assert ((got.slots >= -1) & (got.slots < 7 * 32)).all() and ((got.block_tables >= 0) & (got.block_tables <= 6)).all()
+
+
+def kv4_args(device, D=64, H=4, KV=2, T=3):
+    to = lambda t: t.to(device)  # noqa: E731
+    return dict(qkv=to(torch.randn(T, (H + 2 * KV) * D).to(BF16)), positions=to(torch.arange(T, dtype=torch.int32)), slots=to(torch.arange(T)), q_norm_w=to(torch.ones(D, dtype=BF16)),
+                k_norm_w=to(torch.ones(D, dtype=BF16)), cos=to(torch.ones(9, D // 2)), sin=to(torch.zeros(9, D // 2)), k_cache=to(torch.zeros(2, KV, 32, row_bytes(D), dtype=torch.uint8)),
+                v_cache=to(torch.zeros(2, KV, 32, row_bytes(D), dtype=torch.uint8)), H=H, KV=KV, D=D, eps=1e-6)
+
+
+BAD_WRITES = [
+    dict(rotate="thirds"), dict(D=96), dict(H=5), dict(KV=3), dict(cos=None), dict(k_norm_w=None), dict(positions=slice(0, 2)), dict(slots=slice(0, 2)), dict(slots=torch.int32),
+    dict(k_cache=torch.int8), dict(v_cache=(2, 2, 32, 41)), dict(v_cache=(3, 2, 32, 40)), dict(cos=(9, 33), sin=(9, 33)), dict(sin=(8, 32)), dict(k_cache=(2, 2, 16, 40), v_cache=(2, 2, 16, 40)),
+]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("change", BAD_WRITES)
+def test_write_refuses(device, change):
+    a = kv4_args(device)
+    for name, c in change.items():
+        t = a.get(name)
+        a[name] = t[c] if isinstance(c, slice) else t.to(c) if isinstance(c, torch.dtype) else torch.zeros(c, dtype=t.dtype, device=device) if isinstance(c, tuple) else c
+    with pytest.raises((ValueError, RuntimeError)):
+        rope_kv4(**a)
+    done(device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_write_reports_slots_behind_the_cache(device):
+    a = kv4_args(device)
+    a["slots"] = torch.tensor([0, 64, 1 << 40], device=device)
+    if device == "cpu":
+        with pytest.raises(IndexError):
+            rope_kv4(**a)
+    else:
+        rope_kv4(**a)
+        with pytest.raises(RuntimeError, match="bad kernel arguments"):
+            ops.check_status()
+        assert (a["k_cache"][:, :, 1:] == 0).all() and a["k_cache"][0, :, 0].any()
+
+
+def attention_args(device, B=2, D=64, KV=2, G=2):
+    to = lambda t: t.to(device)  # noqa: E731
+    return dict(q=to(torch.randn(B, KV * G * D).to(BF16)), k_cache=to(random_cache(4, KV, 32, D)), v_cache=to(random_cache(4, KV, 32, D)),
+                block_tables=to(torch.tensor([[1, 2], [3, 0]], dtype=torch.int32)), ctx_lens=to(torch.tensor([40, 5], dtype=torch.int32)), H=KV * G, scale=0.1)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("change", [dict(H=3), dict(H=8), dict(window=-1), dict(softcap=-1.0), dict(block_tables=torch.int64), dict(ctx_lens=slice(0, 1)), dict(block_tables=slice(0, 1)),
+                                    dict(k_cache=slice(0, 3)), dict(v_cache=torch.int8)])
+def test_decode_refuses(device, change):
+    a = attention_args(device)
+    for name, c in change.items():
+        t = a.get(name)
+        a[name] = t[c] if isinstance(c, slice) else t.to(c) if isinstance(c, torch.dtype) else c
+    with pytest.raises((ValueError, RuntimeError)):
+        decode_attention4(**a)
+    done(device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("change", [dict(block_tables=[[1, 9], [3, 0]]), dict(block_tables=[[1, -2], [3, 0]]), dict(ctx_lens=[65, 5]), dict(ctx_lens=[40, -1])])
+def test_decode_reports_bad_tables(device, change):
+    a = attention_args(device)
+    for name, c in change.items():
+        a[name] = torch.tensor(c, dtype=torch.int32, device=device)
+    if device == "cpu":
+        with pytest.raises((ValueError, IndexError)):
+            decode_attention4(**a)
+    else:
+        assert decode_attention4(**a).shape == a["q"].shape
+        with pytest.raises(RuntimeError, match="bad kernel arguments"):
+            ops.check_status()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_expand_reports_pages_outside(device):
+    k = random_cache(3, 1, 32, 64).to(device)
+    for pages in ([0, 3], [-1]):
+        pages = torch.tensor(pages, dtype=torch.int32, device=device)
+        if device == "cpu":
+            with pytest.raises(IndexError):
+                expand4(k, k, pages)
+        else:
+            expand4(k, k, pages)
+            with pytest.raises(RuntimeError, match="bad kernel arguments"):
+                ops.check_status()
+    with pytest.raises(ValueError):
+        expand4(k, k, torch.zeros(1, dtype=torch.int32, device=device), torch.float64)
+
+
+@pytest.mark.parametrize("device", GPU)
+def test_prefill_reports(device):
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    a = attention_args(device)
+    q, rest = torch.randn(4, 256, device=device).to(BF16), (a["k_cache"], a["v_cache"])
+    run = lambda table, news, lens, **kw: prefill_attention4(q, *rest, i32(table), i32([0, 3]), i32(news), i32(lens), 4, 0.1, **kw)  # noqa: E731
+    with pytest.raises(ValueError):
+        run([[1, 2], [3, 0]], [3, 2], [40, 5])
+    with pytest.raises(ValueError):
+        run([[1, 2], [3, 0]], [3, 1], [2, 5])
+    run([[1, 7], [3, 0]], [3, 1], [40, 5])
+    with pytest.raises(RuntimeError, match="bad kernel arguments"):
+        ops.check_status()
+    run([[1, 2], [3, 0]], [3, 1], [70, 5])
+    with pytest.raises(RuntimeError, match="bad kernel arguments"):
+        ops.check_status()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_operators_together(device):
+    """Two prompts, one behind a cached prefix, then three decode steps: tables, write, attention, as a layer uses them; the attention against 64 bits over what the cache holds."""
+    D, H, KV, page = 128, 8, 2, 32
+    tol = lambda want, mass, reach: want.abs() * HALF_STEP + mass * (2 * HALF_STEP + reach * 2.0**-16) + 1e-30  # noqa: E731
+    to = lambda t: t.to(device)  # noqa: E731
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    cos, sin = (to(t) for t in rotary(None, 32, 400))
+    qn, kn = to(torch.randn(D).to(BF16)), to(torch.randn(D).to(BF16))
+    kc, vc = to(random_cache(12, KV, page, D)), to(random_cache(12, KV, page, D, False))
+    pages = [[3, 7, 1, 9, 4], [2, 11, 5]]
+    cached, flat, first = [40, 0], i32(pages[0] + pages[1]), i32([0, 5, 8])
+    for new in ([77, 50], [1, 1], [1, 1], [1, 1]):
+        T = sum(new)
+        t = step_tables(flat, first, i32(cached), i32(cached), i32(new), T, 6, page, 64, sum(-(-n // 64) for n in new))
+        qkv = to(torch.randn(T, (H + 2 * KV) * D).to(BF16))
+        q = rope_kv4(qkv, t.positions, t.slots, qn, kn, cos, sin, kc, vc, H, KV, D, 1e-6)
+        if T > 2:
+            got = prefill_attention4(q, kc, vc, t.block_tables, t.q_start, i32(new), t.ctx_len, H, D**-0.5)
+        else:
+            got = decode_attention4(q, kc, vc, t.block_tables, t.ctx_len, H, D**-0.5)
+        done(device)
+        lens = [a + b for a, b in zip(cached, new)]
+        values = (lambda x: ref.kv4_unpack(x, BF16)) if device == "cuda" and T > 2 else ref.kv4_unpack
+        want, mass, reach = plain_attention(q.cpu(), kc.cpu(), vc.cpu(), t.block_tables.cpu(), lens, new, KV, D**-0.5, 0.0, 0, values)
+        assert ((got.cpu().double() - want).abs() <= tol(want, mass, reach)).all()
+        v_new = qkv.view(T, H + 2 * KV, D)[:, H + KV :].cpu()
+        held = vc.cpu().transpose(1, 2).flatten(0, 1)[t.slots.cpu()]
+        assert torch.equal(held, ref.kv4_pack(v_new))
+        cached = lens
