@@ -22,7 +22,7 @@
 // Every wait is bounded (common.cuh); on expiry the CTA records a status word, skips its stores, lets its copies and MMAs drain
 // (bounded), frees tensor memory and returns; CTAs that start after a recorded failure leave at once.
 //
-// Three layouts share the kernel (template parameters LATENT, KM):
+// Four layouts share the kernel (template parameters LATENT, KM):
 //   paged   q [T, H * dk], K and V rows in the paged cache, GQA groups; the real widths dk and dv may be smaller than DK and DV (multiples
 //           of 8): tensor-map bounds fill the columns behind a cache row with zeros, and query columns that reach into the next head meet
 //           zeros. The first `keep_first` keys stay visible beside a sliding window (their key tiles are listed in front of the window's),
@@ -43,6 +43,10 @@
 //           softmax groups take its key tiles in turn, each with an accumulator, maximum and sum of its own; they meet in the epilogue. Warps 0 and 3
 //           then issue the Q K^T of one group's tiles each, from halves of the key ring: a group of eight MMAs behind a wait costs its thread about a
 //           thousand cycles, twice the MMAs themselves (one thread 337 us for 16 heads over rows of 512 columns, whatever the depth of the ring).
+//
+//   fp16    (KM = 4) the paged layout with keys and values in fp16, unpacked from a 4-bit cache (kv4.cu), whose numbers have 11 bits: in bf16 their rounding and that of the
+//           probabilities is most of the result's error (2.5 times that of rounding the result, 4 x 2048 tokens). The softmax warps turn the query rows into fp16 where the copy has put
+//           them; head widths of 64, 128, 256, no sink.
 //
 // Replaces the reference's packed prefill attention (core/.../generator/CausalSelfAttention.java:458-502: per head QK^T GEMM over
 // the visible pages, causal scaled softmax with optional soft-cap, saxpy with V).
@@ -97,6 +101,8 @@ __device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem_addr, uint3
   d |= static_cast<uint64_t>(2) << 61;
   return d;
 }
+// operand types of an instruction descriptor: bf16 (bits 7 and 10) to fp16
+__host__ __device__ constexpr uint32_t umma_idesc_f16(uint32_t bf16) { return bf16 & ~((1u << 7) | (1u << 10)); }
 // kind::f16, bf16 x bf16 -> fp32, A K-major, B MN-major
 __host__ __device__ constexpr uint32_t umma_idesc_bf16_bmn(int m, int n) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (0u << 15) | (1u << 16) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
@@ -227,7 +233,7 @@ __global__ void __launch_bounds__(AttnTcLayout<DK, DV, QT, KM>::T::kThreads, 1)
                            const AttnTcParams p) {
   using L = typename AttnTcLayout<DK, DV, QT, KM>::T;
   constexpr int NS = L::kStages, NSV = L::kStagesV, SUBK = L::kSubK, SUBV = L::kSubV;
-  constexpr bool PIECES = KM == 1 || KM == 2;
+  constexpr bool PIECES = KM == 1 || KM == 2, F16 = KM == 4;
   const int pieces = PIECES ? (p.k_subs + kAtPiece - 1) / kAtPiece : 1;  // K stages per key tile
   constexpr int kProducer = 1, kIssuer = 0, kIssuerPV = 2, kIssuer2 = 3;  // (kIssuer2: SPLIT, the second softmax group's Q K^T)
   extern __shared__ uint8_t at_raw[];
@@ -242,7 +248,7 @@ __global__ void __launch_bounds__(AttnTcLayout<DK, DV, QT, KM>::T::kThreads, 1)
   uint64_t* bar_pv_done = bar_p_full + 4;  // [2][2] the P V that read the slot's probabilities has retired
   uint64_t* bar_o_final = bar_pv_done + 4;
   uint64_t* bar_drain = bar_o_final + 1;    // [3] an issuing thread's MMAs have retired (only used when a wait ran out)
-  uint64_t* bar_ml = bar_drain + 3;         // SPLIT: maxima and sums of both softmax groups are in shared memory
+  uint64_t* bar_ml = bar_drain + 3;         // SPLIT: maxima and sums of both softmax groups are in shared memory; F16: the queries are fp16
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_ml + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -296,7 +302,7 @@ __global__ void __launch_bounds__(AttnTcLayout<DK, DV, QT, KM>::T::kThreads, 1)
     mbar_init(smem_u32(&bar_drain[1]), 1);
     mbar_init(smem_u32(&bar_drain[2]), 1);
     mbar_init(smem_u32(bar_o_final), 1);
-    mbar_init(smem_u32(bar_ml), 8);
+    mbar_init(smem_u32(bar_ml), F16 && !two ? 4 : 8);
     *abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&map_q);
@@ -438,8 +444,8 @@ __global__ void __launch_bounds__(AttnTcLayout<DK, DV, QT, KM>::T::kThreads, 1)
     // free again (the P V that read the probabilities kept there has retired) and its K tile has landed; one thread of warp 2
     // issues the P V of every item once its probabilities are written and its V tile has landed. While one of them waits, the other
     // feeds the pipe. Everything the two depend on travels through mbarriers; tcgen05.commit covers the MMAs of its own thread.
-    constexpr uint32_t idesc_s = umma_idesc_bf16(kAtBM, kAtBN);
-    constexpr uint32_t idesc_o = umma_idesc_bf16_bmn(kAtBM, DV);
+    constexpr uint32_t idesc_s = F16 ? umma_idesc_f16(umma_idesc_bf16(kAtBM, kAtBN)) : umma_idesc_bf16(kAtBM, kAtBN);
+    constexpr uint32_t idesc_o = F16 ? umma_idesc_f16(umma_idesc_bf16_bmn(kAtBM, DV)) : umma_idesc_bf16_bmn(kAtBM, DV);
     auto valid = [&](int u, int q) {
       if (SPLIT) return (u & 1) == q;
       const int j = tile_at(u);
@@ -465,7 +471,7 @@ __global__ void __launch_bounds__(AttnTcLayout<DK, DV, QT, KM>::T::kThreads, 1)
       int u = 0, q = 0;
       if (n_tiles > 0 && !valid(u, q)) advance(u, q);
       if (warp != kIssuerPV) {
-        if (KM != 2) ok = wait(bar_q, 0);
+        if (KM != 2) ok = wait(F16 ? bar_ml : bar_q, 0);
         if (warp == kIssuer2) {
           u = 1;
           q = 1;
@@ -568,8 +574,44 @@ __global__ void __launch_bounds__(AttnTcLayout<DK, DV, QT, KM>::T::kThreads, 1)
     const int my_kept = min(kept_tiles, ja), my_tiles = SPLIT ? (n_tiles - q + 1) / 2 : my_kept + jb - ja;
     const int my_pos = my_first + r;
     const float c_log2 = 1.4426950408889634f;
+    [[maybe_unused]] bool converted = true;
+    float row_scale = p.scale;
+    if constexpr (F16) {
+      // This thread's query row, as the copy has left it in shared memory, becomes fp16: divided by the power of two that brings its largest number to [1, 2), so that whatever bf16 holds fits
+      // (what is lost is below 2^-24 of that number). Its 16-byte chunks are visited in the order that the swizzle gives neighbouring rows different banks in.
+      converted = __all_sync(0xffffffffu, mbar_wait(smem_u32(bar_q), 0, abort_flag, p.status)) != 0;
+      if (converted) {
+        uint8_t* row = smem + q * L::kTileQ + r * 128;
+        auto chunk = [&](int i) { return reinterpret_cast<uint4*>(row + (i >> 3) * (kAtBM * 128) + (((i ^ r) & 7) << 4)); };
+        uint32_t top = 0;  // largest magnitude, as bits
+        for (int i = 0; i < DK / 8; ++i) {
+          const uint4 v = *chunk(i);
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = max(top, max(w[e] << 16 & 0x7FFF0000u, w[e] & 0x7FFF0000u));
+        }
+        const uint32_t e = min(max(top >> 23, 1u), 253u);
+        const float down = __uint_as_float((254u - e) << 23);
+        row_scale *= __uint_as_float(e << 23);
+        for (int i = 0; i < DK / 8; ++i) {
+          uint4 v = *chunk(i);
+          uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+          for (int e2 = 0; e2 < 4; ++e2) {
+            const float2 f = unpack_bf162(w[e2]);
+            const __half2 hf = __floats2half2_rn(f.x * down, f.y * down);
+            w[e2] = *reinterpret_cast<const uint32_t*>(&hf);
+          }
+          *chunk(i) = v;
+        }
+        fence_proxy_async_smem();
+      }
+      __syncwarp();
+      if (converted && lane == 0) mbar_arrive(smem_u32(bar_ml));
+    }
     // scores stay in the units the tensor core delivers; kf turns a difference of scores into a base-2 exponent
-    const float kf = p.softcap > 0.f ? c_log2 : p.scale * c_log2;
+    const float kf = p.softcap > 0.f ? c_log2 : row_scale * c_log2;
+    constexpr float kShift = F16 ? 7.f : 0.f;  // probabilities of fp16 are held 2^7 times as large (up to 2^15), which leaves 2^-31 of the largest as their smallest
     float m_run = -INFINITY, l_run = 0.f;
     // gate logits of this row; threads behind the last row read that row's (every branch around tensor-memory accesses stays warp-uniform)
     const int q_rows = SPLIT ? 0 : q * kAtBM;  // rows in front of this group's
@@ -578,7 +620,7 @@ __global__ void __launch_bounds__(AttnTcLayout<DK, DV, QT, KM>::T::kThreads, 1)
     const bool gate_vec = grow != nullptr && (p.dv & 7) == 0;  // (then rows, heads and the gate are 16-byte aligned)
     if (grow != nullptr)
       for (int c = 0; c < p.dv; c += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(grow + c));
-    bool ok = true;
+    bool ok = converted;
     for (int t = 0; t < my_tiles && ok; ++t) {
       const int j = SPLIT ? lo + 2 * t + q : (t < my_kept ? t : ja + t - my_kept);
       const uint32_t slot = q * 2 + (t & 1);
@@ -596,7 +638,7 @@ __global__ void __launch_bounds__(AttnTcLayout<DK, DV, QT, KM>::T::kThreads, 1)
         tmem_ld_wait();
       }
       if (p.softcap > 0.f) {
-        softcap_tile(f, p.scale / p.softcap, p.softcap);
+        softcap_tile(f, row_scale / p.softcap, p.softcap);
       }
       // is the whole tile visible to all 128 rows? (row 0 sees the fewest late keys, row 127 the fewest early ones)
       const bool full = key_base + kAtBN <= min(ctx, p.causal ? my_first + 1 : ctx) && (p.window <= 0 || key_base >= my_first + kAtBM - p.window || key_base + kAtBN <= p.keep_first) && my_rows == kAtBM;
@@ -642,8 +684,8 @@ __global__ void __launch_bounds__(AttnTcLayout<DK, DV, QT, KM>::T::kThreads, 1)
         l_run *= alpha;
       }
       m_run = m_new;
-      const float neg_mk = m_new == -INFINITY ? 0.f : -m_new * kf;
-      // probabilities -> packed bf16 over the first half of the score slot's columns (every score is in registers by now)
+      const float neg_mk = (m_new == -INFINITY ? 0.f : -m_new * kf) + kShift;
+      // probabilities -> packed bf16 (F16: fp16) over the first half of the score slot's columns (every score is in registers by now)
       float ls4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < kAtBN / 32; ++c) {
@@ -656,8 +698,14 @@ __global__ void __launch_bounds__(AttnTcLayout<DK, DV, QT, KM>::T::kThreads, 1)
           ls4[1] += p1;
           ls4[2] += p2;
           ls4[3] += p3;
-          pk[i >> 1] = pack_bf162(p0, p1);
-          pk[(i >> 1) + 1] = pack_bf162(p2, p3);
+          if constexpr (F16) {
+            const __half2 h0 = __floats2half2_rn(p0, p1), h1 = __floats2half2_rn(p2, p3);
+            pk[i >> 1] = *reinterpret_cast<const uint32_t*>(&h0);
+            pk[(i >> 1) + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+          } else {
+            pk[i >> 1] = pack_bf162(p0, p1);
+            pk[(i >> 1) + 1] = pack_bf162(p2, p3);
+          }
         }
         tmem_st_x16(sb + c * 16, pk);
       }
@@ -793,7 +841,7 @@ static int launch_prefill_tc_maps(const CUtensorMap& mq, const CUtensorMap& mk, 
   return 0;
 }
 
-template <int DK, int DV, int QT>
+template <int DK, int DV, int QT, int KM = 0>
 static int launch_prefill_tc_t(const void* q, long long q_stride, long long T, const void* kc, const void* vc, long long cache_rows, const AttnTcParams& p,
                                int num_tiles, cudaStream_t st) {
   CUtensorMap mq, mk, mv;
@@ -801,7 +849,7 @@ static int launch_prefill_tc_t(const void* q, long long q_stride, long long T, c
   const uint32_t box_rows = p.page_size < kAtBN ? p.page_size : kAtBN;
   encode_map_2d(&mk, 0, kc, static_cast<uint64_t>(cache_rows), p.dk, static_cast<uint64_t>(p.dk) * 2, box_rows, 64, 128);
   encode_map_2d(&mv, 0, vc, static_cast<uint64_t>(cache_rows), p.dv, static_cast<uint64_t>(p.dv) * 2, box_rows, 64, 128);
-  return launch_prefill_tc_maps<DK, DV, QT, false>(mq, mk, mv, mv, p, num_tiles, st);
+  return launch_prefill_tc_maps<DK, DV, QT, false, KM>(mq, mk, mv, mv, p, num_tiles, st);
 }
 
 // ---- latent layout -----------------------------------------------------------------------------------------------------
@@ -930,9 +978,10 @@ int prefill_attention_tc_tile_rows(int D) { return D <= 128 ? 256 : 128; }
 int launch_prefill_attention_tc(const void* q, long long q_stride, long long T, const void* kc, const void* vc, long long num_pages, const int* bt,
                                 int bt_stride, const int* q_start, const int* q_len, const int* ctx, const int* tile_seq, const int* tile_q0,
                                 int num_tiles, void* out, int H, int KV, int dk, int dv, int page, float scale, float cap, int window, int causal,
-                                AttnExtra x, int* status, cudaStream_t st) {
+                                AttnExtra x, int* status, cudaStream_t st, bool f16) {
   if (num_tiles == 0) return 0;
   const int D = dk > dv ? dk : dv;
+  if (f16 && (dk != dv || (D != 64 && D != 128 && D != 256) || x.sink != nullptr)) return 1;
   if ((page != 32 && page != 64 && page != 128) || dk % 8 != 0 || dv % 8 != 0 || dk <= 0 || dv <= 0 || D > 256) return 1;
   AttnTcParams p = {};
   p.block_tables = bt;
@@ -961,6 +1010,11 @@ int launch_prefill_attention_tc(const void* q, long long q_stride, long long T, 
   p.out_pitch = x.out_pitch > 0 ? x.out_pitch : static_cast<long long>(H) * dv;
   p.status = status;
   const long long cache_rows = num_pages * KV * page;
+  if (f16) {
+    if (D == 64) return launch_prefill_tc_t<64, 64, 2, 4>(q, q_stride, T, kc, vc, cache_rows, p, num_tiles, st);
+    if (D == 128) return launch_prefill_tc_t<128, 128, 2, 4>(q, q_stride, T, kc, vc, cache_rows, p, num_tiles, st);
+    return launch_prefill_tc_t<256, 256, 1, 4>(q, q_stride, T, kc, vc, cache_rows, p, num_tiles, st);
+  }
   if (D <= 64) return launch_prefill_tc_t<64, 64, 2>(q, q_stride, T, kc, vc, cache_rows, p, num_tiles, st);
   if (D <= 128 && dv <= 64) return launch_prefill_tc_t<128, 64, 2>(q, q_stride, T, kc, vc, cache_rows, p, num_tiles, st);
   if (D <= 128) return launch_prefill_tc_t<128, 128, 2>(q, q_stride, T, kc, vc, cache_rows, p, num_tiles, st);

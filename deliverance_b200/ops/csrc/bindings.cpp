@@ -1886,6 +1886,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv4_write", &kv4_write);
   m.def("kv4_expand", &kv4_expand);
   m.def("kv4_expand_seqs", &kv4_expand_seqs);
+  m.def("kv4_prefill", &kv4_prefill);
   m.def("kv4_decode", &kv4_decode);
   m.def("step_tables", &step_tables);
   m.def("q4_quantize", &q4_quantize);

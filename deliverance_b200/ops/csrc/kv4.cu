@@ -177,8 +177,8 @@ void launch_kv4_expand(const Kv4ExpandArgs& a, cudaStream_t st) {
   }
 }
 
-// The pages of a step's sequences -> bf16 pages next to one another (sequence by sequence), for prompt attention, with block tables that name them. Rows behind a
-// sequence's end are zeros there. A thread takes four units of 8 numbers, keys and values; grid (units of a page / 1024, pages of the longest sequence, S).
+// The pages of a step's sequences -> fp16 pages next to one another (sequence by sequence), for prompt attention, with block tables that name them; a page becomes page / out_page of them.
+// Rows behind a sequence's end are zeros there. fp16, because a value is the sum of two fp16 numbers: 2^-12 of it are lost, where bf16 would lose 2^-9. A thread takes four units of 8 numbers, keys and values; grid (units of a page / 1024, pages of the longest sequence, S).
 template <int D>
 __global__ void __launch_bounds__(256) kv4_expand_seqs_kernel(const Kv4SeqsArgs a) {
   pdl_trigger();
@@ -199,7 +199,8 @@ __global__ void __launch_bounds__(256) kv4_expand_seqs_kernel(const Kv4SeqsArgs 
   if (first) {
     const bool bad = given != ctx || own > a.longest || base + own > a.total || (s == a.S - 1 && base + own != a.total);
     if (bad && threadIdx.x == 0) atomicCAS(a.status, kStatusOk, kStatusBadArgs);
-    for (int c = threadIdx.x; c < a.width; c += 256) a.out_tables[static_cast<long long>(s) * a.width + c] = c < own && base + c < a.total ? base + c : 0;
+    const int cut = a.page / a.out_page;
+    for (int c = threadIdx.x; c < a.width * cut; c += 256) a.out_tables[static_cast<long long>(s) * a.width * cut + c] = c < own * cut && base + c / cut < a.total ? base * cut + c : 0;
     if (j >= own) return;
   }
   if (base + j >= a.total) return;
@@ -233,7 +234,12 @@ __global__ void __launch_bounds__(256) kv4_expand_seqs_kernel(const Kv4SeqsArgs 
     for (int kv = 0; kv < 2; ++kv) {
       float v[8];
       kv4_values(codes[i][kv], side[i][kv], v);
-      io_st8(static_cast<__nv_bfloat16*>(kv ? a.vo : a.ko) + (dst + row) * D + e0, v);
+      const int head = row / a.page, at = row % a.page, part = at / a.out_page;  // row of the page -> part, head, row of the part
+      const long long to = (dst + (part * a.KV + head) * a.out_page + at % a.out_page) * D + e0;
+      __half2 h[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) h[e] = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
+      *reinterpret_cast<uint4*>(static_cast<__half*>(kv ? a.vo : a.ko) + to) = *reinterpret_cast<const uint4*>(h);
     }
   }
 }

@@ -39,10 +39,10 @@ struct Kv4SeqsArgs {
   const uint8_t *k, *v;
   const int* tables;  // [S, width]
   const int* ctx;     // [S]
-  void *ko, *vo;      // bf16 [total, KV, page, D]
-  int* out_tables;    // [S, width]
+  void *ko, *vo;      // fp16 [total * page / out_page, KV, out_page, D]
+  int* out_tables;    // [S, width * page / out_page]
   int* status;
-  int S, width, longest, total, pages, KV, page, D;  // longest: pages of a sequence, at most
+  int S, width, longest, total, pages, KV, page, out_page, D;  // longest: pages of a sequence, at most
 };
 void launch_kv4_expand_seqs(const Kv4SeqsArgs& a, cudaStream_t st);
 

@@ -112,19 +112,19 @@ def _plain(q, k_cache, v_cache, block_tables, q_start, q_len, ctx_lens, H, scale
     return o.to(q.dtype).reshape(T, H * D)
 
 
-EXPAND_PAGES_BYTES = 512 << 20  # bf16 pages that a call of prefill_attention4 makes at one time (at least one sequence's)
+EXPAND_PAGES_BYTES = 512 << 20  # fp16 pages that a call of prefill_attention4 makes at one time (at least one sequence's)
 
 
 def prefill_attention4(q, k_cache, v_cache, block_tables, q_start, q_len, ctx_lens, H: int, scale: float, softcap: float = 0.0, window: int = 0, causal: bool = True,
                        q_len_host: Optional[list] = None, ctx_len_host: Optional[list] = None, tiles_for=None):
     """:func:`ops.prefill_attention` for 4-bit caches: packed query rows of sequences of different lengths (``q_start`` adds ``q_len`` up), which are the last rows of their ``ctx_lens`` cached ones. On
-    GPUs the pages in use are unpacked to bf16 next to one another, :data:`EXPAND_PAGES_BYTES` of them at a time, and attended to there. ``q_len_host`` / ``ctx_len_host``: the lengths on the
+    GPUs the pages in use are unpacked to fp16 next to one another, :data:`EXPAND_PAGES_BYTES` of them at a time, and attended to there. ``q_len_host`` / ``ctx_len_host``: the lengths on the
     host (else they are read back); ``tiles_for`` as there. Pages outside the caches and lengths that do not fit the table or the host's are reported by :func:`ops.check_status`."""
     T, D = q.shape[0], q.shape[1] // H
+    if H % k_cache.shape[1] or window < 0 or softcap < 0:
+        raise ValueError("KV heads must divide the query heads, window and softcap not negative")
     if not q.is_cuda:
         _check_caches(k_cache, v_cache, D)
-        if H % k_cache.shape[1] or window < 0 or softcap < 0:
-            raise ValueError("KV heads must divide the query heads, window and softcap not negative")
         return _plain(q, k_cache, v_cache, block_tables, q_start, q_len, ctx_lens, H, scale, softcap, window, causal)
     ext = ops.require_ext()
     news = q_len_host if q_len_host is not None else q_len.tolist()
@@ -132,6 +132,9 @@ def prefill_attention4(q, k_cache, v_cache, block_tables, q_start, q_len, ctx_le
     S, KV, page = len(news), k_cache.shape[1], k_cache.shape[2]
     if sum(news) != T or len(lens) != S or any(not 0 <= n <= m for n, m in zip(news, lens)):
         raise ValueError("the query rows must be those of the sequences, no more than their cached rows")
+    if q.stride(1) != 1 or q.stride(0) % 8 or q.data_ptr() % 16:
+        q = q.contiguous().clone() if q.data_ptr() % 16 else q.contiguous()
+    rows = ext.prefill_tc_tile_rows(D)
     outs, i, row = [], 0, 0
     while i < S or not outs:
         j, n_pages, n_rows = i, 0, 0
@@ -141,8 +144,12 @@ def prefill_attention4(q, k_cache, v_cache, block_tables, q_start, q_len, ctx_le
             j += 1
         part, whole = slice(i, j), j - i == S
         ctx, new, at = (ctx_lens, q_len, q_start) if whole else (ctx_lens[part], q_len[part], q_start[part] - row)
-        ops._count()
-        k, v, table = ext.kv4_expand_seqs(k_cache, v_cache, block_tables[part], ctx, n_pages, max([-(-n // page) for n in lens[part]] + [0]), D)
-        outs.append(ops.prefill_attention(q[row : row + n_rows], k, v, table, at, new, ctx, H, scale, softcap, window, causal, q_len_host=news[part], tiles_for=tiles_for if whole else None))
+        if tiles_for is not None and whole:
+            tile_seq, tile_q0 = tiles_for(rows)
+        else:
+            tile_seq, tile_q0 = (torch.tensor(t, dtype=torch.int32, device=q.device) for t in ops.prefill_tiles(news[part], rows))
+        ops._count(2)
+        k, v, table = ext.kv4_expand_seqs(k_cache, v_cache, block_tables[part], ctx, n_pages, max([-(-n // page) for n in lens[part]] + [0]), D, page if page in (32, 64, 128) else 32)
+        outs.append(ext.kv4_prefill(q[row : row + n_rows], k, v, table, at, new, ctx, tile_seq, tile_q0, H, scale, softcap, window, causal))
         i, row = j, row + n_rows
     return outs[0] if len(outs) == 1 else torch.cat(outs)

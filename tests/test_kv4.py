@@ -296,9 +296,9 @@ def run_prefill(device, D, KV, G, news, befores, softcap=0.0, window=0, page=32)
     if device == "cpu":
         want, mass, reach = plain_attention(q, k, v, table, lens, news, KV, D**-0.5, softcap, window)
         tol = want.abs() * HALF_STEP + mass * (2.0**-16 + reach * 2.0**-16)
-    else:  # keys and values in bf16, as the kernel behind reads them (unpacking is tested by itself): probabilities in bf16, numerator and denominator, the result in bf16
-        want, mass, reach = plain_attention(q, k, v, table, lens, news, KV, D**-0.5, softcap, window, lambda t: ref.kv4_unpack(t, BF16))
-        tol = want.abs() * HALF_STEP + mass * (2 * HALF_STEP + reach * 2.0**-16)
+    else:  # keys and values in fp16, as the kernel behind reads them (2^-12 of a value, tested by itself): probabilities in fp16, numerator and denominator, fp32 sums as in decoding, the result in bf16
+        want, mass, reach = plain_attention(q, k, v, table, lens, news, KV, D**-0.5, softcap, window, lambda t: ref.kv4_unpack(t, torch.float16))
+        tol = want.abs() * HALF_STEP + mass * (2.0**-10 + reach * 2.0**-16)
     assert ((got.cpu().double() - want).abs() <= tol + 1e-30).all(), ((got.cpu().double() - want).abs() / (tol + 1e-30)).max()
 
 
@@ -503,7 +503,7 @@ def test_prefill_reports(device):
 def test_operators_together(device):
     """Two prompts, one behind a cached prefix, then three decode steps: tables, write, attention, as a layer uses them; the attention against 64 bits over what the cache holds."""
     D, H, KV, page = 128, 8, 2, 32
-    tol = lambda want, mass, reach: want.abs() * HALF_STEP + mass * (2 * HALF_STEP + reach * 2.0**-16) + 1e-30  # noqa: E731
+    tol = lambda want, mass, reach: want.abs() * HALF_STEP + mass * (2.0**-10 + reach * 2.0**-16) + 1e-30  # noqa: E731
     to = lambda t: t.to(device)  # noqa: E731
     i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
     cos, sin = (to(t) for t in rotary(None, 32, 400))
@@ -522,7 +522,7 @@ def test_operators_together(device):
             got = decode_attention4(q, kc, vc, t.block_tables, t.ctx_len, H, D**-0.5)
         done(device)
         lens = [a + b for a, b in zip(cached, new)]
-        values = (lambda x: ref.kv4_unpack(x, BF16)) if device == "cuda" and T > 2 else ref.kv4_unpack
+        values = (lambda x: ref.kv4_unpack(x, torch.float16)) if device == "cuda" and T > 2 else ref.kv4_unpack
         want, mass, reach = plain_attention(q.cpu(), kc.cpu(), vc.cpu(), t.block_tables.cpu(), lens, new, KV, D**-0.5, 0.0, 0, values)
         assert ((got.cpu().double() - want).abs() <= tol(want, mass, reach)).all()
         v_new = qkv.view(T, H + 2 * KV, D)[:, H + KV :].cpu()
