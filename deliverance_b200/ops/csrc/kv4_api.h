@@ -47,17 +47,22 @@ struct Kv4SeqsArgs {
 void launch_kv4_expand_seqs(const Kv4SeqsArgs& a, cudaStream_t st);
 
 struct Kv4DecodeArgs {
-  const void* q;  // bf16 [B, H * D], rows q_stride elements apart
+  const void* q;  // bf16 [B, H * D], rows q_stride elements apart, 16-byte aligned
   long long q_stride;
   const uint8_t *k, *v;
   const int* tables;  // [B, width]
   const int* ctx;     // [B]
   void* out;          // bf16 [B, H * D]
+  int* sums;          // [B + 1] 32-key tiles of a KV head in front of every sequence (written by the first launch for the second)
+  float *part_o, *part_ml;  // partial results: 2 per warp, [G, D] and [G, 2]
   int* status;
   int B, H, KV, D, page, pages, width, window;
   float scale, softcap;
 };
-int launch_kv4_decode(const Kv4DecodeArgs& a, cudaStream_t st);
+constexpr int kKv4MaxCtas = 1024;
+int kv4_decode_ctas(int B, int KV, int G, int D, long long rows, int sms);  // CTAs for sequences of up to `rows` keys
+long long kv4_decode_room(int ctas, int G, int D);                   // floats of partial results
+void launch_kv4_decode(const Kv4DecodeArgs& a, int ctas, cudaStream_t st);  // two launches
 
 struct StepTablesArgs {
   const int *pages, *page_start, *cached, *start, *fresh;  // [n_pages], [S + 1], [S], [S], [S]
