@@ -107,7 +107,8 @@ __global__ void __launch_bounds__(kWarps * 32, Kv4Ring<D, NT>::kCtas) kv4_decode
   constexpr int OT = D == 64 ? 4 : 8;           // products per group
   extern __shared__ __align__(128) uint8_t ring_all[];
   __shared__ __align__(8) uint64_t bars[kWarps][R::kStages];
-  __shared__ int4 notes[kWarps][R::kStages];  // pair, first key of the tile, length, flags (1: the pair's first tile, 2: its last)
+  __shared__ int4 notes[kWarps][64];  // of the tiles that are copied and those to come: pair, first key of the tile, length, flags (1: the pair's first tile, 2: its last)
+  __shared__ long long places[kWarps][64];  // where their rows lie in the caches
   __shared__ int scan[kWarps], begin[kWarps][2], sum_all, abort_word;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
   volatile int* abort_flag = &abort_word;
@@ -176,43 +177,36 @@ __global__ void __launch_bounds__(kWarps * 32, Kv4Ring<D, NT>::kCtas) kv4_decode
     cur_b = begin[warp][0];
     cur_base = begin[warp][1];
   }
-  int my_pair = 0, my_key = 0, my_ctx = 0, my_flags = 0;
-  long long my_at = 0;
   auto load = [&](int j) {
     if ((j & 31) == 0) {
       const int i = lo + j + lane;
       if (j + lane < n_mine) {
-        int fk, ft, n = tiles_of(a, clamped(a, a.ctx[cur_b]), fk, ft);
+        int fk, ft, ctx = clamped(a, a.ctx[cur_b]), n = tiles_of(a, ctx, fk, ft);
         while (i >= cur_base + n * a.KV) {
           cur_base += n * a.KV;
           ++cur_b;
-          n = tiles_of(a, clamped(a, a.ctx[cur_b]), fk, ft);
+          ctx = clamped(a, a.ctx[cur_b]);
+          n = tiles_of(a, ctx, fk, ft);
         }
-        const int kvh = (i - cur_base) / n, tile = (i - cur_base) - kvh * n;
-        my_pair = cur_b * a.KV + kvh;
-        my_key = (ft + tile) * kTile;
-        my_ctx = clamped(a, a.ctx[cur_b]);
-        my_flags = (tile == 0 ? 1 : 0) | (tile == n - 1 ? 2 : 0);
-        int page = a.tables[static_cast<long long>(cur_b) * a.width + my_key / a.page];
+        const int kvh = (i - cur_base) / n, tile = (i - cur_base) - kvh * n, key = (ft + tile) * kTile, in_page = key / a.page;
+        int page = a.tables[static_cast<long long>(cur_b) * a.width + in_page];
         if (page < 0 || page >= a.pages) {
           atomicCAS(a.status, kStatusOk, kStatusBadArgs);
           page = 0;
         }
-        my_at = ((static_cast<long long>(page) * a.KV + kvh) * a.page + my_key % a.page) * R::kRow;
+        notes[warp][(j + lane) & 63] = make_int4(cur_b * a.KV + kvh, key, ctx, (tile == 0 ? 1 : 0) | (tile == n - 1 ? 2 : 0));
+        places[warp][(j + lane) & 63] = ((static_cast<long long>(page) * a.KV + kvh) * a.page + (key - in_page * a.page)) * R::kRow;
       }
       __syncwarp();
     }
-    const int stage = j % R::kStages, src = j & 31;
-    const long long at = __shfl_sync(0xffffffffu, my_at, src);
-    const int4 note = make_int4(__shfl_sync(0xffffffffu, my_pair, src), __shfl_sync(0xffffffffu, my_key, src), __shfl_sync(0xffffffffu, my_ctx, src), __shfl_sync(0xffffffffu, my_flags, src));
     if (lane == 0) {
-      notes[warp][stage] = note;
+      const int stage = j % R::kStages;
+      const long long at = places[warp][j & 63];
       const uint32_t bar = smem_u32(&bars[warp][stage]), dst = smem_u32(ring + stage * R::kStage);
       mbar_expect_tx(bar, R::kStage);
       bulk_load_1d(dst, a.k + at, R::kCopy, bar);
       bulk_load_1d(dst + R::kCopy, a.v + at, R::kCopy, bar);
     }
-    __syncwarp();
   };
   int issued = 0;
   for (; issued < R::kStages - 1 && issued < n_mine; ++issued) load(issued);
@@ -366,15 +360,26 @@ __global__ void __launch_bounds__(kWarps * 32, Kv4Ring<D, NT>::kCtas) kv4_decode
     const int stage = j % R::kStages;
     ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bars[warp][stage]), (j / R::kStages) & 1, abort_flag, a.status));
     if (!ok) break;
-    const int4 note = notes[warp][stage];
+    const int4 note = notes[warp][j & 63];
     if (note.x != pair) {
       open(note.x);
       from_start = note.w & 1;
     }
-    const uint8_t *sk = ring + stage * R::kStage, *sv = sk + R::kCopy;
+    uint8_t *sk = ring + stage * R::kStage, *sv = sk + R::kCopy;
     const int first_key = a.window > 0 && note.z > a.window ? note.z - a.window : 0;
     const int live_lo = first_key - note.y, live_hi = note.z - note.y;  // keys of the tile that count
     const bool whole = live_lo <= 0 && live_hi >= kTile;
+    if (!whole) {  // what stands in rows that do not count may be anything: steps and minima of zero make zeros of it
+      if (lane < live_lo || lane >= live_hi) {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          *reinterpret_cast<uint32_t*>(sk + lane * R::kRow + D / 2 + 4 * i) = 0u;
+          *reinterpret_cast<uint32_t*>(sv + lane * R::kRow + D / 2 + 4 * i) = 0u;
+        }
+      }
+      fence_proxy_async_smem();  // (in front of the next copy into this stage)
+      __syncwarp();
+    }
 
     // ---- scores of two times 16 keys
     float s[2][NT][4];
@@ -417,24 +422,25 @@ __global__ void __launch_bounds__(kWarps * 32, Kv4Ring<D, NT>::kCtas) kv4_decode
         mma_f16(s[mt][nt], low[0][0], low[1][0], CH == 2 ? low[0][CH - 1] : 0u, CH == 2 ? low[1][CH - 1] : 0u, q_sum[nt][0], CH == 2 ? q_sum[nt][CH - 1] : 0u);
     }
     // ---- probabilities
+#pragma unroll
+    for (int i = 0; i < 8 * NT; ++i) s[i / 4 & 1][i / 8][i & 3] *= factor[i / 8][i & 1];
+    if (a.softcap > 0.f) {
+#pragma unroll
+      for (int i = 0; i < 8 * NT; ++i) s[i / 4 & 1][i / 8][i & 3] = tanhf(s[i / 4 & 1][i / 8][i & 3]) * (a.softcap * kLog2e);
+    }
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < 8 * NT; ++i) {
+        const int key = (i / 4 & 1) * 16 + g + (i >> 1 & 1) * 8;
+        if (key < live_lo || key >= live_hi) s[i / 4 & 1][i / 8][i & 3] = -INFINITY;
+      }
+    }
     uint32_t pf[2][NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float most[2] = {-INFINITY, -INFINITY};
+      float most[2];
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float x = s[mt][nt][i] * factor[nt][i & 1];
-          if (a.softcap > 0.f) x = tanhf(x) * (a.softcap * kLog2e);
-          if (!whole) {
-            const int key = mt * 16 + g + (i >> 1) * 8;
-            x = key >= live_lo && key < live_hi ? x : -INFINITY;
-          }
-          s[mt][nt][i] = x;
-          most[i & 1] = fmaxf(most[i & 1], x);
-        }
-      }
+      for (int i = 0; i < 2; ++i) most[i] = fmaxf(fmaxf(s[0][nt][i], s[0][nt][2 + i]), fmaxf(s[1][nt][i], s[1][nt][2 + i]));
       if (__any_sync(0xffffffffu, most[0] > top[nt][0] + kSlack || most[1] > top[nt][1] + kSlack)) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -478,12 +484,7 @@ __global__ void __launch_bounds__(kWarps * 32, Kv4Ring<D, NT>::kCtas) kv4_decode
             const int word = og * 16 + hf * 8 + g;
             const uint8_t *ra = r0 + ks * 8 * R::kRow, *rb = ra + R::kRow;
             const uint32_t wa = *reinterpret_cast<const uint32_t*>(ra + word * 4), wb = *reinterpret_cast<const uint32_t*>(rb + word * 4);
-            uint32_t sa = *reinterpret_cast<const uint32_t*>(ra + D / 2 + (word >> 2) * 4), sb = *reinterpret_cast<const uint32_t*>(rb + D / 2 + (word >> 2) * 4);
-            if (!whole) {  // (what stands behind the end may be anything: step and minimum of zero make zeros of it)
-              const int key = mt * 16 + 2 * t4 + ks * 8;
-              if (key < live_lo || key >= live_hi) sa = 0u;
-              if (key + 1 < live_lo || key + 1 >= live_hi) sb = 0u;
-            }
+            const uint32_t sa = *reinterpret_cast<const uint32_t*>(ra + D / 2 + (word >> 2) * 4), sb = *reinterpret_cast<const uint32_t*>(rb + D / 2 + (word >> 2) * 4);
             const int at = ks * 2 + hf;
             lo16[at] = __byte_perm(wa, wb, 0x5410);
             hi16[at] = __byte_perm(wa, wb, 0x7632);
