@@ -54,14 +54,17 @@ struct Kv4DecodeArgs {
   const int* ctx;     // [B]
   void* out;          // bf16 [B, H * D]
   int* sums;          // [B + 1] 32-key tiles of a KV head in front of every sequence (written by the first launch for the second)
-  float *part_o, *part_ml;  // partial results: 2 per warp, [G, D] and [G, 2]
+  int* counts;        // [B * KV] partial results of every (sequence, KV head) pair, -1: finished
+  float *part_o, *part_ml;  // partial results, [G, D] and [G, 2]
+  int near;           // as many of every pair lie next to one another
   int* status;
   int B, H, KV, D, page, pages, width, window;
   float scale, softcap;
 };
 constexpr int kKv4MaxCtas = 1024;
 int kv4_decode_ctas(int B, int KV, int G, int D, long long rows, int sms);  // CTAs for sequences of up to `rows` keys
-long long kv4_decode_room(int ctas, int G, int D);                   // floats of partial results
+int kv4_decode_near(int ctas, int pairs);
+long long kv4_decode_parts(int ctas, int pairs, int near);  // partial results that have a place
 void launch_kv4_decode(const Kv4DecodeArgs& a, int ctas, cudaStream_t st);  // two launches
 
 struct StepTablesArgs {
