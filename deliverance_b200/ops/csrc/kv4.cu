@@ -2,141 +2,259 @@
 #include "kv4.cuh"
 #include "kv4_api.h"
 #include "io.cuh"
+#include "mma_pair.cuh"
 
 namespace dlv {
 
-// Head norms, rotation, queries out, keys and values quantised into their rows. A thread has 8 neighbouring numbers of a head, D / 8 threads a head, four a block; what it is rotated
-// with it reads (and norms) once more, from cache. grid (T, threads of a row / 256).
-// The cache holds codes, which change by whole steps: every operation in front of them rounds by itself (no contraction), and sums of squares are in 64 bits (exact for bf16
-// numbers within 2^18 of one another), so that the codes do not depend on who computes them.
+// Head norms, rotation, queries out, keys and values quantised into their rows. The cache holds codes, which change by whole steps: every operation in front of them rounds by itself (no contraction), and the
+// statistics are in 64 bits (sums of squares exact for bf16 numbers within 2^18 of one another), so that the codes do not depend on who computes them.
+//
+// A thread has two times 8 neighbouring numbers of one head: what is rotated together is in one thread, and four neighbouring threads have a block of either half. A CTA has all heads of a token, or a part of them, and
+// goes through further tokens with the same heads: a thread reads its norm weights once, and copies what it needs of the next two tokens ahead into shared memory, each warp the tables' rows for itself. Bound by
+// instructions (some 440 per thread and token): 8,192 rows of 32 + 2 x 8 heads of 128 62 us (177 MB: 27 at the copy rate), 121 with 8 numbers per thread, a partner's numbers read and normed again, and nothing ahead.
+template <int D>
+constexpr int kWriteHead = D / 16;  // threads of a head
+constexpr int kWriteStages = 3;
+
+// what is written of 8 numbers of a key or value
+template <int D>
+__device__ __forceinline__ void kv4_store(const Kv4WriteArgs& a, float2 (&y)[4], int e, uint32_t group, uint8_t* dst) {
+  float lo = fmin3(fmin3(y[0].x, y[0].y, y[1].x), fmin3(y[1].y, y[2].x, y[2].y), fminf(y[3].x, y[3].y));
+  float hi = fmax3_nan(fmax3_nan(y[0].x, y[0].y, y[1].x), fmax3_nan(y[1].y, y[2].x, y[2].y), fmax3_nan(y[3].x, y[3].y, y[3].y));
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {  // the threads of a block
+    const float other = __shfl_xor_sync(group, hi, o);
+    lo = fminf(lo, __shfl_xor_sync(group, lo, o));
+    hi = fmax3_nan(hi, other, other);
+  }
+  const bool nan = hi != hi;
+  if (nan || hi > kKv4Limit || lo < -kKv4Limit) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = make_float2(fminf(fmaxf(y[i].x, -kKv4Limit), kKv4Limit), fminf(fmaxf(y[i].y, -kKv4Limit), kKv4Limit));
+    lo = fminf(fmaxf(lo, -kKv4Limit), kKv4Limit);
+    hi = fminf(fmaxf(hi, -kKv4Limit), kKv4Limit);
+  }
+  const Kv4Block b(lo, hi, nan);
+  const uint32_t codes = b.codes(y);
+  if (dst == nullptr) return;
+  *reinterpret_cast<uint32_t*>(dst + e / 2) = codes;
+  if (e % 32 == 0) *reinterpret_cast<uint32_t*>(dst + D / 2 + e / 8) = b.side();
+}
+// the row of KV head 0 that a slot names (-1: none)
+__device__ __forceinline__ int kv4_row(const Kv4WriteArgs& a, long long slot) {
+  if (slot >= a.rows) atomicCAS(a.status, kStatusOk, kStatusBadArgs);
+  if (slot < 0 || slot >= a.rows) return -1;
+  const int s = static_cast<int>(slot), block = a.by_page.of(s);  // (a cache has fewer than 2^31 rows)
+  return block * a.KV * a.page + (s - block * a.page);
+}
+
 template <int D, bool PAIRS>
-__global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4WriteArgs a) {
+__global__ void __launch_bounds__(512) kv4_write_kernel(const Kv4WriteArgs a) {
+  pdl_trigger();
+  constexpr int TPH = kWriteHead<D>, STAGES = kWriteStages;
+  extern __shared__ __align__(16) uint4 pieces[];  // [STAGES][2][threads] a thread's own, then [STAGES][warps][64] the position's cosines and sines
+  const int threads = blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = threadIdx.x % TPH, h = blockIdx.y * (threads / TPH) + threadIdx.x / TPH, half = a.half;
+  const bool live = h < a.H + 2 * a.KV, norm = live && a.q_norm != nullptr && h < a.H + a.KV, is_q = h < a.H;
+  const uint32_t group = ((1u << TPH) - 1u) << (lane / TPH * TPH);  // the lanes of this head: heads of one warp may be of different kinds
+  // halves: element e with e + half, what is not rotated cut in two; pairs: neighbours, the head cut in two
+  const bool turns = !PAIRS && 8 * j < half;
+  const int ea = PAIRS || turns ? 8 * j : 8 * j + half, eb = PAIRS ? D / 2 + 8 * j : turns ? half + 8 * j : D / 2 + 8 * j;
+  const bool wide = half % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.cos_t) | reinterpret_cast<uintptr_t>(a.sin_t)) & 15) == 0;  // (whole pieces of the tables)
+  const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(a.qkv) + static_cast<long long>(live ? h : 0) * D;
+  float* tables = reinterpret_cast<float*>(pieces + STAGES * 2 * threads + warp * 64);
+  const int table_stage = threads / 32 * 256;
+  auto place = [&](int t) { return t < a.T ? a.positions[t] : 0; };  // (brought into the tables where it is used: what looks at it here would wait for it)
+  auto inside = [&](int pos) { return max(0, min(pos, a.max_pos - 1)); };
+  auto fetch = [&](int t, int pos, int stage) {
+    if (t < a.T) {
+      const __nv_bfloat16* src = row + t * a.pitch;
+      const uint32_t dst = smem_u32(pieces + stage * 2 * threads + threadIdx.x);
+      cp16(dst, src + ea, true);
+      cp16(dst + threads * 16, src + eb, true);
+      if (wide && lane * 4 < half) {
+        const long long at = static_cast<long long>(inside(pos)) * half + lane * 4;
+        const uint32_t tab = smem_u32(tables + stage * table_stage) + lane * 16;
+        cp16(tab, a.cos_t + at, true);
+        cp16(tab + 512, a.sin_t + at, true);
+      }
+    }
+    cp_commit();
+  };
+  pdl_wait();
+  const int step = gridDim.x;
+  int t = blockIdx.x, pos_here = place(t), pos_next = place(t + step), pos_after = place(t + 2 * step);
+  long long slot_next = a.slots[t];
+  fetch(t, pos_here, 0);
+  fetch(t + step, pos_next, 1);
+  float2 w[8];  // norm weights
+  if (norm) {
+    const __nv_bfloat16* weights = static_cast<const __nv_bfloat16*>(is_q ? a.q_norm : a.k_norm);
+    io_ld8(weights + ea, reinterpret_cast<float*>(w));
+    io_ld8(weights + eb, reinterpret_cast<float*>(w + 4));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = make_float2(__fadd_rn(w[i].x, a.offset), __fadd_rn(w[i].y, a.offset));
+  }
+  const int kvh = h - a.H - (h < a.H + a.KV ? 0 : a.KV);
+  uint8_t* cache = (h < a.H + a.KV ? a.k : a.v) + static_cast<long long>(kvh) * a.page * kv4_row_bytes(D);
+  for (int stage = 0; t < a.T; t += step, stage = stage + 1 == STAGES ? 0 : stage + 1) {
+    const int pos = inside(pos_here);
+    const long long slot = slot_next;
+    fetch(t + 2 * step, pos_after, stage == 0 ? STAGES - 1 : stage - 1);
+    pos_here = pos_next;
+    pos_next = pos_after;
+    pos_after = place(t + 3 * step);
+    slot_next = t + step < a.T ? a.slots[t + step] : -1;
+    cp_wait<STAGES - 1>();
+    __syncwarp();
+    if (live) {
+      float2 x[8];
+      const uint4 ra = pieces[stage * 2 * threads + threadIdx.x], rb = pieces[(stage * 2 + 1) * threads + threadIdx.x];
+      x[0] = unpack_bf162(ra.x);
+      x[1] = unpack_bf162(ra.y);
+      x[2] = unpack_bf162(ra.z);
+      x[3] = unpack_bf162(ra.w);
+      x[4] = unpack_bf162(rb.x);
+      x[5] = unpack_bf162(rb.y);
+      x[6] = unpack_bf162(rb.z);
+      x[7] = unpack_bf162(rb.w);
+      if (norm) {
+        double ss = 0.0, s2 = 0.0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          ss = fma(static_cast<double>(x[i].x), static_cast<double>(x[i].x), ss);
+          s2 = fma(static_cast<double>(x[i].y), static_cast<double>(x[i].y), s2);
+        }
+        ss += s2;
+#pragma unroll
+        for (int o = 1; o < TPH; o <<= 1) ss += __shfl_xor_sync(group, ss, o);
+        const float inv = static_cast<float>(rsqrt(ss / D + a.eps));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = mul2(mul2(x[i], make_float2(inv, inv)), w[i]);
+      }
+      if (h < a.H + a.KV && half > 0) {
+        const float* tab = tables + stage * table_stage;
+        const long long at = static_cast<long long>(pos) * half;
+        if constexpr (PAIRS) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int k = (i < 4 ? ea / 2 : eb / 2 - 4) + i;
+            if (k < half) {
+              const float c = wide ? tab[k] : a.cos_t[at + k], n = wide ? tab[128 + k] : a.sin_t[at + k];
+              x[i] = add2(mul2(x[i], make_float2(c, c)), mul2(make_float2(x[i].y, x[i].x), make_float2(-n, n)));
+            }
+          }
+        } else if (turns) {
+          float2 c[4], n[4];
+          if (wide) {
+            io_ld8(tab + 8 * j, reinterpret_cast<float*>(c));
+            io_ld8(tab + 128 + 8 * j, reinterpret_cast<float*>(n));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              c[i] = make_float2(a.cos_t[at + 8 * j + 2 * i], a.cos_t[at + 8 * j + 2 * i + 1]);
+              n[i] = make_float2(a.sin_t[at + 8 * j + 2 * i], a.sin_t[at + 8 * j + 2 * i + 1]);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 u = x[i], v = x[4 + i];
+            x[i] = sub2(mul2(u, c[i]), mul2(v, n[i]));
+            x[4 + i] = add2(mul2(v, c[i]), mul2(u, n[i]));
+          }
+        }
+      }
+      if (is_q) {
+        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.q) + (static_cast<long long>(t) * a.H + h) * D;
+        *reinterpret_cast<uint4*>(dst + ea) = make_uint4(pack_bf162(x[0].x, x[0].y), pack_bf162(x[1].x, x[1].y), pack_bf162(x[2].x, x[2].y), pack_bf162(x[3].x, x[3].y));
+        *reinterpret_cast<uint4*>(dst + eb) = make_uint4(pack_bf162(x[4].x, x[4].y), pack_bf162(x[5].x, x[5].y), pack_bf162(x[6].x, x[6].y), pack_bf162(x[7].x, x[7].y));
+      } else {
+        const int at = kv4_row(a, slot);
+        uint8_t* dst = at < 0 ? nullptr : cache + static_cast<long long>(at) * kv4_row_bytes(D);
+        kv4_store<D>(a, reinterpret_cast<float2(&)[4]>(x[0]), ea, group, dst);
+        kv4_store<D>(a, reinterpret_cast<float2(&)[4]>(x[4]), eb, group, dst);
+      }
+    }
+    __syncwarp();  // (the tables have been read)
+  }
+}
+
+// The same where halves are rotated whose blocks lie otherwise (half no multiple of 32): 8 numbers per thread, partners by shuffles. grid (T, threads of a row / 256).
+template <int D>
+__global__ void __launch_bounds__(256) kv4_write_odd_kernel(const Kv4WriteArgs a) {
   pdl_trigger();
   pdl_wait();
   constexpr int TPH = D / 8;  // threads of a head
-  const int t = blockIdx.x, unit = blockIdx.y * 256 + threadIdx.x, h = unit / TPH, e0 = unit % TPH * 8;
-  const bool live = h < a.H + 2 * a.KV;
-  const bool is_q = h < a.H, is_k = !is_q && h < a.H + a.KV;
-  const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(a.qkv) + t * a.pitch + static_cast<long long>(live ? h : 0) * D;
-  float x[8];
-  io_ld8(row + e0, x);
-  if (is_q || is_k) {
-    const __nv_bfloat16* w = static_cast<const __nv_bfloat16*>(is_q ? a.q_norm : a.k_norm);
-    float inv = 1.f;
-    if (w != nullptr) {  // (whole heads, and the same in all threads: the shuffles below are for full groups of a head)
+  const int t = blockIdx.x, lane = threadIdx.x & 31, h = (blockIdx.y * 256 + threadIdx.x) / TPH, e0 = threadIdx.x % TPH * 8, half = a.half;
+  if (h >= a.H + 2 * a.KV) return;  // (whole heads)
+  const uint32_t group = TPH == 32 ? 0xffffffffu : ((1u << (TPH & 31)) - 1u) << (lane / TPH * TPH);
+  float2 x[4];
+  io_ld8(static_cast<const __nv_bfloat16*>(a.qkv) + t * a.pitch + static_cast<long long>(h) * D + e0, reinterpret_cast<float*>(x));
+  if (h < a.H + a.KV) {
+    if (a.q_norm != nullptr) {
       double ss = 0.0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fma(static_cast<double>(x[i]), static_cast<double>(x[i]), ss);
-      const uint32_t group = TPH == 32 ? 0xffffffffu : ((1u << TPH) - 1u) << ((threadIdx.x & 31) / TPH * TPH);
+      for (int i = 0; i < 4; ++i) ss = fma(static_cast<double>(x[i].y), static_cast<double>(x[i].y), fma(static_cast<double>(x[i].x), static_cast<double>(x[i].x), ss));
 #pragma unroll
       for (int o = 1; o < TPH; o <<= 1) ss += __shfl_xor_sync(group, ss, o);
-      inv = static_cast<float>(1.0 / sqrt(ss / D + a.eps));
+      const float inv = static_cast<float>(rsqrt(ss / D + a.eps));
+      float2 w[4];
+      io_ld8(static_cast<const __nv_bfloat16*>(h < a.H ? a.q_norm : a.k_norm) + e0, reinterpret_cast<float*>(w));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = mul2(mul2(x[i], make_float2(inv, inv)), make_float2(__fadd_rn(w[i].x, a.offset), __fadd_rn(w[i].y, a.offset)));
     }
-    auto normed = [&](float v, int e) { return w == nullptr ? v : __fmul_rn(__fmul_rn(v, inv), __fadd_rn(bf2f(w[e]), a.offset)); };
-    float y[8];
+    const long long at = static_cast<long long>(max(0, min(a.positions[t], a.max_pos - 1))) * half;
+    float v[8], r[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = normed(x[i], e0 + i);
-    const int half = a.half;
-    if (e0 < 2 * half) {
-      int pos = a.positions[t];
-      pos = pos < 0 ? 0 : (pos >= a.max_pos ? a.max_pos - 1 : pos);
-      const float *cs = a.cos_t + static_cast<long long>(pos) * half, *sn = a.sin_t + static_cast<long long>(pos) * half;
-      if constexpr (PAIRS) {
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = x[i].x;
+      v[2 * i + 1] = x[i].y;
+    }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int p = e0 / 2 + i;
-          if (p < half) {
-            const float c = cs[p], n = sn[p], u = y[2 * i], v = y[2 * i + 1];
-            y[2 * i] = __fsub_rn(__fmul_rn(u, c), __fmul_rn(v, n));
-            y[2 * i + 1] = __fadd_rn(__fmul_rn(v, c), __fmul_rn(u, n));
-          }
-        }
-      } else {
-        float z[8], c[8], n[8];
-        if (half % 8 == 0) {  // the partners are 8 neighbours too
-          const int other = e0 < half ? e0 + half : e0 - half, p = e0 < half ? e0 : e0 - half;
-          io_ld8(row + other, z);
-          const bool wide = ((reinterpret_cast<uintptr_t>(cs + p) | reinterpret_cast<uintptr_t>(sn + p)) & 15) == 0;
-          if (wide) {
-            io_ld8(cs + p, c);
-            io_ld8(sn + p, n);
-          }
+    for (int i = 0; i < 8; ++i) {  // element e0 + i with e0 + i + half or - half: of one thread or of two
+      const int e = e0 + i, other = e < half ? e + half : e < 2 * half ? e - half : e;
+      float z = 0.f;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (!wide) {
-              c[i] = cs[p + i];
-              n[i] = sn[p + i];
-            }
-            z[i] = normed(z[i], other + i);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int e = e0 + i, other = e < half ? e + half : e - half, p = e < half ? e : e - half;
-            const bool in = e < 2 * half;
-            z[i] = in ? normed(bf2f(row[other]), other) : 0.f;
-            c[i] = in ? cs[p] : 1.f;
-            n[i] = in ? sn[p] : 0.f;
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float m = __fmul_rn(z[i], n[i]);
-          if (e0 + i < half) y[i] = __fsub_rn(__fmul_rn(y[i], c[i]), m);
-          else if (e0 + i < 2 * half) y[i] = __fadd_rn(__fmul_rn(y[i], c[i]), m);
-        }
+      for (int k = 0; k < 8; ++k) {
+        const float theirs = __shfl_sync(group, v[k], lane / TPH * TPH + other / 8);
+        z = other % 8 == k ? theirs : z;
       }
+      const int k = e < half ? e : e - half;
+      r[i] = v[i];
+      if (e < 2 * half) r[i] = __fadd_rn(__fmul_rn(v[i], a.cos_t[at + k]), __fmul_rn(z, e < half ? -a.sin_t[at + k] : a.sin_t[at + k]));
     }
-    if (is_q) {
-      io_st8(static_cast<__nv_bfloat16*>(a.q) + (static_cast<long long>(t) * a.H + h) * D + e0, y);
-      return;
-    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = y[i];
+    for (int i = 0; i < 4; ++i) x[i] = make_float2(r[2 * i], r[2 * i + 1]);
   }
-  if (!live) return;
-  float lo = INFINITY, hi = -INFINITY;
-  bool nan = false;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    nan = nan || x[i] != x[i];
-    x[i] = fminf(fmaxf(x[i], -kKv4Limit), kKv4Limit);
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-  }
-  const uint32_t four = 0xfu << (threadIdx.x & 28);  // the threads of a block
-#pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(four, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(four, hi, o));
-    nan = __shfl_xor_sync(four, static_cast<int>(nan), o) || nan;
-  }
-  const Kv4Block b(lo, hi, nan);
-  uint32_t codes = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) codes |= b.code(x[i]) << (4 * i);
-  const long long slot = a.slots[t];
-  if (slot < 0) return;
-  if (slot >= a.rows) {
-    if (unit % TPH == 0) atomicCAS(a.status, kStatusOk, kStatusBadArgs);
+  if (h < a.H) {
+    *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.q) + (static_cast<long long>(t) * a.H + h) * D + e0) =
+        make_uint4(pack_bf162(x[0].x, x[0].y), pack_bf162(x[1].x, x[1].y), pack_bf162(x[2].x, x[2].y), pack_bf162(x[3].x, x[3].y));
     return;
   }
-  const int kvh = is_k ? h - a.H : h - a.H - a.KV;
-  const bool narrow = slot <= 0xffffffffll;
-  const long long page = narrow ? static_cast<unsigned>(slot) / static_cast<unsigned>(a.page) : slot / a.page;
-  uint8_t* dst = (is_k ? a.k : a.v) + ((page * a.KV + kvh) * a.page + (slot - page * a.page)) * kv4_row_bytes(D);
-  *reinterpret_cast<uint32_t*>(dst + e0 / 2) = codes;
-  if (e0 % 32 == 0) *reinterpret_cast<uint32_t*>(dst + D / 2 + e0 / 8) = b.side();
+  const int at = kv4_row(a, a.slots[t]), kvh = h - a.H - (h < a.H + a.KV ? 0 : a.KV);
+  kv4_store<D>(a, x, e0, group, at < 0 ? nullptr : (h < a.H + a.KV ? a.k : a.v) + static_cast<long long>(at + kvh * a.page) * kv4_row_bytes(D));
 }
 
+template <int D, bool PAIRS>
+static void launch_write_t(const Kv4WriteArgs& a, cudaStream_t st) {
+  constexpr int TPH = kWriteHead<D>, most = 512;
+  static PerDeviceOnce once;
+  if (once.first()) cudaFuncSetAttribute(kv4_write_kernel<D, PAIRS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWriteStages * (2 * most + most * 2) * 16);
+  // a token's heads in one CTA where there are tokens for all SMs, otherwise in parts of 128 threads
+  const int heads = a.H + 2 * a.KV, want = heads * TPH < (a.T < 148 ? 128 : most) ? heads * TPH : (a.T < 148 ? 128 : most), threads = (want + 31) / 32 * 32, y = (heads * TPH + threads - 1) / threads;
+  const int smem = kWriteStages * (2 * threads + threads * 2) * 16, per_sm = 1024 / threads < 8 ? (1024 / threads < 1 ? 1 : 1024 / threads) : 8, room = 148 * per_sm / y < 1 ? 1 : 148 * per_sm / y;
+  launch_pdl(kv4_write_kernel<D, PAIRS>, dim3(a.T < room ? a.T : room, y), dim3(threads), smem, st, a);
+}
+template <int D>
+static void launch_write_d(const Kv4WriteArgs& a, cudaStream_t st) {
+  if (a.pairs) launch_write_t<D, true>(a, st);
+  else if (a.half % 32 == 0) launch_write_t<D, false>(a, st);
+  else launch_pdl(kv4_write_odd_kernel<D>, dim3(a.T, ((a.H + 2 * a.KV) * (D / 8) + 255) / 256), dim3(256), 0, st, a);
+}
 void launch_kv4_write(const Kv4WriteArgs& a, cudaStream_t st) {
   if (a.T == 0) return;
-  const dim3 grid(static_cast<unsigned>(a.T), static_cast<unsigned>(((a.H + 2 * a.KV) * (a.D / 8) + 255) / 256));
-#define DLV_KV4_WRITE(DD) (a.pairs ? launch_pdl(kv4_write_kernel<DD, true>, grid, dim3(256), 0, st, a) : launch_pdl(kv4_write_kernel<DD, false>, grid, dim3(256), 0, st, a))
-  if (a.D == 64) DLV_KV4_WRITE(64);
-  else if (a.D == 128) DLV_KV4_WRITE(128);
-  else DLV_KV4_WRITE(256);
-#undef DLV_KV4_WRITE
+  if (a.D == 64) launch_write_d<64>(a, st);
+  else if (a.D == 128) launch_write_d<128>(a, st);
+  else launch_write_d<256>(a, st);
 }
 
 // Pages -> bf16 or fp32 pages: what prompt attention reads, and what shows a cache's contents. 8 numbers per thread; grid (8-number units of a page / 256, n, keys | values).

@@ -11,6 +11,21 @@ namespace dlv {
 
 constexpr float kKv4Limit = 472.f;
 
+// two products or sums, each rounded by itself (mul.rn.f32x2 followed by add.rn.f32x2 comes back from the assembler with one rounding)
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return make_float2(__fmul_rn(a.x, b.x), __fmul_rn(a.y, b.y)); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)); }
+__device__ __forceinline__ float2 sub2(float2 a, float2 b) { return make_float2(__fsub_rn(a.x, b.x), __fsub_rn(a.y, b.y)); }
+__device__ __forceinline__ float fmin3(float a, float b, float c) {
+  float y;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {  // NaN if one of them is
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
 // step and minimum of a block whose (clamped) numbers lie in [lo, hi], and the reciprocal of the step; every operation rounds by itself
 struct Kv4Block {
   __half s, m;
@@ -29,9 +44,17 @@ struct Kv4Block {
       mf = inv = 0.f;
     }
   }
-  __device__ __forceinline__ uint32_t code(float x) const {
-    const float c = rintf(__fmul_rn(__fsub_rn(x, mf), inv));
-    return static_cast<uint32_t>(fminf(fmaxf(c, 0.f), 15.f));  // (a NaN: 0)
+  // Eight codes. The sum with 1.5 2^23 rounds halves to even, as rint does, and leaves the integer in its last bits: the products with 16^i put the codes side by side, above a constant. No code is above
+  // 15: the step is no less than a fifteenth of the range.
+  __device__ __forceinline__ uint32_t codes(const float2* x) const {
+    uint32_t r = 0u - 0x4B400000u * 0x11111111u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float2 c = mul2(add2(x[i], make_float2(-mf, -mf)), make_float2(inv, inv));
+      c = add2(make_float2(fmaxf(c.x, 0.f), fmaxf(c.y, 0.f)), make_float2(12582912.f, 12582912.f));
+      r += __float_as_uint(c.x) * (1u << (8 * i)) + __float_as_uint(c.y) * (16u << (8 * i));
+    }
+    return r;
   }
   __device__ __forceinline__ uint32_t side() const { return static_cast<uint32_t>(__half_as_ushort(s)) | static_cast<uint32_t>(__half_as_ushort(m)) << 16; }
 };

@@ -3,6 +3,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "divisor.h"
+
 namespace dlv {
 
 constexpr int kv4_row_bytes(int D) { return D / 2 + D / 8; }
@@ -18,6 +20,7 @@ struct Kv4WriteArgs {
   uint8_t *k, *v;               // [pages, KV, page, row bytes]
   int* status;
   long long rows;  // pages * page
+  Divisor by_page;
   int T, H, KV, D, page, half, max_pos;
   bool pairs;
   double eps;

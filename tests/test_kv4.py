@@ -155,6 +155,23 @@ def test_write_of_extremes_has_the_plain_bytes(device):
     assert torch.equal(kc.cpu(), k) and torch.equal(vc.cpu(), v)
 
 
+@pytest.mark.parametrize("device", GPU)
+@pytest.mark.parametrize("D,rotate,half", [(64, "halves", 32), (128, "halves", 64), (128, "halves", 32), (256, "pairs", 128), (128, "pairs", 21), (256, "halves", 24)])
+def test_write_of_many_rows_has_the_plain_bytes(device, D, rotate, half):
+    """Any operation that is contracted with another one shows in some thousand rows."""
+    T, H, KV = 3000, 4, 2
+    x, cos, sin = torch.randn(T, (H + 2 * KV) * D).to(BF16), *rotary(None, half, 5000)
+    qn, kn = torch.randn(D).to(BF16), torch.randn(D).to(BF16)
+    k, v = (torch.zeros(T // 32 + 1, KV, 32, row_bytes(D), dtype=torch.uint8) for _ in range(2))
+    kc, vc = k.to(device), v.to(device)
+    slots, positions = torch.randperm(T), torch.randint(0, 5000, (T,), dtype=torch.int32)
+    q = ref.rope_kv4(x, positions, slots, qn, kn, cos, sin, k, v, H, KV, D, 1e-6, 0.0, rotate == "pairs")
+    to = lambda t: t.to(device)  # noqa: E731
+    got = rope_kv4(to(x), to(positions), to(slots), to(qn), to(kn), to(cos), to(sin), kc, vc, H, KV, D, 1e-6, 0.0, rotate)
+    done(device)
+    assert torch.equal(kc.cpu(), k) and torch.equal(vc.cpu(), v) and torch.equal(got.cpu(), q)
+
+
 def random_cache(pages, KV, page, D, loud=True):
     x = torch.randn(pages, KV, page, D)
     if loud:
