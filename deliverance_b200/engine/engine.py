@@ -123,6 +123,11 @@ class Engine:
                 raise ValueError("a bounded cache needs 0 <= keep_recent <= keep_tokens, keep_every >= 1 and keep_capacity > keep_tokens (or 0)")
             if not getattr(model, "supports_key_weights", lambda: False)():
                 raise ValueError("this model's cache cannot be bounded: it needs attention over all cached rows in every layer")
+        if kvs.bits != 16:
+            if self.bounded:
+                raise ValueError("a bounded cache holds its rows in 16 bits")
+            if not getattr(model, "supports_kv4", lambda: False)():
+                raise ValueError("this model's cache cannot be held in 4 bits: it needs plain attention with heads of 64, 128 or 256, at most 16 query heads per KV head")
         pages = self.config.num_pages or self._auto_pages(layout)
         tp = getattr(model, "tp", None)
         if self.config.num_pages is None and tp is not None and tp.enabled and tp.collectives is not None:
@@ -172,7 +177,7 @@ class Engine:
         return score_room(next((b for b in _BUCKETS if b >= n), n), self.model.n_heads, rows, self._weight_capacity())
 
     def _auto_pages(self, layout) -> int:
-        per = max(1, PagedKVCache.bytes_per_page(layout, self.config.kv.block_size, self.model.dtype))
+        per = max(1, PagedKVCache.bytes_per_page(layout, self.config.kv.block_size, self.model.dtype, self.config.kv.bits))
         if self.device.type == "cuda":
             free, _ = torch.cuda.mem_get_info(self.device)
             free -= (1 + self._state_slots(layout)) * PagedKVCache.bytes_per_state_slot(layout)

@@ -62,8 +62,9 @@ def _unpack(f: SafeTensorFile) -> dict:
 
 
 class DiskPrefixStore:
-    def __init__(self, directory: str, compression: str = "LZ4", bits: int = 4, max_bytes: int = 8 << 30, max_age_s: float = 0.0):
+    def __init__(self, directory: str, compression: str = "LZ4", bits: int = 4, max_bytes: int = 8 << 30, max_age_s: float = 0.0, rows: str = "values"):
         self.dir = directory
+        self.suffix = ".kv4" if rows == "bytes" else ".kv"  # (an engine finds only what fits its cache; the limits hold for both)
         self.compression = compression
         self.bits = bits
         self.max_bytes = max_bytes
@@ -72,7 +73,7 @@ class DiskPrefixStore:
         self.metrics = {"disk_writes": 0, "disk_hits": 0, "disk_misses": 0, "disk_evict": 0, "disk_bytes": 0}
 
     def _path(self, key: bytes) -> str:
-        return os.path.join(self.dir, key.hex() + ".kv")
+        return os.path.join(self.dir, key.hex() + self.suffix)
 
     def has(self, key: bytes) -> bool:
         return os.path.exists(self._path(key))
@@ -116,7 +117,7 @@ class DiskPrefixStore:
             p = os.path.join(self.dir, f)
             try:
                 age = now - os.path.getmtime(p)
-                if (f.endswith(".kv") and self.max_age_s > 0 and age > self.max_age_s) or (f.endswith(".tmp") and age > 600):
+                if (f.endswith((".kv", ".kv4")) and self.max_age_s > 0 and age > self.max_age_s) or (f.endswith(".tmp") and age > 600):
                     os.remove(p)
                     removed += 1
             except OSError:
@@ -127,7 +128,7 @@ class DiskPrefixStore:
     def _trim(self) -> None:
         self.sweep()
         files = [(os.path.getmtime(os.path.join(self.dir, f)), os.path.getsize(os.path.join(self.dir, f)), os.path.join(self.dir, f))
-                 for f in os.listdir(self.dir) if f.endswith(".kv")]
+                 for f in os.listdir(self.dir) if f.endswith((".kv", ".kv4"))]
         total = sum(s for _, s, _ in files)
         for _, size, path in sorted(files):
             if total <= self.max_bytes:

@@ -12,7 +12,7 @@ What differs by design: the reference copies a full KV snapshot per checkpoint; 
 whose reference counts are bumped, so a hit costs no copy and no extra memory, and the 512-token cap
 (``max_prefix_tokens``) is a setting, not a limit of the data structure.
 
-Layout per attention layer: ``k[pages, KV, page_size, D]`` and ``v[...]`` in the working dtype; page 0 is a scratch page
+Layout per attention layer: ``k[pages, KV, page_size, D]`` and ``v[...]`` in the working dtype, or with ``KvCacheSettings.bits`` 4 rows of bytes (``ops.kv4``); page 0 is a scratch page
 that padded batch rows write to. Latent-attention layers use the same pair with one "head": ``k`` holds the compressed vectors, ``v``
 the rotated key parts shared by all heads (a width of its own, ``v_dim_per_layer``). Recurrent layers (Mamba2, gated linear
 attention) have no pages: a sequence holds one state slot, an index into the fp32 tensors named by the layout's ``state_shapes`` (one
@@ -29,6 +29,8 @@ from typing import Optional
 
 import torch
 
+from ..ops.kv4 import row_bytes
+
 PAGE_SIZE = 32
 
 
@@ -44,6 +46,7 @@ class KvCacheSettings:
     anchors: tuple = (32, 64, 128)
     enabled: bool = True
     compression: str = "NONE"  # NONE | LZ4 | DEFLATE | MSE_TURBOQUANT (host snapshots only, see kv.turboquant)
+    bits: int = 16  # per cached number on the device: 16 (the model's working type) or 4 (ops.kv4)
     # Bounded cache: a decoding sequence that holds more than keep_tokens rows is shortened to that many every keep_every steps, to its newest keep_recent rows
     # and those of the others that had the most attention since (ops.evict). 0: off. Rows at or behind keep_capacity (0: the model's context) are not weighed;
     # a sequence that reaches it is shortened at once.
@@ -242,6 +245,8 @@ class PagedKVCache:
         self.page_size = self.settings.block_size
         if self.page_size % 32:
             raise ValueError("page size must be a multiple of 32")
+        self.bits = self.settings.bits
+        self._check_bits(layout, self.bits)
         self.device = torch.device(device)
         self.dtype = dtype
         self.num_pages = num_pages
@@ -265,6 +270,10 @@ class PagedKVCache:
                 self.v.append(self.v[shared[i]])
             else:
                 shape = (num_pages, heads[i], self.page_size)
+                if self.bits == 4:
+                    self.k.append(torch.zeros(shape + (row_bytes(dims[i]),), dtype=torch.uint8, device=self.device))
+                    self.v.append(torch.zeros(shape + (row_bytes(v_dims[i]),), dtype=torch.uint8, device=self.device))
+                    continue
                 self.k.append(torch.zeros(shape + (dims[i],), dtype=dtype, device=self.device))
                 self.v.append(torch.zeros(shape + (v_dims[i],), dtype=dtype, device=self.device))
         self.allocator = PageAllocator(num_pages)
@@ -300,13 +309,23 @@ class PagedKVCache:
         return sum(4 * math.prod(shape) for shapes in layout.get("state_shapes") or [] if shapes for shape in shapes.values())
 
     @staticmethod
-    def bytes_per_page(layout: dict, page_size: int, dtype) -> int:
+    def _check_bits(layout: dict, bits: int) -> None:
+        if bits not in (16, 4):
+            raise ValueError("cached numbers have 16 or 4 bits")
+        if bits == 4 and (layout.get("v_dim_per_layer") or layout.get("shared_from") or layout.get("head_dim_per_layer") or layout["head_dim"] not in (64, 128, 256)):
+            raise ValueError("a cache in 4 bits needs keys and values of 64, 128 or 256 numbers per head, the same in all layers")
+
+    @staticmethod
+    def bytes_per_page(layout: dict, page_size: int, dtype, bits: int = 16) -> int:
         kinds = layout["layer_kinds"]
         heads = layout.get("kv_heads_per_layer") or [layout["kv_heads"]] * len(kinds)
         dims = layout.get("head_dim_per_layer") or [layout["head_dim"]] * len(kinds)
         shared = layout.get("shared_from") or [-1] * len(kinds)
         v_dims = layout.get("v_dim_per_layer") or dims
         paged = PagedKVCache.paged_layers(layout)
+        if bits == 4:
+            PagedKVCache._check_bits(layout, bits)
+            return sum(heads[i] * 2 * row_bytes(dims[i]) for i in range(len(kinds)) if paged[i]) * page_size
         rows = sum(heads[i] * (dims[i] + v_dims[i]) for i in range(len(kinds)) if paged[i] and shared[i] < 0)
         return rows * page_size * torch.empty((), dtype=dtype).element_size()
 
@@ -404,11 +423,13 @@ class PagedKVCache:
         """Spill evicted prefixes to ``directory`` and pull them back on later hits (attention-only models)."""
         from .disk import DiskPrefixStore
 
-        self.prefix.disk = DiskPrefixStore(directory, compression, bits, max_bytes, max_age_s)
+        if self.bits == 4 and compression == "MSE_TURBOQUANT":
+            raise ValueError("rows of a 4-bit cache are stored as they are (NONE, LZ4, DEFLATE), not quantised again")
+        self.prefix.disk = DiskPrefixStore(directory, compression, bits, max_bytes, max_age_s, rows="bytes" if self.bits == 4 else "values")
         return self.prefix.disk
 
     def gather_rows(self, layer: int, pages: list[int], n_tokens: int):
-        """Dense ``[KV, n_tokens, D]`` copies of K and V (tests, snapshots, debugging)."""
+        """Dense ``[KV, n_tokens, D]`` copies of K and V (tests, snapshots, debugging); rows of a 4-bit cache as they are stored."""
         idx = torch.tensor(pages[: (n_tokens + self.page_size - 1) // self.page_size], device=self.device, dtype=torch.long)
         kh, hd = self.k[layer].shape[1], self.k[layer].shape[3]
         k = self.k[layer][idx].permute(1, 0, 2, 3).reshape(kh, -1, hd)[:, :n_tokens]

@@ -26,6 +26,7 @@ from ..ckpt.safetensors_io import Q4Tensor
 from ..config import ModelConfig
 from ..ops import LinearWeight, ref
 from ..ops.evict import decode_attention_weighted
+from ..ops.kv4 import decode_attention4, prefill_attention4, rope_kv4
 from ..parallel.context import SINGLE, TensorParallelContext, TensorParallelPlanner
 from .batch import ForwardBatch
 
@@ -358,16 +359,17 @@ class DecoderModel:
         ``rmsnorm(residual)``; otherwise ``y`` is the block output as without the argument."""
         cfg = self.cfg
         k_cache, v_cache = kv.layer(i)
+        in4 = getattr(kv, "bits", 16) == 4
         local_rope = lw.kind == "sliding" and self.cos_local is not None
         cos, sin = (self.cos_local, self.sin_local) if local_rope else (self.cos, self.sin)
-        inside = (self.rope_in_attention and batch.is_decode and batch.key_slots is None and self._sp is None and ops.rope_in_attention(x.device, x.shape[0], self.n_heads, self.n_kv, cfg.head_dim) and
+        inside = (not in4 and self.rope_in_attention and batch.is_decode and batch.key_slots is None and self._sp is None and ops.rope_in_attention(x.device, x.shape[0], self.n_heads, self.n_kv, cfg.head_dim) and
                   batch.rows_apart())  # (else every new key is in the cache before any row reads it)
         if inside:  # norm + rotary + cache write in the attention kernel
             with self._stage("causalselfattention.qkv_projection"):
                 q = self._col_parallel(x, lw.qkv)
                 if lw.lora:
                     q = self._lora(lw, "qkv", x, q)
-        elif self.fused_rope and "qkv" not in lw.lora and self._sp is None:
+        elif not in4 and self.fused_rope and "qkv" not in lw.lora and self._sp is None:
             # norm + rotary + cache write in the projection's epilogue (one launch instead of two, q is written once); a
             # sequence-parallel forward gathers its input inside the projection and keeps the two-kernel form
             with self._stage("causalselfattention.qkv_projection"):
@@ -379,14 +381,19 @@ class DecoderModel:
                 if lw.lora:
                     qkv = self._lora(lw, "qkv", x, qkv)
             with self._stage("causalselfattention.rope"):
-                q = ops.rope_kv(qkv, batch.positions, batch.slots, lw.q_norm, lw.k_norm, cos, sin, k_cache, v_cache,
-                                self.n_heads, self.n_kv, cfg.head_dim, cfg.norm_eps, cfg.norm_weight_offset)
+                q = (rope_kv4 if in4 else ops.rope_kv)(qkv, batch.positions, batch.slots, lw.q_norm, lw.k_norm, cos, sin, k_cache, v_cache,
+                                                       self.n_heads, self.n_kv, cfg.head_dim, cfg.norm_eps, cfg.norm_weight_offset)
         window = cfg.window(i)
         with self._stage("causalselfattention.score_value"):
             if inside:
                 a = ops.decode_attention_rope(q, batch.positions, batch.slots, lw.q_norm, lw.k_norm, cos, sin, k_cache, v_cache, batch.block_tables, batch.ctx_len,
                                               self.n_heads, cfg.scale, cfg.attn_softcap, window, batch.decode_splits, cfg.norm_eps, cfg.norm_weight_offset,
                                               batch.decode_even, lambda *a: batch.decode_plan(i, *a))
+            elif in4 and batch.is_decode:
+                a = decode_attention4(q, k_cache, v_cache, batch.block_tables, batch.ctx_len, self.n_heads, cfg.scale, cfg.attn_softcap, window)
+            elif in4:
+                a = prefill_attention4(q, k_cache, v_cache, batch.block_tables, batch.q_start, batch.q_len, batch.ctx_len, self.n_heads, cfg.scale, cfg.attn_softcap, window, True,
+                                       batch.q_len_host, batch.ctx_len_host, batch.tiles)
             elif batch.is_decode and batch.key_slots is not None:  # bounded cache
                 a = decode_attention_weighted(q, k_cache, v_cache, batch.block_tables, batch.ctx_len, self.n_heads, cfg.scale, kv.key_weights[i], batch.key_slots,
                                               cfg.attn_softcap, 0, batch.decode_splits, batch.decode_even, lambda *a: batch.decode_plan(i, *a), kv.key_scores)
@@ -622,6 +629,10 @@ class DecoderModel:
         cfg = self.cfg
         return (type(self) is DecoderModel and all(cfg.layer_type(i) != "mamba" and not cfg.window(i) for i in range(cfg.num_layers)) and
                 self.n_heads // self.n_kv <= 16)
+
+    def supports_kv4(self) -> bool:
+        """Whether the cache of this model can be held in 4 bits (``KvCacheSettings.bits``)."""
+        return type(self) is DecoderModel and self.cfg.head_dim in (64, 128, 256) and self.n_heads // self.n_kv <= 16
 
     def weight_bytes(self) -> int:
         n = self.embed.numel() * self.embed.element_size()

@@ -13,6 +13,7 @@ tp_local/coordinator.properties; both ``model-name`` and ``modelName`` spellings
     deliverance-model.configs[i].tensor-parallel.enabled | size
     deliverance.kv.prefix.max-tokens | checkpoint-policy | max-checkpoints | compression | turboquant.bits | enabled | max-entries
     deliverance.kv.context-rows-per-page-target | deliverance.kv.disk-dir
+    deliverance.kv.bits                                   16 | 4: bits per cached number on the device (extension)
     deliverance.openai.reasoning-field                    openai | vllm
     deliverance.basic.auth.user | deliverance.basic.auth.password | deliverance.jwt.secret
 
@@ -116,7 +117,7 @@ class ServerConfig:
 _KV_KEYS = {"deliverance.kv.prefix.max-tokens": ("max_prefix_tokens", int), "deliverance.kv.prefix.checkpoint-policy": ("policy", str.upper),
             "deliverance.kv.prefix.max-checkpoints": ("checkpoints", int), "deliverance.kv.prefix.compression": ("compression", str.upper),
             "deliverance.kv.prefix.enabled": ("enabled", lambda v: v.lower() == "true"), "deliverance.kv.prefix.max-entries": ("max_entries", int),
-            "deliverance.kv.keep-tokens": ("keep_tokens", int), "deliverance.kv.keep-recent": ("keep_recent", int),
+            "deliverance.kv.bits": ("bits", int), "deliverance.kv.keep-tokens": ("keep_tokens", int), "deliverance.kv.keep-recent": ("keep_recent", int),
             "deliverance.kv.keep-every": ("keep_every", int), "deliverance.kv.keep-capacity": ("keep_capacity", int),
             "deliverance.kv.prefix.block-size": ("block_size", int), "deliverance.kv.context-rows-per-page-target": ("block_size", int)}
 
