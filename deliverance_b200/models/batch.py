@@ -92,7 +92,8 @@ def make_batch(seqs: list[dict], page_size: int, device, max_pages: Optional[int
     """
     from ..ops import even_lengths, prefill_tiles
 
-    if torch.device(device).type == "cuda" and 0 < len(seqs) <= 8192:
+    # (4 prompts of 2,048 tokens: 493 us, on the host 732; single tokens, whose tables the host keeps too (``rows_apart``), go better there: 64 of them 600 us, by the kernel 819)
+    if torch.device(device).type == "cuda" and len(seqs) <= 8192 and any(len(s["tokens"]) != 1 for s in seqs):
         return _make_batch_there(seqs, page_size, torch.device(device), max_pages)
     toks, pos, slots, qs, ql, cl = [], [], [], [], [], []  # toks / pos / slots: one tensor per sequence
     width = max_pages or max(1, max(len(s["pages"]) for s in seqs))
@@ -169,8 +170,7 @@ def make_batch(seqs: list[dict], page_size: int, device, max_pages: Optional[int
 
 
 def _make_batch_there(seqs: list[dict], page_size: int, dev: torch.device, max_pages: Optional[int]) -> ForwardBatch:
-    """:func:`make_batch` for a GPU: lengths and page lists go there in one copy, a kernel makes positions, slots, block tables and query tiles of them (``ops.tables``)."""
-    from ..ops import even_lengths
+    """:func:`make_batch` of prompts for a GPU: lengths and page lists go there in one copy, a kernel makes positions, slots, block tables and query tiles of them (``ops.tables``)."""
     from ..ops.tables import step_tables
 
     width = max_pages or max(1, max(len(s["pages"]) for s in seqs))
@@ -188,12 +188,11 @@ def _make_batch_there(seqs: list[dict], page_size: int, dev: torch.device, max_p
         pages.extend(s["pages"])
         first.append(len(pages))
     S, T = len(seqs), sum(ql)
-    is_decode = all(n == 1 for n in ql)
     t = lambda v, dt: torch.tensor(v, dtype=dt).pin_memory().to(dev, non_blocking=True)  # noqa: E731
     ints = t(pages + first + rows + start + ql, torch.int32)
     P = len(pages)
     q_len = ints[P + 3 * S + 1 :]
-    tiles = 0 if is_decode else sum((n + 63) // 64 for n in ql)
+    tiles = sum((n + 63) // 64 for n in ql)
     made = step_tables(ints[:P], ints[P : P + S + 1], ints[P + S + 1 : P + 2 * S + 1], ints[P + 2 * S + 1 : P + 3 * S + 1], q_len, T, width, page_size, 64, tiles)
     # (copies behind the kernel: nothing of the step starts before it has written the tables)
     flat: list = []
@@ -207,15 +206,8 @@ def _make_batch_there(seqs: list[dict], page_size: int, dev: torch.device, max_p
             prev.append(int(s.get("prev", -1)))
             prev.extend(int(x) for x in s["tokens"][:-1])
         prev_ids = t(prev, torch.int32)
-    tables = None
-    if is_decode:
-        host = torch.zeros(S, width, dtype=torch.int32)
-        for i, s in enumerate(seqs):
-            host[i, : len(s["pages"])] = torch.tensor(s["pages"], dtype=torch.int32)
-        tables = (host, page_size)
     cl = [a + b for a, b in zip(rows, ql)]
     return ForwardBatch(
-        token_ids=token_ids, positions=made.positions, slots=made.slots, q_start=made.q_start, q_len=q_len, ctx_len=made.ctx_len, block_tables=made.block_tables, is_decode=is_decode,
+        token_ids=token_ids, positions=made.positions, slots=made.slots, q_start=made.q_start, q_len=q_len, ctx_len=made.ctx_len, block_tables=made.block_tables, is_decode=False,
         logits_rows=made.logits_rows, tile_seq=made.tile_seq if tiles else None, tile_q0=made.tile_q0 if tiles else None,
-        state_slots=t([int(s.get("state_slot", 0)) for s in seqs], torch.int64) if any("state_slot" in s for s in seqs) else None, q_len_host=ql, ctx_len_host=cl, prev_ids=prev_ids,
-        decode_even=is_decode and even_lengths(cl), host_tables=tables, key_slots=t([int(s.get("key_slot", 0)) for s in seqs], torch.int64) if is_decode and any("key_slot" in s for s in seqs) else None)
+        state_slots=t([int(s.get("state_slot", 0)) for s in seqs], torch.int64) if any("state_slot" in s for s in seqs) else None, q_len_host=ql, ctx_len_host=cl, prev_ids=prev_ids)

@@ -1,6 +1,7 @@
 // torch <-> kernel-launcher glue. Every entry validates device, dtype, contiguity and alignment on the host before a
 // launch (no kernel is started on arguments that could fault), and launches on the current CUDA stream.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
