@@ -118,11 +118,11 @@ EXPAND_PAGES_BYTES = 512 << 20  # fp16 pages that a call of prefill_attention4 m
 def prefill_attention4(q, k_cache, v_cache, block_tables, q_start, q_len, ctx_lens, H: int, scale: float, softcap: float = 0.0, window: int = 0, causal: bool = True,
                        q_len_host: Optional[list] = None, ctx_len_host: Optional[list] = None, tiles_for=None):
     """:func:`ops.prefill_attention` for 4-bit caches: packed query rows of sequences of different lengths (``q_start`` adds ``q_len`` up), which are the last rows of their ``ctx_lens`` cached ones. On
-    GPUs the pages in use are unpacked to fp16 next to one another, :data:`EXPAND_PAGES_BYTES` of them at a time, and attended to there. ``q_len_host`` / ``ctx_len_host``: the lengths on the
-    host (else they are read back); ``tiles_for`` as there. Pages outside the caches and lengths that do not fit the table or the host's are reported by :func:`ops.check_status`."""
+    GPUs the pages in use are unpacked to fp16 next to one another, :data:`EXPAND_PAGES_BYTES` of them at a time, and attended to there. ``q_len_host`` / ``ctx_len_host``: the same lengths on the
+    host (else they are read back); ``tiles_for`` as there. Pages outside the caches, and cached lengths that are not the host's, are reported by :func:`ops.check_status`."""
     T, D = q.shape[0], q.shape[1] // H
-    if H % k_cache.shape[1] or window < 0 or softcap < 0:
-        raise ValueError("KV heads must divide the query heads, window and softcap not negative")
+    if H % k_cache.shape[1] or window < 0 or softcap < 0 or not scale > 0:
+        raise ValueError("KV heads must divide the query heads, scale must be positive, window and softcap not negative")
     if not q.is_cuda:
         _check_caches(k_cache, v_cache, D)
         return _plain(q, k_cache, v_cache, block_tables, q_start, q_len, ctx_lens, H, scale, softcap, window, causal)
@@ -130,8 +130,8 @@ def prefill_attention4(q, k_cache, v_cache, block_tables, q_start, q_len, ctx_le
     news = q_len_host if q_len_host is not None else q_len.tolist()
     lens = ctx_len_host if ctx_len_host is not None else ctx_lens.tolist()
     S, KV, page = len(news), k_cache.shape[1], k_cache.shape[2]
-    if sum(news) != T or len(lens) != S or any(not 0 <= n <= m for n, m in zip(news, lens)):
-        raise ValueError("the query rows must be those of the sequences, no more than their cached rows")
+    if sum(news) != T or len(lens) != S or any(not 0 <= n <= m for n, m in zip(news, lens)) or max(lens, default=0) > block_tables.shape[1] * page:
+        raise ValueError("the query rows must be those of the sequences, no more than their cached rows, and these no more than the block table has")
     if q.stride(1) != 1 or q.stride(0) % 8 or q.data_ptr() % 16:
         q = q.contiguous().clone() if q.data_ptr() % 16 else q.contiguous()
     rows = ext.prefill_tc_tile_rows(D)

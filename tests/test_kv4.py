@@ -297,6 +297,83 @@ def test_decode_sharp_and_large(device):
     run_decode(device, 64, 1, 8, [200], mult=0.0)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("scale", [-0.2, 0.0])
+def test_decode_scale_of_any_sign(device, scale):
+    D, KV, G, lens = 128, 2, 3, [40, 1, 200]
+    table, pages = tables_for(lens, 32)
+    q, k, v = torch.randn(3, KV * G * D).to(BF16), random_cache(pages, KV, 32, D), random_cache(pages, KV, 32, D, False)
+    to = lambda t: t.to(device)  # noqa: E731
+    got = decode_attention4(to(q), to(k), to(v), to(table), to(torch.tensor(lens, dtype=torch.int32)), KV * G, scale)
+    done(device)
+    want, mass, reach = plain_attention(q, k, v, table, lens, [1] * 3, KV, scale, 0.0, 0)
+    assert ((got.cpu().double() - want).abs() <= want.abs() * HALF_STEP + mass * (2.0**-10 + reach.abs() * 2.0**-15) + 1e-30).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_decode_nan_stays_where_it_is(device):
+    """A NaN in a query is its head's, one in a cached value its block's of the sequences that see it, and a misaligned or strided query is taken as it is."""
+    D, KV, G, lens = 128, 2, 2, [100, 70, 33]
+    table, pages = tables_for(lens, 32)
+    wide = torch.randn(3, KV * G * D + 3).to(BF16)
+    q = wide[:, 1 : 1 + KV * G * D]
+    wide[1, 1 + D + 5] = math.nan  # head 1 of sequence 1
+    k, x = random_cache(pages, KV, 32, D), torch.randn(pages, KV, 32, D)
+    x[table[2, 0].long(), 1, 7, 40] = math.nan  # KV head 1 of sequence 2, block 1
+    v = ref.kv4_pack(x)
+    to = lambda t: t.to(device)  # noqa: E731
+    got = decode_attention4(to(wide)[:, 1 : 1 + KV * G * D], to(k), to(v), to(table), to(torch.tensor(lens, dtype=torch.int32)), KV * G, D**-0.5).cpu().view(3, KV * G, 4, 32)
+    done(device)
+    bad = torch.zeros(3, KV * G, 4, 32, dtype=torch.bool)
+    bad[1, 1] = True
+    bad[2, 2:, 1] = True
+    assert torch.equal(torch.isnan(got), bad)
+    want, mass, reach = plain_attention(torch.nan_to_num(q), k, ref.kv4_pack(torch.nan_to_num(x)), table, lens, [1] * 3, KV, D**-0.5, 0.0, 0)
+    err, tol = (got.double().flatten(1) - want).abs(), want.abs() * HALF_STEP + mass * (2.0**-10 + reach * 2.0**-15) + 1e-30
+    assert (err <= tol)[~bad.flatten(1)].all()
+
+
+@pytest.mark.parametrize("device", GPU)
+def test_captured_calls_on_a_stream(device):
+    """Writing, decode attention and tables in a captured graph, replayed with other lengths, pages and rows, beside calls on another stream."""
+    D, H, KV, B, width = 128, 8, 2, 5, 12
+    to = lambda t: t.to(device)  # noqa: E731
+    cos, sin = (to(t) for t in rotary(None, 64, 400))
+    kc, vc = (to(random_cache(B * width + 1, KV, 32, D, loud)) for loud in (True, False))
+    qkv = torch.zeros(B, (H + 2 * KV) * D, dtype=BF16, device=device)
+    pos, ctx = (torch.zeros(B, dtype=torch.int32, device=device) for _ in range(2))
+    slots, table = torch.zeros(B, dtype=torch.int64, device=device), torch.zeros(B, width, dtype=torch.int32, device=device)
+
+    def step(cache_k, cache_v):
+        q = rope_kv4(qkv, pos, slots, None, None, cos, sin, cache_k, cache_v, H, KV, D, 1e-6)
+        return q, decode_attention4(q, cache_k, cache_v, table, ctx, H, D**-0.5)
+
+    slots.copy_(torch.arange(B))
+    ctx.fill_(1)
+    step(kc.clone(), vc.clone())
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        q, out = step(kc, vc)
+    side = torch.cuda.Stream()
+    for lens in ([1, 1, 1, 1, 1], [300, 2, 33, 64, 384], [7, 384, 384, 1, 90]):
+        pages = (torch.randperm(B * width) + 1).view(B, width).to(torch.int32)
+        new = torch.tensor(lens) - 1
+        qkv.copy_(torch.randn(qkv.shape))
+        pos.copy_(new)
+        ctx.copy_(torch.tensor(lens))
+        table.copy_(pages)
+        slots.copy_(pages.gather(1, (new // 32).view(-1, 1)).view(-1).long() * 32 + new % 32)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            apart = [step(kc.clone(), vc.clone())[1] for _ in range(3)]
+        graph.replay()
+        torch.cuda.synchronize()
+        done(device)
+        assert all(torch.equal(a, out) for a in apart)
+        check_decode(out, q.cpu(), kc.cpu(), vc.cpu(), pages, lens, KV, D**-0.5, 0.0, 0)
+
+
 def run_prefill(device, D, KV, G, news, befores, softcap=0.0, window=0, page=32):
     lens = [a + b for a, b in zip(news, befores)]
     H, T = KV * G, sum(news)
@@ -330,6 +407,22 @@ def test_prefill_matches_plain(device, D, KV, G, news, befores):
 @pytest.mark.parametrize("softcap,window,page", [(30.0, 0, 32), (0.0, 40, 64), (50.0, 7, 32), (0.0, 0, 96)])
 def test_prefill_options(device, softcap, window, page):
     run_prefill(device, 64, 2, 2, [70, 40], [100, 0], softcap, window, page)
+
+
+@pytest.mark.parametrize("device", GPU)
+def test_prefill_ends_of_the_range(device):
+    """Queries at both ends of bf16's range are as good as ordinary ones: their rows are scaled in front of fp16."""
+    D, H, KV = 128, 4, 2
+    table, pages = tables_for([90], 32)
+    k, v = random_cache(pages, KV, 32, D), random_cache(pages, KV, 32, D, False)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    q = torch.randn(50, H * D)
+    for size, scale in ((1.0, 0.09), (1e30, 9e-32), (1e-30, 9e28)):
+        x = (q * size).to(BF16)
+        got = prefill_attention4(x.to(device), k.to(device), v.to(device), table.to(device), i32([0]), i32([50]), i32([90]), H, scale)
+        done(device)
+        want, mass, reach = plain_attention(x, k, v, table, [90], [50], KV, scale, 0.0, 0, lambda t: ref.kv4_unpack(t, torch.float16))
+        assert ((got.cpu().double() - want).abs() <= want.abs() * HALF_STEP + mass * (2.0**-10 + reach * 2.0**-16) + 1e-30).all()
 
 
 @pytest.mark.parametrize("device", GPU)
@@ -511,7 +604,11 @@ def test_prefill_reports(device):
     run([[1, 7], [3, 0]], [3, 1], [40, 5])
     with pytest.raises(RuntimeError, match="bad kernel arguments"):
         ops.check_status()
-    run([[1, 2], [3, 0]], [3, 1], [70, 5])
+    with pytest.raises(ValueError):
+        run([[1, 2], [3, 0]], [3, 1], [70, 5])
+    with pytest.raises(ValueError):
+        prefill_attention4(q, *rest, i32([[1, 2], [3, 0]]), i32([0, 3]), i32([3, 1]), i32([40, 5]), 4, -0.1)
+    run([[1, 2], [3, 0]], [3, 1], [40, 5], ctx_len_host=[30, 5])  # (one page where the device's lengths have two)
     with pytest.raises(RuntimeError, match="bad kernel arguments"):
         ops.check_status()
 
