@@ -37,7 +37,7 @@ struct Kv4Block {
     float sf = __int_as_float((__float_as_int(s0) + 0x1FFFF) & ~0x1FFFF);
     if (s0 < 0x1p-14f) sf = ceilf(s0 * 0x1p20f) * 0x1p-20f;
     s = __float2half_rn(sf);
-    inv = sf > 0.f ? __fdiv_rn(1.f, sf) : 0.f;
+    inv = sf > 0.f ? __frcp_rn(sf) : 0.f;
     if (nan) {
       s = __ushort_as_half(0);
       m = __ushort_as_half(0x7E00);
