@@ -257,23 +257,43 @@ void launch_kv4_write(const Kv4WriteArgs& a, cudaStream_t st) {
   else launch_write_d<256>(a, st);
 }
 
-// Pages -> bf16 or fp32 pages: what prompt attention reads, and what shows a cache's contents. 8 numbers per thread; grid (8-number units of a page / 256, n, keys | values).
+// Pages -> bf16 or fp32 pages: what shows a cache's contents. A thread takes four units of 8 numbers, keys and values; grid (units of a page / 1024, n).
 template <int D, typename TO>
 __global__ void __launch_bounds__(256) kv4_expand_kernel(const Kv4ExpandArgs a) {
   pdl_trigger();
   pdl_wait();
   constexpr int TPR = D / 8, RB = kv4_row_bytes(D);
-  const int unit = blockIdx.x * 256 + threadIdx.x, row = unit / TPR, e0 = unit % TPR * 8, rows = a.KV * a.page;
-  if (row >= rows) return;
+  const int rows = a.KV * a.page, u0 = blockIdx.x * 1024 + threadIdx.x;
   int page = a.list[blockIdx.y];
   if (page < 0 || page >= a.pages) {
-    if (unit == 0) atomicCAS(a.status, kStatusOk, kStatusBadArgs);
+    if (u0 == 0) atomicCAS(a.status, kStatusOk, kStatusBadArgs);
     page = 0;
   }
-  const uint8_t* src = (blockIdx.z ? a.v : a.k) + (static_cast<long long>(page) * rows + row) * RB;
-  float v[8];
-  kv4_values(*reinterpret_cast<const uint32_t*>(src + e0 / 2), *reinterpret_cast<const uint32_t*>(src + D / 2 + e0 / 32 * 4), v);
-  io_st8(static_cast<TO*>(blockIdx.z ? a.vo : a.ko) + (static_cast<long long>(blockIdx.y) * rows + row) * D + e0, v);
+  uint32_t codes[4][2], side[4][2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int u = u0 + 256 * i, row = u / TPR, e0 = u % TPR * 8;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      codes[i][kv] = side[i][kv] = 0;
+      if (row < rows) {
+        const uint8_t* p = (kv ? a.v : a.k) + (static_cast<long long>(page) * rows + row) * RB;
+        codes[i][kv] = *reinterpret_cast<const uint32_t*>(p + e0 / 2);
+        side[i][kv] = *reinterpret_cast<const uint32_t*>(p + D / 2 + e0 / 32 * 4);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int u = u0 + 256 * i, row = u / TPR, e0 = u % TPR * 8;
+    if (row >= rows) break;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      float v[8];
+      kv4_values(codes[i][kv], side[i][kv], v);
+      io_st8(static_cast<TO*>(kv ? a.vo : a.ko) + (static_cast<long long>(blockIdx.y) * rows + row) * D + e0, v);
+    }
+  }
 }
 
 void launch_kv4_expand(const Kv4ExpandArgs& a, cudaStream_t st) {
@@ -285,7 +305,7 @@ void launch_kv4_expand(const Kv4ExpandArgs& a, cudaStream_t st) {
     const long long skip = static_cast<long long>(at) * a.KV * a.page * a.D * (a.f32 ? 4 : 2);
     b.ko = static_cast<uint8_t*>(a.ko) + skip;
     b.vo = static_cast<uint8_t*>(a.vo) + skip;
-    const dim3 grid(static_cast<unsigned>((static_cast<long long>(a.KV) * a.page * (a.D / 8) + 255) / 256), static_cast<unsigned>(b.n), 2);
+    const dim3 grid(static_cast<unsigned>((static_cast<long long>(a.KV) * a.page * (a.D / 8) + 1023) / 1024), static_cast<unsigned>(b.n));
 #define DLV_KV4_EXPAND(DD) \
   (a.f32 ? launch_pdl(kv4_expand_kernel<DD, float>, grid, dim3(256), 0, st, b) : launch_pdl(kv4_expand_kernel<DD, __nv_bfloat16>, grid, dim3(256), 0, st, b))
     if (a.D == 64) DLV_KV4_EXPAND(64);

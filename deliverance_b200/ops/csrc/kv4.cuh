@@ -59,11 +59,17 @@ struct Kv4Block {
   __device__ __forceinline__ uint32_t side() const { return static_cast<uint32_t>(__half_as_ushort(s)) | static_cast<uint32_t>(__half_as_ushort(m)) << 16; }
 };
 
-// eight neighbouring codes and their block's step and minimum -> values
+// eight neighbouring codes and their block's step and minimum -> values: a masked pair of codes under the exponent of 1024 is 1024 + c or 1024 + 16 c, fp16 takes that off exactly, and one fp32 FMA rounds
 __device__ __forceinline__ void kv4_values(uint32_t codes, uint32_t side, float* v) {
   const float s = __half2float(__ushort_as_half(static_cast<unsigned short>(side))), m = __half2float(__ushort_as_half(static_cast<unsigned short>(side >> 16)));
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = fmaf(static_cast<float>((codes >> (4 * i)) & 15u), s, m);
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = (i < 2 ? codes : codes >> 8) & (i % 2 ? 0x00F000F0u : 0x000F000Fu) | 0x64006400u;
+    const __half2 x = *reinterpret_cast<const __half2*>(&w);
+    const float2 c = __half22float2(i % 2 ? __hfma2(x, __floats2half2_rn(0.0625f, 0.0625f), __floats2half2_rn(-64.f, -64.f)) : __hadd2(x, __floats2half2_rn(-1024.f, -1024.f)));
+    v[i] = fmaf(c.x, s, m);
+    v[i + 4] = fmaf(c.y, s, m);
+  }
 }
 
 }  // namespace dlv

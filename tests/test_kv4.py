@@ -645,6 +645,24 @@ def test_operators_together(device):
         cached = lens
 
 
+@pytest.mark.parametrize("device", GPU)
+def test_outputs_stay_inside_their_guard_areas(device):
+    ops.set_bounds_check(True)
+    try:
+        for D, KV, G, lens in ((64, 2, 5, [700, 31, 32, 0]), (128, 1, 16, [64] * 40), (256, 2, 1, [5000])):
+            run_decode(device, D, KV, G, lens)
+        run_prefill(device, 64, 2, 3, [33, 5], [0, 70])
+        run_prefill(device, 128, 1, 2, [5], [3], page=96)
+        test_expand_matches_plain(device, 128, 1, 96)
+        test_step_tables(device, [5, 0, 0, 129, 0], 64, 32)
+        test_write_matches_plain(device, 128, 6, 2, 37, "halves", 64, True)
+        test_write_matches_plain(device, 64, 4, 1, 9, "halves", 5, True)
+        torch.cuda.synchronize()
+        ops.check_guards()
+    finally:
+        ops.set_bounds_check(False)
+
+
 # ---------------------------------------------------------------------------------------------------------------- engine
 HEADS = dict(hidden_size=256, num_attention_heads=4, num_key_value_heads=2, head_dim=64)
 
