@@ -978,7 +978,7 @@ int prefill_attention_tc_tile_rows(int D) { return D <= 128 ? 256 : 128; }
 int launch_prefill_attention_tc(const void* q, long long q_stride, long long T, const void* kc, const void* vc, long long num_pages, const int* bt,
                                 int bt_stride, const int* q_start, const int* q_len, const int* ctx, const int* tile_seq, const int* tile_q0,
                                 int num_tiles, void* out, int H, int KV, int dk, int dv, int page, float scale, float cap, int window, int causal,
-                                AttnExtra x, int* status, cudaStream_t st, bool f16) {
+                                AttnExtra x, int* status, cudaStream_t st, bool f16, int rows) {
   if (num_tiles == 0) return 0;
   const int D = dk > dv ? dk : dv;
   if (f16 && (dk != dv || (D != 64 && D != 128 && D != 256) || x.sink != nullptr)) return 1;
@@ -1011,6 +1011,9 @@ int launch_prefill_attention_tc(const void* q, long long q_stride, long long T, 
   p.status = status;
   const long long cache_rows = num_pages * KV * page;
   if (f16) {
+    if (D == 64 && rows == kAtBM) return launch_prefill_tc_t<64, 64, 1, 4>(q, q_stride, T, kc, vc, cache_rows, p, num_tiles, st);
+    if (D == 128 && rows == kAtBM) return launch_prefill_tc_t<128, 128, 1, 4>(q, q_stride, T, kc, vc, cache_rows, p, num_tiles, st);
+    if (rows != prefill_attention_tc_tile_rows(D)) return 1;
     if (D == 64) return launch_prefill_tc_t<64, 64, 2, 4>(q, q_stride, T, kc, vc, cache_rows, p, num_tiles, st);
     if (D == 128) return launch_prefill_tc_t<128, 128, 2, 4>(q, q_stride, T, kc, vc, cache_rows, p, num_tiles, st);
     return launch_prefill_tc_t<256, 256, 1, 4>(q, q_stride, T, kc, vc, cache_rows, p, num_tiles, st);

@@ -1886,7 +1886,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("beam_move", &beam_move, py::arg("tensors"), py::arg("slots"), py::arg("parents"), py::arg("rows") = py::none(), py::arg("paged") = false);
   m.def("kv4_write", &kv4_write);
   m.def("kv4_expand", &kv4_expand);
-  m.def("kv4_expand_seqs", &kv4_expand_seqs);
   m.def("kv4_prefill", &kv4_prefill);
   m.def("kv4_decode", &kv4_decode);
   m.def("step_tables", &step_tables);

@@ -38,7 +38,7 @@ enum : int { kFirst = 1, kLast = 2, kOpen = 4, kClose = 8, kPartial = 16 };  // 
 template <int D, int NT>
 struct Kv4Ring {
   static constexpr int kRow = kv4_row_bytes(D), kCopy = kTile * kRow, kStage = 2 * kCopy;
-  static constexpr int kStages = D == 64 ? 4 : 2;
+  static constexpr int kStages = 2;
   static constexpr int kCtas = (D == 64 ? 4 : D == 128 ? 3 : 2) - (NT - 1);  // per SM, as registers allow
   static constexpr int kBytes = kWarps * kStages * kStage;
 };

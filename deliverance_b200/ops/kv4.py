@@ -135,21 +135,29 @@ def prefill_attention4(q, k_cache, v_cache, block_tables, q_start, q_len, ctx_le
     if q.stride(1) != 1 or q.stride(0) % 8 or q.data_ptr() % 16:
         q = q.contiguous().clone() if q.data_ptr() % 16 else q.contiguous()
     rows = ext.prefill_tc_tile_rows(D)
-    outs, i, row = [], 0, 0
-    while i < S or not outs:
-        j, n_pages, n_rows = i, 0, 0
-        while j < S and (j == i or (n_pages + -(-lens[j] // page)) * KV * page * D * 4 <= EXPAND_PAGES_BYTES):
-            n_pages += -(-lens[j] // page)
-            n_rows += news[j]
-            j += 1
-        part, whole = slice(i, j), j - i == S
-        ctx, new, at = (ctx_lens, q_len, q_start) if whole else (ctx_lens[part], q_len[part], q_start[part] - row)
-        if tiles_for is not None and whole:
-            tile_seq, tile_q0 = tiles_for(rows)
-        else:
-            tile_seq, tile_q0 = (torch.tensor(t, dtype=torch.int32, device=q.device) for t in ops.prefill_tiles(news[part], rows))
+    # A CTA takes a tile of query rows of one head. Tiles of half the height where all of them run at one time on the 148 SMs: the softmax of a key tile has half the rows to wait for (heads of 128, us:
+    # 700 rows of 16 heads 23.2 for 26.4, 2,048 of 8 heads 45.3 for 53.4, 200 rows behind 9,000 of 32 heads 193 for 221). Beyond that the second wave costs more (1,024 rows of 32 heads 45.7 for 35.7).
+    if sum(-(-n // 128) for n in news) * H <= 148:
+        rows = 128
+    pages = [-(-n // page) for n in lens]
+    if sum(pages) * KV * page * D * 4 <= EXPAND_PAGES_BYTES or S == 1:
+        tile_seq, tile_q0 = tiles_for(rows) if tiles_for is not None else _tiles(news, rows, q.device)
         ops._count(2)
-        k, v, table = ext.kv4_expand_seqs(k_cache, v_cache, block_tables[part], ctx, n_pages, max([-(-n // page) for n in lens[part]] + [0]), D, page if page in (32, 64, 128) else 32)
-        outs.append(ext.kv4_prefill(q[row : row + n_rows], k, v, table, at, new, ctx, tile_seq, tile_q0, H, scale, softcap, window, causal))
-        i, row = j, row + n_rows
-    return outs[0] if len(outs) == 1 else torch.cat(outs)
+        return ext.kv4_prefill(q, k_cache, v_cache, block_tables, q_start, q_len, ctx_lens, tile_seq, tile_q0, H, scale, softcap, window, causal, sum(pages), max(pages, default=0), rows)
+    outs, i, row = [], 0, 0
+    while i < S:
+        j, n_pages = i, 0
+        while j < S and (j == i or (n_pages + pages[j]) * KV * page * D * 4 <= EXPAND_PAGES_BYTES):
+            n_pages += pages[j]
+            j += 1
+        part, n = slice(i, j), sum(news[i:j])
+        tile_seq, tile_q0 = _tiles(news[part], rows, q.device)
+        ops._count(2)
+        outs.append(ext.kv4_prefill(q[row : row + n], k_cache, v_cache, block_tables[part], q_start[part] - row, q_len[part], ctx_lens[part], tile_seq, tile_q0, H, scale, softcap, window, causal,
+                                    n_pages, max(pages[part]), rows))
+        i, row = j, row + n
+    return torch.cat(outs)
+
+
+def _tiles(news, rows: int, device):
+    return tuple(torch.tensor(t, dtype=torch.int32, device=device) for t in ops.prefill_tiles(news, rows))

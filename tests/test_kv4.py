@@ -410,6 +410,33 @@ def test_prefill_options(device, softcap, window, page):
 
 
 @pytest.mark.parametrize("device", GPU)
+@pytest.mark.parametrize("D,KV,G,news,befores", [(64, 4, 8, [600, 1, 129], [0, 64, 300]), (128, 8, 4, [257, 500], [40, 0]), (128, 8, 4, [128] * 4 + [1], [0] * 5), (128, 8, 4, [128] * 4, [0] * 4)])
+def test_prefill_tile_heights(device, D, KV, G, news, befores):
+    """Calls on both sides of the rule on query tiles; a sequence has the same bits whichever height its call takes."""
+    run_prefill(device, D, KV, G, news, befores)
+    lens, H = [a + b for a, b in zip(news, befores)], KV * G
+    table, pages = tables_for(lens, 32)
+    k, v = (random_cache(pages, KV, 32, D, False).to(device) for _ in range(2))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    q, start = torch.randn(sum(news), H * D, device=device).to(BF16), [sum(news[:i]) for i in range(len(news))]
+    whole = prefill_attention4(q, k, v, table.to(device), i32(start), i32(news), i32(lens), H, D**-0.5)
+    for b, (at, n) in enumerate(zip(start, news)):
+        alone = prefill_attention4(q[at : at + n], k, v, table[b : b + 1].to(device), i32([0]), i32([n]), i32([lens[b]]), H, D**-0.5)
+        assert torch.equal(alone, whole[at : at + n])
+    done(device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_prefill_of_nothing(device):
+    k = random_cache(2, 2, 32, 64).to(device)
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device=device)  # noqa: E731
+    q = torch.zeros(0, 256, dtype=BF16, device=device)
+    assert prefill_attention4(q, k, k, i32(0, 1), i32(0), i32(0), i32(0), 4, 0.1).shape == (0, 256)
+    assert prefill_attention4(q, k, k, i32(2, 1), i32(2), i32(2), i32(2), 4, 0.1).shape == (0, 256)
+    done(device)
+
+
+@pytest.mark.parametrize("device", GPU)
 def test_prefill_ends_of_the_range(device):
     """Queries at both ends of bf16's range are as good as ordinary ones: their rows are scaled in front of fp16."""
     D, H, KV = 128, 4, 2
