@@ -46,7 +46,8 @@
 //
 //   fp16    (KM = 4) the paged layout with keys and values in fp16, unpacked from a 4-bit cache (kv4.cu), whose numbers have 11 bits: in bf16 their rounding and that of the
 //           probabilities is most of the result's error (2.5 times that of rounding the result, 4 x 2048 tokens). The softmax warps turn the query rows into fp16 where the copy has put
-//           them; head widths of 64, 128, 256, no sink.
+//           them; head widths of 64, 128, 256, no sink. Where few query tiles see many keys (a new turn behind a long cache) a tile's keys are cut into gridDim.z equal parts, a CTA each:
+//           a key tile takes a CTA some 1.25 us however few the CTAs are. The parts' accumulators and sums are joined by prefill_parts_kernel.
 //
 // Replaces the reference's packed prefill attention (core/.../generator/CausalSelfAttention.java:458-502: per head QK^T GEMM over
 // the visible pages, causal scaled softmax with optional soft-cap, saxpy with V).
@@ -87,6 +88,9 @@ struct AttnTcParams {
   int gate_heads;
   float out_mult;
   int k_subs;                  // wide layout: 64-column blocks of a key row
+  float* part_o;               // fp16 layout, a query tile's keys in gridDim.z > 1 parts: accumulators [parts, T, H, dv] ...
+  float2* part_note;           // ... and (base-2 exponent that they are relative to, sum) [parts, T, H]
+  long long rows;              // T
 };
 
 // MN-major shared-memory descriptor (128-byte swizzle): the operand tile is stored as rows of the K dimension, each row 64 elements of
@@ -279,6 +283,12 @@ __global__ void __launch_bounds__(AttnTcLayout<DK, DV, QT, KM>::T::kThreads, 1)
     a_q[q] = key_lo / kAtBN;
     b_q[q] = rows_q[q] > 0 ? (key_hi + kAtBN - 1) / kAtBN : a_q[q];
   }
+  constexpr bool PARTED = F16 && QT == 1;
+  if (PARTED && p.part_o != nullptr) {  // this CTA's share of the tile's keys, perhaps nothing
+    const int share = (b_q[0] - a_q[0] + static_cast<int>(gridDim.z) - 1) / static_cast<int>(gridDim.z), end = b_q[0];
+    a_q[0] = min(end, a_q[0] + static_cast<int>(blockIdx.z) * share);
+    b_q[0] = min(end, a_q[0] + share);
+  }
   const int a0 = a_q[0], b0 = b_q[0], a1 = a_q[1], b1 = two ? b_q[1] : a_q[1];
   // key tiles this CTA loads, in this order: those that hold kept first tokens in front of the window, then [lo, hi)
   const int kept_tiles = (min(p.keep_first, ctx) + kAtBN - 1) / kAtBN;
@@ -286,6 +296,12 @@ __global__ void __launch_bounds__(AttnTcLayout<DK, DV, QT, KM>::T::kThreads, 1)
   const int n_kept = min(kept_tiles, lo);
   const int n_tiles = n_kept + hi - lo;
   auto tile_at = [&](int u) { return u < n_kept ? u : lo + u - n_kept; };
+  if (PARTED && p.part_o != nullptr && n_tiles == 0) {
+    pdl_wait();
+    const int r = static_cast<int>(threadIdx.x);
+    if (r < rows_q[0]) p.part_note[(static_cast<size_t>(blockIdx.z) * p.rows + qs + q0 + r) * p.H + h] = make_float2(-INFINITY, 0.f);
+    return;
+  }
 
   if (threadIdx.x == 0) {
     mbar_init(smem_u32(bar_q), 1);
@@ -613,6 +629,7 @@ __global__ void __launch_bounds__(AttnTcLayout<DK, DV, QT, KM>::T::kThreads, 1)
     const float kf = p.softcap > 0.f ? c_log2 : row_scale * c_log2;
     constexpr float kShift = F16 ? 7.f : 0.f;  // probabilities of fp16 are held 2^7 times as large (up to 2^15), which leaves 2^-31 of the largest as their smallest
     float m_run = -INFINITY, l_run = 0.f;
+    [[maybe_unused]] float m_exp = 0.f;  // PARTED: the exponent that probabilities are relative to, as they were computed with it
     // gate logits of this row; threads behind the last row read that row's (every branch around tensor-memory accesses stays warp-uniform)
     const int q_rows = SPLIT ? 0 : q * kAtBM;  // rows in front of this group's
     const size_t gate_row = static_cast<size_t>(qs + q0 + q_rows + max(0, min(r, my_rows - 1)));
@@ -685,6 +702,7 @@ __global__ void __launch_bounds__(AttnTcLayout<DK, DV, QT, KM>::T::kThreads, 1)
       }
       m_run = m_new;
       const float neg_mk = (m_new == -INFINITY ? 0.f : -m_new * kf) + kShift;
+      if constexpr (PARTED) m_exp = -neg_mk;
       // probabilities -> packed bf16 (F16: fp16) over the first half of the score slot's columns (every score is in registers by now)
       float ls4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -728,7 +746,21 @@ __global__ void __launch_bounds__(AttnTcLayout<DK, DV, QT, KM>::T::kThreads, 1)
         ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(bar_ml), 0, abort_flag, p.status));
       }
     }
-    if (ok) {
+    if (PARTED && ok && p.part_o != nullptr) {  // as it stands, for prefill_parts_kernel
+      tc_fence_after();
+      const size_t at = (static_cast<size_t>(blockIdx.z) * p.rows + qs + q0 + r) * p.H + h;
+      if (r < my_rows) p.part_note[at] = make_float2(l_run == 0.f ? -INFINITY : (l_run == l_run ? m_exp : l_run), l_run);
+#pragma unroll 1
+      for (int c0 = 0; my_tiles > 0 && c0 < DV; c0 += 32) {
+        __syncwarp();
+        uint32_t v[32];
+        tmem_ld_x32(lane_addr + kColO + c0, v);
+        tmem_ld_wait();
+        if (r < my_rows)
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(p.part_o + at * DV + c0 + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+      }
+    } else if (ok) {
       tc_fence_after();
       float w_mine = 1.f, w_other = 0.f;  // SPLIT: weights of this group's and the other one's accumulator
       if constexpr (SPLIT) {
@@ -819,7 +851,7 @@ __global__ void __launch_bounds__(AttnTcLayout<DK, DV, QT, KM>::T::kThreads, 1)
 
 template <int DK, int DV, int QT, bool LATENT, int KM = 0>
 static int launch_prefill_tc_maps(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mr, const AttnTcParams& p,
-                                  int num_tiles, cudaStream_t st) {
+                                  int num_tiles, cudaStream_t st, int parts = 1) {
   using L = typename AttnTcLayout<DK, DV, QT, KM>::T;
   static PerDeviceOnce attr_once;
   if (attr_once.first()) {
@@ -827,7 +859,7 @@ static int launch_prefill_tc_maps(const CUtensorMap& mq, const CUtensorMap& mk, 
     if (e != cudaSuccess) throw std::runtime_error(std::string("prefill attention (tcgen05): cudaFuncSetAttribute: ") + cudaGetErrorString(e));
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(num_tiles, p.H);
+  cfg.gridDim = dim3(num_tiles, p.H, parts);
   cfg.blockDim = dim3(L::kThreads);
   cfg.dynamicSmemBytes = L::kBytes;
   cfg.stream = st;
@@ -843,13 +875,13 @@ static int launch_prefill_tc_maps(const CUtensorMap& mq, const CUtensorMap& mk, 
 
 template <int DK, int DV, int QT, int KM = 0>
 static int launch_prefill_tc_t(const void* q, long long q_stride, long long T, const void* kc, const void* vc, long long cache_rows, const AttnTcParams& p,
-                               int num_tiles, cudaStream_t st) {
+                               int num_tiles, cudaStream_t st, int parts = 1) {
   CUtensorMap mq, mk, mv;
   encode_map_2d(&mq, 0, q, static_cast<uint64_t>(T), static_cast<uint64_t>(p.H) * p.dk, static_cast<uint64_t>(q_stride) * 2, kAtBM, 64, 128);
   const uint32_t box_rows = p.page_size < kAtBN ? p.page_size : kAtBN;
   encode_map_2d(&mk, 0, kc, static_cast<uint64_t>(cache_rows), p.dk, static_cast<uint64_t>(p.dk) * 2, box_rows, 64, 128);
   encode_map_2d(&mv, 0, vc, static_cast<uint64_t>(cache_rows), p.dv, static_cast<uint64_t>(p.dv) * 2, box_rows, 64, 128);
-  return launch_prefill_tc_maps<DK, DV, QT, false, KM>(mq, mk, mv, mv, p, num_tiles, st);
+  return launch_prefill_tc_maps<DK, DV, QT, false, KM>(mq, mk, mv, mv, p, num_tiles, st, parts);
 }
 
 // ---- latent layout -----------------------------------------------------------------------------------------------------
@@ -973,12 +1005,67 @@ int launch_prefill_wide_tc(const WideTcArgs& a, AttnExtra x, cudaStream_t st) {
 // tensor memory beside the two score slots.
 int prefill_attention_tc_tile_rows(int D) { return D <= 128 ? 256 : 128; }
 
+// o = sum_z 2^(e_z - e) O_z / sum_z 2^(e_z - e) l_z with e the largest e_z: a warp per query row and head. A part in which a row sees no key has e_z = -inf and nothing to read; it is the
+// bytes of the parts that count (L2), for which all of a row's parts are asked for four at a time.
+template <int D>
+__global__ void __launch_bounds__(256) prefill_parts_kernel(const float* po, const float2* notes, __nv_bfloat16* out, long long rows, int parts) {
+  constexpr int N = D / 32;  // columns of a lane, next to one another
+  const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_trigger();
+  if (row >= rows) return;
+  const float2 mine = lane < parts ? notes[lane * rows + row] : make_float2(-INFINITY, 0.f);
+  float top = mine.x;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  const float w = mine.x == -INFINITY ? 0.f : ex2_approx(mine.x - top);  // (NaN stays NaN)
+  float sum = w * mine.y;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  float acc[N] = {};
+  for (int z0 = 0; z0 < parts; z0 += 4) {
+    float v[4][N], wz[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      wz[k] = __shfl_sync(0xffffffffu, w, z0 + k);  // (lanes behind the last part: 0)
+      const bool there = __shfl_sync(0xffffffffu, mine.x, z0 + k) != -INFINITY;
+      const float* from = po + ((z0 + k) * rows + row) * D + lane * N;
+      if constexpr (N == 2) {
+        const float2 f = there ? *reinterpret_cast<const float2*>(from) : make_float2(0.f, 0.f);
+        v[k][0] = f.x;
+        v[k][1] = f.y;
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+          const float4 f = there ? *reinterpret_cast<const float4*>(from + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+          v[k][i] = f.x;
+          v[k][i + 1] = f.y;
+          v[k][i + 2] = f.z;
+          v[k][i + 3] = f.w;
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[i] = fmaf(wz[k], v[k][i], acc[i]);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint32_t packed[N / 2];
+#pragma unroll
+  for (int i = 0; i < N; i += 2) packed[i / 2] = pack_bf162(acc[i] * inv, acc[i + 1] * inv);
+  uint32_t* to = reinterpret_cast<uint32_t*>(out + row * D + lane * N);
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) to[i] = packed[i];
+}
+
 // tile arrays: prefill_attention_tc_tile_rows(max(dk, dv)) query rows per tile. page_size must be 32, 64 or 128. Returns 1 for an unsupported
 // head size (multiples of 8 up to 256) or page size.
 int launch_prefill_attention_tc(const void* q, long long q_stride, long long T, const void* kc, const void* vc, long long num_pages, const int* bt,
                                 int bt_stride, const int* q_start, const int* q_len, const int* ctx, const int* tile_seq, const int* tile_q0,
                                 int num_tiles, void* out, int H, int KV, int dk, int dv, int page, float scale, float cap, int window, int causal,
-                                AttnExtra x, int* status, cudaStream_t st, bool f16, int rows) {
+                                AttnExtra x, int* status, cudaStream_t st, bool f16, int rows, int parts, float* part_o, void* part_note) {
   if (num_tiles == 0) return 0;
   const int D = dk > dv ? dk : dv;
   if (f16 && (dk != dv || (D != 64 && D != 128 && D != 256) || x.sink != nullptr)) return 1;
@@ -1011,12 +1098,23 @@ int launch_prefill_attention_tc(const void* q, long long q_stride, long long T, 
   p.status = status;
   const long long cache_rows = num_pages * KV * page;
   if (f16) {
-    if (D == 64 && rows == kAtBM) return launch_prefill_tc_t<64, 64, 1, 4>(q, q_stride, T, kc, vc, cache_rows, p, num_tiles, st);
-    if (D == 128 && rows == kAtBM) return launch_prefill_tc_t<128, 128, 1, 4>(q, q_stride, T, kc, vc, cache_rows, p, num_tiles, st);
-    if (rows != prefill_attention_tc_tile_rows(D)) return 1;
-    if (D == 64) return launch_prefill_tc_t<64, 64, 2, 4>(q, q_stride, T, kc, vc, cache_rows, p, num_tiles, st);
-    if (D == 128) return launch_prefill_tc_t<128, 128, 2, 4>(q, q_stride, T, kc, vc, cache_rows, p, num_tiles, st);
-    return launch_prefill_tc_t<256, 256, 1, 4>(q, q_stride, T, kc, vc, cache_rows, p, num_tiles, st);
+    if (rows != kAtBM && (rows != prefill_attention_tc_tile_rows(D) || parts != 1)) return 1;
+    if (parts < 1 || parts > kMaxPrefillParts || (parts > 1 && (part_o == nullptr || part_note == nullptr || x.gate != nullptr || p.out_mult != 1.f || p.out_pitch != static_cast<long long>(H) * D))) return 1;
+    p.part_o = parts > 1 ? part_o : nullptr;
+    p.part_note = static_cast<float2*>(part_note);
+    p.rows = T;
+    if (rows != kAtBM && D == 64) return launch_prefill_tc_t<64, 64, 2, 4>(q, q_stride, T, kc, vc, cache_rows, p, num_tiles, st);
+    if (rows != kAtBM) return launch_prefill_tc_t<128, 128, 2, 4>(q, q_stride, T, kc, vc, cache_rows, p, num_tiles, st);
+    if (D == 64) launch_prefill_tc_t<64, 64, 1, 4>(q, q_stride, T, kc, vc, cache_rows, p, num_tiles, st, parts);
+    else if (D == 128) launch_prefill_tc_t<128, 128, 1, 4>(q, q_stride, T, kc, vc, cache_rows, p, num_tiles, st, parts);
+    else launch_prefill_tc_t<256, 256, 1, 4>(q, q_stride, T, kc, vc, cache_rows, p, num_tiles, st, parts);
+    if (parts == 1) return 0;
+    const long long n = T * H;
+    const dim3 grid(static_cast<unsigned>((n + 7) / 8));
+    if (D == 64) launch_pdl(prefill_parts_kernel<64>, grid, dim3(256), 0, st, static_cast<const float*>(part_o), static_cast<const float2*>(p.part_note), p.out, n, parts);
+    else if (D == 128) launch_pdl(prefill_parts_kernel<128>, grid, dim3(256), 0, st, static_cast<const float*>(part_o), static_cast<const float2*>(p.part_note), p.out, n, parts);
+    else launch_pdl(prefill_parts_kernel<256>, grid, dim3(256), 0, st, static_cast<const float*>(part_o), static_cast<const float2*>(p.part_note), p.out, n, parts);
+    return 0;
   }
   if (D <= 64) return launch_prefill_tc_t<64, 64, 2>(q, q_stride, T, kc, vc, cache_rows, p, num_tiles, st);
   if (D <= 128 && dv <= 64) return launch_prefill_tc_t<128, 64, 2>(q, q_stride, T, kc, vc, cache_rows, p, num_tiles, st);

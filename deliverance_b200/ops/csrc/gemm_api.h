@@ -225,7 +225,10 @@ extern bool g_gemv_simt_only;  // gemm.cu: grouped JQ4 GEMV on CUDA cores instea
 int launch_prefill_attention_tc(const void* q, long long q_stride, long long T, const void* kc, const void* vc, long long num_pages, const int* bt,
                                 int bt_stride, const int* q_start, const int* q_len, const int* ctx, const int* tile_seq, const int* tile_q0,
                                 int num_tiles, void* out, int H, int KV, int dk, int dv, int page, float scale, float cap, int window, int causal,
-                                AttnExtra x, int* status, cudaStream_t st, bool f16 = false, int rows = 0);  // f16: tiles of `rows` (128, or as many as the layout's)
+                                AttnExtra x, int* status, cudaStream_t st, bool f16 = false, int rows = 0,
+                                int parts = 1, float* part_o = nullptr, void* part_note = nullptr);
+// f16: tiles of `rows` (128, or as many as the layout's); with 128 a tile's keys may be cut into `parts`: part_o fp32 [parts, T, H, D], part_note fp32 pairs [parts, T, H]
+constexpr int kMaxPrefillParts = 32;
 // wide rows: query tile height for keys of k_width columns and values of dv columns per head, 0 when the kernel does not take them
 int prefill_attention_wide_tile_rows(int k_width, int dv);
 // q [T, H * W], gathered keys k [kv_rows, W] (W: k_width padded with zeros to a multiple of 64) and values v [kv_rows, KV * dv]

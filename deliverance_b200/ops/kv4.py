@@ -139,11 +139,12 @@ def prefill_attention4(q, k_cache, v_cache, block_tables, q_start, q_len, ctx_le
     # 700 rows of 16 heads 23.2 for 26.4, 2,048 of 8 heads 45.3 for 53.4, 200 rows behind 9,000 of 32 heads 193 for 221). Beyond that the second wave costs more (1,024 rows of 32 heads 45.7 for 35.7).
     if sum(-(-n // 128) for n in news) * H <= 148:
         rows = 128
+    parts = _parts(news, lens, rows, H, window)
     pages = [-(-n // page) for n in lens]
     if sum(pages) * KV * page * D * 4 <= EXPAND_PAGES_BYTES or S == 1:
         tile_seq, tile_q0 = tiles_for(rows) if tiles_for is not None else _tiles(news, rows, q.device)
-        ops._count(2)
-        return ext.kv4_prefill(q, k_cache, v_cache, block_tables, q_start, q_len, ctx_lens, tile_seq, tile_q0, H, scale, softcap, window, causal, sum(pages), max(pages, default=0), rows)
+        ops._count(2 + (parts > 1))
+        return ext.kv4_prefill(q, k_cache, v_cache, block_tables, q_start, q_len, ctx_lens, tile_seq, tile_q0, H, scale, softcap, window, causal, sum(pages), max(pages, default=0), rows, parts)
     outs, i, row = [], 0, 0
     while i < S:
         j, n_pages = i, 0
@@ -154,9 +155,20 @@ def prefill_attention4(q, k_cache, v_cache, block_tables, q_start, q_len, ctx_le
         tile_seq, tile_q0 = _tiles(news[part], rows, q.device)
         ops._count(2)
         outs.append(ext.kv4_prefill(q[row : row + n], k_cache, v_cache, block_tables[part], q_start[part] - row, q_len[part], ctx_lens[part], tile_seq, tile_q0, H, scale, softcap, window, causal,
-                                    n_pages, max(pages[part]), rows))
+                                    n_pages, max(pages[part]), rows, 1))
         i, row = j, row + n
     return torch.cat(outs)
+
+
+def _parts(news, lens, rows: int, H: int, window: int) -> int:
+    """In how many parts, a CTA each, a call cuts the keys of its query tiles: as many as the 148 SMs hold at one time, of 128 keys or more. A part costs its CTA's start and a pass over its accumulator, so
+    that a second wave loses (100 rows behind 9,000 of 32 heads of 128, us: 192 whole, 109 in 2 parts, 67 in 4, 74 in 8; 300 behind 30,000 of 8 heads 616, 144 in 6, 150 in 12; 20 behind 400 of 32 heads
+    17.4, 14.5 in 4, 20.6 in 8)."""
+    tiles = sum(-(-n // 128) for n in news) * H
+    if rows != 128 or tiles * 2 > 148 or tiles == 0:
+        return 1
+    keys = max(min(m, window + 128) if window else m for m in lens)  # (of any tile, at most)
+    return max(1, min(148 // tiles, keys // 128, 32))
 
 
 def _tiles(news, rows: int, device):

@@ -411,9 +411,12 @@ def test_prefill_options(device, softcap, window, page):
 
 @pytest.mark.parametrize("device", GPU)
 @pytest.mark.parametrize("D,KV,G,news,befores", [(64, 4, 8, [600, 1, 129], [0, 64, 300]), (128, 8, 4, [257, 500], [40, 0]), (128, 8, 4, [128] * 4 + [1], [0] * 5), (128, 8, 4, [128] * 4, [0] * 4)])
-def test_prefill_tile_heights(device, D, KV, G, news, befores):
-    """Calls on both sides of the rule on query tiles; a sequence has the same bits whichever height its call takes."""
+def test_prefill_tile_heights(device, D, KV, G, news, befores, monkeypatch):
+    """Calls on both sides of the rule on query tiles; a sequence has the same bits whichever height its call takes (its keys in one part)."""
+    from deliverance_b200.ops import kv4
+
     run_prefill(device, D, KV, G, news, befores)
+    monkeypatch.setattr(kv4, "_parts", lambda *args: 1)
     lens, H = [a + b for a, b in zip(news, befores)], KV * G
     table, pages = tables_for(lens, 32)
     k, v = (random_cache(pages, KV, 32, D, False).to(device) for _ in range(2))
@@ -424,6 +427,45 @@ def test_prefill_tile_heights(device, D, KV, G, news, befores):
         alone = prefill_attention4(q[at : at + n], k, v, table[b : b + 1].to(device), i32([0]), i32([n]), i32([lens[b]]), H, D**-0.5)
         assert torch.equal(alone, whole[at : at + n])
     done(device)
+
+
+@pytest.mark.parametrize("device", GPU)
+@pytest.mark.parametrize("D,KV,G", [(64, 2, 3), (128, 1, 4), (256, 2, 1)])
+@pytest.mark.parametrize("news,befores,softcap,window", [([1], [1023], 0.0, 0), ([1], [5000], 0.0, 0), ([33, 5], [2100, 70], 0.0, 0), ([130, 1, 64], [3, 4031, 0], 30.0, 0), ([3, 0, 2], [2000, 40, 9], 0.0, 0),
+                                                         ([300], [3000], 0.0, 1500), ([129, 2], [100, 4000], 0.5, 1000), ([128], [1408], 0.0, 0), ([2000], [0], 0.0, 0)])
+def test_prefill_in_parts(device, D, KV, G, news, befores, softcap, window):
+    """Few query rows behind many keys: the keys are cut into parts."""
+    from deliverance_b200.ops import kv4
+
+    tiles = sum(-(-n // 128) for n in news) * KV * G
+    assert kv4._parts(news, [a + b for a, b in zip(news, befores)], 128, KV * G, window) > 1 or 148 // tiles == 1  # (16 tiles of 6 heads are 96: whole)
+    run_prefill(device, D, KV, G, news, befores, softcap, window)
+
+
+@pytest.mark.parametrize("device", GPU)
+def test_prefill_in_parts_keeps_nan(device):
+    """A NaN block reaches the rows and heads that see it, whichever part holds it, and no others."""
+    KV, D, H, page, lens = 2, 64, 4, 32, [4000]
+    table, pages = tables_for(lens, page)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    q = torch.randn(20, H * D).to(BF16).to(device)
+    for cache, pos in ((0, 5), (0, 3000), (1, 5), (1, 2500), (0, 3990)):
+        kv = [random_cache(pages, KV, page, D, False) for _ in range(2)]
+        kv[cache][table[0, pos // page].long(), 1, pos % page, D // 2 :] = 0x7F
+        got = prefill_attention4(q, kv[0].to(device), kv[1].to(device), table.to(device), i32([0]), i32([20]), i32(lens), H, 0.1).cpu().float().reshape(20, H, D)
+        done(device)
+        sees = torch.arange(20) + 3980 >= pos
+        assert got[sees][:, 2:].isnan().all() and not got[:, :2].isnan().any()
+        if cache == 0:
+            assert not got[~sees].isnan().any()
+
+
+def test_prefill_parts_rule():
+    from deliverance_b200.ops.kv4 import _parts
+
+    assert _parts([], [], 128, 4, 0) == 1 and _parts([1], [100], 128, 32, 0) == 1 and _parts([1], [10**6], 256, 32, 0) == 1
+    assert _parts([100], [9000], 128, 32, 0) == 4 and _parts([200], [9000], 128, 32, 0) == 2 and _parts([300], [9000], 128, 32, 0) == 1
+    assert _parts([1], [2**20], 128, 1, 0) == 32 and _parts([1], [2**20], 128, 1, 100) == 1 and _parts([0], [0], 128, 1, 0) == 1
 
 
 @pytest.mark.parametrize("device", DEVICES)
