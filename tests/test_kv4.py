@@ -1,4 +1,4 @@
-"""The KV cache in 4 bits (quantising write, unpacking, decode and prompt attention) and step tables against plain statements in 64 bits, on the CPU and, on a GPU box, on the CUDA kernels."""
+"""The KV cache in 4 bits (quantising write, unpacking, decode and prompt attention) and step tables against plain statements in 64 bits, on the CPU and, where there is a GPU, on the CUDA kernels."""
 import math
 
 import pytest
@@ -443,6 +443,38 @@ def test_prefill_in_parts(device, D, KV, G, news, befores, softcap, window):
 
 
 @pytest.mark.parametrize("device", GPU)
+def test_prefill_in_parts_captured(device):
+    """Two captured calls with workspaces of their own, replayed in turn on two streams, with other tokens behind the same addresses."""
+    KV, D, H, page, lens, news = 2, 64, 4, 32, [3000, 700], [40, 7]
+    table, pages = tables_for(lens, page)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    k, v = (random_cache(pages, KV, page, D, False).to(device) for _ in range(2))
+    rest = (k, v, table.to(device), i32([0, 40]), i32(news), i32(lens), H, 0.1)
+    tiles = tuple(i32(t) for t in ops.prefill_tiles(news, 128))
+    qs = [torch.randn(47, H * D).to(BF16).to(device) for _ in range(2)]
+    run = lambda q: prefill_attention4(q, *rest, q_len_host=news, ctx_len_host=lens, tiles_for=lambda rows: tiles)  # noqa: E731
+    run(qs[0])
+    torch.cuda.synchronize()
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in qs]
+    for q in qs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(run(q))
+    for _ in range(3):
+        for q in qs:
+            q.copy_(torch.randn(47, H * D).to(BF16))
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        for q, out in zip(qs, outs):
+            assert torch.equal(out, run(q))
+    done(device)
+
+
+@pytest.mark.parametrize("device", GPU)
 def test_prefill_in_parts_keeps_nan(device):
     """A NaN block reaches the rows and heads that see it, whichever part holds it, and no others."""
     KV, D, H, page, lens = 2, 64, 4, 32, [4000]
@@ -722,6 +754,7 @@ def test_outputs_stay_inside_their_guard_areas(device):
             run_decode(device, D, KV, G, lens)
         run_prefill(device, 64, 2, 3, [33, 5], [0, 70])
         run_prefill(device, 128, 1, 2, [5], [3], page=96)
+        run_prefill(device, 128, 1, 2, [5], [3000])
         test_expand_matches_plain(device, 128, 1, 96)
         test_step_tables(device, [5, 0, 0, 129, 0], 64, 32)
         test_write_matches_plain(device, 128, 6, 2, 37, "halves", 64, True)
