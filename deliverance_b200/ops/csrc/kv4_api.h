@@ -4,6 +4,7 @@
 #include <stdint.h>
 
 #include "divisor.h"
+#include "kv4_parts.h"
 
 namespace dlv {
 
@@ -67,7 +68,6 @@ struct Kv4DecodeArgs {
 constexpr int kKv4MaxCtas = 1024;
 int kv4_decode_ctas(int B, int KV, int G, int D, long long rows, int sms);  // CTAs for sequences of up to `rows` keys
 int kv4_decode_near(int ctas, int pairs);
-long long kv4_decode_parts(int ctas, int pairs, int near);  // partial results that have a place
 void launch_kv4_decode(const Kv4DecodeArgs& a, int ctas, cudaStream_t st);  // two launches
 
 struct StepTablesArgs {

@@ -27,8 +27,8 @@ namespace dlv {
 namespace {
 
 constexpr int kTile = 32;      // keys of a tile
-constexpr int kWarps = 4;
-constexpr int kMinTiles = 2;   // of a share
+constexpr int kWarps = kKv4Warps;
+constexpr int kMinTiles = kKv4MinTiles;
 constexpr int kNear = 8;       // partial results of a pair that the second launch fetches at once
 constexpr float kShift = 12.f, kSlack = 3.f;
 constexpr float kLog2e = 1.44269504088896341f;
@@ -42,47 +42,6 @@ struct Kv4Ring {
   static constexpr int kCtas = (D == 64 ? 4 : D == 128 ? 3 : 2) - (NT - 1);  // per SM, as registers allow
   static constexpr int kBytes = kWarps * kStages * kStage;
 };
-
-// A share of the tiles: tile i of the step belongs to warp i / per.
-struct Kv4Shares {
-  int total, per;
-  __device__ Kv4Shares(int total_, int workers) : total(total_), per(max(kMinTiles, (total_ + workers - 1) / workers)) {}
-};
-
-// The parts of a pair's result. Parts in order: of the first CTA that has some of it, one of each CTA in the middle, of the last; a CTA whose shares all lie inside the pair makes one of them.
-struct Kv4Parts {
-  int parts, n0, mid, w0, c0, c1, first, per;
-  bool j0, j1;
-  __device__ Kv4Parts(const Kv4Shares& shares, int first_, int n) : first(first_), per(shares.per) {
-    const int last = first + n - 1, w1 = last / per, cta = kWarps * per;
-    w0 = first / per;
-    c0 = w0 / kWarps;
-    c1 = w1 / kWarps;
-    auto joined = [&](int c) {
-      const int lo = c * cta, hi = min(shares.total, lo + cta);
-      return hi - lo > per && first <= lo && hi <= last + 1;
-    };
-    j0 = joined(c0);
-    j1 = joined(c1);
-    n0 = j0 ? 1 : min(w1, c0 * kWarps + kWarps - 1) - w0 + 1;
-    mid = max(0, c1 - c0 - 1);
-    parts = n0 + mid + (c1 == c0 ? 0 : j1 ? 1 : w1 - c1 * kWarps + 1);
-  }
-  __device__ int number(int w) const {  // of the part that warp w (or its CTA) makes
-    const int c = w / kWarps;
-    return c == c0 ? (j0 ? 0 : w - w0) : c < c1 ? n0 + c - c0 - 1 : n0 + mid + (j1 ? 0 : w - c1 * kWarps);
-  }
-  __device__ int maker(int i) const {  // the (first) warp that makes part i, and which of its two parts that is
-    const bool middle = i >= n0 && i < n0 + mid, own = i < n0 ? !j0 : !middle && !j1;
-    const int w = i < n0 ? (j0 ? c0 * kWarps : w0 + i) : middle ? (c0 + 1 + i - n0) * kWarps : c1 * kWarps + (i - n0 - mid);
-    return w * 2 + (own && first >= w * per ? 1 : 0);
-  }
-};
-// Where part i of a pair lies, in [G, D] rows of part_o, for kv4_merge_kernel: the first `near` of every pair next to one another, so that the second launch can fetch them before it knows how many there are; the others with the warp
-// that makes them (`maker`).
-__device__ __forceinline__ long long kv4_place(const Kv4DecodeArgs& a, int pair, int i, long long maker) {
-  return i < a.near ? static_cast<long long>(pair) * a.near + i : static_cast<long long>(a.B) * a.KV * a.near + maker;
-}
 
 __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t magic) {
   uint32_t y;
@@ -615,7 +574,7 @@ __global__ void __launch_bounds__(kWarps * 32, Kv4Ring<D, NT>::kCtas) kv4_decode
       if (a.near > 0 && (all || !together)) {
         const int2 span = spans[warp][j & 63];
         const Kv4Parts parts(shares, span.x, span.y);
-        at = kv4_place(a, pair, parts.number(worker), at);
+        at = kv4_place(a.B * a.KV, a.near, pair, parts.number(worker), at);
         if (from_start && lane == 0) a.counts[pair] = all ? -1 : parts.parts;
       }
       if (!all && !together) write_part(a.part_o + at * G * D, a.part_ml + at * G * 2);
@@ -642,7 +601,7 @@ __global__ void __launch_bounds__(kWarps * 32, Kv4Ring<D, NT>::kCtas) kv4_decode
   if (a.near > 0) {
     const int n = tiles_at(cta_b), kvh = static_cast<int>((cta_lo - cta_base) / n), first = cta_base + kvh * n, cta_pair = cta_b * a.KV + kvh;
     const Kv4Parts parts(shares, first, n);
-    slot = kv4_place(a, cta_pair, parts.number(blockIdx.x * kWarps), slot);
+    slot = kv4_place(a.B * a.KV, a.near, cta_pair, parts.number(blockIdx.x * kWarps), slot);
     if (tid == 0 && first == cta_lo) a.counts[cta_pair] = parts.parts;
   }
   for (int i = tid; i < G * (D / 4); i += kWarps * 32) {
@@ -724,16 +683,18 @@ __global__ void __launch_bounds__(128) kv4_merge_kernel(const Kv4DecodeArgs a, i
     if (i < near) add(i);
   }
   if (count > near) {
+    // (a warp whose wait ran out has left no count: what stands there is anything, and the parts that there can be are the limit)
     const int n = behind - before;
     const Kv4Parts p(Kv4Shares(total * a.KV, workers), before * a.KV + kvh * n, n);
-    for (int i0 = near; i0 < count; i0 += AHEAD) {
+    const int most = p.most(count);
+    for (int i0 = near; i0 < most; i0 += AHEAD) {
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
-        if (i0 + i < count) fetch(i, kv4_place(a, pair, i0 + i, p.maker(i0 + i)));
+        if (i0 + i < most) fetch(i, kv4_place(a.B * a.KV, a.near, pair, i0 + i, p.maker(i0 + i)));
       }
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
-        if (i0 + i < count) add(i);
+        if (i0 + i < most) add(i);
       }
     }
   }
@@ -842,7 +803,6 @@ int kv4_decode_near(int ctas, int pairs) {
   const int n = ctas * kWarps / pairs + 2;
   return n <= kNear ? n : 0;
 }
-long long kv4_decode_parts(int ctas, int pairs, int near) { return static_cast<long long>(ctas) * kWarps * 2 + static_cast<long long>(pairs) * near; }
 
 void launch_kv4_decode(const Kv4DecodeArgs& a, int ctas, cudaStream_t st) {
   const bool two = a.H / a.KV > 8;

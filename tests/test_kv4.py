@@ -988,3 +988,64 @@ def test_batches_made_there(device, kind):
         assert a.rows_apart() == b.rows_apart() if a.is_decode else b.host_tables is None
     with pytest.raises(ValueError):
         make_batch([dict(seqs[0], pages=[])], 32, device)
+
+
+# ---------------------------------------------------------------------------------------------------------------- ends of the operators
+PARTS = """
+#include <cstdio>
+#include <cstdlib>
+#include <set>
+#include <vector>
+#include "kv4_parts.h"
+using namespace dlv;
+int main() {
+  srand(7);
+  for (int round = 0; round < 4000; ++round) {
+    const int KV = 1 + rand() % 8, B = 1 + rand() % 40, ctas = 1 + rand() % (round % 3 ? 12 : 1024), workers = ctas * kKv4Warps, near = rand() % 9, pairs = B * KV;
+    std::vector<int> n(B), front(B + 1, 0);
+    for (int b = 0; b < B; ++b) {
+      n[b] = rand() % 4 ? rand() % (round % 2 ? 9 : 400) : 0;
+      front[b + 1] = front[b] + n[b];
+    }
+    const Kv4Shares shares(front[B] * KV, workers);
+    const long long room = kv4_decode_parts(ctas, pairs, near);
+    std::set<long long> places;
+    for (int pair = 0; pair < pairs; ++pair) {
+      const int b = pair / KV, h = pair % KV;
+      const Kv4Parts p(shares, front[b] * KV + h * n[b], n[b]);
+      if (n[b] == 0 && p.parts != 0) return 1;
+      const bool whole = p.parts == 1 && !p.j0;  // seen whole by one warp, which writes the result and no part
+      for (int i = 0; i < p.parts && !whole; ++i) {  // every part has a place of its own
+        const long long at = kv4_place(pairs, near, pair, i, p.maker(i));
+        if (at < 0 || at >= room || !places.insert(at).second) return 2;
+      }
+      const int counts[] = {p.parts, 0, -1, 1, near + 1, 1 << 30, 0x7fffffff, 0x3f800000, -0x7fffffff - 1};
+      for (int count : counts) {  // what the second launch reads, whatever stands where the count should be
+        for (int i = 0; i < near; ++i)
+          if (kv4_place(pairs, near, pair, i, 0) >= room) return 3;
+        for (int i = count < near ? count : near; i >= 0 && i < p.most(count); ++i) {
+          const long long at = kv4_place(pairs, near, pair, i, p.maker(i));
+          if (at < 0 || at >= room) return 4;
+        }
+      }
+      if (p.most(p.parts) != p.parts) return 5;
+    }
+  }
+  puts("ok");
+}
+"""
+
+
+def test_decode_parts_stay_in_their_workspace(tmp_path):
+    """The places of partial results, from the header that the kernels use: different ones, and inside the workspace even for a count that no warp has written."""
+    import os
+    import shutil
+    import subprocess
+
+    from deliverance_b200.ops import build
+
+    if shutil.which("g++") is None:
+        pytest.skip("no g++")
+    (tmp_path / "parts.cpp").write_text(PARTS)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover", "-I", build.CSRC, str(tmp_path / "parts.cpp"), "-o", str(tmp_path / "parts")], check=True, timeout=120)
+    assert subprocess.run([str(tmp_path / "parts")], capture_output=True, text=True, timeout=120, env=dict(os.environ)).stdout == "ok\n"
