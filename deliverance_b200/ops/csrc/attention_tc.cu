@@ -65,7 +65,7 @@ void encode_map_2d(CUtensorMap* map, int dtype_code, const void* base, uint64_t 
 
 struct AttnTcParams {
   const int* block_tables;
-  int bt_stride;
+  int bt_stride;               // (fp16 layout: also the columns of a row)
   const int* q_start;
   const int* q_len;
   const int* ctx_lens;
@@ -90,7 +90,7 @@ struct AttnTcParams {
   int k_subs;                  // wide layout: 64-column blocks of a key row
   float* part_o;               // fp16 layout, a query tile's keys in gridDim.z > 1 parts: accumulators [parts, T, H, dv] ...
   float2* part_note;           // ... and (base-2 exponent that they are relative to, sum) [parts, T, H]
-  long long rows;              // T
+  long long rows;              // fp16 layout: T
 };
 
 // MN-major shared-memory descriptor (128-byte swizzle): the operand tile is stored as rows of the K dimension, each row 64 elements of
@@ -265,10 +265,13 @@ __global__ void __launch_bounds__(AttnTcLayout<DK, DV, QT, KM>::T::kThreads, 1)
   auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };  // (one value for the CTA, told to the compiler)
   const int seq = uniform(p.tile_seq[tile]), q0 = uniform(p.tile_q0[tile]), h = blockIdx.y;
   const int kvh = h / (p.H / p.KV);
-  const int qs = uniform(p.q_start[seq]), ql = uniform(p.q_len[seq]), ctx = uniform(p.ctx_lens[seq]);
+  const int qs = uniform(p.q_start[seq]), ql_given = uniform(p.q_len[seq]), ctx_given = uniform(p.ctx_lens[seq]);
+  // (F16: lengths that are not those the tables were made for are reported by the kernel in front, perhaps after this CTA has looked at the status: here they end where tables and rows do)
+  const int ctx = F16 ? max(0, min(ctx_given, p.bt_stride * p.page_size)) : ctx_given, ql = F16 ? max(0, min(ql_given, ctx)) : ql_given;
   const int pos0 = ctx - ql;  // position of the sequence's first query row
   constexpr bool SPLIT = PIECES && QT == 2;  // one query tile, its key tiles alternate between the softmax groups
-  const int rows_all = min((SPLIT ? 1 : QT) * kAtBM, ql - q0);
+  const int rows_left = F16 ? (qs < 0 ? 0 : static_cast<int>(max(0ll, min(static_cast<long long>(ql - q0), p.rows - qs - q0)))) : ql - q0;
+  const int rows_all = min((SPLIT ? 1 : QT) * kAtBM, rows_left);
   const bool two = QT == 2 && (SPLIT || rows_all > kAtBM);  // two query tiles share every K / V tile
   // key tiles [a, b) each query tile sees
   int rows_q[2], first_q[2], a_q[2], b_q[2];

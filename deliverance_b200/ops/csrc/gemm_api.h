@@ -227,7 +227,7 @@ int launch_prefill_attention_tc(const void* q, long long q_stride, long long T, 
                                 int num_tiles, void* out, int H, int KV, int dk, int dv, int page, float scale, float cap, int window, int causal,
                                 AttnExtra x, int* status, cudaStream_t st, bool f16 = false, int rows = 0,
                                 int parts = 1, float* part_o = nullptr, void* part_note = nullptr);
-// f16: tiles of `rows` (128, or as many as the layout's); with 128 a tile's keys may be cut into `parts`: part_o fp32 [parts, T, H, D], part_note fp32 pairs [parts, T, H]
+// f16: block tables without gaps (bt_stride columns); lengths beyond them or beyond T end there; tiles of `rows` (128, or as many as the layout's); with 128 a tile's keys may be cut into `parts`: part_o fp32 [parts, T, H, D], part_note fp32 pairs [parts, T, H]
 constexpr int kMaxPrefillParts = 32;
 // wide rows: query tile height for keys of k_width columns and values of dv columns per head, 0 when the kernel does not take them
 int prefill_attention_wide_tile_rows(int k_width, int dv);

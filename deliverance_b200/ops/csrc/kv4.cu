@@ -335,7 +335,8 @@ __global__ void __launch_bounds__(256) kv4_expand_seqs_kernel(const Kv4SeqsArgs 
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) base += __shfl_xor_sync(0xffffffffu, base, o);
   if (first) {
-    const bool bad = given != ctx || own > a.longest || base + own > a.total || (s == a.S - 1 && base + own != a.total);
+    const int qs = a.q_start[s], ql = a.q_len[s];
+    const bool bad = given != ctx || own > a.longest || base + own > a.total || (s == a.S - 1 && base + own != a.total) || ql < 0 || ql > ctx || qs < 0 || static_cast<long long>(qs) + ql > a.T;
     if (bad && threadIdx.x == 0) atomicCAS(a.status, kStatusOk, kStatusBadArgs);
     const int cut = a.page / a.out_page;
     for (int c = threadIdx.x; c < a.width * cut; c += 256) a.out_tables[static_cast<long long>(s) * a.width * cut + c] = c < own * cut && base + c / cut < a.total ? base * cut + c : 0;

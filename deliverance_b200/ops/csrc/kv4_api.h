@@ -42,10 +42,11 @@ void launch_kv4_expand(const Kv4ExpandArgs& a, cudaStream_t st);
 struct Kv4SeqsArgs {
   const uint8_t *k, *v;
   const int* tables;  // [S, width]
-  const int* ctx;     // [S]
+  const int *ctx, *q_start, *q_len;  // [S]
   void *ko, *vo;      // fp16 [total * page / out_page, KV, out_page, D]
   int* out_tables;    // [S, width * page / out_page]
   int* status;
+  long long T;        // query rows
   int S, width, longest, total, pages, KV, page, out_page, D;  // longest: pages of a sequence, at most
 };
 void launch_kv4_expand_seqs(const Kv4SeqsArgs& a, cudaStream_t st);

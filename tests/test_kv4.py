@@ -1049,3 +1049,33 @@ def test_decode_parts_stay_in_their_workspace(tmp_path):
     (tmp_path / "parts.cpp").write_text(PARTS)
     subprocess.run(["g++", "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover", "-I", build.CSRC, str(tmp_path / "parts.cpp"), "-o", str(tmp_path / "parts")], check=True, timeout=120)
     assert subprocess.run([str(tmp_path / "parts")], capture_output=True, text=True, timeout=120, env=dict(os.environ)).stdout == "ok\n"
+
+
+@pytest.mark.parametrize("device", GPU)
+@pytest.mark.parametrize("D,news,befores", [(64, [3, 200], [90, 40]), (128, [150, 7], [3000, 10]), (256, [2, 2], [10, 30])])
+def test_prefill_reports_other_lengths(device, D, news, befores):
+    """Lengths on the device that are not the host's, beyond the tables and below zero, are reported; the kernels stay inside tables and rows, and the next call is as good as any."""
+    KV, H, page, lens = 2, 4, 32, [a + b for a, b in zip(news, befores)]
+    table, pages = tables_for(lens, page)
+    k, v = random_cache(pages, KV, page, D, False).to(device), random_cache(pages, KV, page, D, False).to(device)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    q, start, width = torch.randn(sum(news), H * D, device=device).to(BF16), [0, news[0]], table.shape[1]
+    call = lambda ctx, new=news: prefill_attention4(q, k, v, table.to(device), i32(start), i32(new), i32(ctx), H, D**-0.5, q_len_host=news, ctx_len_host=lens)  # noqa: E731
+    want = call(lens)
+    done(device)
+    ops.set_bounds_check(True)
+    try:
+        for ctx in ([lens[0], width * page + 999], [2**31 - 1, lens[1]], [-5, lens[1]], [0, 0], [lens[0], -(2**31)]):
+            call(ctx)
+            with pytest.raises(RuntimeError, match="bad kernel arguments"):
+                ops.check_status()
+        for new in ([news[0], news[1] + 4000], [lens[0] + 1, news[1]], [-1, news[1]], [news[0], 2**31 - 1]):
+            call(lens, new)
+            with pytest.raises(RuntimeError, match="bad kernel arguments"):
+                ops.check_status()
+        torch.cuda.synchronize()
+        ops.check_guards()
+    finally:
+        ops.set_bounds_check(False)
+    assert torch.equal(call(lens), want)
+    done(device)
