@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(kWarps * 32, Kv4Ring<D, NT>::kCtas) kv4_decode
       }
     }
   };
-  // unnormalised rows, maximum and sum of every head: dst [G][D], ml [G][2]
+  // unnormalised rows, maximum and sum of every head: dst [G][D], ml [G][2]. Maxima pass NaN over: a NaN in the sum stands as the maximum too, so that no join takes the part for one without keys.
   auto write_part = [&](float* dst, float* ml) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(kWarps * 32, Kv4Ring<D, NT>::kCtas) kv4_decode
           }
         }
         if (g == 0) {
-          ml[2 * h] = top[nt][i];
+          ml[2 * h] = ol[nt][i] == ol[nt][i] ? top[nt][i] : ol[nt][i];
           ml[2 * h + 1] = ol[nt][i];
         }
       }
@@ -623,7 +623,7 @@ __global__ void __launch_bounds__(kWarps * 32, Kv4Ring<D, NT>::kCtas) kv4_decode
       v.w += f[w] * p.w;
     }
     *reinterpret_cast<float4*>(a.part_o + slot * G * D + h * D + d) = v;
-    if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * G + h) * 2) = make_float2(up, sum);
+    if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * G + h) * 2) = make_float2(sum == sum ? up : sum, sum);
   }
 }
 
@@ -666,7 +666,7 @@ __global__ void __launch_bounds__(128) kv4_merge_kernel(const Kv4DecodeArgs a, i
   auto add = [&](int i) {
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
-      if (h0 + (k * 32 + lane) / DQ < G && ml[i][k].x > -INFINITY) {
+      if (h0 + (k * 32 + lane) / DQ < G && ml[i][k].x != -INFINITY) {  // (NaN goes into everything)
         const float top = fmaxf(up[k], ml[i][k].x), f = ex2(up[k] - top), w = ex2(ml[i][k].x - top);
         up[k] = top;
         sum[k] = sum[k] * f + w * ml[i][k].y;

@@ -1079,3 +1079,30 @@ def test_prefill_reports_other_lengths(device, D, news, befores):
         ops.set_bounds_check(False)
     assert torch.equal(call(lens), want)
     done(device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D,KV,G,lens,first,count", [
+    (128, 2, 2, [4000], 64, 512), (128, 2, 2, [4000], 3968, 32), (128, 2, 2, [4000], 0, 4000), (64, 1, 3, [20000], 4096, 2048),  # one sequence, cut into many shares
+    (128, 2, 2, [4000], 256, 256), (128, 8, 4, [2176] * 64, 0, 128), (128, 8, 4, [2176] * 64, 0, 384), (128, 8, 4, [2176] * 64, 1792, 384), (128, 8, 4, [2176] * 64, 0, 544), (128, 8, 4, [2176] * 64, 1088, 1088), (64, 4, 8, [3000, 100] * 8, 512, 1024), (256, 2, 12, [3000, 7, 900] * 4, 64, 800),  # many pairs
+])
+@pytest.mark.parametrize("cache", ["keys", "values"])
+def test_decode_keeps_nan_whatever_the_shares(device, D, KV, G, lens, first, count, cache):
+    """Runs of rows without a number, long enough for whole shares of the work to hold nothing else: the heads that see them are NaN, all others are what they are without them."""
+    if device == "cpu" and sum(lens) * KV * G * D > 5e7:
+        pytest.skip("large for the CPU")
+    table, pages = tables_for(lens, 32)
+    H, q = KV * G, torch.randn(len(lens), KV * G * D).to(BF16)
+    k, v = random_cache(pages, KV, 32, D), random_cache(pages, KV, 32, D, False)
+    to = lambda t: t.to(device)  # noqa: E731
+    call = lambda: decode_attention4(to(q), to(k), to(v), to(table), to(torch.tensor(lens, dtype=torch.int32)), H, D**-0.5).cpu().view(len(lens), KV, G * D)  # noqa: E731
+    clean = call()
+    hit = [b for b, n in enumerate(lens) if b % 3 == 0 and first + count <= n]
+    for b in hit:
+        for j in range(first, first + count):
+            (k if cache == "keys" else v)[table[b, j // 32].long(), KV - 1, j % 32, D // 2 :] = 0x7E  # (steps and minima that are no numbers)
+    got = call()
+    done(device)
+    bad = torch.zeros(len(lens), KV, dtype=torch.bool)
+    bad[hit, KV - 1] = True
+    assert hit and got[bad].isnan().all() and torch.equal(got[~bad], clean[~bad])
