@@ -611,7 +611,7 @@ __global__ void __launch_bounds__(AttnTcLayout<DK, DV, QT, KM>::T::kThreads, 1)
         }
         const uint32_t e = min(max(top >> 23, 1u), 253u);
         const float down = __uint_as_float((254u - e) << 23);
-        row_scale *= __uint_as_float(e << 23);
+        row_scale = fmaxf(row_scale * __uint_as_float(e << 23), 0x1p-126f);  // (zero would make NaN of the -inf of hidden keys; scores that small are zero in either case)
         for (int i = 0; i < DK / 8; ++i) {
           uint4 v = *chunk(i);
           uint32_t* w = reinterpret_cast<uint32_t*>(&v);

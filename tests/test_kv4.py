@@ -1106,3 +1106,22 @@ def test_decode_keeps_nan_whatever_the_shares(device, D, KV, G, lens, first, cou
     bad = torch.zeros(len(lens), KV, dtype=torch.bool)
     bad[hit, KV - 1] = True
     assert hit and got[bad].isnan().all() and torch.equal(got[~bad], clean[~bad])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D,news,befores,softcap", [(64, [70, 3], [100, 0], 0.0), (128, [5], [2000], 0.0), (256, [40], [9], 30.0)])
+def test_prefill_of_zero_rows_at_small_scales(device, D, news, befores, softcap):
+    """Query rows of zeros, and scales that take scores below the smallest numbers: every visible key counts alike, those that are not visible not at all."""
+    KV, H, page, lens = 2, 4, 32, [a + b for a, b in zip(news, befores)]
+    table, pages = tables_for(lens, page)
+    k, v = random_cache(pages, KV, page, D, False), random_cache(pages, KV, page, D, False)
+    to, i32 = lambda t: t.to(device), lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    q = torch.randn(sum(news), H, D)
+    q[:, ::2] = 0.0
+    q = q.flatten(1).to(BF16)
+    for scale in (1e-8, 1e-20, 1e-37):
+        got = prefill_attention4(to(q), to(k), to(v), to(table), i32([0, news[0]][: len(news)]), i32(news), i32(lens), H, scale, softcap).cpu().double()
+        done(device)
+        want, mass, _ = plain_attention(q, k, v, table, lens, news, KV, scale, softcap, 0)
+        # the result's rounding, values and probabilities in fp16 (half a step each; numerator and denominator)
+        assert ((got - want).abs() <= want.abs() * HALF_STEP + mass * (2.0**-11 + 2.0**-10) + 2.0**-24).all()
