@@ -316,7 +316,7 @@ void launch_kv4_expand(const Kv4ExpandArgs& a, cudaStream_t st) {
 }
 
 // The pages of a step's sequences -> fp16 pages next to one another (sequence by sequence), for prompt attention, with block tables that name them; a page becomes page / out_page of them.
-// Rows behind a sequence's end are zeros there. fp16, because a value is the sum of two fp16 numbers: 2^-12 of it are lost, where bf16 would lose 2^-9. A thread takes four units of 8 numbers, keys and values; grid (units of a page / 1024, pages of the longest sequence, S).
+// Rows behind a sequence's end, and rows that no window reaches, are zeros there: what stands in them does not matter, not even NaN. fp16, because a value is the sum of two fp16 numbers: 2^-12 of it are lost, where bf16 would lose 2^-9. A thread takes four units of 8 numbers, keys and values; grid (units of a page / 1024, pages of the longest sequence, S).
 template <int D>
 __global__ void __launch_bounds__(256) kv4_expand_seqs_kernel(const Kv4SeqsArgs a) {
   pdl_trigger();
@@ -349,7 +349,8 @@ __global__ void __launch_bounds__(256) kv4_expand_seqs_kernel(const Kv4SeqsArgs 
     page = 0;
   }
   const long long src = static_cast<long long>(page) * rows, dst = static_cast<long long>(base + j) * rows;
-  const int left = ctx - j * a.page;  // rows of this page in use
+  // rows of this page in use, and those in front of all query rows' windows
+  const int left = ctx - j * a.page, front = a.window > 0 ? ctx - max(0, min(a.q_len[s], ctx)) + 1 - a.window - j * a.page : 0;
   uint32_t codes[4][2], side[4][2];
   const int u0 = blockIdx.x * 1024 + threadIdx.x;
 #pragma unroll
@@ -358,7 +359,7 @@ __global__ void __launch_bounds__(256) kv4_expand_seqs_kernel(const Kv4SeqsArgs 
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
       codes[i][kv] = side[i][kv] = 0;
-      if (row < rows && row % a.page < left) {
+      if (row < rows && row % a.page < left && row % a.page >= front) {
         const uint8_t* p = (kv ? a.v : a.k) + (src + row) * RB;
         codes[i][kv] = *reinterpret_cast<const uint32_t*>(p + e0 / 2);
         side[i][kv] = *reinterpret_cast<const uint32_t*>(p + D / 2 + e0 / 32 * 4);

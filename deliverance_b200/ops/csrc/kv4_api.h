@@ -47,7 +47,7 @@ struct Kv4SeqsArgs {
   int* out_tables;    // [S, width * page / out_page]
   int* status;
   long long T;        // query rows
-  int S, width, longest, total, pages, KV, page, out_page, D;  // longest: pages of a sequence, at most
+  int S, width, longest, total, pages, KV, page, out_page, D, window;  // longest: pages of a sequence, at most
 };
 void launch_kv4_expand_seqs(const Kv4SeqsArgs& a, cudaStream_t st);
 

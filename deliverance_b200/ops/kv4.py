@@ -119,7 +119,7 @@ def prefill_attention4(q, k_cache, v_cache, block_tables, q_start, q_len, ctx_le
                        q_len_host: Optional[list] = None, ctx_len_host: Optional[list] = None, tiles_for=None):
     """:func:`ops.prefill_attention` for 4-bit caches: packed query rows of sequences of different lengths (``q_start`` adds ``q_len`` up), which are the last rows of their ``ctx_lens`` cached ones. On
     GPUs the pages in use are unpacked to fp16 next to one another, :data:`EXPAND_PAGES_BYTES` of them at a time, and attended to there. ``q_len_host`` / ``ctx_len_host``: the same lengths on the
-    host (else they are read back); ``tiles_for`` as there. Pages outside the caches, cached lengths that are not the host's, and more query rows than
+    host (else they are read back); ``tiles_for`` as there. What pages hold behind a sequence's end or in front of all its rows' windows does not matter. Pages outside the caches, cached lengths that are not the host's, and more query rows than
     there are or than cached ones, are reported by :func:`ops.check_status`."""
     T, D = q.shape[0], q.shape[1] // H
     if H % k_cache.shape[1] or window < 0 or softcap < 0 or not scale > 0:

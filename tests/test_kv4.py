@@ -1125,3 +1125,24 @@ def test_prefill_of_zero_rows_at_small_scales(device, D, news, befores, softcap)
         want, mass, _ = plain_attention(q, k, v, table, lens, news, KV, scale, softcap, 0)
         # the result's rounding, values and probabilities in fp16 (half a step each; numerator and denominator)
         assert ((got - want).abs() <= want.abs() * HALF_STEP + mass * (2.0**-11 + 2.0**-10) + 2.0**-24).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D,news,befores,window,page", [(64, [70, 1], [200, 300], 40, 32), (128, [5], [2000], 100, 96), (128, [20, 0, 33], [700, 40, 0], 7, 64), (256, [150], [333], 64, 32), (64, [300], [1000], 1, 32)])
+def test_prefill_in_front_of_a_window(device, D, news, befores, window, page):
+    """What stands in rows that no query row's window reaches does not matter, not even infinities and NaN."""
+    KV, H, lens = 2, 6, [a + b for a, b in zip(news, befores)]
+    table, pages = tables_for(lens, page)
+    k, v = random_cache(pages, KV, page, D, False), random_cache(pages, KV, page, D, False)
+    to, i32 = lambda t: t.to(device), lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    q, start = torch.randn(sum(news), H * D).to(BF16), [sum(news[:i]) for i in range(len(news))]
+    call = lambda: prefill_attention4(to(q), to(k), to(v), to(table), i32(start), i32(news), i32(lens), H, D**-0.5, 0.0, window).cpu()  # noqa: E731
+    clean = call()
+    want, mass, reach = plain_attention(q, k, v, table, lens, news, KV, D**-0.5, 0.0, window)
+    # the result's rounding; keys, values and probabilities in fp16 (a key's half step reaches the exponent; numerator and denominator)
+    assert ((clean.double() - want).abs() <= want.abs() * HALF_STEP + mass * (2.0**-10 + 2.0**-11 + reach * (2.0**-10 + 2.0**-16)) + 2.0**-24).all()
+    for b, (n, m) in enumerate(zip(lens, news)):
+        for j in range(n - m + 1 - window if m else n):
+            k[table[b, j // page].long(), :, j % page] = v[table[b, j // page].long(), :, j % page] = 0x7D if j % 2 else 0xFE
+    assert torch.equal(call(), clean)
+    done(device)
