@@ -133,8 +133,8 @@ def prefill_attention4(q, k_cache, v_cache, block_tables, q_start, q_len, ctx_le
     S, KV, page = len(news), k_cache.shape[1], k_cache.shape[2]
     if sum(news) != T or len(lens) != S or any(not 0 <= n <= m for n, m in zip(news, lens)) or max(lens, default=0) > block_tables.shape[1] * page:
         raise ValueError("the query rows must be those of the sequences, no more than their cached rows, and these no more than the block table has")
-    if q.stride(1) != 1 or q.stride(0) % 8 or q.data_ptr() % 16:
-        q = q.contiguous().clone() if q.data_ptr() % 16 else q.contiguous()
+    if q.stride(1) != 1 or q.stride(0) % 8 or q.stride(0) < q.shape[1] or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)  # (``contiguous`` leaves a single row its stride)
     rows = ext.prefill_tc_tile_rows(D)
     # A CTA takes a tile of query rows of one head. Tiles of half the height where all of them run at one time on the 148 SMs: the softmax of a key tile has half the rows to wait for (heads of 128, us:
     # 700 rows of 16 heads 23.2 for 26.4, 2,048 of 8 heads 45.3 for 53.4, 200 rows behind 9,000 of 32 heads 193 for 221). Beyond that the second wave costs more (1,024 rows of 32 heads 45.7 for 35.7).

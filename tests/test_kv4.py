@@ -1146,3 +1146,19 @@ def test_prefill_in_front_of_a_window(device, D, news, befores, window, page):
             k[table[b, j // page].long(), :, j % page] = v[table[b, j // page].long(), :, j % page] = 0x7D if j % 2 else 0xFE
     assert torch.equal(call(), clean)
     done(device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("rows", [1, 4])
+def test_prefill_takes_query_rows_as_they_lie(device, rows):
+    """Rows of any distance (none: the same row again) and alignment, a single one too."""
+    KV, H, D, page = 2, 4, 64, 32
+    table, pages = tables_for([40 + rows], page)
+    to, i32 = lambda t: t.to(device), lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    k, v = to(random_cache(pages, KV, page, D)), to(random_cache(pages, KV, page, D, False))
+    wide = to(torch.randn(rows, H * D + 3).to(BF16))
+    call = lambda q: prefill_attention4(q, k, v, to(table), i32([0]), i32([rows]), i32([40 + rows]), H, 0.1)  # noqa: E731
+    same = wide[:1, : H * D].contiguous()
+    for q in (wide[:, : H * D], wide[:, 1 : 1 + H * D], same.expand(rows, -1), torch.randn(H * D, rows, device=device).to(BF16).t()):
+        assert torch.equal(call(q), call(q.clone(memory_format=torch.contiguous_format)))
+    done(device)
