@@ -120,19 +120,23 @@ def prefill_attention4(q, k_cache, v_cache, block_tables, q_start, q_len, ctx_le
     """:func:`ops.prefill_attention` for 4-bit caches: packed query rows of sequences of different lengths (``q_start`` adds ``q_len`` up), which are the last rows of their ``ctx_lens`` cached ones. On
     GPUs the pages in use are unpacked to fp16 next to one another, :data:`EXPAND_PAGES_BYTES` of them at a time, and attended to there. ``q_len_host`` / ``ctx_len_host``: the same lengths on the
     host (else they are read back); ``tiles_for`` as there. What pages hold behind a sequence's end or in front of all its rows' windows does not matter. Pages outside the caches, cached lengths that are not the host's, and more query rows than
-    there are or than cached ones, are reported by :func:`ops.check_status`."""
+    there are or than cached ones, are reported by :func:`ops.check_status` (on the CPU: raised)."""
     T, D = q.shape[0], q.shape[1] // H
     if H % k_cache.shape[1] or window < 0 or softcap < 0 or not scale > 0:
         raise ValueError("KV heads must divide the query heads, scale must be positive, window and softcap not negative")
-    if not q.is_cuda:
-        _check_caches(k_cache, v_cache, D)
-        return _plain(q, k_cache, v_cache, block_tables, q_start, q_len, ctx_lens, H, scale, softcap, window, causal)
-    ext = ops.require_ext()
-    news = q_len_host if q_len_host is not None else q_len.tolist()
-    lens = ctx_len_host if ctx_len_host is not None else ctx_lens.tolist()
+    news = q_len_host if q_len_host is not None and q.is_cuda else q_len.tolist()
+    lens = ctx_len_host if ctx_len_host is not None and q.is_cuda else ctx_lens.tolist()
     S, KV, page = len(news), k_cache.shape[1], k_cache.shape[2]
     if sum(news) != T or len(lens) != S or any(not 0 <= n <= m for n, m in zip(news, lens)) or max(lens, default=0) > block_tables.shape[1] * page:
         raise ValueError("the query rows must be those of the sequences, no more than their cached rows, and these no more than the block table has")
+    if not q.is_cuda:
+        _check_caches(k_cache, v_cache, D)
+        if block_tables.dim() != 2 or block_tables.shape[0] != S or any(t.dtype != torch.int32 for t in (block_tables, q_start, q_len, ctx_lens)) or q_start.tolist() != [sum(news[:i]) for i in range(S)]:
+            raise ValueError("block_tables int32 [S, pages]; q_start, q_len, ctx_lens int32 [S], q_start the sums of q_len")
+        if (q_len_host is not None and list(q_len_host) != news) or (ctx_len_host is not None and list(ctx_len_host) != lens):
+            raise ValueError("the lengths on the host are other ones")
+        return _plain(q, k_cache, v_cache, block_tables, q_start, q_len, ctx_lens, H, scale, softcap, window, causal)
+    ext = ops.require_ext()
     if q.stride(1) != 1 or q.stride(0) % 8 or q.stride(0) < q.shape[1] or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)  # (``contiguous`` leaves a single row its stride)
     rows = ext.prefill_tc_tile_rows(D)

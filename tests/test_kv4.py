@@ -1162,3 +1162,29 @@ def test_prefill_takes_query_rows_as_they_lie(device, rows):
     for q in (wide[:, : H * D], wide[:, 1 : 1 + H * D], same.expand(rows, -1), torch.randn(H * D, rows, device=device).to(BF16).t()):
         assert torch.equal(call(q), call(q.clone(memory_format=torch.contiguous_format)))
     done(device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("change", [dict(ctx_lens=[70, 5]), dict(ctx_lens=[2, 5]), dict(ctx_lens=[40, -1]), dict(q_len=[3, 2]), dict(q_len=[5, -1]), dict(ctx_lens=[40, 5, 5]), dict(block_tables=[[1, 2]]),
+                                    dict(block_tables=torch.int64), dict(ctx_lens=torch.int64), dict(H=3), dict(H=8), dict(window=-1), dict(softcap=-1.0), dict(scale=0.0), dict(scale=math.nan), dict(k_cache=slice(0, 3))])
+def test_prefill_refuses(device, change):
+    """The same calls on the CPU and on a GPU, before anything is computed."""
+    a = attention_args(device, B=4)
+    a.update(q_start=torch.tensor([0, 3], dtype=torch.int32, device=device), q_len=torch.tensor([3, 1], dtype=torch.int32, device=device))
+    assert prefill_attention4(**a).shape == a["q"].shape
+    for name, c in change.items():
+        a[name] = a[name].to(c) if isinstance(c, torch.dtype) else a[name][c] if isinstance(c, slice) else torch.tensor(c, dtype=torch.int32, device=device) if isinstance(c, list) else c
+    with pytest.raises((ValueError, RuntimeError)):
+        prefill_attention4(**a)
+    done(device)
+
+
+def test_prefill_raises_on_the_cpu():
+    a = attention_args("cpu", B=4)
+    a.update(q_start=torch.tensor([0, 3], dtype=torch.int32), q_len=torch.tensor([3, 1], dtype=torch.int32))
+    for change in (dict(q_len_host=[2, 2]), dict(ctx_len_host=[40, 6]), dict(q_start=torch.tensor([0, 2], dtype=torch.int32))):
+        with pytest.raises(ValueError):
+            prefill_attention4(**{**a, **change})
+    for table in ([[1, 9], [3, 0]], [[1, -2], [3, 0]]):
+        with pytest.raises(IndexError):
+            prefill_attention4(**{**a, "block_tables": torch.tensor(table, dtype=torch.int32)})
