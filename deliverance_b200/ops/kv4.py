@@ -144,24 +144,24 @@ def prefill_attention4(q, k_cache, v_cache, block_tables, q_start, q_len, ctx_le
     # 700 rows of 16 heads 23.2 for 26.4, 2,048 of 8 heads 45.3 for 53.4, 200 rows behind 9,000 of 32 heads 193 for 221). Beyond that the second wave costs more (1,024 rows of 32 heads 45.7 for 35.7).
     if sum(-(-n // 128) for n in news) * H <= 148:
         rows = 128
-    parts = _parts(news, lens, rows, H, window)
     pages = [-(-n // page) for n in lens]
+    tile_seq, tile_q0 = tiles_for(rows) if tiles_for is not None else _tiles(news, rows, q.device)
     if sum(pages) * KV * page * D * 4 <= EXPAND_PAGES_BYTES or S == 1:
-        tile_seq, tile_q0 = tiles_for(rows) if tiles_for is not None else _tiles(news, rows, q.device)
+        parts = _parts(news, lens, rows, H, window)
         ops._count(2 + (parts > 1))
         return ext.kv4_prefill(q, k_cache, v_cache, block_tables, q_start, q_len, ctx_lens, tile_seq, tile_q0, H, scale, softcap, window, causal, sum(pages), max(pages, default=0), rows, parts)
-    outs, i, row = [], 0, 0
+    outs, i, row, tile = [], 0, 0, 0  # (nothing comes from the host here: the portions' tables are cut out of the call's)
     while i < S:
         j, n_pages = i, 0
         while j < S and (j == i or (n_pages + pages[j]) * KV * page * D * 4 <= EXPAND_PAGES_BYTES):
             n_pages += pages[j]
             j += 1
-        part, n = slice(i, j), sum(news[i:j])
-        tile_seq, tile_q0 = _tiles(news[part], rows, q.device)
-        ops._count(2)
-        outs.append(ext.kv4_prefill(q[row : row + n], k_cache, v_cache, block_tables[part], q_start[part] - row, q_len[part], ctx_lens[part], tile_seq, tile_q0, H, scale, softcap, window, causal,
-                                    n_pages, max(pages[part]), rows, 1))
-        i, row = j, row + n
+        part, n, n_tiles = slice(i, j), sum(news[i:j]), sum(-(-m // rows) for m in news[i:j])
+        parts = _parts(news[part], lens[part], rows, H, window)
+        ops._count(2 + (parts > 1))
+        outs.append(ext.kv4_prefill(q[row : row + n], k_cache, v_cache, block_tables[part], q_start[part] - row, q_len[part], ctx_lens[part], tile_seq[tile : tile + n_tiles] - i,
+                                    tile_q0[tile : tile + n_tiles], H, scale, softcap, window, causal, n_pages, max(pages[part]), rows, parts))
+        i, row, tile = j, row + n, tile + n_tiles
     return torch.cat(outs)
 
 

@@ -1188,3 +1188,36 @@ def test_prefill_raises_on_the_cpu():
     for table in ([[1, 9], [3, 0]], [[1, -2], [3, 0]]):
         with pytest.raises(IndexError):
             prefill_attention4(**{**a, "block_tables": torch.tensor(table, dtype=torch.int32)})
+
+
+@pytest.mark.parametrize("device", GPU)
+def test_prefill_in_portions_captured(device, monkeypatch):
+    """Portions take the tiles that the caller has (nothing is copied from the host: such a call can be captured), and their keys in parts where they have few tiles."""
+    from deliverance_b200.ops import kv4
+
+    KV, D, H, page, news, befores = 2, 64, 4, 32, [70, 0, 40, 1, 300], [100, 50, 0, 2000, 5]
+    lens = [a + b for a, b in zip(news, befores)]
+    table, pages = tables_for(lens, page)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    k, v = (random_cache(pages, KV, page, D, False) for _ in range(2))
+    start = [sum(news[:i]) for i in range(len(news))]
+    args = (k.to(device), v.to(device), table.to(device), i32(start), i32(news), i32(lens), H, 0.1)
+    tiles, asked = {rows: tuple(i32(t) for t in ops.prefill_tiles(news, rows)) for rows in (128, 256)}, []
+    run = lambda q: prefill_attention4(q, *args, q_len_host=news, ctx_len_host=lens, tiles_for=lambda rows: asked.append(rows) or tiles[rows])  # noqa: E731
+    q = torch.randn(sum(news), H * D).to(BF16).to(device)
+    monkeypatch.setattr(kv4, "EXPAND_PAGES_BYTES", 20 * KV * page * D * 4)
+    seen, rule = [], kv4._parts
+    monkeypatch.setattr(kv4, "_parts", lambda *a: seen.append(rule(*a)) or seen[-1])
+    run(q)
+    torch.cuda.synchronize()
+    assert asked and max(seen) > 1 and len(seen) > 1
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(q)
+    for _ in range(2):
+        q.copy_(torch.randn(q.shape))
+        graph.replay()
+        torch.cuda.synchronize()
+        want, mass, reach = plain_attention(q.cpu(), k, v, table, lens, news, KV, 0.1, 0.0, 0)
+        assert ((out.cpu().double() - want).abs() <= want.abs() * HALF_STEP + mass * (2.0**-10 + 2.0**-11 + reach * (2.0**-10 + 2.0**-16)) + 2.0**-24).all()
+    done(device)
