@@ -147,6 +147,8 @@ def _codec_for(codec: MseTurboQuantCodec, dim: int, bits: int) -> MseTurboQuantC
 
 def snapshot_pages(kv, pages: list[int], n_tokens: int, compression: str = "NONE", bits: int = 3) -> dict:
     """Host copy of the K/V rows of ``pages`` for every attention layer (``NONE`` | ``LZ4`` | ``DEFLATE`` | ``MSE_TURBOQUANT``)."""
+    if compression == "MSE_TURBOQUANT" and getattr(kv, "bits", 16) == 4:
+        raise ValueError("rows of a 4-bit cache are stored as they are (NONE, LZ4, DEFLATE), not quantised again")
     out = {"compression": compression, "n_tokens": n_tokens, "layers": {}}
     codec = None
     for i, k in enumerate(kv.k):

@@ -1221,3 +1221,21 @@ def test_prefill_in_portions_captured(device, monkeypatch):
         want, mass, reach = plain_attention(q.cpu(), k, v, table, lens, news, KV, 0.1, 0.0, 0)
         assert ((out.cpu().double() - want).abs() <= want.abs() * HALF_STEP + mass * (2.0**-10 + 2.0**-11 + reach * (2.0**-10 + 2.0**-16)) + 2.0**-24).all()
     done(device)
+
+
+@pytest.mark.parametrize("compression", ["NONE", "LZ4", "DEFLATE", "MSE_TURBOQUANT"])
+def test_snapshots_hold_the_rows_as_they_are(compression):
+    from deliverance_b200.kv.paged import KvCacheSettings, PagedKVCache
+    from deliverance_b200.kv.turboquant import restore_pages, snapshot_pages
+
+    layout = dict(layer_kinds=["full"] * 2, kv_heads=2, head_dim=64)
+    a, b = (PagedKVCache(layout, 8, "cpu", torch.float32, KvCacheSettings(bits=4)) for _ in range(2))
+    for t in a.k + a.v:
+        t.copy_(random_cache(8, 2, 32, 64))
+    if compression == "MSE_TURBOQUANT":  # (a codec for numbers: bytes do not come back)
+        with pytest.raises(ValueError, match="4-bit"):
+            snapshot_pages(a, [5, 2], 40, compression)
+        return
+    restore_pages(b, snapshot_pages(a, [5, 2], 40, compression), [3, 7])
+    for s, t in zip(a.k + a.v, b.k + b.v):
+        assert torch.equal(t[3], s[5]) and torch.equal(t[7, :, :8], s[2, :, :8])
