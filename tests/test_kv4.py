@@ -1239,3 +1239,158 @@ def test_snapshots_hold_the_rows_as_they_are(compression):
     restore_pages(b, snapshot_pages(a, [5, 2], 40, compression), [3, 7])
     for s, t in zip(a.k + a.v, b.k + b.v):
         assert torch.equal(t[3], s[5]) and torch.equal(t[7, :, :8], s[2, :, :8])
+
+
+# what else decoders have around their attention: biases, local and global layers, recurrent layers, experts
+FAMILIES = [("qwen2", {}), ("gemma3_text", {}), ("mixtral", {}), ("qwen3_moe", {}), ("granitemoehybrid", dict(mamba_n_heads=16))]
+
+
+def replayed(e, tokens, cuts):
+    """Logits of all positions, ``tokens`` fed in portions of the given sizes and the rest one by one."""
+    r, out, at = e.open_replay(), [], 0
+    for n in list(cuts) + [1] * (len(tokens) - sum(cuts)):
+        out.append(e.replay_step([(r, tokens[at : at + n], list(range(n)))]))
+        at += n
+    return torch.cat(out)
+
+
+@pytest.mark.parametrize("family,over", FAMILIES)
+def test_engine_families(tmp_path, family, over):
+    """A prompt whole, in portions, and token by token. (Tokens alone prove nothing here: fp32 sums of other lengths move a number by 2^-23 of its size, which now and then falls on the other side of a code's
+    border; a step is a fifteenth of a block's range, and what it moves in the logits is a few per cent of their spread.)"""
+    model = tiny_model(tmp_path, family=family, **{**HEADS, **over})
+    assert model.supports_kv4()
+    e, tokens = engine_of(model, max_batch_tokens=4096, kv={"enabled": False}), prompt_of(110)
+    whole, portions, single = (replayed(e, tokens, cuts) for cuts in ([110], [33, 60], [1]))
+    assert all(k is None or k.dtype == torch.uint8 for k in e.kv.k)
+    rms = lambda x: x.double().square().mean().sqrt()  # noqa: E731
+    assert rms(whole - portions) < 0.05 * rms(whole) and rms(whole - single) < 0.05 * rms(whole)
+    assert rms(whole - replayed(engine_of(model, 16, max_batch_tokens=4096, kv={"enabled": False}), tokens, [110])) > 1e-3 * rms(whole)  # (fp32 noise is 1e-5)
+    e = engine_of(model)
+    first = e.generate(prompt_of(90), params_of(12))
+    again = e.generate(prompt_of(90), params_of(12))
+    assert len(first.token_ids) == 12 and again.prefix_hit_tokens > 0
+    e.kv.audit([])
+
+
+@pytest.mark.parametrize("device", GPU)
+@pytest.mark.parametrize("family,over", [f for f in FAMILIES if f[0] not in ("mixtral", "qwen3_moe")])
+def test_engine_families_match_the_cpu(tmp_path, device, family, over):
+    """Logits of a prompt, of a portion behind it and of decode steps against the plain forms in fp32 of the same checkpoint."""
+    got, tokens = {}, prompt_of(100)
+    for d in ("cpu", device):
+        model = tiny_model(tmp_path, d, family, **{**HEADS, **over})
+        for bits in (16, 4):
+            got[d, bits] = replayed(engine_of(model, bits, max_batch_tokens=4096, kv={"enabled": False}), tokens, [60, 20]).double()
+    # A number lies within 7.5 steps s of its block's middle. Rounded to bf16 it is off by up to 7.5 s 2^-8 = 0.03 s, and so are the roundings in front of it: with probability 0.03 or so it gets another code, s away,
+    # which makes sqrt(0.03) s = 0.17 s in the mean square, where quantising itself makes s / sqrt(12) = 0.29 s. Hence: off by less than what bf16 makes without codes, and what quantising makes, together.
+    err = lambda a, b: (got[a] - got[b]).square().mean(1).sqrt().mean()  # noqa: E731
+    assert err((device, 4), ("cpu", 4)) < err((device, 16), ("cpu", 16)) + err(("cpu", 16), ("cpu", 4))
+    done(device)
+
+
+@pytest.mark.parametrize("device", GPU)
+@pytest.mark.parametrize("family,over", [("llama", {}), ("qwen3", dict(hidden_size=512, head_dim=128)), ("gemma2", {})])
+def test_captured_steps_have_the_logits_of_single_launches(tmp_path, device, family, over):
+    """The two divide the keys of decode attention otherwise (by the widest block table there can be, and by the batch's own), so that they agree up to roundings, and codes by a step where those decide."""
+    model = tiny_model(tmp_path, device, family, **{**HEADS, **over})
+    rows = []
+    for graphs in (True, False):
+        e = engine_of(model, max_batch_tokens=4096, kv={"enabled": False}, cuda_graphs=graphs)
+        open_, parts = [e.open_replay() for _ in range(3)], []
+        texts = [prompt_of(n + 30, k) for k, n in enumerate((70, 5, 133))]
+        e.replay_step([(r, t[:-30], []) for r, t in zip(open_, texts)])
+        for i in range(-30, 0):
+            parts.append(e.replay_step([(r, [t[i]], [0]) for r, t in zip(open_, texts)]))
+        rows.append(torch.stack(parts))
+        assert (e.metrics["graph_replays"] > 0) == graphs
+    err, spread = (rows[0] - rows[1]).double().square().mean(-1).sqrt(), rows[0].double().std()
+    assert err.mean() < 0.05 * spread
+    assert (rows[0][:, 0] - rows[1][:, 1]).double().square().mean(-1).sqrt().mean() > 0.5 * spread  # (those of another sequence)
+    done(device)
+
+
+def adapter_of(tmp, model):
+    import json
+    import os
+
+    from deliverance_b200.ckpt.lora import lora_names
+    from deliverance_b200.ckpt.safetensors_io import write_safetensors
+
+    c, tensors = model.cfg, {}
+    shapes = {"q_proj": c.num_heads * c.head_dim, "k_proj": c.num_kv_heads * c.head_dim, "v_proj": c.num_kv_heads * c.head_dim}
+    for i in range(c.num_layers):
+        for proj, n in shapes.items():
+            a, b = lora_names(f"model.layers.{i}.self_attn.{proj}.weight")
+            tensors[a], tensors[b] = torch.randn(4, model.embed.shape[1]) * 0.2, torch.randn(n, 4) * 0.2
+    os.makedirs(tmp)
+    write_safetensors(os.path.join(tmp, "adapter_model.safetensors"), tensors)
+    with open(os.path.join(tmp, "adapter_config.json"), "w") as f:
+        json.dump({"r": 4, "lora_alpha": 8, "target_modules": list(shapes)}, f)
+    return tmp
+
+
+def test_engine_lora(tmp_path):
+    """Queries, keys and values with an adapter's share: swapped in, the same as merged into the weights."""
+    from deliverance_b200.api import AutoModelForCausalLM
+    from deliverance_b200.kv.paged import KvCacheSettings
+
+    model = tiny_model(tmp_path, **HEADS)
+    d, settings = str(next(tmp_path.iterdir())), KvCacheSettings(bits=4)
+    adapter = adapter_of(str(tmp_path / "adapter"), model)
+    build = lambda b: b.with_device("cpu").with_kv_cache_settings(settings).build()  # noqa: E731
+    base, merged = build(AutoModelForCausalLM.new_builder(d)), build(AutoModelForCausalLM.new_builder(d).with_lora_adapter(adapter))
+    prompt, p = prompt_of(40), params_of(20)
+    plain, want = base.generate(prompt, p).token_ids, merged.generate(prompt, p).token_ids
+    assert base.engine.kv.bits == merged.engine.kv.bits == 4
+    base.activate_lora(base.register_lora(adapter))
+    assert base.generate(prompt, p).token_ids == want != plain
+    base.activate_lora(None)
+    assert base.generate(prompt, p).token_ids == plain
+
+
+@pytest.mark.parametrize("family", ["llama", "qwen3", "gemma2"])
+def test_engine_tensor_parallel(tmp_path, family):
+    """Two ranks with a KV head each in 4 bits answer as one with both."""
+    import threading
+
+    from deliverance_b200.ckpt.loader import WeightLoader
+    from deliverance_b200.config import load_config
+    from deliverance_b200.models.transformer import DecoderModel, TensorParallelContext
+    from deliverance_b200.parallel.context import InProcessCollectives, InProcessGroup
+
+    one = tiny_model(tmp_path, family=family, **HEADS)
+    d = str(next(tmp_path.iterdir()))
+    prompts = [prompt_of(40), prompt_of(7, 1)]
+    want = [r.token_ids for r in engine_of(one).generate_batch(prompts, params_of(20))]
+    group, got = InProcessGroup(2, timeout=60), [None, None]
+
+    def rank(r):
+        try:
+            model = DecoderModel(load_config(d), "cpu", tp=TensorParallelContext(r, 2, InProcessCollectives(group, r))).load(WeightLoader(d))
+            e = engine_of(model)
+            assert e.kv.k[0].shape[1] == 1 and e.kv.k[0].dtype == torch.uint8
+            got[r] = [x.token_ids for x in e.generate_batch(prompts, params_of(20))]
+        except Exception as e:  # noqa: BLE001
+            got[r] = e
+
+    threads = [threading.Thread(target=rank, args=(r,)) for r in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert got[0] == got[1] == want, got
+
+
+@pytest.mark.parametrize("device", GPU)
+@pytest.mark.parametrize("D,KV,G,news,befores,softcap", [(64, 2, 3, [33, 5], [2100, 70], 0.0), (128, 8, 4, [257, 500], [40, 0], 0.0), (128, 1, 4, [130, 1, 64], [3, 4031, 0], 30.0), (256, 2, 1, [70, 300], [0, 900], 0.0)])
+def test_prefill_against_what_the_cache_holds(device, D, KV, G, news, befores, softcap):
+    """Against 64 bits over the cached values themselves: fp16 keys and values count as the kernels' errors."""
+    lens, H = [a + b for a, b in zip(news, befores)], KV * G
+    table, pages = tables_for(lens, 32)
+    k, v = random_cache(pages, KV, 32, D), random_cache(pages, KV, 32, D, False)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    q, start = torch.randn(sum(news), H * D).to(BF16), [sum(news[:i]) for i in range(len(news))]
+    got = prefill_attention4(q.to(device), k.to(device), v.to(device), table.to(device), i32(start), i32(news), i32(lens), H, D**-0.5, softcap).cpu().double()
+    done(device)
+    want, mass, reach = plain_attention(q, k, v, table, lens, news, KV, D**-0.5, softcap, 0)
+    # the result in bf16; probabilities and values in fp16 (half a step each, 2^-11; probabilities in numerator and denominator); a key in fp16 moves its score by 2^-11 of sum |q| |k| (numerator and denominator), fp32 sums as in decoding
+    assert ((got - want).abs() <= want.abs() * HALF_STEP + mass * (2.0**-10 + 2.0**-11 + reach * (2.0**-10 + 2.0**-16)) + 2.0**-24).all()
