@@ -1394,3 +1394,60 @@ def test_prefill_against_what_the_cache_holds(device, D, KV, G, news, befores, s
     want, mass, reach = plain_attention(q, k, v, table, lens, news, KV, D**-0.5, softcap, 0)
     # the result in bf16; probabilities and values in fp16 (half a step each, 2^-11; probabilities in numerator and denominator); a key in fp16 moves its score by 2^-11 of sum |q| |k| (numerator and denominator), fp32 sums as in decoding
     assert ((got - want).abs() <= want.abs() * HALF_STEP + mass * (2.0**-10 + 2.0**-11 + reach * (2.0**-10 + 2.0**-16)) + 2.0**-24).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D,news,befores", [(64, [70, 3], [100, 0]), (128, [5], [2000]), (256, [130, 1], [9, 0])])
+def test_prefill_that_is_not_causal(device, D, news, befores):
+    KV, H, page, lens = 2, 4, 32, [a + b for a, b in zip(news, befores)]
+    table, pages = tables_for(lens, page)
+    k, v = random_cache(pages, KV, page, D), random_cache(pages, KV, page, D, False)
+    to, i32 = lambda t: t.to(device), lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    q = torch.randn(sum(news), H * D).to(BF16)
+    got = prefill_attention4(to(q), to(k), to(v), to(table), i32([0, news[0]][: len(news)]), i32(news), i32(lens), H, D**-0.5, causal=False).cpu().double()
+    done(device)
+    # every query row sees all keys, as the last row of its sequence does
+    seq = torch.repeat_interleave(torch.arange(len(news)), torch.tensor(news))
+    want, mass, reach = plain_attention(q, k, v, table[seq], [lens[b] for b in seq.tolist()], [1] * len(seq), KV, D**-0.5, 0.0, 0)
+    assert ((got - want).abs() <= want.abs() * HALF_STEP + mass * (2.0**-10 + 2.0**-11 + reach * (2.0**-10 + 2.0**-16)) + 2.0**-24).all()
+
+
+@pytest.mark.parametrize("device", GPU)
+def test_caches_beyond_32_bits(device):
+    """Rows whose bytes lie more than 2^32 behind the first ones: write, decode and prompt attention, unpacking."""
+    D, H, KV, page, lens = 128, 16, 8, 32, [90, 33]
+    pages = 2**32 // (KV * page * row_bytes(D)) + 40
+    kc, vc = (torch.zeros(pages, KV, page, row_bytes(D), dtype=torch.uint8, device=device) for _ in range(2))
+    far = [[pages - 1, pages - 7, pages - 3], [pages - 2, pages - 9]]
+    table = torch.tensor([far[0], far[1] + [0]], dtype=torch.int32)
+    slots = torch.tensor([far[b][j // page] * page + j % page for b, n in enumerate(lens) for j in range(n)])
+    T, at = sum(lens), [0, lens[0]]
+    x, i32 = torch.randn(T, (H + 2 * KV) * D).to(BF16), lambda v: torch.tensor(v, dtype=torch.int32, device=device)  # noqa: E731
+    q = rope_kv4(x.to(device), torch.zeros(T, dtype=torch.int32, device=device), slots.to(device), None, None, None, None, kc, vc, H, KV, D, 1e-6).cpu()
+    done(device)
+    assert torch.equal(q, x[:, : H * D]) and not kc[: pages - 9].any() and not vc[: pages - 9].any()
+    k, v = kc[pages - 9 :].cpu(), vc[pages - 9 :].cpu()
+    near = torch.where(table > 0, table - (pages - 9), 0)
+    for cache, cols in ((k, x.view(T, -1, D)[:, H : H + KV]), (v, x.view(T, -1, D)[:, H + KV :])):
+        rows = torch.cat([cache[near[b].long()].transpose(1, 2).flatten(0, 1)[:n] for b, n in enumerate(lens)])
+        assert torch.equal(rows, ref.kv4_pack(cols))
+    whole = prefill_attention4(q.to(device), kc, vc, table.to(device), i32(at), i32(lens), i32(lens), H, D**-0.5).cpu().double()
+    want, mass, reach = plain_attention(q, k, v, near, lens, lens, KV, D**-0.5, 0.0, 0)
+    assert ((whole - want).abs() <= want.abs() * HALF_STEP + mass * (2.0**-10 + 2.0**-11 + reach * (2.0**-10 + 2.0**-16)) + 2.0**-24).all()
+    last = q[[lens[0] - 1, T - 1]]
+    got = decode_attention4(last.to(device), kc, vc, table.to(device), i32(lens), H, D**-0.5)
+    check_decode(got, last, k, v, near, lens, KV, D**-0.5, 0.0, 0)
+    for a, b in zip(expand4(kc, vc, i32([pages - 1, pages - 9]), torch.float32), (k, v)):
+        assert torch.equal(a.cpu(), ref.kv4_unpack(b[[8, 0]]))
+    done(device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("B,KV", [(1, 1), (3, 2), (50, 4), (600, 8)])
+def test_decode_without_keys(device, B, KV):
+    k = random_cache(3, KV, 32, 64).to(device)
+    q = torch.randn(B, KV * 2 * 64, device=device).to(BF16)
+    zero = torch.zeros(B, dtype=torch.int32, device=device)
+    assert (decode_attention4(q, k, k, torch.zeros(B, 9, dtype=torch.int32, device=device), zero, KV * 2, 0.1) == 0).all()
+    assert decode_attention4(q[:0], k, k, torch.zeros(0, 9, dtype=torch.int32, device=device), zero[:0], KV * 2, 0.1).shape == (0, KV * 128)
+    done(device)
