@@ -1451,3 +1451,30 @@ def test_decode_without_keys(device, B, KV):
     assert (decode_attention4(q, k, k, torch.zeros(B, 9, dtype=torch.int32, device=device), zero, KV * 2, 0.1) == 0).all()
     assert decode_attention4(q[:0], k, k, torch.zeros(0, 9, dtype=torch.int32, device=device), zero[:0], KV * 2, 0.1).shape == (0, KV * 128)
     done(device)
+
+
+@pytest.mark.parametrize("device", GPU)
+def test_batches_made_there_of_odd_entries(device):
+    """Entries without tokens, tokens in a tensor, pages in reserve, many sequences: the host's batch, field by field."""
+    from deliverance_b200.models.batch import make_batch
+
+    one = lambda n, start, pages, **kw: {"tokens": [(7 * i) % 99 for i in range(n)], "start": start, "pages": pages, **kw}  # noqa: E731
+    cases = [
+        [one(0, 5, [3]), one(4, 0, [9, 2])],
+        [one(0, 0, []), one(0, 0, [])],
+        [one(3, 0, [1])] * 9000,  # (more than the kernel takes: made on the host)
+        [one(2, 62, [4, 5, 6, 7, 8]), one(1, 0, [1])] * 2000,
+        [dict(one(0, 0, [2, 3]), tokens=torch.arange(40, dtype=torch.int64)), dict(one(0, 7, [5], cached=3), tokens=torch.tensor([8, 9]))],
+    ]
+    for seqs in cases:
+        a, b = make_batch(seqs, 32, "cpu"), make_batch(seqs, 32, device)
+        done(device)
+        for name in ("token_ids", "positions", "slots", "q_start", "q_len", "ctx_len", "block_tables", "logits_rows", "tile_seq", "tile_q0"):
+            x, y = getattr(a, name), getattr(b, name)
+            assert (x is None) == (y is None) and (x is None or (x.dtype == y.dtype and torch.equal(x, y.cpu()))), name
+        assert (a.is_decode, a.q_len_host, a.ctx_len_host) == (b.is_decode, b.q_len_host, b.ctx_len_host)
+    for seqs, kw in (([one(40, 0, [1])], {}), ([one(4, 0, [1, 2, 3])], {"max_pages": 2})):
+        for d in ("cpu", device):
+            with pytest.raises((ValueError, RuntimeError)):
+                make_batch(seqs, 32, d, **kw)
+    done(device)
