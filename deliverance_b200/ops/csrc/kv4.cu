@@ -316,7 +316,7 @@ void launch_kv4_expand(const Kv4ExpandArgs& a, cudaStream_t st) {
 }
 
 // The pages of a step's sequences -> fp16 pages next to one another (sequence by sequence), for prompt attention, with block tables that name them; a page becomes page / out_page of them.
-// Rows behind a sequence's end, and rows that no window reaches, are zeros there: what stands in them does not matter, not even NaN. fp16, because a value is the sum of two fp16 numbers: 2^-12 of it are lost, where bf16 would lose 2^-9. A thread takes four units of 8 numbers, keys and values; grid (units of a page / 1024, pages of the longest sequence, S).
+// Rows behind a sequence's end, and rows that no window reaches, are zeros there: what stands in them does not matter, not even NaN. fp16, because a value is the sum of two fp16 numbers: up to 2^-11 of it are lost, where bf16 would lose 2^-8. A thread takes four units of 8 numbers, keys and values; grid (units of a page / 1024, pages of the longest sequence, S).
 template <int D>
 __global__ void __launch_bounds__(256) kv4_expand_seqs_kernel(const Kv4SeqsArgs a) {
   pdl_trigger();

@@ -56,7 +56,7 @@ def rope_kv4(qkv, positions, slots, q_norm_w, k_norm_w, cos, sin, k_cache, v_cac
 
 
 def expand4(k_cache, v_cache, pages, dtype: torch.dtype = torch.bfloat16):
-    """The values of some pages (int32 ``[n]``, any order, repeats allowed) as ``[n, KV, page, D]`` keys and values in bf16 or fp32 (fp32: exact). Pages outside the caches are
+    """The values of some pages (int32 ``[n]``, any order, repeats allowed) as ``[n, KV, page, D]`` keys and values in bf16 or fp32, each rounded once. Pages outside the caches are
     reported by :func:`ops.check_status` (on the CPU: an IndexError)."""
     D = k_cache.shape[3] * 8 // 5
     if dtype not in (torch.bfloat16, torch.float32):

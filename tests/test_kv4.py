@@ -1478,3 +1478,13 @@ def test_batches_made_there_of_odd_entries(device):
             with pytest.raises((ValueError, RuntimeError)):
                 make_batch(seqs, 32, d, **kw)
     done(device)
+
+
+@pytest.mark.parametrize("device", GPU)
+def test_prefill_portions_without_rows(device, monkeypatch):
+    """Sequences without new tokens that fill portions of their own."""
+    from deliverance_b200.ops import kv4
+
+    monkeypatch.setattr(kv4, "EXPAND_PAGES_BYTES", 8 * 2 * 32 * 64 * 4)
+    run_prefill(device, 64, 2, 2, [0, 5, 0, 0, 130], [400, 300, 700, 0, 20])
+    run_prefill(device, 64, 2, 2, [0, 0], [400, 300])
